@@ -520,6 +520,58 @@ int ts2_op_attention_backward_limited(int device, void *stream, int variant, con
                                       const float *lse, const float *dscale, const int32_t *span_start, const int32_t *span_finish, int T,
                                       int head_count, float alibi_slope, void *dq, void *dk, void *dv, int64_t score_gradient_bytes);
 
+/* Parts of a training step that the engine does not run itself, for callers that build their own layers or optimizer (no
+ * counterparts in the reference's backward path).  All pointers but coef are device pointers; the calls are asynchronous on
+ * `stream`, take their scratch from the library's pool (ts2_dev_trim) and may be captured into a graph after a first call outside
+ * of one.  type: element type of the arrays without another one in their description: TS2_OUT_F32, TS2_OUT_F16 or TS2_OUT_BF16; fp16
+ * results saturate at +-65504.  Arrays need the alignment of their elements only; rows whose pitch and base allow 16-byte (the
+ * recurrence: two-element) accesses are read faster.  An output may not overlap anything else the call uses, unless said
+ * otherwise.  The results do not depend on the schedule: the same call gives the same bits. */
+
+/* Gated linear recurrence of a sequence-mixing layer over packed sequences, per channel:
+ *     h[t] = a[t] h[t-1] + (1 - a[t]) x[t],   a[t] = 1 / (1 + exp(-gate[t]))
+ * gate, x, h: [T][D], rows of *_ld elements.  seq_ptr[n_seq + 1] ascends inside [0, T]: sequence s is the nodes
+ * [seq_ptr[s], seq_ptr[s + 1]), possibly none; null: one sequence (n_seq 1) over all T nodes.  Nodes before the first and
+ * behind the last sequence are left as they were.  h0 (optional): fp32 [n_seq][D], the state before each sequence's first node
+ * (zero without it); h_last (optional): fp32 [n_seq][D], the state behind its last one, h0's where a sequence is empty.  A
+ * sequence of one token with h0 and h_last is a step of generation.  States are fp32 inside a call.  T up to 2^30. */
+int ts2_op_recurrence_forward(int device, void *stream, int type, const void *gate, int64_t gate_ld, const void *x, int64_t x_ld, int T, int D,
+                              int n_seq, const int32_t *seq_ptr, const float *h0, void *h, int64_t h_ld, float *h_last);
+/* Its backward pass: h is what the forward call left; dh [T][D] the gradient of h, dh_last (optional) that of h_last ->
+ * dgate, dx [T][D], dh0 (optional) fp32 [n_seq][D].  All are gradients of the same sign. */
+int ts2_op_recurrence_backward(int device, void *stream, int type, const void *gate, int64_t gate_ld, const void *x, int64_t x_ld, const void *h,
+                               int64_t h_ld, int T, int D, int n_seq, const int32_t *seq_ptr, const float *h0, const void *dh, int64_t dh_ld,
+                               const float *dh_last, void *dgate, int64_t dgate_ld, void *dx, int64_t dx_ld, float *dh0);
+
+/* Load balance of a mixture-of-experts router over the choices ts2_moe_route makes.  With p[t] = softmax(logits[t]), N tokens
+ * that count, C[e] choices of expert e among theirs:
+ *     loss = expert_count / (selected N) sum_e C[e] prob[e],   prob[e] = mean_t p[t][e]
+ * (1 where all experts get the same, up to expert_count; 0 without tokens).  logits [T][expert_count], rows of ld elements;
+ * ids int32 [T][selected], an id outside [0, expert_count) is a choice not made; token_mask (optional) [T]: tokens with a zero
+ * byte do not count, whatever their logits and ids are.  A row of logits that is -inf throughout has no probabilities, but its
+ * token counts.  counts: int32 [expert_count + 1], C and behind it N; prob fp32 [expert_count]; loss fp32 [1].
+ * expert_count up to 1024, T up to 2^30, T * selected below 2^31. */
+int ts2_op_moe_balance_forward(int device, void *stream, int type, const void *logits, int64_t ld, int64_t T, int expert_count, int selected,
+                               const int32_t *ids, const uint8_t *token_mask, int32_t *counts, float *prob, float *loss);
+/* dlogits[t][e] (+)= *dloss * scale * expert_count / (selected N^2) p[t][e] (C[e] - sum_j C[j] p[t][j]), the gradient of that
+ * loss; tokens that do not count get zeros.  counts: of the forward call, or summed over ranks (then the loss is that of the
+ * whole batch and every rank has its rows' part of the gradient).  dloss: fp32 [1], null: 1.  add: dlogits += instead of =.
+ * With a negative scale it is an ascent direction, as the engine's gradients are. */
+int ts2_op_moe_balance_backward(int device, void *stream, int type, const void *logits, int64_t ld, int64_t T, int expert_count, int selected,
+                                const uint8_t *token_mask, const int32_t *counts, const float *dloss, float scale, void *dlogits, int64_t dlogits_ld,
+                                int add);
+
+/* Orthogonalised update: out = out_scale * U q(S / |G|) V^T for every matrix G = U S V^T of a batch, q = `steps` times
+ * p(s) = coef[0] s + coef[1] s^3 + coef[2] s^5 (a host array), |G| the Frobenius norm: Newton-Schulz products that take the
+ * singular values to about one.  g: [batch] matrices [rows][cols] of `type`, rows of ld elements, g_stride elements apart (may
+ * be 0); out: bf16, alike (out_ld, out_stride); out may be g itself where type is TS2_OUT_BF16 and the pitches agree.  A zero
+ * matrix gives zeros, one with a NaN or an infinity NaNs; the scale of g does not matter.  Products are fp16 with fp32 sums, the
+ * iterate is held in 32 bits: the result is within 2e-3 (relative L2, before its rounding to bf16) of the formula for the usual
+ * coefficients (3.4445, -4.7750, 2.0315), 5 steps.  TS2_ERR_UNSUPPORTED for coefficients that take a singular value beyond 3.9, which
+ * the fp16 scaling does not allow.  Up to 64 steps, 65535 matrices, 2^20 rows and columns. */
+int ts2_op_orthogonalize(int device, void *stream, int type, const void *g, int64_t ld, int64_t g_stride, int batch, int64_t rows, int64_t cols,
+                         const float coef[3], int steps, float out_scale, void *out, int64_t out_ld, int64_t out_stride);
+
 #ifdef __cplusplus
 }
 #endif

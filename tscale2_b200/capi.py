@@ -163,6 +163,11 @@ def _declare(lib):
         "ts2_attention_forward": (i32, [i32, vp, i32, vp, vp, vp, vp, vp, i32, i32, f32, vp, vp]),
         "ts2_attention_backward": (i32, [i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, f32, vp, vp, vp]),
         "ts2_op_attention_backward_limited": (i32, [i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, f32, vp, vp, vp, i64]),
+        "ts2_op_recurrence_forward": (i32, [i32, vp, i32, vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, i64, vp]),
+        "ts2_op_recurrence_backward": (i32, [i32, vp, i32, vp, i64, vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, i64, vp, vp, i64, vp, i64, vp]),
+        "ts2_op_moe_balance_forward": (i32, [i32, vp, i32, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp]),
+        "ts2_op_moe_balance_backward": (i32, [i32, vp, i32, vp, i64, i64, i32, i32, vp, vp, vp, f32, vp, i64, i32]),
+        "ts2_op_orthogonalize": (i32, [i32, vp, i32, vp, i64, i64, i32, i64, i64, P(f32), i32, f32, vp, i64, i64]),
         "ts2_gemm_dw": (i32, [i32, vp, i32, i32, i64, i64, i64, vp, vp, vp, f32, vp, C.c_size_t]),
     }
     missing = []

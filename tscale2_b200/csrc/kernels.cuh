@@ -231,6 +231,20 @@ int moe_combine_backward(const Ctx &c, const void *y, bool y16, const int *slot_
 int moe_router_backward(const Ctx &c, const float *dmoe_part, int tiles, const int *ids, const float *weights, const int *slot_of, int T,
                         int k, int E, int ld, void *dl);
 
+// ---- kernels_balance.cu, kernels_recurrence.cu, kernels_orth.cu ---------------------
+// what the ts2_op_* calls of the same names do (include/ts2_b200.h); type: TS2_OUT_F32, TS2_OUT_F16 or TS2_OUT_BF16
+int moe_balance_forward(const Ctx &c, int type, const void *logits, int64_t ld, int64_t T, int E, int selected, const int *ids,
+                        const uint8_t *mask, int *counts, float *prob, float *loss);
+int moe_balance_backward(const Ctx &c, int type, const void *logits, int64_t ld, int64_t T, int E, int selected, const uint8_t *mask,
+                         const int *counts, const float *dloss, float scale, void *dlogits, int64_t ld_d, bool add);
+int recurrence_forward(const Ctx &c, int type, const void *gate, int64_t gate_ld, const void *x, int64_t x_ld, int T, int D, int n_seq,
+                       const int *seq_ptr, const float *h0, void *h, int64_t h_ld, float *h_last);
+int recurrence_backward(const Ctx &c, int type, const void *gate, int64_t gate_ld, const void *x, int64_t x_ld, const void *h, int64_t h_ld,
+                        int T, int D, int n_seq, const int *seq_ptr, const float *h0, const void *dh, int64_t dh_ld, const float *dh_last,
+                        void *dgate, int64_t dgate_ld, void *dx, int64_t dx_ld, float *dh0);
+int orthogonalize(const Ctx &c, int type, const void *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
+                  float out_scale, void *out, int64_t ld_out, int64_t out_stride);
+
 // ---- kernels_opt.cu ----------------------------------------------------------------
 // ---- flat, sharded optimizer + requantiser (kernels_opt.cu) -------------------------
 // the part [a, b) (elements inside the matrix, multiples of 4) of one matrix that a rank owns

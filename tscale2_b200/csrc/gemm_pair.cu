@@ -17,6 +17,7 @@
 // Units (tile, K split) are assigned statically to clusters.  Every wait is bounded, as in gemm.cu; a CTA leaves only
 // after a cluster barrier, so no barrier or copy of its peer can still refer to it.
 #include "gemm_params.cuh"
+#include "pair_ptx.cuh"
 #include "row_math.cuh"
 
 namespace ts2 {
@@ -38,64 +39,6 @@ struct PairSmem {
     static constexpr int TOTAL = BAR_OFF + 1024 + 1024;
     static_assert(TOTAL <= 232448, "shared memory budget");
 };
-
-__device__ __forceinline__ uint32_t cluster_rank()
-{
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t map_to_leader(uint32_t addr)
-{
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
-{
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// a copy into this CTA's shared memory that completes on a barrier of either CTA of the pair
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1)
-{
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-                 "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
-                 : "memory");
-}
-template <int MMA>
-__device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
-{
-    if constexpr (MMA == 0)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-                     "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-                     : "memory");
-    else if constexpr (MMA == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-                     "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-                     : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-                     "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-                     : "memory");
-}
-// arrives at the barrier at this offset in both CTAs when the MMAs issued so far are complete
-__device__ __forceinline__ void commit_both(uint32_t bar)
-{
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                 "h"((uint16_t)3)
-                 : "memory");
-}
-__device__ __forceinline__ void commit_own(uint32_t bar)
-{
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
 
 struct PairUnit {
     int m0, n0, nt, kb0, kb1;

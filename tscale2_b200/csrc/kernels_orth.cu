@@ -9,7 +9,8 @@
 // 1.8e-4 with X in two halves; flat spectra 2.0e-3 and 1.3e-3).  All fp16 values are scaled by powers of two that keep them
 // below 65504 for every X the coefficients can reach (orth_check).
 #include "kernels.cuh"
-#include "gemm.cuh"
+#include "pair_ptx.cuh"
+#include <cuda.h>
 #include <algorithm>
 #include <cmath>
 
@@ -103,22 +104,367 @@ __global__ void __launch_bounds__(256) orth_store_kernel(const __half *__restric
     }
 }
 
-// B = b A + c A A
-__global__ void __launch_bounds__(256) orth_poly_kernel(const __half *__restrict__ a, const float *__restrict__ aa, size_t n, float b, float c,
-                                                        __half *out)
+// ---- the products ----------------------------------------------------------------------------------------------------
+// Pairs of CTAs on tiles of 256 x 256 (as in gemm_pair.cu), one launch for a product of every matrix of the batch.
+//   SQUARE  A = X X^T     POLY  B = b A + c A A     both operands K-contiguous; symmetric, so only tiles on and above the diagonal are
+//                         computed, and what is above it leaves a second time as its transpose
+//   UPDATE  X = a X + B X   B is K-contiguous (it is its own transpose), X is contiguous along N; writes the high halves to a second
+//                         array, since other tiles still read them, and the low halves in place
+//   PARTIAL a K range of SQUARE or POLY in fp32, for outputs of few tiles; orth_join_kernel adds the ranges
+// Residual inputs come in by TMA a block of 32 x 32 ahead, into the block that takes the result.
+enum Form { SQUARE, POLY, UPDATE, PARTIAL };
+constexpr int PT = 256, BK = 64, STAGES = 4, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
+constexpr int SLOT = 4096, STG_OFF = STAGES * STAGE, BAR_OFF = STG_OFF + 8 * 3 * SLOT, SMEM = BAR_OFF + 1024 + 1024;
+static_assert(SMEM <= 232448, "shared memory budget");
+
+struct ProductArgs {
+    int n, cols;         // rows and columns of the output (of every matrix)
+    int tiles, col_tiles; // a matrix's tiles; UPDATE: in col_tiles columns
+    int units, k_blocks, splits, kb_per_split;
+    float alpha, beta; // POLY: alpha acc + beta A; UPDATE: alpha acc + beta X; else alpha acc
+    float *part;       // PARTIAL: [matrix][tile][split][256][256]
+    int32_t *status;
+};
+struct Unit {
+    int matrix, row, col, kb0, kb1, index;
+};
+// the r-th tile on or above the diagonal of a square of tiles, column by column
+__device__ __forceinline__ void upper_tile(int r, int &row, int &col)
 {
-    grid_dep_wait();
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const float v = SB * (b / SA * __half2float(a[i]) + c / (SA * SA) * aa[i]);
-        out[i] = __low2half(sat_half2(v, v));
-    }
+    col = (int)((sqrtf(8.f * r + 1.f) - 1.f) * 0.5f);
+    while (col * (col + 1) / 2 > r)
+        --col;
+    while ((col + 1) * (col + 2) / 2 <= r)
+        ++col;
+    row = r - col * (col + 1) / 2;
 }
-// X = a X + B X
-__global__ void __launch_bounds__(256) orth_update_kernel(__half *hi, __half *lo, const float *__restrict__ bx, size_t n, float a)
+template <int FORM>
+__device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
+{
+    Unit t;
+    const int tile = u / p.splits, split = u - tile * p.splits;
+    t.index = u;
+    t.matrix = tile / p.tiles;
+    const int r = tile - t.matrix * p.tiles;
+    if (FORM == UPDATE)
+        t.row = r / p.col_tiles, t.col = r - t.row * p.col_tiles;
+    else
+        upper_tile(r, t.row, t.col);
+    t.row *= PT, t.col *= PT;
+    t.kb0 = split * p.kb_per_split;
+    t.kb1 = min(p.k_blocks, t.kb0 + p.kb_per_split);
+    return t;
+}
+
+// tmA, tmB: boxes of 128 rows x 64 (UPDATE: tmB 64 rows x 64); tmR, tmL: residual, tmC, tmD: outputs, boxes of 32 rows x 32, 64-byte swizzle
+template <int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
+    orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmR,
+                        const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
+                        const ProductArgs p)
+{
+    constexpr int RES = FORM == POLY ? 1 : FORM == UPDATE ? 2 : 0; // residual blocks of 2 KB
+    extern __shared__ uint8_t orth_smem[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)orth_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
+    uint64_t *bars = (uint64_t *)(smem + BAR_OFF);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), tfull0 = smem_u32(bars + 2 * STAGES),
+                   tempty0 = smem_u32(bars + 2 * STAGES + 2), drain = smem_u32(bars + 2 * STAGES + 4), res0 = smem_u32(bars + 2 * STAGES + 5);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 5 + 24);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull0 + 8 * a, 1);
+            mbar_init(tempty0 + 8 * a, 16); // the leader's counts the epilogue warps of both CTAs
+        }
+        for (int i = 0; i < 24; ++i)
+            mbar_init(res0 + 8 * i, 1);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmA);
+        prefetch_tmap(&tmB);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); // both CTAs' barriers exist
+    tc_fence_after();
+    grid_dep_wait();
+    const uint32_t tmem_base = *tmem_slot;
+    const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+
+    if (warp == 0) {
+        // TMA producer of the CTA's halves; all copies of a stage complete on the leader's barrier
+        if (lane == 0) {
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int u = first; u < p.units && ok; u += step) {
+                const Unit un = product_unit<FORM>(p, u);
+                const int am = un.row + (int)rank * 128, bn = un.col + (int)rank * 128;
+                for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = map_to_leader(full0 + 8 * stage);
+                    if (rank == 0)
+                        mbar_arrive_expect_tx(full0 + 8 * stage, 2 * STAGE);
+                    const uint32_t sa = smem_u32(smem + stage * STAGE), sb = sa + HALF;
+                    tma_load_3d_pair(sa, &tmA, fb, kb * BK, am, un.matrix);
+                    if constexpr (FORM == UPDATE) {
+                        tma_load_3d_pair(sb, &tmB, fb, bn, kb * BK, un.matrix);
+                        tma_load_3d_pair(sb + BK * 128, &tmB, fb, bn + 64, kb * BK, un.matrix);
+                    } else {
+                        tma_load_3d_pair(sb, &tmB, fb, kb * BK, bn, un.matrix);
+                    }
+                    ++issued;
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok && rank == 0) { // copies in flight land (a bounded wait) before the CTA may leave
+                int s = stage;
+                uint32_t ph = phase;
+                for (int i = 0; i < min(issued, STAGES); ++i) {
+                    if (--s < 0) {
+                        s = STAGES - 1;
+                        ph ^= 1;
+                    }
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(full0 + 8 * s, ph) && clock64() - t0 < 200000000ll) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // MMA issuer (leader)
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = (1u << 4) | ((FORM == UPDATE ? 1u : 0u) << 16) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int u = first; u < p.units && ok; u += step) {
+                const Unit un = product_unit<FORM>(p, u);
+                if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag))
+                    break;
+                tc_fence_after();
+                const uint32_t tmem_d = tmem_base + acc * PT;
+                for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                    if (!mbar_wait(full0 + 8 * stage, phase, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + stage * STAGE);
+                    const uint64_t adesc = umma_smem_desc(sa, 16, 1024);
+                    const uint64_t bdesc = umma_smem_desc(sa + HALF, FORM == UPDATE ? BK * 128 : 16, 1024);
+                    constexpr uint64_t a_step = 2, b_step = FORM == UPDATE ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_pair<1>(tmem_d, adesc + k * a_step, bdesc + k * b_step, idesc, (kb > un.kb0 || k > 0) ? 1u : 0u);
+                    commit_both(empty0 + 8 * stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (ok)
+                    commit_both(tfull0 + 8 * acc);
+                acc ^= 1;
+                if (acc == 0)
+                    acc_phase ^= 1;
+            }
+            commit_own(drain); // every MMA issued so far has completed once this arrives
+            const long long t0 = clock64();
+            while (!mbar_try_wait(drain, 0) && clock64() - t0 < 1500000000ll) {
+            }
+        }
+    } else {
+        // epilogue: a warp takes 32 rows x 128 columns in four blocks of 32 x 32, thread = row
+        const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
+        uint8_t *const slots = smem + STG_OFF + ew * 3 * SLOT; // of 4 KB: a block and the low halves or the transpose
+        const uint32_t res_bar = res0 + 8 * 3 * ew;
+        const int sw = (lane >> 1) & 3; // the 64-byte swizzle of the thread's row
+        auto row_of = [&](const Unit &un) { return un.row + (int)rank * 128 + quarter * 32; };
+        auto col_of = [&](const Unit &un, int c) { return un.col + half * 128 + c * 32; };
+        auto fetch = [&](const Unit &un, int c, int slot) { // lane 0
+            mbar_arrive_expect_tx(res_bar + 8 * slot, RES * 2048);
+            tma_load_3d(smem_u32(slots + slot * SLOT), &tmR, res_bar + 8 * slot, col_of(un, c), row_of(un), un.matrix);
+            if (RES == 2)
+                tma_load_3d(smem_u32(slots + slot * SLOT + 2048), &tmL, res_bar + 8 * slot, col_of(un, c), row_of(un), un.matrix);
+        };
+        int acc = 0, slot = 0;
+        uint32_t acc_phase = 0, slot_phase = 0;
+        bool ok = true;
+        if (RES && lane == 0 && first < p.units)
+            fetch(product_unit<FORM>(p, first), 0, 0);
+        for (int u = first; u < p.units && ok; u += step) {
+            const Unit un = product_unit<FORM>(p, u);
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PT + half * 128;
+            const int row0 = row_of(un);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                const int next = slot == 2 ? 0 : slot + 1;
+                if constexpr (RES > 0) {
+                    if (lane == 0) {
+                        bulk_wait_read<1>(); // the stores that last used the next slot have read it
+                        if (c < 3)
+                            fetch(un, c + 1, next);
+                        else if (u + step < p.units)
+                            fetch(product_unit<FORM>(p, u + step), 0, next);
+                    }
+                } else if constexpr (FORM == SQUARE) {
+                    if (lane == 0)
+                        bulk_wait_read<2>();
+                }
+                __syncwarp();
+                if (c == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag));
+                    if (!ok)
+                        break;
+                    tc_fence_after();
+                }
+                if constexpr (RES > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(res_bar + 8 * slot, slot_phase, abort_flag));
+                    if (!ok)
+                        break;
+                }
+                uint32_t r[32];
+                tmem_ld32(taddr + c * 32, r);
+                tmem_ld_wait();
+                if (c == 3) { // the accumulator is read: the next tile may have it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive_cluster(map_to_leader(tempty0 + 8 * acc));
+                }
+                const int col = col_of(un, c);
+                if constexpr (FORM == PARTIAL) {
+                    float4 *to = (float4 *)(p.part + ((size_t)un.index * PT + (row0 - un.row) + lane) * PT + (col - un.col));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        to[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
+                                            __uint_as_float(r[4 * i + 3]));
+                } else {
+                    uint8_t *const block = slots + slot * SLOT, *const second = block + 2048;
+                    const bool mirror = FORM != UPDATE && un.row != un.col;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { // 8 columns
+                        uint4 *const at = (uint4 *)(block + lane * 64 + ((i ^ sw) << 4)), *const at2 = (uint4 *)(second + lane * 64 + ((i ^ sw) << 4));
+                        uint32_t out[4], low[4];
+                        const uint4 x4 = RES > 0 ? *at : make_uint4(0, 0, 0, 0), l4 = RES == 2 ? *at2 : make_uint4(0, 0, 0, 0);
+                        const uint32_t xs[4] = {x4.x, x4.y, x4.z, x4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float v0 = p.alpha * __uint_as_float(r[8 * i + 2 * j]), v1 = p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]);
+                            if constexpr (RES > 0) {
+                                float2 x = __half22float2(*(const __half2 *)&xs[j]);
+                                if constexpr (RES == 2) {
+                                    const float2 l = __half22float2(*(const __half2 *)&ls[j]);
+                                    x.x = fmaf(l.x, 1.f / LO, x.x), x.y = fmaf(l.y, 1.f / LO, x.y);
+                                }
+                                v0 = fmaf(p.beta, x.x, v0), v1 = fmaf(p.beta, x.y, v1);
+                            }
+                            const __half2 h = sat_half2(v0, v1);
+                            out[j] = *(const uint32_t *)&h;
+                            if constexpr (FORM == UPDATE) {
+                                const float2 b = __half22float2(h);
+                                const __half2 l = sat_half2((v0 - b.x) * LO, (v1 - b.y) * LO);
+                                low[j] = *(const uint32_t *)&l;
+                            } else if (mirror) {
+                                // element (column, row) of the transpose: a column's 32 rows are the 64 bytes of one row there
+                                const int k = 8 * i + 2 * j;
+                                *(__half *)(second + k * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __low2half(h);
+                                *(__half *)(second + (k + 1) * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __high2half(h);
+                            }
+                        }
+                        *at = make_uint4(out[0], out[1], out[2], out[3]);
+                        if constexpr (FORM == UPDATE)
+                            *at2 = make_uint4(low[0], low[1], low[2], low[3]);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (row0 < p.n && col < p.cols) {
+                            tma_store_3d(&tmC, smem_u32(block), col, row0, un.matrix);
+                            if (FORM == UPDATE)
+                                tma_store_3d(&tmD, smem_u32(second), col, row0, un.matrix);
+                            else if (mirror)
+                                tma_store_3d(&tmC, smem_u32(second), row0, col, un.matrix);
+                        }
+                        bulk_commit();
+                    }
+                }
+                slot = next;
+                if (slot == 0)
+                    slot_phase ^= 1;
+            }
+            acc ^= 1;
+            if (acc == 0)
+                acc_phase ^= 1;
+        }
+        if (lane == 0) {
+            if (RES && !ok) { // residual blocks in flight land before the CTA may leave
+                const long long t0 = clock64();
+                const int next = slot == 2 ? 0 : slot + 1;
+                while (!(mbar_try_wait(res_bar + 8 * slot, slot_phase) && mbar_try_wait(res_bar + 8 * next, next == 0 ? slot_phase ^ 1 : slot_phase)) &&
+                       clock64() - t0 < 200000000ll) {
+                }
+            }
+            bulk_wait_read<0>(); // the blocks must outlive the stores that read them
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); // nothing of the peer refers to this CTA any more
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    if (threadIdx.x == 0 && *abort_flag)
+        atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);
+}
+
+// The K ranges of SQUARE or (with a) POLY added in their order; 32 x 32 of a tile per block
+__global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict__ part, const ProductArgs p, const __half *__restrict__ a, __half *out)
 {
     grid_dep_wait();
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256)
-        split(fmaf(a, joined(hi[i], lo[i]), bx[i] * (1.f / SB)), hi[i], lo[i]);
+    __shared__ float tile[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    int row, col;
+    upper_tile(blockIdx.y, row, col);
+    const bool mirror = row != col;
+    const int i0 = (blockIdx.x >> 3) * 32, j0 = (blockIdx.x & 7) * 32;
+    row = row * PT + i0, col = col * PT + j0;
+    if (row >= p.n || col >= p.n)
+        return;
+    part += ((size_t)blockIdx.z * p.tiles + blockIdx.y) * p.splits * PT * PT;
+    out += (size_t)blockIdx.z * p.n * p.n;
+    for (int k = ty; k < 32; k += 8) {
+        float sum = 0.f;
+        for (int s = 0; s < p.splits; ++s)
+            sum += part[((size_t)s * PT + i0 + k) * PT + j0 + tx];
+        sum *= p.alpha;
+        if (a)
+            sum = fmaf(p.beta, __half2float(a[((size_t)blockIdx.z * p.n + row + k) * p.n + col + tx]), sum);
+        tile[k][tx] = sum;
+        out[(size_t)(row + k) * p.n + col + tx] = __low2half(sat_half2(sum, sum));
+    }
+    if (!mirror)
+        return;
+    __syncthreads();
+    for (int k = ty; k < 32; k += 8)
+        out[(size_t)(col + k) * p.n + row + tx] = __low2half(sat_half2(tile[tx][k], tile[tx][k]));
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -153,6 +499,62 @@ static bool orth_check(const float coef[3], int steps)
     return x * 1.02 <= MAX_X;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// [batch][rows][cols] halves; box: `wide` elements (64: 128-byte swizzle, 32: 64-byte) x `high` rows
+static int half_map(CUtensorMap *tm, const void *base, int64_t cols, int64_t rows, int64_t batch, int wide, int high)
+{
+    static const EncodeTiledFn encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return (EncodeTiledFn)f;
+    }();
+    if (!encode)
+        return fail(TS2_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+    const cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)(cols * rows * 2)};
+    const cuuint32_t box[3] = {(cuuint32_t)wide, (cuuint32_t)high, 1}, estr[3] = {1, 1, 1};
+    const CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              wide == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? TS2_OK : fail(TS2_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+}
+
+template <int FORM>
+static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, const CUtensorMap &R, const CUtensorMap &L, const CUtensorMap &C,
+                   const CUtensorMap &D, const ProductArgs &p)
+{
+    static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
+    const unsigned bit = 1u << (c.device & 15);
+    if (!(ready.load() & bit)) {
+        TS2_CUDA(cudaFuncSetAttribute((const void *)orth_product_kernel<FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        ready.fetch_or(bit);
+    }
+    const int pairs = std::min(sm_count(c.device) / 2, p.units);
+    TS2_LAUNCH((orth_product_kernel<FORM>), 2 * pairs, 320, SMEM, c.stream, A, B, R, L, C, D, p);
+    return TS2_OK;
+}
+
+// K ranges of a symmetric product: the number with the least estimated time, in K blocks of a tile (0.27 us each).  A tile costs 4
+// more, joining the ranges a launch (10) and its bytes.
+static int choose_splits(int pairs, int64_t tiles, int k_blocks)
+{
+    double best = 1e30;
+    int splits = 1;
+    for (int s = 1; s <= 64 && s <= k_blocks; ++s) {
+        const int per = (int)ceil_div(k_blocks, s), used = (int)ceil_div(k_blocks, per);
+        if (used != s)
+            continue;
+        const double cost = (double)ceil_div(tiles * s, pairs) * (per + 4) + (s > 1 ? 10 + 0.3 * tiles * s : 0.);
+        if (cost < best)
+            best = cost, splits = s;
+    }
+    return splits;
+}
+
 struct Scratch {
     void *p = nullptr;
     cudaStream_t stream;
@@ -172,46 +574,67 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
                                float out_scale, __nv_bfloat16 *out, int64_t ld_out, int64_t out_stride)
 {
     const bool tall = rows > cols;
-    const int n = std::min(rows, cols), m = std::max(rows, cols), np = (int)ceil_div(n, 128) * 128, mp = (int)ceil_div(m, 128) * 128;
-    const int n_part = std::min(rows, 64);
-    const size_t x = (size_t)np * mp, a = (size_t)np * np;
-    size_t ws = gemm_workspace_bytes(c.device, KIND_F16, false, np, np, mp);
-    ws = std::max(ws, gemm_workspace_bytes(c.device, KIND_F16, false, np, np, np));
-    ws = (std::max(ws, gemm_workspace_bytes(c.device, KIND_F16, true, np, mp, np)) + 255) / 256 * 256;
-    Scratch s(c, ws + batch * x * 4 + a * 4 + x * 4 + (size_t)batch * n_part * 8);
+    const int n = std::min(rows, cols), m = std::max(rows, cols), np = (int)ceil_div(n, 64) * 64, mp = (int)ceil_div(m, 64) * 64;
+    const int n_part = std::min(rows, 64), pairs = sm_count(c.device) / 2;
+    const int nt = (int)ceil_div(np, PT), mt = (int)ceil_div(mp, PT), upper = nt * (nt + 1) / 2;
+    const size_t x = (size_t)batch * np * mp, a = (size_t)batch * np * np;
+    const int split1 = choose_splits(pairs, (int64_t)batch * upper, mp / BK), split2 = choose_splits(pairs, (int64_t)batch * upper, np / BK);
+    const int most = std::max(split1, split2);
+    const size_t part_bytes = most > 1 ? (size_t)batch * upper * most * PT * PT * 4 : 0;
+    Scratch s(c, part_bytes + x * 6 + a * 4 + (size_t)batch * n_part * 8);
     if (s.rc != TS2_OK)
         return s.rc;
-    __half *hi = (__half *)((uint8_t *)s.p + ws), *lo = hi + batch * x, *A = lo + batch * x, *B = A + a;
-    float *prod = (float *)(B + a);
-    double *part = (double *)(prod + x);
+    float *part = (float *)s.p;
+    __half *hi[2] = {(__half *)((uint8_t *)s.p + part_bytes), (__half *)((uint8_t *)s.p + part_bytes) + x}, *lo = hi[1] + x, *A = lo + x, *B = A + a;
+    double *sums = (double *)(B + a);
 
-    TS2_LAUNCH((orth_sum2_kernel<T>), dim3(n_part, batch), 256, 0, c.stream, g, ld, stride, rows, cols, part);
-    TS2_LAUNCH((orth_load_kernel<T>), dim3(mp / 32, np / 32, batch), 256, 0, c.stream, g, ld, stride, rows, cols, tall, part, n_part, np, mp, hi, lo);
-    GemmArgs p;
-    p.device = c.device, p.stream = c.stream, p.kind = KIND_F16, p.workspace = s.p, p.workspace_bytes = ws;
-    const int grid = sm_count(c.device) * 8;
-    for (int i = 0; i < batch; ++i) {
-        __half *xh = hi + i * x, *xl = lo + i * x;
-        for (int k = 0; k < steps; ++k) {
-            p.mn_major = false;
-            p.M = p.N = np, p.K = mp, p.A = p.B = xh, p.lda = p.ldb = mp, p.C = A, p.ldc = np;
-            p.epi.out_kind = TS2_OUT_F16, p.epi.alpha = SA / (SX * SX);
-            if (int rc = gemm(p))
-                return rc;
-            p.K = np, p.A = p.B = A, p.lda = p.ldb = np, p.C = prod;
-            p.epi.out_kind = TS2_OUT_F32, p.epi.alpha = 1.f;
-            if (int rc = gemm(p))
-                return rc;
-            TS2_LAUNCH(orth_poly_kernel, (unsigned)std::min<size_t>(grid, a / 256), 256, 0, c.stream, A, prod, a, coef[1], coef[2], B);
-            p.mn_major = true; // B is its own transpose
-            p.N = mp, p.A = B, p.B = xh, p.ldb = p.ldc = mp;
-            if (int rc = gemm(p))
-                return rc;
-            TS2_LAUNCH(orth_update_kernel, (unsigned)std::min<size_t>(grid, x / 256), 256, 0, c.stream, xh, xl, prod, x, coef[0]);
-        }
+    TS2_LAUNCH((orth_sum2_kernel<T>), dim3(n_part, batch), 256, 0, c.stream, g, ld, stride, rows, cols, sums);
+    TS2_LAUNCH((orth_load_kernel<T>), dim3(mp / 32, np / 32, batch), 256, 0, c.stream, g, ld, stride, rows, cols, tall, sums, n_part, np, mp, hi[0],
+               lo);
+    CUtensorMap x_rows[2], x_cols[2], x_block[2], lo_block, a_rows, a_block, b_rows, b_block;
+    int rc = TS2_OK;
+    for (int i = 0; i < 2 && rc == TS2_OK; ++i) {
+        rc = half_map(&x_rows[i], hi[i], mp, np, batch, 64, 128);
+        if (rc == TS2_OK)
+            rc = half_map(&x_cols[i], hi[i], mp, np, batch, 64, 64);
+        if (rc == TS2_OK)
+            rc = half_map(&x_block[i], hi[i], mp, np, batch, 32, 32);
     }
-    TS2_LAUNCH(orth_store_kernel, dim3(mp / 32, np / 32, batch), 256, 0, c.stream, hi, lo, np, mp, tall, out_scale / SX, out, ld_out, out_stride, rows,
-               cols);
+    if (rc != TS2_OK || (rc = half_map(&lo_block, lo, mp, np, batch, 32, 32)) || (rc = half_map(&a_rows, A, np, np, batch, 64, 128)) ||
+        (rc = half_map(&a_block, A, np, np, batch, 32, 32)) || (rc = half_map(&b_rows, B, np, np, batch, 64, 128)) ||
+        (rc = half_map(&b_block, B, np, np, batch, 32, 32)))
+        return rc;
+    ProductArgs p = {};
+    p.status = device_status_word(c.device);
+    if (!p.status)
+        return fail(TS2_ERR_CUDA, "no device status word");
+    p.n = np;
+    p.part = part;
+    const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &res, const CUtensorMap &to, __half *dst) {
+        p.cols = np, p.tiles = upper, p.col_tiles = 0;
+        p.k_blocks = k / BK, p.splits = splits, p.kb_per_split = (int)ceil_div(p.k_blocks, splits), p.units = batch * upper * splits;
+        if (splits == 1)
+            return poly ? product<POLY>(c, in, in, res, res, to, to, p) : product<SQUARE>(c, in, in, res, res, to, to, p);
+        if (int e = product<PARTIAL>(c, in, in, res, res, to, to, p))
+            return e;
+        TS2_LAUNCH(orth_join_kernel, dim3(64, upper, batch), 256, 0, c.stream, part, p, poly ? A : (const __half *)nullptr, dst);
+        return TS2_OK;
+    };
+    for (int k = 0; k < steps; ++k) {
+        const int now = k & 1;
+        p.alpha = SA / (SX * SX), p.beta = 0.f;
+        if ((rc = symmetric(false, mp, split1, x_rows[now], a_block, a_block, A)))
+            return rc;
+        p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA;
+        if ((rc = symmetric(true, np, split2, a_rows, a_block, b_block, B)))
+            return rc;
+        p.alpha = 1.f / SB, p.beta = coef[0];
+        p.cols = mp, p.tiles = nt * mt, p.col_tiles = mt, p.k_blocks = np / BK, p.splits = 1, p.kb_per_split = p.k_blocks, p.units = batch * nt * mt;
+        if ((rc = product<UPDATE>(c, b_rows, x_cols[now], x_block[now], lo_block, x_block[now ^ 1], lo_block, p)))
+            return rc;
+    }
+    TS2_LAUNCH(orth_store_kernel, dim3(mp / 32, np / 32, batch), 256, 0, c.stream, hi[steps & 1], lo, np, mp, tall, out_scale / SX, out, ld_out,
+               out_stride, rows, cols);
     return TS2_OK;
 }
 

@@ -4,17 +4,20 @@
 //     d loss / d logits[t][e] = E / (k N^2) p[t][e] (C[e] - sum_j C[j] p[t][j])
 // The counts have no gradient.  The routing weights are exp((l - lmax) / 2), so p is their square, normalised.
 //
-// G lanes share a row, each with its 16-byte pieces of it, so a warp reads 32 / G rows at a time; the softmax is a maximum and a
-// sum over G lanes.  Logits are read once forward, and read once and written once backward: memory bandwidth bounds large calls,
-// the latency of a launch small ones.  The column sums stay in registers until a block's rows are done and are joined in a fixed
-// order; counts are integers, so that the order of their atomics does not matter.
+// G lanes share a row, each with its 16-byte pieces of it, so a warp reads 32 / G rows at a time, the next ones while it works on
+// these; the softmax is a maximum and a sum over G lanes.  Logits are read once forward, and read once and written once
+// backward: memory bandwidth bounds large calls, the latency of a launch small ones.  The column sums stay in registers until a
+// block's rows are done; the blocks of a cluster join theirs through distributed shared memory, so that a small call is one
+// launch and a large one leaves a partial result per cluster to a second.  All sums have a fixed order; counts are integers, so
+// that the order of their atomics does not matter.
 #include "kernels.cuh"
 #include <algorithm>
 
 namespace ts2 {
 
-static constexpr int THREADS = 256, WARPS = THREADS / 32;
-static constexpr int MAX_EXPERTS = 1024;
+static constexpr int THREADS = 256, WARPS = THREADS / 32;                // backward
+static constexpr int SUM_THREADS = 512, SUM_WARPS = SUM_THREADS / 32;    // forward
+static constexpr int MAX_EXPERTS = 1024, CLUSTER = 8, MAX_CLUSTERS = 32;
 
 template <class T>
 __device__ __forceinline__ float widen(T v) { return (float)v; }
@@ -39,22 +42,24 @@ struct Row {
     float v[VALUES];
 
     static __device__ __forceinline__ int column(int i) { return ((i / VEC) * G + (int)(threadIdx.x & (G - 1))) * VEC + i % VEC; }
-    __device__ __forceinline__ void load(const T *row, int E)
+    // the lane's pieces of the row as they lie in memory; E = 0: nothing is read.  VEC > 1: E is a multiple of it
+    struct Raw {
+        Piece<T, VEC> p[N];
+        __device__ __forceinline__ void load(const T *row, int E)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (column(i * VEC) < E)
+                    p[i] = *(const Piece<T, VEC> *)(row + column(i * VEC));
+        }
+    };
+    __device__ __forceinline__ void widen_from(const Raw &raw, int E)
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = column(i * VEC);
-            if (c < E) { // VEC > 1: E is a multiple of it
-                const Piece<T, VEC> p = *(const Piece<T, VEC> *)(row + c);
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    v[i * VEC + j] = widen(p.v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    v[i * VEC + j] = -INFINITY;
-            }
-        }
+            for (int j = 0; j < VEC; ++j)
+                v[i * VEC + j] = column(i * VEC) < E ? widen(raw.p[i].v[j]) : -INFINITY;
     }
     __device__ __forceinline__ void store(T *row, int E, bool add) const
     {
@@ -104,8 +109,8 @@ struct BalanceArgs {
     const uint8_t *mask;
     long long rows_per_block;
     // forward
-    float *part_prob; // [blocks][E]
-    int *part_count;  // [blocks][E + 1], the last one: rows that count
+    float *part_prob; // [clusters][E]
+    int *part_count;  // [clusters][E + 1], the last one: rows that count
     int *counts;
     float *prob, *loss;
     // backward
@@ -116,105 +121,232 @@ struct BalanceArgs {
     int add;
 };
 
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// this CTA's shared-memory address `p`, in CTA `rank` of the cluster
+template <class V>
+__device__ __forceinline__ uint32_t in_rank(const V *p, unsigned rank)
+{
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float ld_float(uint32_t a)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_int(uint32_t a)
+{
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// an expert's part of the loss
+__device__ __forceinline__ double loss_term(double mean, int count, int tokens, int E, int selected)
+{
+    return tokens ? mean * count * E / ((double)tokens * selected) : 0.;
+}
+__device__ __forceinline__ double warp_sum(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 template <class T, int VEC, int G, int N>
-__global__ void __launch_bounds__(THREADS) balance_sums_kernel(const BalanceArgs p)
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS) balance_sums_kernel(const BalanceArgs p)
 {
     grid_dep_wait();
     using R = Row<T, VEC, G, N>;
-    constexpr int ROWS = 32 / G;
-    __shared__ float sums[MAX_EXPERTS];
+    constexpr int ROWS = 32 / G, WIDTH = VEC * G * N < MAX_EXPERTS ? VEC * G * N : MAX_EXPERTS; // columns there is room for
+    constexpr int PARTS = WIDTH <= 256 ? SUM_WARPS : 1; // warps that leave their sums side by side
+    __shared__ float sums[PARTS][WIDTH];
     __shared__ int count[MAX_EXPERTS + 1];
+    __shared__ double terms[CLUSTER], warp_terms[SUM_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.E;
-    for (int e = threadIdx.x; e <= E; e += THREADS)
+    for (int e = threadIdx.x; e <= E; e += SUM_THREADS)
         count[e] = 0;
     __syncthreads();
-    const long long t_begin = blockIdx.x * p.rows_per_block, t_end = min(p.T, t_begin + p.rows_per_block);
+    // the block's rows, counted from 0; what is read ahead of them: logits (of rows that do not count, too: waiting for the mask
+    // would cost more), mask and each lane's first choice
+    constexpr int STEP = SUM_WARPS * ROWS;
+    const long long t_begin = blockIdx.x * p.rows_per_block;
+    const int rows = (int)max(0ll, min(p.rows_per_block, p.T - t_begin)), own = warp * ROWS + lane / G, choice_row = lane / p.selected;
+    const T *from = (const T *)p.logits + (t_begin + own) * p.ld;
+    const uint8_t *mask = p.mask ? p.mask + t_begin + own : nullptr;
+    const int *ids = p.ids + (t_begin + warp * ROWS) * p.selected + lane;
+    const long long step_from = STEP * p.ld;
     float acc[R::VALUES];
 #pragma unroll
     for (int i = 0; i < R::VALUES; ++i)
         acc[i] = 0.f;
-    for (long long base = t_begin + warp * ROWS; base < t_end; base += WARPS * ROWS) {
-        const long long t = base + lane / G;
+    typename R::Raw raw;
+    bool on;
+    int id = -1;
+    const auto fetch = [&](int r) { // r: the warp's first row
+        const bool there = r + lane / G < rows;
+        raw.load(from, there ? E : 0);
+        on = there && (!mask || *mask);
+        id = choice_row < ROWS && r + choice_row < rows ? *ids : -1;
+        from += step_from, ids += STEP * p.selected;
+        if (mask)
+            mask += STEP;
+    };
+    fetch(warp * ROWS);
+    for (int r = warp * ROWS; r < rows; r += STEP) {
         R row;
-        const bool on = t < t_end && (!p.mask || p.mask[t]);
-        row.load((const T *)p.logits + t * p.ld, on ? E : 0);
+        const bool now = on;
+        row.widen_from(raw, now ? E : 0);
+        const unsigned m = __ballot_sync(0xffffffffu, now && (lane & (G - 1)) == 0);
+        const int e = id;
+        const int *more = ids - STEP * p.selected; // of these rows
+        fetch(r + STEP);
+        if (lane == 0 && m)
+            atomicAdd(&count[E], __popc(m));
+        if ((m >> ((choice_row * G) & 31) & 1) && e >= 0 && e < E)
+            atomicAdd(&count[e], 1);
+        for (int i = lane + 32; i < ROWS * p.selected; i += 32) { // what 32 lanes do not hold
+            more += 32;
+            const int at = i / p.selected;
+            if (m >> at * G & 1) {
+                const int f = *more;
+                if (f >= 0 && f < E)
+                    atomicAdd(&count[f], 1);
+            }
+        }
         row.softmax();
-        if (on) {
+        if (now) {
 #pragma unroll
             for (int i = 0; i < R::VALUES; ++i)
                 acc[i] += row.v[i];
         }
-        const unsigned m = __ballot_sync(0xffffffffu, on && (lane & (G - 1)) == 0);
-        if (lane == 0 && m)
-            atomicAdd(&count[E], __popc(m));
-    }
-    for (long long i = t_begin * p.selected + threadIdx.x; i < t_end * p.selected; i += THREADS) {
-        const int e = p.ids[i];
-        if (e >= 0 && e < E && (!p.mask || p.mask[i / p.selected]))
-            atomicAdd(&count[e], 1);
     }
 #pragma unroll
     for (int i = 0; i < R::VALUES; ++i)
 #pragma unroll
         for (int o = G; o < 32; o <<= 1)
             acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    for (int w = 0; w < WARPS; ++w) { // warp by warp: a fixed order
-        if (warp == w && lane < G) {
+    if (PARTS > 1) {
+        if (lane < G)
 #pragma unroll
-            for (int i = 0; i < R::VALUES; ++i) {
-                const int c = R::column(i);
-                if (c < E)
-                    sums[c] = w ? sums[c] + acc[i] : acc[i];
-            }
-        }
+            for (int i = 0; i < R::VALUES; ++i)
+                sums[warp % PARTS][R::column(i)] = acc[i];
         __syncthreads();
+        for (int e = threadIdx.x; e < E; e += SUM_THREADS) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < PARTS; ++w)
+                sum += sums[w][e];
+            sums[0][e] = sum;
+        }
+    } else {
+        for (int w = 0; w < SUM_WARPS; ++w) { // warp by warp
+            if (warp == w && lane < G)
+#pragma unroll
+                for (int i = 0; i < R::VALUES; ++i)
+                    sums[0][R::column(i)] = w ? sums[0][R::column(i)] + acc[i] : acc[i];
+            __syncthreads();
+        }
     }
-    for (int e = threadIdx.x; e < E; e += THREADS)
-        p.part_prob[(size_t)blockIdx.x * E + e] = sums[e];
-    for (int e = threadIdx.x; e <= E; e += THREADS)
-        p.part_count[(size_t)blockIdx.x * (E + 1) + e] = count[e];
+    // every CTA joins the columns rank, rank + 8, .. of the cluster
+    cluster_sync();
+    const unsigned rank = cluster_rank();
+    const bool alone = gridDim.x == CLUSTER;
+    int tokens = 0;
+#pragma unroll
+    for (int r = 0; r < CLUSTER; ++r)
+        tokens += ld_int(in_rank(&count[E], r));
+    double loss = 0.;
+    const size_t cluster = blockIdx.x / CLUSTER;
+    for (int e = (int)rank + CLUSTER * threadIdx.x; e < E; e += CLUSTER * SUM_THREADS) {
+        double sum = 0.;
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) {
+            sum += ld_float(in_rank(&sums[0][e], r));
+            n += ld_int(in_rank(&count[e], r));
+        }
+        if (alone) {
+            const double mean = tokens ? sum / tokens : 0.;
+            p.prob[e] = (float)mean;
+            p.counts[e] = n;
+            loss += loss_term(mean, n, tokens, E, p.selected);
+        } else {
+            p.part_prob[cluster * E + e] = (float)sum;
+            p.part_count[cluster * (E + 1) + e] = n;
+        }
+    }
+    if (rank == 0 && threadIdx.x == 0)
+        *(alone ? &p.counts[E] : &p.part_count[cluster * (E + 1) + E]) = tokens;
+    if (alone) {
+        loss = warp_sum(loss);
+        if (lane == 0)
+            warp_terms[warp] = loss;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < SUM_WARPS; ++w)
+                loss += warp_terms[w];
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_rank(&terms[rank], 0)), "d"(loss) : "memory");
+        }
+    }
+    cluster_sync(); // nobody reads a CTA's shared memory any more; the terms of the loss are there
+    if (alone && rank == 0 && threadIdx.x == 0) {
+        for (int r = 1; r < CLUSTER; ++r)
+            loss += terms[r];
+        *p.loss = (float)loss;
+    }
 }
 
-// one block: the blocks' sums, in their order
-__global__ void __launch_bounds__(MAX_EXPERTS) balance_finish_kernel(const BalanceArgs p, int blocks)
+// one block: the clusters' sums, in their order; a warp a column, a lane a cluster
+__global__ void __launch_bounds__(1024) balance_finish_kernel(const BalanceArgs p, int clusters)
 {
     grid_dep_wait();
-    __shared__ int total;
     __shared__ double terms[32];
-    const int E = p.E, e = threadIdx.x, lane = e & 31, warp = e >> 5;
-    if (warp == 0) {
-        int n = 0;
-        for (int b = lane; b < blocks; b += 32)
-            n += p.part_count[(size_t)b * (E + 1) + E];
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0)
-            total = n, p.counts[E] = n;
-    }
-    double sum = 0.;
-    int n = 0;
-    if (e < E) {
-        for (int b = 0; b < blocks; ++b) {
-            sum += p.part_prob[(size_t)b * E + e];
-            n += p.part_count[(size_t)b * (E + 1) + e];
-        }
-        p.counts[e] = n;
-    }
-    __syncthreads();
-    const double tokens = total;
-    const double mean = total ? sum / tokens : 0.;
-    if (e < E)
-        p.prob[e] = (float)mean;
-    double term = total ? mean * n * E / (tokens * p.selected) : 0.;
+    const int E = p.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tokens = __reduce_add_sync(0xffffffffu, lane < clusters ? p.part_count[(size_t)lane * (E + 1) + E] : 0);
+    double loss = 0.;
+    for (int e0 = warp; e0 < E; e0 += 128) { // four columns' loads at a time
+        float part[4];
+        int count[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        term += __shfl_xor_sync(0xffffffffu, term, o);
+        for (int i = 0; i < 4; ++i) {
+            const int e = e0 + 32 * i;
+            const bool in = lane < clusters && e < E;
+            part[i] = in ? p.part_prob[(size_t)lane * E + e] : 0.f;
+            count[i] = in ? p.part_count[(size_t)lane * (E + 1) + e] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = e0 + 32 * i;
+            const double sum = warp_sum((double)part[i]), mean = tokens ? sum / tokens : 0.;
+            const int n = __reduce_add_sync(0xffffffffu, count[i]);
+            if (e >= E)
+                continue;
+            if (lane == 0)
+                p.prob[e] = (float)mean, p.counts[e] = n;
+            loss += loss_term(mean, n, tokens, E, p.selected);
+        }
+    }
     if (lane == 0)
-        terms[warp] = term;
+        terms[warp] = loss;
     __syncthreads();
-    if (e == 0) {
-        for (int w = 1; w < (int)blockDim.x / 32; ++w)
-            term += terms[w];
-        *p.loss = (float)term;
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 32; ++w)
+            loss += terms[w];
+        *p.loss = (float)loss;
+        p.counts[E] = tokens;
     }
 }
 
@@ -227,6 +359,18 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance
     using R = Row<T, VEC, G, N>;
     constexpr int ROWS = 32 / G;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.E;
+    long long t = ((long long)blockIdx.x * WARPS + warp) * ROWS + lane / G;
+    const long long step = (long long)gridDim.x * WARPS * ROWS, step_from = step * p.ld, step_to = step * p.ld_d;
+    const T *from = (const T *)p.logits + t * p.ld;
+    T *to = (T *)p.dlogits + t * p.ld_d;
+    typename R::Raw raw;
+    bool on_next;
+    const auto fetch = [&](long long t) {
+        raw.load(from, t < p.T ? E : 0);
+        on_next = t < p.T && (!p.mask || p.mask[t]);
+        from += step_from;
+    };
+    fetch(t);
     const double tokens = p.counts[E];
     const double even = tokens * p.selected / E;
     const double unit = tokens > 0 ? (p.dloss ? (double)*p.dloss : 1.) * p.scale * E / (p.selected * tokens * tokens) : 0.;
@@ -234,11 +378,11 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance
 #pragma unroll
     for (int i = 0; i < R::VALUES; ++i)
         f[i] = R::column(i) < E ? (float)((p.counts[R::column(i)] - even) * unit) : 0.f;
-    for (long long base = ((long long)blockIdx.x * WARPS + warp) * ROWS; base < p.T; base += (long long)gridDim.x * WARPS * ROWS) {
-        const long long t = base + lane / G;
-        const bool on = t < p.T && (!p.mask || p.mask[t]);
+    for (; t - lane / G < p.T; t += step, to += step_to) { // a warp together
+        const bool on = on_next;
         R row;
-        row.load((const T *)p.logits + t * p.ld, on ? E : 0);
+        row.widen_from(raw, on ? E : 0);
+        fetch(t + step);
         row.softmax();
         float dot = 0.f;
 #pragma unroll
@@ -251,7 +395,7 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance
         for (int i = 0; i < R::VALUES; ++i)
             row.v[i] = on ? row.v[i] * (f[i] - dot) : 0.f;
         if (t < p.T && (on || !p.add)) // a row that does not count has no gradient: zeros, or nothing added
-            row.store((T *)p.dlogits + t * p.ld_d, E, p.add && on);
+            row.store(to, E, p.add && on);
     }
 }
 
@@ -259,22 +403,28 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance
 template <class T, int VEC, int G, int N>
 static int launch(const Ctx &c, BalanceArgs &p, bool backward)
 {
-    const int rows = 32 / G * WARPS, cap = sm_count(c.device) * 4;
     if (backward) {
+        const int rows = 32 / G * WARPS, cap = sm_count(c.device) * 4;
         TS2_LAUNCH((balance_backward_kernel<T, VEC, G, N>), (unsigned)std::max<int64_t>(1, std::min<int64_t>(cap, ceil_div(p.T, rows))), THREADS, 0,
                    c.stream, p);
         return TS2_OK;
     }
-    p.rows_per_block = std::max<int64_t>(rows, ceil_div(ceil_div(p.T, cap), rows) * rows);
-    const int blocks = (int)std::max<int64_t>(1, ceil_div(p.T, p.rows_per_block));
+    // one cluster for up to four rounds of its warps, and then as many as the device holds at once
+    const int64_t round = (int64_t)32 / G * SUM_WARPS, clusters_wanted = ceil_div(p.T, round * CLUSTER);
+    const int clusters = clusters_wanted <= 4 ? 1 : (int)std::min<int64_t>(clusters_wanted, MAX_CLUSTERS);
+    p.rows_per_block = ceil_div(ceil_div(p.T, (int64_t)clusters * CLUSTER), 32 / G) * (32 / G);
+    if (clusters == 1) {
+        TS2_LAUNCH((balance_sums_kernel<T, VEC, G, N>), CLUSTER, SUM_THREADS, 0, c.stream, p);
+        return TS2_OK;
+    }
     void *scratch;
-    if (int rc = scratch_alloc(c.device, (size_t)blocks * (2 * p.E + 1) * 4, c.stream, &scratch))
+    if (int rc = scratch_alloc(c.device, (size_t)clusters * (2 * p.E + 1) * 4, c.stream, &scratch))
         return rc;
     p.part_prob = (float *)scratch;
-    p.part_count = (int *)scratch + (size_t)blocks * p.E;
+    p.part_count = (int *)scratch + (size_t)clusters * p.E;
     const auto work = [&] {
-        TS2_LAUNCH((balance_sums_kernel<T, VEC, G, N>), blocks, THREADS, 0, c.stream, p);
-        TS2_LAUNCH(balance_finish_kernel, 1, (p.E + 31) / 32 * 32, 0, c.stream, p, blocks);
+        TS2_LAUNCH((balance_sums_kernel<T, VEC, G, N>), clusters * CLUSTER, SUM_THREADS, 0, c.stream, p);
+        TS2_LAUNCH(balance_finish_kernel, 1, 1024, 0, c.stream, p, clusters);
         return TS2_OK;
     };
     const int rc = work();

@@ -32,23 +32,55 @@ __device__ __forceinline__ void split(float x, __half &hi, __half &lo)
 }
 __device__ __forceinline__ float joined(__half hi, __half lo) { return fmaf(__half2float(lo), 1.f / LO, __half2float(hi)); }
 
-// ---- G -> X ----------------------------------------------------------------------------------------------------------
-// partial sums of squares in fp64: no input over- or underflows, and nothing is lost over 2^32 terms
+// ---- G -> X and X -> out ---------------------------------------------------------------------------------------------
+// 8 elements of a row from column c on as floats, zeros from column `cols` on; vec: 16-byte accesses are aligned
 template <class T>
-__global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, double *part)
+__device__ __forceinline__ void load8(const T *row, int c, int cols, bool vec, float (&v)[8])
+{
+    if (vec && c + 8 <= cols) {
+        constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8 / PER; ++i) {
+            const uint4 raw = *(const uint4 *)(row + c + i * PER);
+            const T *e = (const T *)&raw;
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                v[i * PER + j] = widen(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = c + i < cols ? widen(row[c + i]) : 0.f;
+    }
+}
+__device__ __forceinline__ double warp_sum(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// partial sums of squares in fp64: no input over- or underflows, and nothing is lost over 2^40 terms
+template <class T>
+__global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, bool vec,
+                                                        double *part)
 {
     grid_dep_wait();
     __shared__ double warps[8];
     g += blockIdx.y * stride;
+    const int pieces = (cols + 7) / 8;
+    const long long total = (long long)rows * pieces;
     double sum = 0.;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < cols; c += 256) {
-            const double v = widen(g[r * ld + c]);
-            sum += v * v;
-        }
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int r = (int)(i / pieces), c = (int)(i - (long long)r * pieces) * 8;
+        float v[8];
+        load8(g + r * ld, c, cols, vec, v);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int j = 0; j < 8; ++j)
+            sum = fma((double)v[j], (double)v[j], sum);
+    }
+    sum = warp_sum(sum);
     if ((threadIdx.x & 31) == 0)
         warps[threadIdx.x >> 5] = sum;
     __syncthreads();
@@ -59,48 +91,109 @@ __global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g,
     }
 }
 
-// 32 x 32 blocks of X [n][m] (padded to np x mp with zeros) from G, transposed where G has more rows than columns
-template <class T>
-__global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, bool tall,
+// 64 x 64 of X [n][m] (padded to np x mp with zeros) from G, transposed where G has more rows than columns
+template <class T, bool TALL>
+__global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, bool vec,
                                                         const double *part, int n_part, int np, int mp, __half *hi, __half *lo)
 {
     grid_dep_wait();
-    __shared__ float tile[32][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, b = blockIdx.z;
-    double sum = 0.;
-    for (int i = 0; i < n_part; ++i)
-        sum += part[b * n_part + i];
-    const double scale = sum == 0. ? 0. : SX / sqrt(sum);
-    const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32; // rows and columns of X
+    __shared__ double norm;
+    __shared__ float tile[TALL ? 64 : 1][65];
+    const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, q = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8;
     g += b * stride;
-    for (int k = ty; k < 32; k += 8) {
-        const int r = (tall ? j0 : i0) + k, c = (tall ? i0 : j0) + tx;
-        tile[k][tx] = r < rows && c < cols ? (float)(widen(g[r * ld + c]) * scale) : 0.f;
+    float v[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) { // 32 rows of G at a time
+        const int r = (TALL ? j0 : i0) + q + 32 * h;
+        if (r < rows)
+            load8(g + r * ld, (TALL ? i0 : j0) + c8, cols, vec, v[h]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[h][j] = 0.f;
+    }
+    if (threadIdx.x < 32) {
+        double sum = 0.;
+        for (int i = threadIdx.x; i < n_part; i += 32)
+            sum += part[b * n_part + i];
+        sum = warp_sum(sum);
+        if (threadIdx.x == 0)
+            norm = sum == 0. ? 0. : SX / sqrt(sum);
+    }
+    if (TALL) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                tile[q + 32 * h][c8 + j] = v[h][j];
     }
     __syncthreads();
-    for (int k = ty; k < 32; k += 8) {
-        const size_t at = ((size_t)b * np + i0 + k) * mp + j0 + tx;
-        split(tall ? tile[tx][k] : tile[k][tx], hi[at], lo[at]);
+    // fp32 holds the scale unless G is all but denormal; then the product is made in fp64
+    const double scale = norm;
+    const bool small = !(scale < 1e30);
+    const float scale32 = (float)scale;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = q + 32 * h;
+        alignas(16) __half hs[8], ls[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = TALL ? tile[c8 + j][i] : v[h][j];
+            split(small ? (float)(x * scale) : x * scale32, hs[j], ls[j]);
+        }
+        const size_t at = ((size_t)b * np + i0 + i) * mp + j0 + c8;
+        *(uint4 *)(hi + at) = *(uint4 *)hs;
+        *(uint4 *)(lo + at) = *(uint4 *)ls;
     }
 }
 
-__global__ void __launch_bounds__(256) orth_store_kernel(const __half *__restrict__ hi, const __half *__restrict__ lo, int np, int mp, bool tall,
-                                                         float scale, __nv_bfloat16 *out, long long ld, long long stride, int rows, int cols)
+template <bool TALL>
+__global__ void __launch_bounds__(256) orth_store_kernel(const __half *__restrict__ hi, const __half *__restrict__ lo, int np, int mp, float scale,
+                                                         __nv_bfloat16 *out, long long ld, long long stride, int rows, int cols, bool vec)
 {
     grid_dep_wait();
-    __shared__ float tile[32][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, b = blockIdx.z;
-    const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
-    for (int k = ty; k < 32; k += 8) {
-        const size_t at = ((size_t)b * np + i0 + k) * mp + j0 + tx;
-        tile[k][tx] = joined(hi[at], lo[at]) * scale;
-    }
-    __syncthreads();
+    __shared__ float tile[TALL ? 64 : 1][65];
+    const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, q = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8;
     out += b * stride;
-    for (int k = ty; k < 32; k += 8) {
-        const int r = (tall ? j0 : i0) + k, c = (tall ? i0 : j0) + tx;
-        if (r < rows && c < cols)
-            out[r * ld + c] = __float2bfloat16_rn(tall ? tile[tx][k] : tile[k][tx]);
+    float v[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const size_t at = ((size_t)b * np + i0 + q + 32 * h) * mp + j0 + c8;
+        const uint4 rh = *(const uint4 *)(hi + at), rl = *(const uint4 *)(lo + at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[h][j] = joined(((const __half *)&rh)[j], ((const __half *)&rl)[j]) * scale;
+    }
+    if (TALL) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                tile[q + 32 * h][c8 + j] = v[h][j];
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[h][j] = tile[c8 + j][q + 32 * h];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = (TALL ? j0 : i0) + q + 32 * h, c = (TALL ? i0 : j0) + c8;
+        if (r >= rows || c >= cols)
+            continue;
+        alignas(16) __nv_bfloat16 o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            o[j] = __float2bfloat16_rn(v[h][j]);
+        if (vec && c + 8 <= cols) {
+            *(uint4 *)(out + r * ld + c) = *(uint4 *)o;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < cols)
+                    out[r * ld + c + j] = o[j];
+        }
     }
 }
 
@@ -111,10 +204,14 @@ __global__ void __launch_bounds__(256) orth_store_kernel(const __half *__restric
 //   UPDATE  X = a X + B X   B is K-contiguous (it is its own transpose), X is contiguous along N; writes the high halves to a second
 //                         array, since other tiles still read them, and the low halves in place
 //   PARTIAL a K range of SQUARE or POLY in fp32, for outputs of few tiles; orth_join_kernel adds the ranges
-// Residual inputs come in by TMA a block of 32 x 32 ahead, into the block that takes the result.
+// Residual inputs are read by the epilogue's threads, a row of 32 each; results leave as blocks of 32 x 32 by TMA.
 enum Form { SQUARE, POLY, UPDATE, PARTIAL };
-constexpr int PT = 256, BK = 64, STAGES = 4, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
-constexpr int SLOT = 4096, STG_OFF = STAGES * STAGE, BAR_OFF = STG_OFF + 8 * 3 * SLOT, SMEM = BAR_OFF + 1024 + 1024;
+constexpr int PT = 256, BK = 64, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
+// Six stages and eight epilogue warps with two blocks each against four, sixteen and three: 32 x 1024 x 1024 1042 -> 1019 us, 8192 x
+// 2048 775 -> 732
+constexpr int STAGES = 6, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS, BLOCKS = 2;
+constexpr int PART = PT / (EPI_WARPS / 4); // columns of an epilogue warp
+constexpr int BLOCK = 2048, STG_OFF = STAGES * STAGE, BAR_OFF = STG_OFF + EPI_WARPS * BLOCKS * BLOCK, SMEM = BAR_OFF + 1024 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 
 struct ProductArgs {
@@ -123,6 +220,7 @@ struct ProductArgs {
     int units, k_blocks, splits, kb_per_split;
     float alpha, beta; // POLY: alpha acc + beta A; UPDATE: alpha acc + beta X; else alpha acc
     float *part;       // PARTIAL: [matrix][tile][split][256][256]
+    const __half *res, *res_lo; // A, or the halves of X
     int32_t *status;
 };
 struct Unit {
@@ -156,20 +254,19 @@ __device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
     return t;
 }
 
-// tmA, tmB: boxes of 128 rows x 64 (UPDATE: tmB 64 rows x 64); tmR, tmL: residual, tmC, tmD: outputs, boxes of 32 rows x 32, 64-byte swizzle
+// tmA, tmB: boxes of 128 rows x 64 (UPDATE: tmB 64 rows x 64); tmC, tmD: outputs, boxes of 32 rows x 32, 64-byte swizzle
 template <int FORM>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
-    orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmR,
-                        const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
-                        const ProductArgs p)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                        const __grid_constant__ CUtensorMap tmD, const ProductArgs p)
 {
-    constexpr int RES = FORM == POLY ? 1 : FORM == UPDATE ? 2 : 0; // residual blocks of 2 KB
+    constexpr int RES = FORM == POLY ? 1 : FORM == UPDATE ? 2 : 0; // residual arrays
     extern __shared__ uint8_t orth_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)orth_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
     uint64_t *bars = (uint64_t *)(smem + BAR_OFF);
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), tfull0 = smem_u32(bars + 2 * STAGES),
-                   tempty0 = smem_u32(bars + 2 * STAGES + 2), drain = smem_u32(bars + 2 * STAGES + 4), res0 = smem_u32(bars + 2 * STAGES + 5);
-    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 5 + 24);
+                   tempty0 = smem_u32(bars + 2 * STAGES + 2), drain = smem_u32(bars + 2 * STAGES + 4);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 5);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -180,10 +277,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull0 + 8 * a, 1);
-            mbar_init(tempty0 + 8 * a, 16); // the leader's counts the epilogue warps of both CTAs
+            mbar_init(tempty0 + 8 * a, 2 * EPI_WARPS); // the leader's counts the epilogue warps of both CTAs
         }
-        for (int i = 0; i < 24; ++i)
-            mbar_init(res0 + 8 * i, 1);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -292,65 +387,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
             }
         }
     } else {
-        // epilogue: a warp takes 32 rows x 128 columns in four blocks of 32 x 32, thread = row
-        const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
-        uint8_t *const slots = smem + STG_OFF + ew * 3 * SLOT; // of 4 KB: a block and the low halves or the transpose
-        const uint32_t res_bar = res0 + 8 * 3 * ew;
+        // epilogue: a warp takes 32 rows x 64 columns in two blocks of 32 x 32, thread = row
+        const int quarter = warp & 3, ew = warp - 2, part = ew >> 2;
+        uint8_t *const blocks = smem + STG_OFF + ew * BLOCKS * BLOCK; // in turn, a store's each
         const int sw = (lane >> 1) & 3; // the 64-byte swizzle of the thread's row
-        auto row_of = [&](const Unit &un) { return un.row + (int)rank * 128 + quarter * 32; };
-        auto col_of = [&](const Unit &un, int c) { return un.col + half * 128 + c * 32; };
-        auto fetch = [&](const Unit &un, int c, int slot) { // lane 0
-            mbar_arrive_expect_tx(res_bar + 8 * slot, RES * 2048);
-            tma_load_3d(smem_u32(slots + slot * SLOT), &tmR, res_bar + 8 * slot, col_of(un, c), row_of(un), un.matrix);
-            if (RES == 2)
-                tma_load_3d(smem_u32(slots + slot * SLOT + 2048), &tmL, res_bar + 8 * slot, col_of(un, c), row_of(un), un.matrix);
-        };
-        int acc = 0, slot = 0;
-        uint32_t acc_phase = 0, slot_phase = 0;
-        bool ok = true;
-        if (RES && lane == 0 && first < p.units)
-            fetch(product_unit<FORM>(p, first), 0, 0);
-        for (int u = first; u < p.units && ok; u += step) {
+        int acc = 0, block = 0;
+        uint32_t acc_phase = 0;
+        for (int u = first; u < p.units; u += step) {
             const Unit un = product_unit<FORM>(p, u);
-            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PT + half * 128;
-            const int row0 = row_of(un);
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                const int next = slot == 2 ? 0 : slot + 1;
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PT + part * PART;
+            const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
+            const auto there = [&](int c) { return row0 < p.n && col0 + c * 32 < p.cols; }; // multiples of 32: a block is there or not
+            uint4 xs[4], ls[4];
+            const size_t at = ((size_t)un.matrix * p.n + row0 + lane) * p.cols + col0;
+            auto residual = [&](int c) {
                 if constexpr (RES > 0) {
-                    if (lane == 0) {
-                        bulk_wait_read<1>(); // the stores that last used the next slot have read it
-                        if (c < 3)
-                            fetch(un, c + 1, next);
-                        else if (u + step < p.units)
-                            fetch(product_unit<FORM>(p, u + step), 0, next);
+                    if (!there(c))
+                        return;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        xs[i] = *(const uint4 *)(p.res + at + c * 32 + i * 8);
+                        if (RES == 2)
+                            ls[i] = *(const uint4 *)(p.res_lo + at + c * 32 + i * 8);
                     }
-                } else if constexpr (FORM == SQUARE) {
-                    if (lane == 0)
-                        bulk_wait_read<2>();
                 }
-                __syncwarp();
-                if (c == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag));
-                    if (!ok)
-                        break;
-                    tc_fence_after();
-                }
-                if constexpr (RES > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(res_bar + 8 * slot, slot_phase, abort_flag));
-                    if (!ok)
-                        break;
-                }
+            };
+            residual(0);
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag)))
+                break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < PART / 32; ++c) {
                 uint32_t r[32];
                 tmem_ld32(taddr + c * 32, r);
                 tmem_ld_wait();
-                if (c == 3) { // the accumulator is read: the next tile may have it
+                if (c == PART / 32 - 1) { // the accumulator is read: the next tile may have it
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0)
                         mbar_arrive_cluster(map_to_leader(tempty0 + 8 * acc));
                 }
-                const int col = col_of(un, c);
+                const int col = col0 + c * 32;
                 if constexpr (FORM == PARTIAL) {
                     float4 *to = (float4 *)(p.part + ((size_t)un.index * PT + (row0 - un.row) + lane) * PT + (col - un.col));
 #pragma unroll
@@ -358,21 +435,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
                         to[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
                                             __uint_as_float(r[4 * i + 3]));
                 } else {
-                    uint8_t *const block = slots + slot * SLOT, *const second = block + 2048;
                     const bool mirror = FORM != UPDATE && un.row != un.col;
+                    const int other = block == BLOCKS - 1 ? 0 : block + 1;
+                    uint8_t *const first_block = blocks + block * BLOCK, *const second = blocks + other * BLOCK;
+                    block = other == BLOCKS - 1 ? 0 : other + 1;
+                    if (lane == 0)
+                        bulk_wait_read<BLOCKS - 2>(); // the stores that last used the two blocks have read them
+                    __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) { // 8 columns
-                        uint4 *const at = (uint4 *)(block + lane * 64 + ((i ^ sw) << 4)), *const at2 = (uint4 *)(second + lane * 64 + ((i ^ sw) << 4));
                         uint32_t out[4], low[4];
-                        const uint4 x4 = RES > 0 ? *at : make_uint4(0, 0, 0, 0), l4 = RES == 2 ? *at2 : make_uint4(0, 0, 0, 0);
-                        const uint32_t xs[4] = {x4.x, x4.y, x4.z, x4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
+                        const uint32_t xw[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w}, lw[4] = {ls[i].x, ls[i].y, ls[i].z, ls[i].w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             float v0 = p.alpha * __uint_as_float(r[8 * i + 2 * j]), v1 = p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]);
                             if constexpr (RES > 0) {
-                                float2 x = __half22float2(*(const __half2 *)&xs[j]);
+                                float2 x = __half22float2(*(const __half2 *)&xw[j]);
                                 if constexpr (RES == 2) {
-                                    const float2 l = __half22float2(*(const __half2 *)&ls[j]);
+                                    const float2 l = __half22float2(*(const __half2 *)&lw[j]);
                                     x.x = fmaf(l.x, 1.f / LO, x.x), x.y = fmaf(l.y, 1.f / LO, x.y);
                                 }
                                 v0 = fmaf(p.beta, x.x, v0), v1 = fmaf(p.beta, x.y, v1);
@@ -390,41 +470,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
                                 *(__half *)(second + (k + 1) * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __high2half(h);
                             }
                         }
-                        *at = make_uint4(out[0], out[1], out[2], out[3]);
+                        *(uint4 *)(first_block + lane * 64 + ((i ^ sw) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
                         if constexpr (FORM == UPDATE)
-                            *at2 = make_uint4(low[0], low[1], low[2], low[3]);
+                            *(uint4 *)(second + lane * 64 + ((i ^ sw) << 4)) = make_uint4(low[0], low[1], low[2], low[3]);
                     }
+                    if (c + 1 < PART / 32)
+                        residual(c + 1);
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        if (row0 < p.n && col < p.cols) {
-                            tma_store_3d(&tmC, smem_u32(block), col, row0, un.matrix);
-                            if (FORM == UPDATE)
-                                tma_store_3d(&tmD, smem_u32(second), col, row0, un.matrix);
-                            else if (mirror)
-                                tma_store_3d(&tmC, smem_u32(second), row0, col, un.matrix);
-                        }
+                        if (there(c))
+                            tma_store_3d(&tmC, smem_u32(first_block), col, row0, un.matrix);
+                        bulk_commit();
+                        if (there(c) && FORM == UPDATE)
+                            tma_store_3d(&tmD, smem_u32(second), col, row0, un.matrix);
+                        else if (there(c) && mirror)
+                            tma_store_3d(&tmC, smem_u32(second), row0, col, un.matrix);
                         bulk_commit();
                     }
                 }
-                slot = next;
-                if (slot == 0)
-                    slot_phase ^= 1;
             }
             acc ^= 1;
             if (acc == 0)
                 acc_phase ^= 1;
         }
-        if (lane == 0) {
-            if (RES && !ok) { // residual blocks in flight land before the CTA may leave
-                const long long t0 = clock64();
-                const int next = slot == 2 ? 0 : slot + 1;
-                while (!(mbar_try_wait(res_bar + 8 * slot, slot_phase) && mbar_try_wait(res_bar + 8 * next, next == 0 ? slot_phase ^ 1 : slot_phase)) &&
-                       clock64() - t0 < 200000000ll) {
-                }
-            }
+        if (lane == 0)
             bulk_wait_read<0>(); // the blocks must outlive the stores that read them
-        }
     }
     tc_fence_before();
     __syncthreads();
@@ -435,36 +506,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
         atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);
 }
 
-// The K ranges of SQUARE or (with a) POLY added in their order; 32 x 32 of a tile per block
+// The K ranges of SQUARE or (with a) POLY added in their order; 64 x 64 of a tile per block
 __global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict__ part, const ProductArgs p, const __half *__restrict__ a, __half *out)
 {
     grid_dep_wait();
-    __shared__ float tile[32][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    __shared__ float tile[64][65];
+    const int q = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8;
     int row, col;
     upper_tile(blockIdx.y, row, col);
     const bool mirror = row != col;
-    const int i0 = (blockIdx.x >> 3) * 32, j0 = (blockIdx.x & 7) * 32;
+    const int i0 = (blockIdx.x >> 2) * 64, j0 = (blockIdx.x & 3) * 64;
     row = row * PT + i0, col = col * PT + j0;
     if (row >= p.n || col >= p.n)
         return;
     part += ((size_t)blockIdx.z * p.tiles + blockIdx.y) * p.splits * PT * PT;
     out += (size_t)blockIdx.z * p.n * p.n;
-    for (int k = ty; k < 32; k += 8) {
-        float sum = 0.f;
-        for (int s = 0; s < p.splits; ++s)
-            sum += part[((size_t)s * PT + i0 + k) * PT + j0 + tx];
-        sum *= p.alpha;
+    if (a)
+        a += (size_t)blockIdx.z * p.n * p.n;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = q + 32 * h;
+        float sum[8] = {};
+        for (int s = 0; s < p.splits; ++s) {
+            const float4 *from = (const float4 *)(part + ((size_t)s * PT + i0 + i) * PT + j0 + c8);
+            const float4 x = from[0], y = from[1];
+            sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w, sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
+        }
+        const size_t at = (size_t)(row + i) * p.n + col + c8;
+        uint4 old = make_uint4(0, 0, 0, 0);
         if (a)
-            sum = fmaf(p.beta, __half2float(a[((size_t)blockIdx.z * p.n + row + k) * p.n + col + tx]), sum);
-        tile[k][tx] = sum;
-        out[(size_t)(row + k) * p.n + col + tx] = __low2half(sat_half2(sum, sum));
+            old = *(const uint4 *)(a + at);
+        alignas(16) __half o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = a ? fmaf(p.beta, __half2float(((const __half *)&old)[j]), p.alpha * sum[j]) : p.alpha * sum[j];
+            tile[i][c8 + j] = v;
+            o[j] = __low2half(sat_half2(v, v));
+        }
+        *(uint4 *)(out + at) = *(uint4 *)o;
     }
     if (!mirror)
         return;
     __syncthreads();
-    for (int k = ty; k < 32; k += 8)
-        out[(size_t)(col + k) * p.n + row + tx] = __low2half(sat_half2(tile[tx][k], tile[tx][k]));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = q + 32 * h;
+        alignas(16) __half o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            o[j] = __low2half(sat_half2(tile[c8 + j][i], 0.f));
+        *(uint4 *)(out + (size_t)(col + i) * p.n + row + c8) = *(uint4 *)o;
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -524,8 +616,7 @@ static int half_map(CUtensorMap *tm, const void *base, int64_t cols, int64_t row
 }
 
 template <int FORM>
-static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, const CUtensorMap &R, const CUtensorMap &L, const CUtensorMap &C,
-                   const CUtensorMap &D, const ProductArgs &p)
+static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, const CUtensorMap &C, const CUtensorMap &D, const ProductArgs &p)
 {
     static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
     const unsigned bit = 1u << (c.device & 15);
@@ -534,7 +625,7 @@ static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, con
         ready.fetch_or(bit);
     }
     const int pairs = std::min(sm_count(c.device) / 2, p.units);
-    TS2_LAUNCH((orth_product_kernel<FORM>), 2 * pairs, 320, SMEM, c.stream, A, B, R, L, C, D, p);
+    TS2_LAUNCH((orth_product_kernel<FORM>), 2 * pairs, THREADS, SMEM, c.stream, A, B, C, D, p);
     return TS2_OK;
 }
 
@@ -575,7 +666,8 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
 {
     const bool tall = rows > cols;
     const int n = std::min(rows, cols), m = std::max(rows, cols), np = (int)ceil_div(n, 64) * 64, mp = (int)ceil_div(m, 64) * 64;
-    const int n_part = std::min(rows, 64), pairs = sm_count(c.device) / 2;
+    const int pairs = sm_count(c.device) / 2;
+    const int n_part = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div((int64_t)rows * cols, 8192), std::max(1, 4 * sm_count(c.device) / batch)));
     const int nt = (int)ceil_div(np, PT), mt = (int)ceil_div(mp, PT), upper = nt * (nt + 1) / 2;
     const size_t x = (size_t)batch * np * mp, a = (size_t)batch * np * np;
     const int split1 = choose_splits(pairs, (int64_t)batch * upper, mp / BK), split2 = choose_splits(pairs, (int64_t)batch * upper, np / BK);
@@ -588,9 +680,13 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     __half *hi[2] = {(__half *)((uint8_t *)s.p + part_bytes), (__half *)((uint8_t *)s.p + part_bytes) + x}, *lo = hi[1] + x, *A = lo + x, *B = A + a;
     double *sums = (double *)(B + a);
 
-    TS2_LAUNCH((orth_sum2_kernel<T>), dim3(n_part, batch), 256, 0, c.stream, g, ld, stride, rows, cols, sums);
-    TS2_LAUNCH((orth_load_kernel<T>), dim3(mp / 32, np / 32, batch), 256, 0, c.stream, g, ld, stride, rows, cols, tall, sums, n_part, np, mp, hi[0],
-               lo);
+    const bool vec = ((uintptr_t)g | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(stride * sizeof(T))) % 16 == 0;
+    TS2_LAUNCH((orth_sum2_kernel<T>), dim3(n_part, batch), 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums);
+    const dim3 blocks(mp / 64, np / 64, batch);
+    if (tall)
+        TS2_LAUNCH((orth_load_kernel<T, true>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lo);
+    else
+        TS2_LAUNCH((orth_load_kernel<T, false>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lo);
     CUtensorMap x_rows[2], x_cols[2], x_block[2], lo_block, a_rows, a_block, b_rows, b_block;
     int rc = TS2_OK;
     for (int i = 0; i < 2 && rc == TS2_OK; ++i) {
@@ -610,31 +706,36 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
         return fail(TS2_ERR_CUDA, "no device status word");
     p.n = np;
     p.part = part;
-    const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &res, const CUtensorMap &to, __half *dst) {
+    const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &to, __half *dst) {
         p.cols = np, p.tiles = upper, p.col_tiles = 0;
         p.k_blocks = k / BK, p.splits = splits, p.kb_per_split = (int)ceil_div(p.k_blocks, splits), p.units = batch * upper * splits;
         if (splits == 1)
-            return poly ? product<POLY>(c, in, in, res, res, to, to, p) : product<SQUARE>(c, in, in, res, res, to, to, p);
-        if (int e = product<PARTIAL>(c, in, in, res, res, to, to, p))
+            return poly ? product<POLY>(c, in, in, to, to, p) : product<SQUARE>(c, in, in, to, to, p);
+        if (int e = product<PARTIAL>(c, in, in, to, to, p))
             return e;
-        TS2_LAUNCH(orth_join_kernel, dim3(64, upper, batch), 256, 0, c.stream, part, p, poly ? A : (const __half *)nullptr, dst);
+        TS2_LAUNCH(orth_join_kernel, dim3(16, upper, batch), 256, 0, c.stream, part, p, poly ? A : (const __half *)nullptr, dst);
         return TS2_OK;
     };
     for (int k = 0; k < steps; ++k) {
         const int now = k & 1;
         p.alpha = SA / (SX * SX), p.beta = 0.f;
-        if ((rc = symmetric(false, mp, split1, x_rows[now], a_block, a_block, A)))
+        if ((rc = symmetric(false, mp, split1, x_rows[now], a_block, A)))
             return rc;
-        p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA;
-        if ((rc = symmetric(true, np, split2, a_rows, a_block, b_block, B)))
+        p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA, p.res = A;
+        if ((rc = symmetric(true, np, split2, a_rows, b_block, B)))
             return rc;
-        p.alpha = 1.f / SB, p.beta = coef[0];
+        p.alpha = 1.f / SB, p.beta = coef[0], p.res = hi[now], p.res_lo = lo;
         p.cols = mp, p.tiles = nt * mt, p.col_tiles = mt, p.k_blocks = np / BK, p.splits = 1, p.kb_per_split = p.k_blocks, p.units = batch * nt * mt;
-        if ((rc = product<UPDATE>(c, b_rows, x_cols[now], x_block[now], lo_block, x_block[now ^ 1], lo_block, p)))
+        if ((rc = product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], lo_block, p)))
             return rc;
     }
-    TS2_LAUNCH(orth_store_kernel, dim3(mp / 32, np / 32, batch), 256, 0, c.stream, hi[steps & 1], lo, np, mp, tall, out_scale / SX, out, ld_out,
-               out_stride, rows, cols);
+    const bool vec_out = ((uintptr_t)out | (uintptr_t)(ld_out * 2) | (uintptr_t)(out_stride * 2)) % 16 == 0;
+    if (tall)
+        TS2_LAUNCH(orth_store_kernel<true>, blocks, 256, 0, c.stream, hi[steps & 1], lo, np, mp, out_scale / SX, out, ld_out, out_stride, rows, cols,
+                   vec_out);
+    else
+        TS2_LAUNCH(orth_store_kernel<false>, blocks, 256, 0, c.stream, hi[steps & 1], lo, np, mp, out_scale / SX, out, ld_out, out_stride, rows, cols,
+                   vec_out);
     return TS2_OK;
 }
 

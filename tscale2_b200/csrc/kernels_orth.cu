@@ -8,7 +8,7 @@
 // that falls off as 1/k^2, 512 x 1024, coefficients 3.4445, -4.7750, 2.0315, 5 steps: relative error 2.0e-2 with X in fp16,
 // 1.8e-4 with X in two halves; flat spectra 2.0e-3 and 1.3e-3).  All fp16 values are scaled by powers of two that keep them
 // below 65504 for every X the coefficients can reach (orth_check).
-#include "kernels.cuh"
+#include "orth.cuh"
 #include "pair_ptx.cuh"
 #include <cuda.h>
 #include <algorithm>
@@ -16,13 +16,8 @@
 
 namespace ts2 {
 
-// X, A = X X^T and B as they are stored: value * 2^14, 2^12, 2^11; |X| <= 3.9, |B| <= 31
-static constexpr float SX = 16384.f, SA = 4096.f, SB = 2048.f;
-static constexpr float MAX_X = 3.9f, MAX_B = 31.f;
+static constexpr float SX = ORTH_SX, SA = ORTH_SA, SB = ORTH_SB, MAX_X = ORTH_MAX_X, MAX_B = ORTH_MAX_B;
 static constexpr float LO = 2048.f; // the low half is stored times 2^11: its values are below 2^-11 of the high half's
-
-template <class T>
-__device__ __forceinline__ float widen(T v) { return (float)v; }
 
 __device__ __forceinline__ void split(float x, __half &hi, __half &lo)
 {
@@ -33,26 +28,6 @@ __device__ __forceinline__ void split(float x, __half &hi, __half &lo)
 __device__ __forceinline__ float joined(__half hi, __half lo) { return fmaf(__half2float(lo), 1.f / LO, __half2float(hi)); }
 
 // ---- G -> X and X -> out ---------------------------------------------------------------------------------------------
-// 8 elements of a row from column c on as floats, zeros from column `cols` on; vec: 16-byte accesses are aligned
-template <class T>
-__device__ __forceinline__ void load8(const T *row, int c, int cols, bool vec, float (&v)[8])
-{
-    if (vec && c + 8 <= cols) {
-        constexpr int PER = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 8 / PER; ++i) {
-            const uint4 raw = *(const uint4 *)(row + c + i * PER);
-            const T *e = (const T *)&raw;
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                v[i * PER + j] = widen(e[j]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = c + i < cols ? widen(row[c + i]) : 0.f;
-    }
-}
 __device__ __forceinline__ double warp_sum(double v)
 {
 #pragma unroll
@@ -75,7 +50,7 @@ __global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g,
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const int r = (int)(i / pieces), c = (int)(i - (long long)r * pieces) * 8;
         float v[8];
-        load8(g + r * ld, c, cols, vec, v);
+        orth_load8(g + r * ld, c, cols, vec, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             sum = fma((double)v[j], (double)v[j], sum);
@@ -106,7 +81,7 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
     for (int h = 0; h < 2; ++h) { // 32 rows of G at a time
         const int r = (TALL ? j0 : i0) + q + 32 * h;
         if (r < rows)
-            load8(g + r * ld, (TALL ? i0 : j0) + c8, cols, vec, v[h]);
+            orth_load8(g + r * ld, (TALL ? i0 : j0) + c8, cols, vec, v[h]);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -744,6 +719,8 @@ int orthogonalize(const Ctx &c, int type, const void *g, int64_t ld, int64_t str
 {
     if (!orth_check(coef, steps))
         return fail(TS2_ERR_UNSUPPORTED, "orthogonalize: the coefficients take singular values beyond %g", (double)MAX_X);
+    if (orth_chip_ranks(rows, cols))
+        return orth_chip(c, type, g, ld, stride, batch, rows, cols, coef, steps, out_scale, out, ld_out, out_stride);
     __nv_bfloat16 *o = (__nv_bfloat16 *)out;
     switch (type) {
     case TS2_OUT_F32: return orthogonalize_typed(c, (const float *)g, ld, stride, batch, rows, cols, coef, steps, out_scale, o, ld_out, out_stride);

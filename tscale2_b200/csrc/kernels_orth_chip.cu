@@ -1,0 +1,423 @@
+// Orthogonalised updates (kernels_orth.cu has the formula and its scaling) of matrices with at most 128 rows or columns, in one launch
+// and without memory in between: a cluster holds a matrix.  Each CTA has the 128 rows (padded with zeros) of up to 384 columns of X:
+// as fp32 in tensor memory, thread = row, and rounded to fp16 in shared memory as the operand of the products
+//     A = X X^T   (the CTAs' parts are added through distributed shared memory, each 128 / cluster rows for all)
+//     B = b A + c A A   (every CTA for itself)      X = a X + B X   (128 columns at a time)
+// A chain of small products: its latency is the bound.  As 15 launches of kernels_orth.cu 128 x 256 took 127 us.
+#include "kernels.cuh"
+#include "orth.cuh"
+#include <algorithm>
+
+namespace ts2 {
+
+namespace {
+
+constexpr int THREADS = 256, MAX_CHUNKS = 3, MAX_CLUSTER = 16;
+constexpr int BLK = 128 * 128;   // 128 rows x 64 columns of fp16, 128-byte swizzle
+constexpr int PITCH = 129;       // fp32 staging of 128 x 128
+constexpr int A_OFF = MAX_CHUNKS * 2 * BLK, B_OFF = A_OFF + 2 * BLK, STG_OFF = B_OFF + 2 * BLK, END_OFF = STG_OFF + 128 * PITCH * 4;
+constexpr int SMEM = END_OFF + 256 + 1024;
+static_assert(SMEM <= 232448, "shared memory budget");
+constexpr uint32_t WORK = MAX_CHUNKS * 128; // tensor-memory columns of the product at hand; X's chunks lie before it
+
+struct ChipArgs {
+    const void *g;
+    long long ld, stride;
+    int rows, cols, chunks; // chunks: of 128 columns of X in a CTA
+    int steps;
+    float a, b, c, out_scale;
+    __nv_bfloat16 *out;
+    long long ld_out, out_stride;
+    bool vec, vec_out;
+    int32_t *status;
+};
+
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_rank(uint32_t addr, unsigned rank)
+{
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+// 16-byte piece c (0 .. 15) of row r of 128 columns of fp16, as two swizzled blocks
+__device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)((c >> 3) * BLK + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+
+// 32 values as fp16 to the columns [32 j, +32) of the thread's row
+__device__ __forceinline__ void put_half(uint8_t *base, int row, int j, const float (&v)[32])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const __half2 h = sat_half2(v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
+            w[k] = *(const uint32_t *)&h;
+        }
+        *(uint4 *)(base + piece(row, 4 * j + i)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <class T, bool TALL>
+__global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
+{
+    extern __shared__ uint8_t chip_smem[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)chip_smem + 1023) & ~(uintptr_t)1023); // the same offset in every CTA of a cluster
+    float *stage = (float *)(smem + STG_OFF);
+    uint64_t *bar_at = (uint64_t *)(smem + END_OFF);
+    uint32_t *tmem_slot = (uint32_t *)(bar_at + 1);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    double *sums = (double *)(smem + END_OFF + 32); // a warp's, the CTA's
+    const uint32_t bar = smem_u32(bar_at);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    if (threadIdx.x == 0) {
+        mbar_init(bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (ranks > 1)
+        cluster_sync(); // all CTAs have started: their shared memory can be used
+    tc_fence_after();
+    grid_dep_wait();
+    const uint32_t tmem = *tmem_slot, lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64; // the thread's row, its half of 128 columns
+    const int row = quarter * 32 + lane, matrix = blockIdx.x / ranks;
+    const int n = TALL ? p.cols : p.rows, m = TALL ? p.rows : p.cols, j0 = (int)rank * p.chunks * 128;
+    const T *g = (const T *)p.g + matrix * p.stride;
+    const auto load32 = [&](uint32_t column, float (&v)[32]) {
+        uint32_t r[32];
+        tmem_ld32(lane_base + column, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            v[i] = __uint_as_float(r[i]);
+    };
+    const auto store32 = [&](uint32_t column, const float (&v)[32]) {
+        uint32_t r[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            r[i] = __float_as_uint(v[i]);
+        tmem_st32(lane_base + column, r);
+    };
+
+    // ---- G -> X, unscaled, and its sum of squares (fp64: nothing over- or underflows) ----
+    double sum = 0.;
+    for (int q = 0; q < p.chunks; ++q) {
+        const int j = j0 + q * 128, part = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+#pragma unroll 4
+        for (int k = 0; k < 8; ++k) {
+            const int r = (TALL ? j : 0) + part + 16 * k; // of G
+            float v[8];
+            if (r < p.rows)
+                orth_load8(g + r * p.ld, (TALL ? 0 : j) + c8, p.cols, p.vec, v);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                stage[TALL ? (c8 + i) * PITCH + part + 16 * k : (part + 16 * k) * PITCH + c8 + i] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                v[i] = stage[row * PITCH + half * 64 + h * 32 + i];
+                sum = fma((double)v[i], (double)v[i], sum);
+            }
+            store32(q * 128 + h * 32, v);
+        }
+        __syncthreads();
+    }
+    tmem_st_wait();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0)
+        sums[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = sums[0];
+        for (int w = 1; w < THREADS / 32; ++w)
+            sum += sums[w];
+        sums[8] = sum;
+    }
+    if (ranks > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    sum = sums[8];
+    if (ranks > 1) {
+        sum = 0.;
+        for (unsigned r = 0; r < ranks; ++r) {
+            double s;
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(s) : "r"(in_rank(smem_u32(sums + 8), r)) : "memory");
+            sum += s;
+        }
+    }
+    {
+        const double scale = sum == 0. ? 0. : (double)ORTH_SX / sqrt(sum);
+        const bool small = !(scale < 1e30); // G is all but denormal, or not finite
+        const float scale32 = (float)scale;
+        for (int q = 0; q < p.chunks; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[32];
+                load32(q * 128 + h * 32, v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    v[i] = small ? (float)(v[i] * scale) : v[i] * scale32;
+                store32(q * 128 + h * 32, v);
+                put_half(smem + q * 2 * BLK, row, half * 2 + h, v);
+            }
+    }
+
+    // ---- steps ----
+    uint32_t phase = 0;
+    // the operands in shared memory are complete and the product's columns are free: one thread issues, all wait for the product
+    const auto product = [&](auto &&issue) {
+        fence_proxy_async();
+        tmem_st_wait();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (threadIdx.x == 0) {
+            issue();
+            tc_commit(bar);
+        }
+        mbar_wait(bar, phase, abort_flag);
+        phase ^= 1;
+        tc_fence_after();
+    };
+    const uint32_t x_at = smem_u32(smem), a_at = smem_u32(smem + A_OFF), b_at = smem_u32(smem + B_OFF), work = tmem + WORK;
+    constexpr uint32_t IDESC = umma_idesc_f16(128, false, false), IDESC_MN = umma_idesc_f16(128, false, true);
+    for (int step = 0; step < p.steps; ++step) {
+        product([&] { // A = X X^T
+            for (int b = 0; b < 2 * p.chunks; ++b) {
+                const uint64_t d = umma_smem_desc(x_at + b * BLK, 16, 1024);
+                umma_f16_x4(work, d, d, IDESC, b > 0, 2, 2);
+            }
+        });
+        constexpr float ALPHA = ORTH_SA / (ORTH_SX * ORTH_SX);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[32];
+            load32(WORK + h * 32, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v[i] *= ALPHA;
+            if (ranks == 1) {
+                put_half(smem + A_OFF, row, half * 2 + h, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    stage[row * PITCH + half * 64 + h * 32 + i] = v[i];
+            }
+        }
+        if (ranks > 1) {
+            cluster_sync();
+            const int rows_each = 128 / (int)ranks;
+            for (int i = threadIdx.x; i < rows_each * 16; i += THREADS) {
+                const int r = (int)rank * rows_each + (i >> 4), c = i & 15;
+                const uint32_t at = smem_u32(stage + r * PITCH + c * 8);
+                float v[8] = {};
+                for (unsigned k = 0; k < ranks; ++k) {
+                    const uint32_t from = in_rank(at, k);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float f;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(from + 4 * e) : "memory");
+                        v[e] += f;
+                    }
+                }
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __half2 h = sat_half2(v[2 * e], v[2 * e + 1]);
+                    w[e] = *(const uint32_t *)&h;
+                }
+                for (unsigned k = 0; k < ranks; ++k)
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(in_rank(a_at + piece(r, c), k)), "r"(w[0]), "r"(w[1]),
+                                 "r"(w[2]), "r"(w[3])
+                                 : "memory");
+            }
+            cluster_sync();
+        }
+        product([&] { // A A
+            for (int b = 0; b < 2; ++b) {
+                const uint64_t d = umma_smem_desc(a_at + b * BLK, 16, 1024);
+                umma_f16_x4(work, d, d, IDESC, b > 0, 2, 2);
+            }
+        });
+        const float kb = ORTH_SB * p.b / ORTH_SA, kc = ORTH_SB * p.c / (ORTH_SA * ORTH_SA);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[32];
+            load32(WORK + h * 32, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 raw = *(const uint4 *)(smem + A_OFF + piece(row, (half * 2 + h) * 4 + i));
+                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = __half22float2(*(const __half2 *)&w[k]);
+                    v[8 * i + 2 * k] = fmaf(kb, f.x, kc * v[8 * i + 2 * k]);
+                    v[8 * i + 2 * k + 1] = fmaf(kb, f.y, kc * v[8 * i + 2 * k + 1]);
+                }
+            }
+            put_half(smem + B_OFF, row, half * 2 + h, v);
+        }
+        const bool last = step == p.steps - 1;
+        for (int q = 0; q < p.chunks; ++q) {
+            product([&] { // B X, 128 columns
+                const uint64_t x = umma_smem_desc(x_at + q * 2 * BLK, BLK, 1024);
+                for (int b = 0; b < 2; ++b)
+                    umma_f16_x4(work, umma_smem_desc(b_at + b * BLK, 16, 1024), x + (uint64_t)(b * 4 * (16 * 128 >> 4)), IDESC_MN, b > 0, 2,
+                                16 * 128 >> 4);
+            });
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[32], x[32];
+                load32(WORK + h * 32, v);
+                load32(q * 128 + h * 32, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    v[i] = fmaf(p.a, x[i], v[i] * (1.f / ORTH_SB));
+                if (last) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        stage[row * PITCH + half * 64 + h * 32 + i] = v[i] * (p.out_scale / ORTH_SX);
+                } else {
+                    store32(q * 128 + h * 32, v);
+                    put_half(smem + q * 2 * BLK, row, half * 2 + h, v);
+                }
+            }
+            if (!last)
+                continue;
+            // X -> out, by rows of out
+            __syncthreads();
+            const int j = j0 + q * 128, part = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+            __nv_bfloat16 *out = p.out + matrix * p.out_stride;
+            for (int k = 0; k < 8; ++k) {
+                const int r = (TALL ? j : 0) + part + 16 * k, c = (TALL ? 0 : j) + c8;
+                if (r >= p.rows || c >= p.cols)
+                    continue;
+                alignas(16) __nv_bfloat16 o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    o[i] = __float2bfloat16_rn(stage[TALL ? (c8 + i) * PITCH + part + 16 * k : (part + 16 * k) * PITCH + c8 + i]);
+                if (p.vec_out && c + 8 <= p.cols) {
+                    *(uint4 *)(out + r * p.ld_out + c) = *(uint4 *)o;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < p.cols)
+                            out[r * p.ld_out + c + i] = o[i];
+                }
+            }
+            // the next chunk's product waits for all threads before the staging is written again
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (ranks > 1)
+        cluster_sync(); // nobody uses another CTA's shared memory any more
+    if (warp == 0)
+        tmem_dealloc(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag)
+        atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);
+    (void)n, (void)m;
+}
+
+template <class T, bool TALL>
+int launch(const Ctx &c, const ChipArgs &p, int batch, int ranks)
+{
+    static std::atomic<unsigned> ready{0}; // a bit a device
+    const unsigned bit = 1u << (c.device & 15);
+    const auto kern = orth_chip_kernel<T, TALL>;
+    if (!(ready.load() & bit)) {
+        TS2_CUDA(cudaFuncSetAttribute((const void *)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        TS2_CUDA(cudaFuncSetAttribute((const void *)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        ready.fetch_or(bit);
+    }
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ranks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = batch * ranks;
+    cfg.blockDim = THREADS;
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = c.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(TS2_ERR_CUDA, "kernel launch failed: %s (%s:%d)", cudaGetErrorString(e), __FILE__, __LINE__);
+    }
+    return TS2_OK;
+}
+
+} // namespace
+
+// CTAs of the cluster that holds a matrix, 0: it does not fit
+int orth_chip_ranks(int rows, int cols)
+{
+    if (std::min(rows, cols) > 128)
+        return 0;
+    const int64_t chunks = ceil_div(std::max(rows, cols), 128);
+    for (int ranks = 1; ranks <= MAX_CLUSTER; ranks *= 2)
+        if (chunks <= (int64_t)ranks * MAX_CHUNKS)
+            return ranks;
+    return 0;
+}
+
+int orth_chip(const Ctx &c, int type, const void *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
+              float out_scale, void *out, int64_t ld_out, int64_t out_stride)
+{
+    const int ranks = orth_chip_ranks(rows, cols), es = type == TS2_OUT_F32 ? 4 : 2;
+    ChipArgs p = {};
+    p.g = g, p.ld = ld, p.stride = stride, p.rows = rows, p.cols = cols;
+    p.chunks = (int)ceil_div(ceil_div(std::max(rows, cols), 128), ranks);
+    p.steps = steps, p.a = coef[0], p.b = coef[1], p.c = coef[2], p.out_scale = out_scale;
+    p.out = (__nv_bfloat16 *)out, p.ld_out = ld_out, p.out_stride = out_stride;
+    p.vec = ((uintptr_t)g | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) % 16 == 0;
+    p.vec_out = ((uintptr_t)out | (uintptr_t)(ld_out * 2) | (uintptr_t)(out_stride * 2)) % 16 == 0;
+    p.status = device_status_word(c.device);
+    if (!p.status)
+        return fail(TS2_ERR_CUDA, "no device status word");
+    const bool tall = rows > cols;
+    switch (type) {
+    case TS2_OUT_F32: return tall ? launch<float, true>(c, p, batch, ranks) : launch<float, false>(c, p, batch, ranks);
+    case TS2_OUT_F16: return tall ? launch<__half, true>(c, p, batch, ranks) : launch<__half, false>(c, p, batch, ranks);
+    default: return tall ? launch<__nv_bfloat16, true>(c, p, batch, ranks) : launch<__nv_bfloat16, false>(c, p, batch, ranks);
+    }
+}
+
+} // namespace ts2

@@ -1,0 +1,39 @@
+// What the kernels of the orthogonalised update share (kernels_orth.cu, kernels_orth_chip.cu).
+#pragma once
+#include "kernels.cuh"
+
+namespace ts2 {
+
+// X, A = X X^T and B = b A + c A A as fp16 holds them: value * 2^14, 2^12, 2^11; |X| <= 3.9, |B| <= 31
+constexpr float ORTH_SX = 16384.f, ORTH_SA = 4096.f, ORTH_SB = 2048.f;
+constexpr float ORTH_MAX_X = 3.9f, ORTH_MAX_B = 31.f;
+
+// the form for matrices that a cluster holds: how many CTAs it takes (0: none), and the call
+int orth_chip_ranks(int rows, int cols);
+int orth_chip(const Ctx &c, int type, const void *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
+              float out_scale, void *out, int64_t ld_out, int64_t out_stride);
+
+#ifdef __CUDACC__
+// 8 elements of a row from column c on as floats, zeros from column `cols` on; vec: 16-byte accesses are aligned
+template <class T>
+__device__ __forceinline__ void orth_load8(const T *row, int c, int cols, bool vec, float (&v)[8])
+{
+    if (vec && c + 8 <= cols) {
+        constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8 / PER; ++i) {
+            const uint4 raw = *(const uint4 *)(row + c + i * PER);
+            const T *e = (const T *)&raw;
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                v[i * PER + j] = (float)e[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = c + i < cols ? (float)row[c + i] : 0.f;
+    }
+}
+#endif
+
+} // namespace ts2

@@ -103,6 +103,24 @@ def test_one_large_matrix():
     near(run("f32", g)[0], g[0])
 
 
+@pytest.mark.parametrize("kind,batch,rows,cols", [("f32", 2, 100, 385), ("bf16", 1, 700, 33), ("f32", 3, 128, 900), ("f16", 1, 1999, 128), ("f32", 1, 5, 3100),
+                                                  ("f32", 1, 128, 6144), ("f32", 1, 6145, 120)])
+def test_long_rows_on_clusters_of_every_size(kind, batch, rows, cols):
+    g = np.stack([spectrum(rows, cols, 0.5, s) for s in range(batch)]).astype(TYPE[kind])
+    got = run(kind, g)
+    for o, m in zip(got, g):
+        near(o, m)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 300, 2500), (30, 200, 264), (13, 520, 300), (1, 2000, 140)])
+def test_products_of_few_and_of_many_tiles(batch, rows, cols):
+    """one matrix whose K is divided, and more matrices than are worked on at a time"""
+    g = np.stack([spectrum(rows, cols, 0.5, s) for s in range(batch)]).astype(np.float32)
+    got = run("f32", g, steps=6)
+    for i in {0, batch // 2, batch - 1}:
+        near(got[i], g[i], steps=6)
+
+
 @pytest.mark.parametrize("batch,rows,cols", [(1, 64, 64), (5, 96, 160), (40, 128, 100), (3, 300, 128), (17, 256, 256)])
 def test_a_batch_is_its_matrices_one_by_one(batch, rows, cols):
     g = np.stack([spectrum(rows, cols, 0.5, s) for s in range(batch)]).astype(np.float32)

@@ -25,9 +25,8 @@ __device__ __forceinline__ void split(float x, __half &hi, __half &lo)
     const float r = (x - __half2float(hi)) * LO;
     lo = __low2half(sat_half2(r, r));
 }
-__device__ __forceinline__ float joined(__half hi, __half lo) { return fmaf(__half2float(lo), 1.f / LO, __half2float(hi)); }
 
-// ---- G -> X and X -> out ---------------------------------------------------------------------------------------------
+// ---- G -> X ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ double warp_sum(double v)
 {
 #pragma unroll
@@ -122,65 +121,17 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
     }
 }
 
-template <bool TALL>
-__global__ void __launch_bounds__(256) orth_store_kernel(const __half *__restrict__ hi, const __half *__restrict__ lo, int np, int mp, float scale,
-                                                         __nv_bfloat16 *out, long long ld, long long stride, int rows, int cols, bool vec)
-{
-    grid_dep_wait();
-    __shared__ float tile[TALL ? 64 : 1][65];
-    const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, q = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8;
-    out += b * stride;
-    float v[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const size_t at = ((size_t)b * np + i0 + q + 32 * h) * mp + j0 + c8;
-        const uint4 rh = *(const uint4 *)(hi + at), rl = *(const uint4 *)(lo + at);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[h][j] = joined(((const __half *)&rh)[j], ((const __half *)&rl)[j]) * scale;
-    }
-    if (TALL) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                tile[q + 32 * h][c8 + j] = v[h][j];
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[h][j] = tile[c8 + j][q + 32 * h];
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = (TALL ? j0 : i0) + q + 32 * h, c = (TALL ? i0 : j0) + c8;
-        if (r >= rows || c >= cols)
-            continue;
-        alignas(16) __nv_bfloat16 o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            o[j] = __float2bfloat16_rn(v[h][j]);
-        if (vec && c + 8 <= cols) {
-            *(uint4 *)(out + r * ld + c) = *(uint4 *)o;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c + j < cols)
-                    out[r * ld + c + j] = o[j];
-        }
-    }
-}
-
 // ---- the products ----------------------------------------------------------------------------------------------------
 // Pairs of CTAs on tiles of 256 x 256 (as in gemm_pair.cu), one launch for a product of every matrix of the batch.
 //   SQUARE  A = X X^T     POLY  B = b A + c A A     both operands K-contiguous; symmetric, so only tiles on and above the diagonal are
 //                         computed, and what is above it leaves a second time as its transpose
 //   UPDATE  X = a X + B X   B is K-contiguous (it is its own transpose), X is contiguous along N; writes the high halves to a second
 //                         array, since other tiles still read them, and the low halves in place
+//   LAST    UPDATE of the last step: writes the result
 //   PARTIAL a K range of SQUARE or POLY in fp32, for outputs of few tiles; orth_join_kernel adds the ranges
 // Residual inputs are read by the epilogue's threads, a row of 32 each; results leave as blocks of 32 x 32 by TMA.
-enum Form { SQUARE, POLY, UPDATE, PARTIAL };
+enum Form { SQUARE, POLY, UPDATE, PARTIAL, LAST };
+constexpr bool updates(int form) { return form == UPDATE || form == LAST; }
 constexpr int PT = 256, BK = 64, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
 // Six stages and eight epilogue warps with two blocks each against four, sixteen and three: 32 x 1024 x 1024 1042 -> 1019 us, 8192 x
 // 2048 775 -> 732
@@ -196,6 +147,12 @@ struct ProductArgs {
     float alpha, beta; // POLY: alpha acc + beta A; UPDATE: alpha acc + beta X; else alpha acc
     float *part;       // PARTIAL: [matrix][tile][split][256][256]
     const __half *res, *res_lo; // A, or the halves of X
+    // LAST
+    __nv_bfloat16 *out;
+    long long ld_out, out_stride;
+    int out_rows, out_cols;
+    float out_scale;
+    bool tall, vec_out;
     int32_t *status;
 };
 struct Unit {
@@ -219,7 +176,7 @@ __device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
     t.index = u;
     t.matrix = tile / p.tiles;
     const int r = tile - t.matrix * p.tiles;
-    if (FORM == UPDATE)
+    if (updates(FORM))
         t.row = r / p.col_tiles, t.col = r - t.row * p.col_tiles;
     else
         upper_tile(r, t.row, t.col);
@@ -229,13 +186,13 @@ __device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
     return t;
 }
 
-// tmA, tmB: boxes of 128 rows x 64 (UPDATE: tmB 64 rows x 64); tmC, tmD: outputs, boxes of 32 rows x 32, 64-byte swizzle
+// tmA, tmB: boxes of 128 rows x 64 (UPDATE, LAST: tmB 64 rows x 64); tmC, tmD: outputs, boxes of 32 rows x 32, 64-byte swizzle
 template <int FORM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
                         const __grid_constant__ CUtensorMap tmD, const ProductArgs p)
 {
-    constexpr int RES = FORM == POLY ? 1 : FORM == UPDATE ? 2 : 0; // residual arrays
+    constexpr int RES = FORM == POLY ? 1 : updates(FORM) ? 2 : 0; // residual arrays
     extern __shared__ uint8_t orth_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)orth_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
     uint64_t *bars = (uint64_t *)(smem + BAR_OFF);
@@ -291,7 +248,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         mbar_arrive_expect_tx(full0 + 8 * stage, 2 * STAGE);
                     const uint32_t sa = smem_u32(smem + stage * STAGE), sb = sa + HALF;
                     tma_load_3d_pair(sa, &tmA, fb, kb * BK, am, un.matrix);
-                    if constexpr (FORM == UPDATE) {
+                    if constexpr (updates(FORM)) {
                         tma_load_3d_pair(sb, &tmB, fb, bn, kb * BK, un.matrix);
                         tma_load_3d_pair(sb + BK * 128, &tmB, fb, bn + 64, kb * BK, un.matrix);
                     } else {
@@ -321,7 +278,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     } else if (warp == 1) {
         // MMA issuer (leader)
         if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = (1u << 4) | ((FORM == UPDATE ? 1u : 0u) << 16) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
+            constexpr uint32_t idesc = (1u << 4) | ((updates(FORM) ? 1u : 0u) << 16) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
@@ -339,8 +296,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + stage * STAGE);
                     const uint64_t adesc = umma_smem_desc(sa, 16, 1024);
-                    const uint64_t bdesc = umma_smem_desc(sa + HALF, FORM == UPDATE ? BK * 128 : 16, 1024);
-                    constexpr uint64_t a_step = 2, b_step = FORM == UPDATE ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
+                    const uint64_t bdesc = umma_smem_desc(sa + HALF, updates(FORM) ? BK * 128 : 16, 1024);
+                    constexpr uint64_t a_step = 2, b_step = updates(FORM) ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         umma_pair<1>(tmem_d, adesc + k * a_step, bdesc + k * b_step, idesc, (kb > un.kb0 || k > 0) ? 1u : 0u);
@@ -409,6 +366,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     for (int i = 0; i < 8; ++i)
                         to[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
                                             __uint_as_float(r[4 * i + 3]));
+                } else if constexpr (FORM == LAST) {
+                    const int i0 = row0 + lane; // X's row: one of the result, or (tall) a column, 32 neighbours a store
+                    __nv_bfloat16 *out = p.out + un.matrix * p.out_stride + (p.tall ? (long long)col * p.ld_out + i0 : (long long)i0 * p.ld_out + col);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { // 8 columns
+                        const uint32_t xw[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w}, lw[4] = {ls[i].x, ls[i].y, ls[i].z, ls[i].w};
+                        __nv_bfloat162 o[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 x = __half22float2(*(const __half2 *)&xw[j]), l = __half22float2(*(const __half2 *)&lw[j]);
+                            const float v0 = fmaf(p.beta, fmaf(l.x, 1.f / LO, x.x), p.alpha * __uint_as_float(r[8 * i + 2 * j]));
+                            const float v1 = fmaf(p.beta, fmaf(l.y, 1.f / LO, x.y), p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]));
+                            o[j] = __floats2bfloat162_rn(v0 * p.out_scale, v1 * p.out_scale);
+                        }
+                        if (p.tall) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (i0 < p.out_cols && col + 8 * i + j < p.out_rows)
+                                    out[(8 * i + j) * p.ld_out] = j & 1 ? __high2bfloat16(o[j / 2]) : __low2bfloat16(o[j / 2]);
+                        } else if (i0 < p.out_rows) {
+                            if (p.vec_out && col + 8 * i + 8 <= p.out_cols)
+                                *(uint4 *)(out + 8 * i) = make_uint4(*(uint32_t *)&o[0], *(uint32_t *)&o[1], *(uint32_t *)&o[2], *(uint32_t *)&o[3]);
+                            else
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    if (col + 8 * i + j < p.out_cols)
+                                        out[8 * i + j] = j & 1 ? __high2bfloat16(o[j / 2]) : __low2bfloat16(o[j / 2]);
+                        }
+                    }
+                    if (c + 1 < PART / 32)
+                        residual(c + 1);
                 } else {
                     const bool mirror = FORM != UPDATE && un.row != un.col;
                     const int other = block == BLOCKS - 1 ? 0 : block + 1;
@@ -701,16 +689,14 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
             return rc;
         p.alpha = 1.f / SB, p.beta = coef[0], p.res = hi[now], p.res_lo = lo;
         p.cols = mp, p.tiles = nt * mt, p.col_tiles = mt, p.k_blocks = np / BK, p.splits = 1, p.kb_per_split = p.k_blocks, p.units = batch * nt * mt;
-        if ((rc = product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], lo_block, p)))
+        if (k == steps - 1) {
+            p.out = out, p.ld_out = ld_out, p.out_stride = out_stride, p.out_rows = rows, p.out_cols = cols, p.out_scale = out_scale / SX, p.tall = tall;
+            p.vec_out = ((uintptr_t)out | (uintptr_t)(ld_out * 2) | (uintptr_t)(out_stride * 2)) % 16 == 0;
+        }
+        if ((rc = k < steps - 1 ? product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], lo_block, p)
+                                : product<LAST>(c, b_rows, x_cols[now], x_block[now ^ 1], lo_block, p)))
             return rc;
     }
-    const bool vec_out = ((uintptr_t)out | (uintptr_t)(ld_out * 2) | (uintptr_t)(out_stride * 2)) % 16 == 0;
-    if (tall)
-        TS2_LAUNCH(orth_store_kernel<true>, blocks, 256, 0, c.stream, hi[steps & 1], lo, np, mp, out_scale / SX, out, ld_out, out_stride, rows, cols,
-                   vec_out);
-    else
-        TS2_LAUNCH(orth_store_kernel<false>, blocks, 256, 0, c.stream, hi[steps & 1], lo, np, mp, out_scale / SX, out, ld_out, out_stride, rows, cols,
-                   vec_out);
     return TS2_OK;
 }
 

@@ -290,17 +290,25 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
             put_half(smem + B_OFF, row, half * 2 + h, v);
         }
         const bool last = step == p.steps - 1;
+        // up to two chunks have tensor memory for their products at once
+        const bool together = p.chunks < MAX_CHUNKS;
         for (int q = 0; q < p.chunks; ++q) {
-            product([&] { // B X, 128 columns
-                const uint64_t x = umma_smem_desc(x_at + q * 2 * BLK, BLK, 1024);
-                for (int b = 0; b < 2; ++b)
-                    umma_f16_x4(work, umma_smem_desc(b_at + b * BLK, 16, 1024), x + (uint64_t)(b * 4 * (16 * 128 >> 4)), IDESC_MN, b > 0, 2,
-                                16 * 128 >> 4);
-            });
+            const uint32_t at = together ? WORK - (p.chunks - 1 - q) * 128 : WORK;
+            if (q == 0 || !together)
+                product([&] { // B X, 128 columns a chunk
+                    for (int k = q; k < (together ? p.chunks : q + 1); ++k) {
+                        const uint64_t x = umma_smem_desc(x_at + k * 2 * BLK, BLK, 1024);
+                        for (int b = 0; b < 2; ++b)
+                            umma_f16_x4(tmem + at + (k - q) * 128, umma_smem_desc(b_at + b * BLK, 16, 1024), x + (uint64_t)(b * 4 * (16 * 128 >> 4)),
+                                        IDESC_MN, b > 0, 2, 16 * 128 >> 4);
+                    }
+                });
+            else if (last)
+                __syncthreads(); // the staging of the chunk before has been read
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float v[32], x[32];
-                load32(WORK + h * 32, v);
+                load32(at + h * 32, v);
                 load32(q * 128 + h * 32, x);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -337,7 +345,6 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                             out[r * p.ld_out + c + i] = o[i];
                 }
             }
-            // the next chunk's product waits for all threads before the staging is written again
         }
     }
     tc_fence_before();

@@ -26,6 +26,14 @@ __device__ __forceinline__ void split(float x, __half &hi, __half &lo)
     lo = __low2half(sat_half2(r, r));
 }
 
+constexpr int PT = 256, BK = 64, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
+// Order of the low halves of a tile of 256 x 256: [CTA of the pair][epilogue warp][block of 32 columns][piece of 8][lane = row]
+constexpr int HALF_PIECES = PT * PT / 8;
+__device__ __forceinline__ int lane_piece(int row, int col) // of the piece at column col
+{
+    return ((((row >> 7) * 8 + (row >> 5 & 3) + 4 * (col >> 7)) * 4 + (col >> 5 & 3)) * 4 + (col >> 3 & 3)) * 32 + (row & 31);
+}
+
 // ---- G -> X ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ double warp_sum(double v)
 {
@@ -68,7 +76,7 @@ __global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g,
 // 64 x 64 of X [n][m] (padded to np x mp with zeros) from G, transposed where G has more rows than columns
 template <class T, bool TALL>
 __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, bool vec,
-                                                        const double *part, int n_part, int np, int mp, __half *hi, __half *lo)
+                                                        const double *part, int n_part, int np, int mp, __half *hi, uint4 *lo, int col_tiles, int tiles)
 {
     grid_dep_wait();
     __shared__ double norm;
@@ -117,7 +125,8 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
         }
         const size_t at = ((size_t)b * np + i0 + i) * mp + j0 + c8;
         *(uint4 *)(hi + at) = *(uint4 *)hs;
-        *(uint4 *)(lo + at) = *(uint4 *)ls;
+        const int row = i0 + i, col = j0 + c8;
+        lo[((size_t)b * tiles + (row / PT) * col_tiles + col / PT) * HALF_PIECES + lane_piece(row % PT, col % PT)] = *(uint4 *)ls;
     }
 }
 
@@ -129,15 +138,15 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
 //                         array, since other tiles still read them, and the low halves in place
 //   LAST    UPDATE of the last step: writes the result
 //   PARTIAL a K range of SQUARE or POLY in fp32, for outputs of few tiles; orth_join_kernel adds the ranges
-// Residual inputs are read by the epilogue's threads, a row of 32 each; results leave as blocks of 32 x 32 by TMA.
+// Residual inputs are read row by row and handed out to the threads, which have a row of 32 each, through shared memory; the low
+// halves, which nothing else reads, lie in the order of these threads (lane_piece).  Results leave as blocks of 32 x 32 by TMA.
 enum Form { SQUARE, POLY, UPDATE, PARTIAL, LAST };
 constexpr bool updates(int form) { return form == UPDATE || form == LAST; }
-constexpr int PT = 256, BK = 64, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
-// Six stages and eight epilogue warps with two blocks each against four, sixteen and three: 32 x 1024 x 1024 1042 -> 1019 us, 8192 x
-// 2048 775 -> 732
-constexpr int STAGES = 6, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS, BLOCKS = 2;
+constexpr int STAGES = 5, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS, BLOCKS = 2;
 constexpr int PART = PT / (EPI_WARPS / 4); // columns of an epilogue warp
-constexpr int BLOCK = 2048, STG_OFF = STAGES * STAGE, BAR_OFF = STG_OFF + EPI_WARPS * BLOCKS * BLOCK, SMEM = BAR_OFF + 1024 + 1024;
+// an epilogue warp's shared memory: two blocks of 32 x 32 on their way out, 32 x 64 of the residual input
+constexpr int BLOCK = 2048, WARP_BYTES = BLOCKS * BLOCK + 4096, STG_OFF = STAGES * STAGE, BAR_OFF = STG_OFF + EPI_WARPS * WARP_BYTES,
+              SMEM = BAR_OFF + 1024 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 
 struct ProductArgs {
@@ -146,7 +155,8 @@ struct ProductArgs {
     int units, k_blocks, splits, kb_per_split;
     float alpha, beta; // POLY: alpha acc + beta A; UPDATE: alpha acc + beta X; else alpha acc
     float *part;       // PARTIAL: [matrix][tile][split][256][256]
-    const __half *res, *res_lo; // A, or the halves of X
+    const __half *res; // A, or the high halves of X
+    uint4 *lo;         // the low halves, [matrix][tile of X] in the order of lane_piece
     // LAST
     __nv_bfloat16 *out;
     long long ld_out, out_stride;
@@ -156,7 +166,7 @@ struct ProductArgs {
     int32_t *status;
 };
 struct Unit {
-    int matrix, row, col, kb0, kb1, index;
+    int matrix, tile, row, col, kb0, kb1, index;
 };
 // the r-th tile on or above the diagonal of a square of tiles, column by column
 __device__ __forceinline__ void upper_tile(int r, int &row, int &col)
@@ -175,7 +185,7 @@ __device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
     const int tile = u / p.splits, split = u - tile * p.splits;
     t.index = u;
     t.matrix = tile / p.tiles;
-    const int r = tile - t.matrix * p.tiles;
+    const int r = t.tile = tile - t.matrix * p.tiles;
     if (updates(FORM))
         t.row = r / p.col_tiles, t.col = r - t.row * p.col_tiles;
     else
@@ -186,11 +196,11 @@ __device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
     return t;
 }
 
-// tmA, tmB: boxes of 128 rows x 64 (UPDATE, LAST: tmB 64 rows x 64); tmC, tmD: outputs, boxes of 32 rows x 32, 64-byte swizzle
+// tmA, tmB: boxes of 128 rows x 64 (UPDATE, LAST: tmB 64 rows x 64); tmC: the output, boxes of 32 rows x 32, 64-byte swizzle
 template <int FORM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-                        const __grid_constant__ CUtensorMap tmD, const ProductArgs p)
+                        const ProductArgs p)
 {
     constexpr int RES = FORM == POLY ? 1 : updates(FORM) ? 2 : 0; // residual arrays
     extern __shared__ uint8_t orth_smem[];
@@ -321,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     } else {
         // epilogue: a warp takes 32 rows x 64 columns in two blocks of 32 x 32, thread = row
         const int quarter = warp & 3, ew = warp - 2, part = ew >> 2;
-        uint8_t *const blocks = smem + STG_OFF + ew * BLOCKS * BLOCK; // in turn, a store's each
+        uint8_t *const blocks = smem + STG_OFF + ew * WARP_BYTES, *const handed = blocks + BLOCKS * BLOCK; // in turn, a store's each
         const int sw = (lane >> 1) & 3; // the 64-byte swizzle of the thread's row
         int acc = 0, block = 0;
         uint32_t acc_phase = 0;
@@ -330,21 +340,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PT + part * PART;
             const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
             const auto there = [&](int c) { return row0 < p.n && col0 + c * 32 < p.cols; }; // multiples of 32: a block is there or not
-            uint4 xs[4], ls[4];
-            const size_t at = ((size_t)un.matrix * p.n + row0 + lane) * p.cols + col0;
-            auto residual = [&](int c) {
+            uint4 rows[8], xs[4], ls[4]; // of 32 rows x 64: 8 lanes a row; of the block at hand: the thread's row
+            const auto fetch = [&](int h) {
                 if constexpr (RES > 0) {
-                    if (!there(c))
+                    if (!there(2 * h))
                         return;
+                    const __half *from = p.res + ((size_t)un.matrix * p.n + row0 + (lane >> 3)) * p.cols + col0 + h * 64 + (lane & 7) * 8;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        xs[i] = *(const uint4 *)(p.res + at + c * 32 + i * 8);
-                        if (RES == 2)
-                            ls[i] = *(const uint4 *)(p.res_lo + at + c * 32 + i * 8);
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        rows[i] = *(const uint4 *)(from + (size_t)(4 * i) * p.cols);
                 }
             };
-            residual(0);
+            uint4 *const lows = p.lo + ((size_t)un.matrix * p.tiles + un.tile) * HALF_PIECES + lane_piece(row0 - un.row + lane, part * PART);
+            const auto fetch_low = [&](int c) {
+                if constexpr (RES == 2)
+                    if (there(c)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            ls[i] = lows[(c * 4 + i) * 32];
+                    }
+            };
+            fetch(0);
+            fetch_low(0);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag)))
                 break;
             tc_fence_after();
@@ -359,13 +376,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (lane == 0)
                         mbar_arrive_cluster(map_to_leader(tempty0 + 8 * acc));
                 }
+                if constexpr (RES > 0) {
+                    if (!(c & 1)) {
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int at = i * 4 + (lane >> 3);
+                            *(uint4 *)(handed + at * 128 + (((lane & 7) ^ (at & 7)) << 4)) = rows[i];
+                        }
+                        __syncwarp();
+                        if (c == 0)
+                            fetch(1);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        xs[i] = *(const uint4 *)(handed + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
+                }
                 const int col = col0 + c * 32;
                 if constexpr (FORM == PARTIAL) {
-                    float4 *to = (float4 *)(p.part + ((size_t)un.index * PT + (row0 - un.row) + lane) * PT + (col - un.col));
+                    // through shared memory, so that 8 lanes write 128 bytes of a row
+                    __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        to[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
-                                            __uint_as_float(r[4 * i + 3]));
+                        *(uint4 *)(handed + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                    __syncwarp();
+                    float *to = p.part + ((size_t)un.index * PT + (row0 - un.row)) * PT + (col - un.col);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int at = i * 4 + (lane >> 3), q = lane & 7;
+                        *(uint4 *)(to + (size_t)at * PT + q * 4) = *(const uint4 *)(handed + at * 128 + ((q ^ (at & 7)) << 4));
+                    }
                 } else if constexpr (FORM == LAST) {
                     const int i0 = row0 + lane; // X's row: one of the result, or (tall) a column, 32 neighbours a store
                     __nv_bfloat16 *out = p.out + un.matrix * p.out_stride + (p.tall ? (long long)col * p.ld_out + i0 : (long long)i0 * p.ld_out + col);
@@ -396,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         }
                     }
                     if (c + 1 < PART / 32)
-                        residual(c + 1);
+                        fetch_low(c + 1);
                 } else {
                     const bool mirror = FORM != UPDATE && un.row != un.col;
                     const int other = block == BLOCKS - 1 ? 0 : block + 1;
@@ -435,19 +475,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         }
                         *(uint4 *)(first_block + lane * 64 + ((i ^ sw) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
                         if constexpr (FORM == UPDATE)
-                            *(uint4 *)(second + lane * 64 + ((i ^ sw) << 4)) = make_uint4(low[0], low[1], low[2], low[3]);
+                            if (there(c))
+                                lows[(c * 4 + i) * 32] = make_uint4(low[0], low[1], low[2], low[3]);
                     }
                     if (c + 1 < PART / 32)
-                        residual(c + 1);
+                        fetch_low(c + 1);
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
                         if (there(c))
                             tma_store_3d(&tmC, smem_u32(first_block), col, row0, un.matrix);
                         bulk_commit();
-                        if (there(c) && FORM == UPDATE)
-                            tma_store_3d(&tmD, smem_u32(second), col, row0, un.matrix);
-                        else if (there(c) && mirror)
+                        if (there(c) && mirror)
                             tma_store_3d(&tmC, smem_u32(second), row0, col, un.matrix);
                         bulk_commit();
                     }
@@ -579,7 +618,7 @@ static int half_map(CUtensorMap *tm, const void *base, int64_t cols, int64_t row
 }
 
 template <int FORM>
-static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, const CUtensorMap &C, const CUtensorMap &D, const ProductArgs &p)
+static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, const CUtensorMap &C, const ProductArgs &p)
 {
     static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
     const unsigned bit = 1u << (c.device & 15);
@@ -588,7 +627,7 @@ static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, con
         ready.fetch_or(bit);
     }
     const int pairs = std::min(sm_count(c.device) / 2, p.units);
-    TS2_LAUNCH((orth_product_kernel<FORM>), 2 * pairs, THREADS, SMEM, c.stream, A, B, C, D, p);
+    TS2_LAUNCH((orth_product_kernel<FORM>), 2 * pairs, THREADS, SMEM, c.stream, A, B, C, p);
     return TS2_OK;
 }
 
@@ -636,21 +675,25 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     const int split1 = choose_splits(pairs, (int64_t)batch * upper, mp / BK), split2 = choose_splits(pairs, (int64_t)batch * upper, np / BK);
     const int most = std::max(split1, split2);
     const size_t part_bytes = most > 1 ? (size_t)batch * upper * most * PT * PT * 4 : 0;
-    Scratch s(c, part_bytes + x * 6 + a * 4 + (size_t)batch * n_part * 8);
+    const size_t low_bytes = (size_t)batch * nt * mt * HALF_PIECES * 16;
+    Scratch s(c, part_bytes + low_bytes + x * 4 + a * 4 + (size_t)batch * n_part * 8);
     if (s.rc != TS2_OK)
         return s.rc;
     float *part = (float *)s.p;
-    __half *hi[2] = {(__half *)((uint8_t *)s.p + part_bytes), (__half *)((uint8_t *)s.p + part_bytes) + x}, *lo = hi[1] + x, *A = lo + x, *B = A + a;
+    uint4 *lows = (uint4 *)((uint8_t *)s.p + part_bytes);
+    __half *hi[2] = {(__half *)((uint8_t *)lows + low_bytes), (__half *)((uint8_t *)lows + low_bytes) + x}, *A = hi[1] + x, *B = A + a;
     double *sums = (double *)(B + a);
 
     const bool vec = ((uintptr_t)g | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(stride * sizeof(T))) % 16 == 0;
     TS2_LAUNCH((orth_sum2_kernel<T>), dim3(n_part, batch), 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums);
     const dim3 blocks(mp / 64, np / 64, batch);
     if (tall)
-        TS2_LAUNCH((orth_load_kernel<T, true>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lo);
+        TS2_LAUNCH((orth_load_kernel<T, true>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lows, mt,
+                   nt * mt);
     else
-        TS2_LAUNCH((orth_load_kernel<T, false>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lo);
-    CUtensorMap x_rows[2], x_cols[2], x_block[2], lo_block, a_rows, a_block, b_rows, b_block;
+        TS2_LAUNCH((orth_load_kernel<T, false>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lows, mt,
+                   nt * mt);
+    CUtensorMap x_rows[2], x_cols[2], x_block[2], a_rows, a_block, b_rows, b_block;
     int rc = TS2_OK;
     for (int i = 0; i < 2 && rc == TS2_OK; ++i) {
         rc = half_map(&x_rows[i], hi[i], mp, np, batch, 64, 128);
@@ -659,7 +702,7 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
         if (rc == TS2_OK)
             rc = half_map(&x_block[i], hi[i], mp, np, batch, 32, 32);
     }
-    if (rc != TS2_OK || (rc = half_map(&lo_block, lo, mp, np, batch, 32, 32)) || (rc = half_map(&a_rows, A, np, np, batch, 64, 128)) ||
+    if (rc != TS2_OK || (rc = half_map(&a_rows, A, np, np, batch, 64, 128)) ||
         (rc = half_map(&a_block, A, np, np, batch, 32, 32)) || (rc = half_map(&b_rows, B, np, np, batch, 64, 128)) ||
         (rc = half_map(&b_block, B, np, np, batch, 32, 32)))
         return rc;
@@ -668,13 +711,14 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     if (!p.status)
         return fail(TS2_ERR_CUDA, "no device status word");
     p.n = np;
+    p.lo = lows;
     p.part = part;
     const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &to, __half *dst) {
         p.cols = np, p.tiles = upper, p.col_tiles = 0;
         p.k_blocks = k / BK, p.splits = splits, p.kb_per_split = (int)ceil_div(p.k_blocks, splits), p.units = batch * upper * splits;
         if (splits == 1)
-            return poly ? product<POLY>(c, in, in, to, to, p) : product<SQUARE>(c, in, in, to, to, p);
-        if (int e = product<PARTIAL>(c, in, in, to, to, p))
+            return poly ? product<POLY>(c, in, in, to, p) : product<SQUARE>(c, in, in, to, p);
+        if (int e = product<PARTIAL>(c, in, in, to, p))
             return e;
         TS2_LAUNCH(orth_join_kernel, dim3(16, upper, batch), 256, 0, c.stream, part, p, poly ? A : (const __half *)nullptr, dst);
         return TS2_OK;
@@ -687,14 +731,14 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
         p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA, p.res = A;
         if ((rc = symmetric(true, np, split2, a_rows, b_block, B)))
             return rc;
-        p.alpha = 1.f / SB, p.beta = coef[0], p.res = hi[now], p.res_lo = lo;
+        p.alpha = 1.f / SB, p.beta = coef[0], p.res = hi[now];
         p.cols = mp, p.tiles = nt * mt, p.col_tiles = mt, p.k_blocks = np / BK, p.splits = 1, p.kb_per_split = p.k_blocks, p.units = batch * nt * mt;
         if (k == steps - 1) {
             p.out = out, p.ld_out = ld_out, p.out_stride = out_stride, p.out_rows = rows, p.out_cols = cols, p.out_scale = out_scale / SX, p.tall = tall;
             p.vec_out = ((uintptr_t)out | (uintptr_t)(ld_out * 2) | (uintptr_t)(out_stride * 2)) % 16 == 0;
         }
-        if ((rc = k < steps - 1 ? product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], lo_block, p)
-                                : product<LAST>(c, b_rows, x_cols[now], x_block[now ^ 1], lo_block, p)))
+        if ((rc = k < steps - 1 ? product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], p)
+                                : product<LAST>(c, b_rows, x_cols[now], x_block[now ^ 1], p)))
             return rc;
     }
     return TS2_OK;

@@ -6,7 +6,8 @@
 // The products are fp16 with fp32 sums on the tensor cores.  X itself is kept in 32 bits, as two halves: small singular values
 // are carried by the term a X and grow by a factor a in every step, so one rounding of X to 16 bits grows with them (a spectrum
 // that falls off as 1/k^2, 512 x 1024, coefficients 3.4445, -4.7750, 2.0315, 5 steps: relative error 2.0e-2 with X in fp16,
-// 1.8e-4 with X in two halves; flat spectra 2.0e-3 and 1.3e-3).  All fp16 values are scaled by powers of two that keep them
+// 1.8e-4 with X in two halves; flat spectra 2.0e-3 and 1.3e-3).  For the same reason the diagonal of B, which is its largest part, stays in fp32 beside the zeros
+// of the operand: X = (a + diagonal) X + B X (flat spectra 1.3e-3 -> 0.8e-3).  All fp16 values are scaled by powers of two that keep them
 // below 65504 for every X the coefficients can reach (orth_check).
 #include "orth.cuh"
 #include "pair_ptx.cuh"
@@ -157,6 +158,7 @@ struct ProductArgs {
     float *part;       // PARTIAL: [matrix][tile][split][256][256]
     const __half *res; // A, or the high halves of X
     uint4 *lo;         // the low halves, [matrix][tile of X] in the order of lane_piece
+    float *diag;       // [matrix][n]: the diagonal of B
     // LAST
     __nv_bfloat16 *out;
     long long ld_out, out_stride;
@@ -362,6 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             };
             fetch(0);
             fetch_low(0);
+            const float beta = p.beta + (RES == 2 && there(0) ? p.diag[(size_t)un.matrix * p.n + row0 + lane] : 0.f);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag)))
                 break;
             tc_fence_after();
@@ -407,8 +410,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         *(uint4 *)(to + (size_t)at * PT + q * 4) = *(const uint4 *)(handed + at * 128 + ((q ^ (at & 7)) << 4));
                     }
                 } else if constexpr (FORM == LAST) {
-                    const int i0 = row0 + lane; // X's row: one of the result, or (tall) a column, 32 neighbours a store
-                    __nv_bfloat16 *out = p.out + un.matrix * p.out_stride + (p.tall ? (long long)col * p.ld_out + i0 : (long long)i0 * p.ld_out + col);
+                    const int i0 = row0 + lane; // X's row: (tall) a column of the result, 32 neighbours a store
+                    __nv_bfloat16 *out = p.out + un.matrix * p.out_stride;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) { // 8 columns
                         const uint32_t xw[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w}, lw[4] = {ls[i].x, ls[i].y, ls[i].z, ls[i].w};
@@ -416,24 +419,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const float2 x = __half22float2(*(const __half2 *)&xw[j]), l = __half22float2(*(const __half2 *)&lw[j]);
-                            const float v0 = fmaf(p.beta, fmaf(l.x, 1.f / LO, x.x), p.alpha * __uint_as_float(r[8 * i + 2 * j]));
-                            const float v1 = fmaf(p.beta, fmaf(l.y, 1.f / LO, x.y), p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]));
+                            const float v0 = fmaf(beta, fmaf(l.x, 1.f / LO, x.x), p.alpha * __uint_as_float(r[8 * i + 2 * j]));
+                            const float v1 = fmaf(beta, fmaf(l.y, 1.f / LO, x.y), p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]));
                             o[j] = __floats2bfloat162_rn(v0 * p.out_scale, v1 * p.out_scale);
                         }
                         if (p.tall) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
                                 if (i0 < p.out_cols && col + 8 * i + j < p.out_rows)
-                                    out[(8 * i + j) * p.ld_out] = j & 1 ? __high2bfloat16(o[j / 2]) : __low2bfloat16(o[j / 2]);
-                        } else if (i0 < p.out_rows) {
-                            if (p.vec_out && col + 8 * i + 8 <= p.out_cols)
-                                *(uint4 *)(out + 8 * i) = make_uint4(*(uint32_t *)&o[0], *(uint32_t *)&o[1], *(uint32_t *)&o[2], *(uint32_t *)&o[3]);
-                            else
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    if (col + 8 * i + j < p.out_cols)
-                                        out[8 * i + j] = j & 1 ? __high2bfloat16(o[j / 2]) : __low2bfloat16(o[j / 2]);
+                                    out[(long long)(col + 8 * i + j) * p.ld_out + i0] = j & 1 ? __high2bfloat16(o[j / 2]) : __low2bfloat16(o[j / 2]);
+                        } else {
+                            *(uint4 *)(blocks + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4)) =
+                                make_uint4(*(uint32_t *)&o[0], *(uint32_t *)&o[1], *(uint32_t *)&o[2], *(uint32_t *)&o[3]);
                         }
+                    }
+                    if (!p.tall && c & 1) { // 32 rows x 64 by rows
+                        __syncwarp();
+                        const int left = col - 32, right = min(p.out_cols - left, 64);
+                        if (p.vec_out) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int at = i * 4 + (lane >> 3), q = lane & 7;
+                                const uint4 eight = *(const uint4 *)(blocks + at * 128 + ((q ^ (at & 7)) << 4));
+                                __nv_bfloat16 *to = out + (long long)(row0 + at) * p.ld_out + left + q * 8;
+                                if (row0 + at >= p.out_rows)
+                                    continue;
+                                if (q * 8 + 8 <= right)
+                                    *(uint4 *)to = eight;
+                                else
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j)
+                                        if (q * 8 + j < right)
+                                            to[j] = ((const __nv_bfloat16 *)&eight)[j];
+                            }
+                        } else {
+                            for (int at = 0; at < 32 && row0 + at < p.out_rows; ++at)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const int k = h * 32 + lane;
+                                    if (k < right)
+                                        out[(long long)(row0 + at) * p.ld_out + left + k] =
+                                            *(const __nv_bfloat16 *)(blocks + at * 128 + (((k >> 3) ^ (at & 7)) << 4) + (k & 7) * 2);
+                                }
+                        }
+                        __syncwarp();
                     }
                     if (c + 1 < PART / 32)
                         fetch_low(c + 1);
@@ -458,8 +487,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                     const float2 l = __half22float2(*(const __half2 *)&lw[j]);
                                     x.x = fmaf(l.x, 1.f / LO, x.x), x.y = fmaf(l.y, 1.f / LO, x.y);
                                 }
-                                v0 = fmaf(p.beta, x.x, v0), v1 = fmaf(p.beta, x.y, v1);
+                                v0 = fmaf(beta, x.x, v0), v1 = fmaf(beta, x.y, v1);
                             }
+                            if constexpr (FORM == POLY)
+                                if (row0 == col && lane >> 1 == 4 * i + j) { // on the diagonal
+                                    if (there(c))
+                                        p.diag[(size_t)un.matrix * p.n + row0 + lane] = (lane & 1 ? v1 : v0) * (1.f / SB);
+                                    (lane & 1 ? v1 : v0) = 0.f;
+                                }
                             const __half2 h = sat_half2(v0, v1);
                             out[j] = *(const uint32_t *)&h;
                             if constexpr (FORM == UPDATE) {
@@ -541,7 +576,11 @@ __global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict_
         alignas(16) __half o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float v = a ? fmaf(p.beta, __half2float(((const __half *)&old)[j]), p.alpha * sum[j]) : p.alpha * sum[j];
+            float v = a ? fmaf(p.beta, __half2float(((const __half *)&old)[j]), p.alpha * sum[j]) : p.alpha * sum[j];
+            if (a && row + i == col + c8 + j) {
+                p.diag[(size_t)blockIdx.z * p.n + row + i] = v * (1.f / SB);
+                v = 0.f;
+            }
             tile[i][c8 + j] = v;
             o[j] = __low2half(sat_half2(v, v));
         }
@@ -676,7 +715,7 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     const int most = std::max(split1, split2);
     const size_t part_bytes = most > 1 ? (size_t)batch * upper * most * PT * PT * 4 : 0;
     const size_t low_bytes = (size_t)batch * nt * mt * HALF_PIECES * 16;
-    Scratch s(c, part_bytes + low_bytes + x * 4 + a * 4 + (size_t)batch * n_part * 8);
+    Scratch s(c, part_bytes + low_bytes + x * 4 + a * 4 + (size_t)batch * n_part * 8 + (size_t)batch * np * 4);
     if (s.rc != TS2_OK)
         return s.rc;
     float *part = (float *)s.p;
@@ -711,7 +750,7 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     if (!p.status)
         return fail(TS2_ERR_CUDA, "no device status word");
     p.n = np;
-    p.lo = lows;
+    p.lo = lows, p.diag = (float *)(sums + (size_t)batch * n_part);
     p.part = part;
     const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &to, __half *dst) {
         p.cols = np, p.tiles = upper, p.col_tiles = 0;

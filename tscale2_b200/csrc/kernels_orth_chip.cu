@@ -2,7 +2,7 @@
 // and without memory in between: a cluster holds a matrix.  Each CTA has the 128 rows (padded with zeros) of up to 384 columns of X:
 // as fp32 in tensor memory, thread = row, and rounded to fp16 in shared memory as the operand of the products
 //     A = X X^T   (the CTAs' parts are added through distributed shared memory, each 128 / cluster rows for all)
-//     B = b A + c A A   (every CTA for itself)      X = a X + B X   (128 columns at a time)
+//     B = b A + c A A   (every CTA for itself)      X = a X + B X   (128 columns at a time; the diagonal of B in fp32)
 // A chain of small products: its latency is the bound.  As 15 launches of kernels_orth.cu 128 x 256 took 127 us.
 #include "kernels.cuh"
 #include "orth.cuh"
@@ -16,7 +16,7 @@ constexpr int THREADS = 256, MAX_CHUNKS = 3, MAX_CLUSTER = 16;
 constexpr int BLK = 128 * 128;   // 128 rows x 64 columns of fp16, 128-byte swizzle
 constexpr int PITCH = 129;       // fp32 staging of 128 x 128
 constexpr int A_OFF = MAX_CHUNKS * 2 * BLK, B_OFF = A_OFF + 2 * BLK, STG_OFF = B_OFF + 2 * BLK, END_OFF = STG_OFF + 128 * PITCH * 4;
-constexpr int SMEM = END_OFF + 256 + 1024;
+constexpr int SMEM = END_OFF + 128 + 512 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 constexpr uint32_t WORK = MAX_CHUNKS * 128; // tensor-memory columns of the product at hand; X's chunks lie before it
 
@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
     uint32_t *tmem_slot = (uint32_t *)(bar_at + 1);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     double *sums = (double *)(smem + END_OFF + 32); // a warp's, the CTA's
+    float *diag = (float *)(smem + END_OFF + 128);  // of B
     const uint32_t bar = smem_u32(bar_at);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
@@ -287,6 +288,12 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                     v[8 * i + 2 * k + 1] = fmaf(kb, f.y, kc * v[8 * i + 2 * k + 1]);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (row == half * 64 + h * 32 + i) {
+                    diag[row] = v[i] * (1.f / ORTH_SB);
+                    v[i] = 0.f;
+                }
             put_half(smem + B_OFF, row, half * 2 + h, v);
         }
         const bool last = step == p.steps - 1;
@@ -312,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                 load32(q * 128 + h * 32, x);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    v[i] = fmaf(p.a, x[i], v[i] * (1.f / ORTH_SB));
+                    v[i] = fmaf(p.a + diag[row], x[i], v[i] * (1.f / ORTH_SB));
                 if (last) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)

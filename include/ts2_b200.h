@@ -534,7 +534,8 @@ int ts2_op_attention_backward_limited(int device, void *stream, int variant, con
  * [seq_ptr[s], seq_ptr[s + 1]), possibly none; null: one sequence (n_seq 1) over all T nodes.  Nodes before the first and
  * behind the last sequence are left as they were.  h0 (optional): fp32 [n_seq][D], the state before each sequence's first node
  * (zero without it); h_last (optional): fp32 [n_seq][D], the state behind its last one, h0's where a sequence is empty.  A
- * sequence of one token with h0 and h_last is a step of generation.  States are fp32 inside a call.  T up to 2^30. */
+ * sequence of one token with h0 and h_last is a step of generation.  States are fp32 inside a call.  T and n_seq up to 2^30, D up to
+ * 65535 * 64. */
 int ts2_op_recurrence_forward(int device, void *stream, int type, const void *gate, int64_t gate_ld, const void *x, int64_t x_ld, int T, int D,
                               int n_seq, const int32_t *seq_ptr, const float *h0, void *h, int64_t h_ld, float *h_last);
 /* Its backward pass: h is what the forward call left; dh [T][D] the gradient of h, dh_last (optional) that of h_last ->
@@ -550,7 +551,7 @@ int ts2_op_recurrence_backward(int device, void *stream, int type, const void *g
  * ids int32 [T][selected], an id outside [0, expert_count) is a choice not made; token_mask (optional) [T]: tokens with a zero
  * byte do not count, whatever their logits and ids are.  A row of logits that is -inf throughout has no probabilities, but its
  * token counts.  counts: int32 [expert_count + 1], C and behind it N; prob fp32 [expert_count]; loss fp32 [1].
- * expert_count up to 1024, T up to 2^30, T * selected below 2^31. */
+ * expert_count up to 1024, selected up to expert_count, T up to 2^30, T * selected below 2^31. */
 int ts2_op_moe_balance_forward(int device, void *stream, int type, const void *logits, int64_t ld, int64_t T, int expert_count, int selected,
                                const int32_t *ids, const uint8_t *token_mask, int32_t *counts, float *prob, float *loss);
 /* dlogits[t][e] (+)= *dloss * scale * expert_count / (selected N^2) p[t][e] (C[e] - sum_j C[j] p[t][j]), the gradient of that
@@ -566,7 +567,7 @@ int ts2_op_moe_balance_backward(int device, void *stream, int type, const void *
  * singular values to about one.  g: [batch] matrices [rows][cols] of `type`, rows of ld elements, g_stride elements apart (may
  * be 0); out: bf16, alike (out_ld, out_stride); out may be g itself where type is TS2_OUT_BF16 and the pitches agree.  A zero
  * matrix gives zeros, one with a NaN or an infinity NaNs; the scale of g does not matter.  Products are fp16 with fp32 sums, the
- * iterate is held in 32 bits: the result is within 2e-3 (relative L2, before its rounding to bf16) of the formula for the usual
+ * iterate is held in 32 bits: the result is within 1.5e-3 (relative L2, before its rounding to bf16) of the formula for the usual
  * coefficients (3.4445, -4.7750, 2.0315), 5 steps.  TS2_ERR_UNSUPPORTED for coefficients that take a singular value beyond 3.9, which
  * the fp16 scaling does not allow.  Up to 64 steps, 65535 matrices, 2^20 rows and columns. */
 int ts2_op_orthogonalize(int device, void *stream, int type, const void *g, int64_t ld, int64_t g_stride, int batch, int64_t rows, int64_t cols,

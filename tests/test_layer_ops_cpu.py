@@ -32,7 +32,7 @@ def refused(lib, name, args, rc=capi.TS2_ERR_INVALID_ARG, **change):
     assert name.split("_op_")[1].split("_")[0].encode() in lib.ts2_last_error(None)
 
 
-@pytest.mark.parametrize("change", [dict(type=1), dict(type=7), dict(type=-1), dict(T=-1), dict(T=(1 << 30) + 1), dict(D=0), dict(D=-5), dict(n_seq=-1),
+@pytest.mark.parametrize("change", [dict(type=1), dict(type=7), dict(type=-1), dict(T=-1), dict(T=(1 << 30) + 1), dict(D=0), dict(D=-5), dict(D=65535 * 64 + 1), dict(n_seq=-1), dict(n_seq=(1 << 30) + 1),
                                     dict(ptr=None), dict(gate=None), dict(x=None), dict(h=None), dict(gate_ld=7), dict(x_ld=7), dict(h_ld=7),
                                     dict(gate_ld=BIG), dict(gate=P + 1), dict(x=P + 1), dict(h=P + 1), dict(h0=P + 2), dict(h_last=P + 2),
                                     dict(ptr=P + 1), dict(type=F32, x=P + 2)])
@@ -47,14 +47,14 @@ def test_recurrence_backward(lib, change):
     refused(lib, "ts2_op_recurrence_backward", BACKWARD, **change)
 
 
-@pytest.mark.parametrize("change", [dict(type=1), dict(T=-1), dict(E=0), dict(k=0), dict(logits=None), dict(ids=None), dict(counts=None), dict(prob=None),
+@pytest.mark.parametrize("change", [dict(type=1), dict(T=-1), dict(E=0), dict(k=0), dict(k=9), dict(logits=None), dict(ids=None), dict(counts=None), dict(prob=None),
                                     dict(loss=None), dict(ld=7), dict(ld=BIG), dict(logits=P + 2), dict(ids=P + 1), dict(counts=P + 2),
                                     dict(prob=P + 1), dict(loss=P + 2), dict(T=1 << 30, k=2), dict(T=(1 << 30) + 1)])
 def test_balance_forward(lib, change):
     refused(lib, "ts2_op_moe_balance_forward", BALANCE, **change)
 
 
-@pytest.mark.parametrize("change", [dict(type=1), dict(T=-1), dict(E=0), dict(k=0), dict(logits=None), dict(counts=None), dict(dl=None), dict(dl_ld=7),
+@pytest.mark.parametrize("change", [dict(type=1), dict(T=-1), dict(E=0), dict(k=0), dict(k=9), dict(logits=None), dict(counts=None), dict(dl=None), dict(dl_ld=7),
                                     dict(ld=7), dict(dl=P + 2), dict(logits=P + 2), dict(counts=P + 1), dict(dloss=P + 2)])
 def test_balance_backward(lib, change):
     refused(lib, "ts2_op_moe_balance_backward", GRADIENT, **change)

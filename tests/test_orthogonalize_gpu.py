@@ -1,7 +1,7 @@
 """The orthogonalised update (ts2_op_orthogonalize) against its formula in float64.
 
-Tolerance: `modelled` computes the formula in float64 with the roundings that the kernels make (X in two halves, the operands of
-the three products in fp16), which says how far these roundings alone carry a result; another order of fp32 sums moves single
+Tolerance: `modelled` computes the formula in float64 with the roundings that the kernels make (X and the diagonal of B in 32 bits, the
+operands of the three products in fp16), which says how far these roundings alone carry a result; another order of fp32 sums moves single
 roundings, so a right kernel is within twice that of the formula, and the final rounding to bf16 adds 2^-8 of an element at most
 (relative L2: 2^-8 / sqrt(3), the mean square of a uniform error)."""
 import ctypes as C
@@ -32,8 +32,9 @@ def exact(g, coef=COEF, steps=5, rounded=False):
     for _ in range(steps):
         h = half(x, 2.0 ** 14)
         a = half(h @ h.T, 2.0 ** 12)
-        b = half(coef[1] * a + coef[2] * (a @ a), 2.0 ** 11)
-        x = coef[0] * x + b @ h
+        b = coef[1] * a + coef[2] * (a @ a)
+        d = np.diag(b).copy() if rounded else np.zeros(len(b))
+        x = (coef[0] + d)[:, None] * x + half(b - np.diag(d), 2.0 ** 11) @ h
     return x.T if tall else x
 
 

@@ -161,6 +161,12 @@ def test_against_the_formula(kind, T, D, n, carry):
     Case(kind, T, D, cut(T, n, T + D), carry, seed=T * D).verify()
 
 
+@pytest.mark.parametrize("kind,T,D,n,carry", [("f16", 20000, 24, 30, True), ("bf16", 20000, 23, 3, True), ("f32", 15000, 22, 1, True),
+                                              ("f16", 9000, 130, 400, False), ("f32", 12000, 65, 1, False)])
+def test_long_arrays_in_segments(kind, T, D, n, carry):
+    Case(kind, T, D, cut(T, n, n + D, first=3, pad=5), carry, seed=T + D).verify()
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_one_sequence_without_a_table(kind):
     Case(kind, 500, 70, [0, 500], True, seed=3).verify(null_ptr=True)

@@ -49,7 +49,7 @@ int ts2_op_recurrence_forward(int device, void *stream, int type, const void *ga
                               int n_seq, const int32_t *seq_ptr, const float *h0, void *h, int64_t h_ld, float *h_last)
 {
     const int es = type_size(type);
-    if (!es || T < 0 || T > 1 << 30 || D < 1 || n_seq < 0 || (!seq_ptr && n_seq != 1) || !rows_ok(gate, gate_ld, T, D, es) ||
+    if (!es || T < 0 || T > 1 << 30 || D < 1 || D > 65535 * 64 || n_seq < 0 || n_seq > 1 << 30 || (!seq_ptr && n_seq != 1) || !rows_ok(gate, gate_ld, T, D, es) ||
         !rows_ok(x, x_ld, T, D, es) || !rows_ok(h, h_ld, T, D, es) || !floats_ok(seq_ptr) || !floats_ok(h0) || !floats_ok(h_last))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_recurrence_forward: bad arguments");
     TS2_ON_DEVICE(device);
@@ -63,7 +63,7 @@ int ts2_op_recurrence_backward(int device, void *stream, int type, const void *g
                                const float *dh_last, void *dgate, int64_t dgate_ld, void *dx, int64_t dx_ld, float *dh0)
 {
     const int es = type_size(type);
-    if (!es || T < 0 || T > 1 << 30 || D < 1 || n_seq < 0 || (!seq_ptr && n_seq != 1) || !rows_ok(gate, gate_ld, T, D, es) ||
+    if (!es || T < 0 || T > 1 << 30 || D < 1 || D > 65535 * 64 || n_seq < 0 || n_seq > 1 << 30 || (!seq_ptr && n_seq != 1) || !rows_ok(gate, gate_ld, T, D, es) ||
         !rows_ok(x, x_ld, T, D, es) || !rows_ok(h, h_ld, T, D, es) || !rows_ok(dh, dh_ld, T, D, es) || !rows_ok(dgate, dgate_ld, T, D, es) ||
         !rows_ok(dx, dx_ld, T, D, es) || !floats_ok(seq_ptr) || !floats_ok(h0) || !floats_ok(dh_last) || !floats_ok(dh0))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_recurrence_backward: bad arguments");
@@ -78,7 +78,7 @@ int ts2_op_moe_balance_forward(int device, void *stream, int type, const void *l
                                const int32_t *ids, const uint8_t *token_mask, int32_t *counts, float *prob, float *loss)
 {
     const int es = type_size(type);
-    if (!es || T < 0 || T > 1 << 30 || expert_count < 1 || selected < 1 || T * selected >= (int64_t)1 << 31 ||
+    if (!es || T < 0 || T > 1 << 30 || expert_count < 1 || selected < 1 || selected > expert_count || T * selected >= (int64_t)1 << 31 ||
         !rows_ok(logits, ld, T, expert_count, es) || (!ids && T) || !floats_ok(ids) || !counts || !prob || !loss || !floats_ok(counts) ||
         !floats_ok(prob) || !floats_ok(loss))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_moe_balance_forward: bad arguments");
@@ -91,7 +91,7 @@ int ts2_op_moe_balance_backward(int device, void *stream, int type, const void *
                                 int add)
 {
     const int es = type_size(type);
-    if (!es || T < 0 || T > 1 << 30 || expert_count < 1 || selected < 1 || !rows_ok(logits, ld, T, expert_count, es) || !counts ||
+    if (!es || T < 0 || T > 1 << 30 || expert_count < 1 || selected < 1 || selected > expert_count || !rows_ok(logits, ld, T, expert_count, es) || !counts ||
         !floats_ok(counts) || !floats_ok(dloss) || !rows_ok(dlogits, dlogits_ld, T, expert_count, es))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_moe_balance_backward: bad arguments");
     TS2_ON_DEVICE(device);

@@ -87,10 +87,12 @@ struct Row {
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = m == -INFINITY ? 0.f : m; // the difference first: it may be of the lowest finite values
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i)
-            sum += v[i] = expf(v[i] - ref);
+        for (int i = 0; i < VALUES; ++i) {
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[i]) : "f"((v[i] - ref) * 1.4426950408889634f));
+            sum += v[i];
+        }
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1)
             sum += __shfl_xor_sync(0xffffffffu, sum, o);

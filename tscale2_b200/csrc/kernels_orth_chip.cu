@@ -3,7 +3,9 @@
 // as fp32 in tensor memory, thread = row, and rounded to fp16 in shared memory as the operand of the products
 //     A = X X^T   (the CTAs' parts are added through distributed shared memory, each 128 / cluster rows for all)
 //     B = b A + c A A   (every CTA for itself)      X = a X + B X   (128 columns at a time; the diagonal of B in fp32)
-// A chain of small products: its latency is the bound.  As 15 launches of kernels_orth.cu 128 x 256 took 127 us.
+// A chain of small products: its latency is the bound, 5 us a step (a tenth of it tensor work), 10 us to bring G in and normalise it,
+// and with more than one CTA the exchange of A, 5 - 8 us a step.  128 x 256: 33 us, as 15 launches of kernels_orth.cu 127;
+// 128 x 4000 on a cluster of 16: 90.
 #include "kernels.cuh"
 #include "orth.cuh"
 #include <algorithm>
@@ -14,8 +16,7 @@ namespace {
 
 constexpr int THREADS = 256, MAX_CHUNKS = 3, MAX_CLUSTER = 16;
 constexpr int BLK = 128 * 128;   // 128 rows x 64 columns of fp16, 128-byte swizzle
-constexpr int PITCH = 129;       // fp32 staging of 128 x 128
-constexpr int A_OFF = MAX_CHUNKS * 2 * BLK, B_OFF = A_OFF + 2 * BLK, STG_OFF = B_OFF + 2 * BLK, END_OFF = STG_OFF + 128 * PITCH * 4;
+constexpr int A_OFF = MAX_CHUNKS * 2 * BLK, B_OFF = A_OFF + 2 * BLK, STG_OFF = B_OFF + 2 * BLK, END_OFF = STG_OFF + 128 * 128 * 4;
 constexpr int SMEM = END_OFF + 128 + 512 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 constexpr uint32_t WORK = MAX_CHUNKS * 128; // tensor-memory columns of the product at hand; X's chunks lie before it
@@ -56,6 +57,10 @@ __device__ __forceinline__ uint32_t in_rank(uint32_t addr, unsigned rank)
 }
 // 16-byte piece c (0 .. 15) of row r of 128 columns of fp16, as two swizzled blocks
 __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)((c >> 3) * BLK + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+
+// fp32 staging of 128 x 128: where 4 elements of row r from column c (a multiple of 4) on lie, so that neither 8 rows nor 8 pieces of a
+// row, nor every eighth row, meet in a bank
+__device__ __forceinline__ int staged(int r, int c) { return r * 128 + (((c >> 2) ^ ((r ^ (r >> 3)) & 7)) << 2); }
 
 // 32 values as fp16 to the columns [32 j, +32) of the thread's row
 __device__ __forceinline__ void put_half(uint8_t *base, int row, int j, const float (&v)[32])
@@ -113,6 +118,11 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         for (int i = 0; i < 32; ++i)
             v[i] = __uint_as_float(r[i]);
     };
+    const auto load64 = [&](uint32_t column, float (&v)[2][32]) { // the thread's half of 128 columns; tmem_ld_wait is the caller's
+        uint32_t(&r)[2][32] = (uint32_t(&)[2][32])v;
+        tmem_ld32(lane_base + column, r[0]);
+        tmem_ld32(lane_base + column + 32, r[1]);
+    };
     const auto store32 = [&](uint32_t column, const float (&v)[32]) {
         uint32_t r[32];
 #pragma unroll
@@ -121,32 +131,63 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         tmem_st32(lane_base + column, r);
     };
 
+    const auto staged32 = [&](int column, float (&v)[32]) { // of the thread's row
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 f = *(const float4 *)(stage + staged(row, column + 4 * i));
+            v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+        }
+    };
+    const auto stage32 = [&](int column, const float (&v)[32]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *(float4 *)(stage + staged(row, column + 4 * i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    };
+
     // ---- G -> X, unscaled, and its sum of squares (fp64: nothing over- or underflows) ----
     double sum = 0.;
     for (int q = 0; q < p.chunks; ++q) {
         const int j = j0 + q * 128, part = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
-#pragma unroll 4
+        float v[8][8]; // all loads of a chunk are on their way together
+#pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int r = (TALL ? j : 0) + part + 16 * k; // of G
-            float v[8];
             if (r < p.rows)
-                orth_load8(g + r * p.ld, (TALL ? 0 : j) + c8, p.cols, p.vec, v);
+                orth_load8(g + r * p.ld, (TALL ? 0 : j) + c8, p.cols, p.vec, v[k]);
             else
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    v[i] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                stage[TALL ? (c8 + i) * PITCH + part + 16 * k : (part + 16 * k) * PITCH + c8 + i] = v[i];
+                    v[k][i] = 0.f;
         }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (TALL) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    stage[staged(c8 + i, (part + 16 * k) & ~3) + (part & 3)] = v[k][i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i += 4)
+                    *(float4 *)(stage + staged(part + 16 * k, c8 + i)) = make_float4(v[k][i], v[k][i + 1], v[k][i + 2], v[k][i + 3]);
+            }
         __syncthreads();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float v[32];
+            float v[32], most = 0.f;
+            staged32(half * 64 + h * 32, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                v[i] = stage[row * PITCH + half * 64 + h * 32 + i];
-                sum = fma((double)v[i], (double)v[i], sum);
+            for (int i = 0; i < 32; ++i)
+                most = fmaxf(most, fabsf(v[i]));
+            if (most > 1e-12f && most < 1e15f) { // 32 squares that fp32 holds; a NaN among them makes the sum one
+                float four[4] = {};
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    four[i & 3] = fmaf(v[i], v[i], four[i & 3]);
+                sum += (double)((four[0] + four[1]) + (four[2] + four[3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    sum = fma((double)v[i], (double)v[i], sum);
             }
             store32(q * 128 + h * 32, v);
         }
@@ -222,19 +263,19 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
             }
         });
         constexpr float ALPHA = ORTH_SA / (ORTH_SX * ORTH_SX);
+        float w2[2][32];
+        load64(WORK, w2);
+        tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float v[32];
-            load32(WORK + h * 32, v);
+            float(&v)[32] = w2[h];
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 v[i] *= ALPHA;
             if (ranks == 1) {
                 put_half(smem + A_OFF, row, half * 2 + h, v);
             } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    stage[row * PITCH + half * 64 + h * 32 + i] = v[i];
+                stage32(half * 64 + h * 32, v);
             }
         }
         if (ranks > 1) {
@@ -242,16 +283,23 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
             const int rows_each = 128 / (int)ranks;
             for (int i = threadIdx.x; i < rows_each * 16; i += THREADS) {
                 const int r = (int)rank * rows_each + (i >> 4), c = i & 15;
-                const uint32_t at = smem_u32(stage + r * PITCH + c * 8);
+                const uint32_t at[2] = {smem_u32(stage + staged(r, c * 8)), smem_u32(stage + staged(r, c * 8 + 4))};
                 float v[8] = {};
-                for (unsigned k = 0; k < ranks; ++k) {
-                    const uint32_t from = in_rank(at, k);
+                for (unsigned k0 = 0; k0 < ranks; k0 += 2) { // in their order, two CTAs' loads at a time
+                    float4 f[2][2];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float f;
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(from + 4 * e) : "memory");
-                        v[e] += f;
-                    }
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(f[k][e].x), "=f"(f[k][e].y), "=f"(f[k][e].z), "=f"(f[k][e].w)
+                                         : "r"(in_rank(at[e], k0 + k))
+                                         : "memory");
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            v[4 * e] += f[k][e].x, v[4 * e + 1] += f[k][e].y, v[4 * e + 2] += f[k][e].z, v[4 * e + 3] += f[k][e].w;
                 }
                 uint32_t w[4];
 #pragma unroll
@@ -273,10 +321,11 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
             }
         });
         const float kb = ORTH_SB * p.b / ORTH_SA, kc = ORTH_SB * p.c / (ORTH_SA * ORTH_SA);
+        load64(WORK, w2);
+        tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float v[32];
-            load32(WORK + h * 32, v);
+            float(&v)[32] = w2[h];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint4 raw = *(const uint4 *)(smem + A_OFF + piece(row, (half * 2 + h) * 4 + i));
@@ -288,12 +337,14 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                     v[8 * i + 2 * k + 1] = fmaf(kb, f.y, kc * v[8 * i + 2 * k + 1]);
                 }
             }
+            if (quarter == half * 2 + h) { // the warp's 32 x 32 on the diagonal
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (row == half * 64 + h * 32 + i) {
-                    diag[row] = v[i] * (1.f / ORTH_SB);
-                    v[i] = 0.f;
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (lane == i) {
+                        diag[row] = v[i] * (1.f / ORTH_SB);
+                        v[i] = 0.f;
+                    }
+            }
             put_half(smem + B_OFF, row, half * 2 + h, v);
         }
         const bool last = step == p.steps - 1;
@@ -312,18 +363,23 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                 });
             else if (last)
                 __syncthreads(); // the staging of the chunk before has been read
+            float x2[2][32];
+            load64(at, w2);
+            load64(q * 128, x2);
+            const float beta = p.a + diag[row];
+            tmem_ld_wait();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float v[32], x[32];
-                load32(at + h * 32, v);
-                load32(q * 128 + h * 32, x);
+                float(&v)[32] = w2[h];
+                const float(&x)[32] = x2[h];
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    v[i] = fmaf(p.a + diag[row], x[i], v[i] * (1.f / ORTH_SB));
+                    v[i] = fmaf(beta, x[i], v[i] * (1.f / ORTH_SB));
                 if (last) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        stage[row * PITCH + half * 64 + h * 32 + i] = v[i] * (p.out_scale / ORTH_SX);
+                        v[i] *= p.out_scale / ORTH_SX;
+                    stage32(half * 64 + h * 32, v);
                 } else {
                     store32(q * 128 + h * 32, v);
                     put_half(smem + q * 2 * BLK, row, half * 2 + h, v);
@@ -342,7 +398,8 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                 alignas(16) __nv_bfloat16 o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    o[i] = __float2bfloat16_rn(stage[TALL ? (c8 + i) * PITCH + part + 16 * k : (part + 16 * k) * PITCH + c8 + i]);
+                    o[i] = __float2bfloat16_rn(TALL ? stage[staged(c8 + i, (part + 16 * k) & ~3) + (part & 3)]
+                                                    : stage[staged(part + 16 * k, c8 + (i & 4)) + (i & 3)]);
                 if (p.vec_out && c + 8 <= p.cols) {
                     *(uint4 *)(out + r * p.ld_out + c) = *(uint4 *)o;
                 } else {
@@ -406,6 +463,8 @@ int orth_chip_ranks(int rows, int cols)
     if (std::min(rows, cols) > 128)
         return 0;
     const int64_t chunks = ceil_div(std::max(rows, cols), 128);
+    // as few as hold it: more CTAs with fewer chunks each save less than the exchange of A costs (100 x 384 in one 47 us, in two 55;
+    // 200 matrices of 128 x 300 117 and 194; only 100 x 700 gains, in four instead of two 77 -> 72)
     for (int ranks = 1; ranks <= MAX_CLUSTER; ranks *= 2)
         if (chunks <= (int64_t)ranks * MAX_CHUNKS)
             return ranks;

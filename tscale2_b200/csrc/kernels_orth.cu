@@ -27,7 +27,7 @@ __device__ __forceinline__ void split(float x, __half &hi, __half &lo)
     lo = __low2half(sat_half2(r, r));
 }
 
-constexpr int PT = 256, BK = 64, HALF = 128 * 128, STAGE = 2 * HALF; // HALF: a CTA's part of an operand, one K block
+constexpr int PT = 256, BK = 64, HALF = 128 * 128; // HALF: a CTA's part of the first operand, one K block
 // Order of the low halves of a tile of 256 x 256: [CTA of the pair][epilogue warp][block of 32 columns][piece of 8][lane = row]
 constexpr int HALF_PIECES = PT * PT / 8;
 __device__ __forceinline__ int lane_piece(int row, int col) // of the piece at column col
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------------
-// Pairs of CTAs on tiles of 256 x 256 (as in gemm_pair.cu), one launch for a product of every matrix of the batch.
+// Pairs of CTAs on tiles of 256 x 256 or 256 x 128 (as in gemm_pair.cu), one launch for a product of every matrix of the batch.
 //   SQUARE  A = X X^T     POLY  B = b A + c A A     both operands K-contiguous; symmetric, so only tiles on and above the diagonal are
 //                         computed, and what is above it leaves a second time as its transpose
 //   UPDATE  X = a X + B X   B is K-contiguous (it is its own transpose), X is contiguous along N; writes the high halves to a second
@@ -144,9 +144,8 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
 enum Form { SQUARE, POLY, UPDATE, PARTIAL, LAST };
 constexpr bool updates(int form) { return form == UPDATE || form == LAST; }
 constexpr int STAGES = 5, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS, BLOCKS = 2;
-constexpr int PART = PT / (EPI_WARPS / 4); // columns of an epilogue warp
 // an epilogue warp's shared memory: two blocks of 32 x 32 on their way out, 32 x 64 of the residual input
-constexpr int BLOCK = 2048, WARP_BYTES = BLOCKS * BLOCK + 4096, STG_OFF = STAGES * STAGE, BAR_OFF = STG_OFF + EPI_WARPS * WARP_BYTES,
+constexpr int BLOCK = 2048, WARP_BYTES = BLOCKS * BLOCK + 4096, STG_OFF = STAGES * 2 * HALF, BAR_OFF = STG_OFF + EPI_WARPS * WARP_BYTES,
               SMEM = BAR_OFF + 1024 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 
@@ -157,7 +156,8 @@ struct ProductArgs {
     float alpha, beta; // POLY: alpha acc + beta A; UPDATE: alpha acc + beta X; else alpha acc
     float *part;       // PARTIAL: [matrix][tile][split][256][256]
     const __half *res; // A, or the high halves of X
-    uint4 *lo;         // the low halves, [matrix][tile of X] in the order of lane_piece
+    uint4 *lo;         // the low halves, [matrix][tile of 256 x 256 of X] in the order of lane_piece
+    int low_tiles, low_cols;
     float *diag;       // [matrix][n]: the diagonal of B
     // LAST
     __nv_bfloat16 *out;
@@ -168,7 +168,7 @@ struct ProductArgs {
     int32_t *status;
 };
 struct Unit {
-    int matrix, tile, row, col, kb0, kb1, index;
+    int matrix, row, col, kb0, kb1, index;
 };
 // the r-th tile on or above the diagonal of a square of tiles, column by column
 __device__ __forceinline__ void upper_tile(int r, int &row, int &col)
@@ -180,30 +180,38 @@ __device__ __forceinline__ void upper_tile(int r, int &row, int &col)
         ++col;
     row = r - col * (col + 1) / 2;
 }
-template <int FORM>
+template <int FORM, int PN>
 __device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
 {
     Unit t;
     const int tile = u / p.splits, split = u - tile * p.splits;
     t.index = u;
     t.matrix = tile / p.tiles;
-    const int r = t.tile = tile - t.matrix * p.tiles;
+    const int r = tile - t.matrix * p.tiles;
     if (updates(FORM))
         t.row = r / p.col_tiles, t.col = r - t.row * p.col_tiles;
-    else
+    else if (PN == PT) {
         upper_tile(r, t.row, t.col);
-    t.row *= PT, t.col *= PT;
+    } else { // p.col_tiles - 2 row of them in a row of tiles
+        int i = r;
+        for (t.row = 0; i >= p.col_tiles - 2 * t.row; ++t.row)
+            i -= p.col_tiles - 2 * t.row;
+        t.col = 2 * t.row + i;
+    }
+    t.row *= PT, t.col *= PN;
     t.kb0 = split * p.kb_per_split;
     t.kb1 = min(p.k_blocks, t.kb0 + p.kb_per_split);
     return t;
 }
 
-// tmA, tmB: boxes of 128 rows x 64 (UPDATE, LAST: tmB 64 rows x 64); tmC: the output, boxes of 32 rows x 32, 64-byte swizzle
-template <int FORM>
+// PN: columns of a tile.  tmA, tmB: boxes of 128 rows x 64 (tmB of UPDATE, LAST and PN = 128: 64 rows x 64); tmC: the output, boxes of
+// 32 rows x 32, 64-byte swizzle
+template <int FORM, int PN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
                         const ProductArgs p)
 {
+    constexpr int STAGE = HALF + PN * 64, PART = PN / 2; // bytes; columns of an epilogue warp
     constexpr int RES = FORM == POLY ? 1 : updates(FORM) ? 2 : 0; // residual arrays
     extern __shared__ uint8_t orth_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)orth_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
@@ -248,8 +256,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             uint32_t phase = 0;
             bool ok = true;
             for (int u = first; u < p.units && ok; u += step) {
-                const Unit un = product_unit<FORM>(p, u);
-                const int am = un.row + (int)rank * 128, bn = un.col + (int)rank * 128;
+                const Unit un = product_unit<FORM, PN>(p, u);
+                const int am = un.row + (int)rank * 128, bn = un.col + (int)rank * (PN / 2);
                 for (int kb = un.kb0; kb < un.kb1; ++kb) {
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
                         ok = false;
@@ -262,7 +270,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     tma_load_3d_pair(sa, &tmA, fb, kb * BK, am, un.matrix);
                     if constexpr (updates(FORM)) {
                         tma_load_3d_pair(sb, &tmB, fb, bn, kb * BK, un.matrix);
-                        tma_load_3d_pair(sb + BK * 128, &tmB, fb, bn + 64, kb * BK, un.matrix);
+                        if (PN == PT)
+                            tma_load_3d_pair(sb + BK * 128, &tmB, fb, bn + 64, kb * BK, un.matrix);
                     } else {
                         tma_load_3d_pair(sb, &tmB, fb, kb * BK, bn, un.matrix);
                     }
@@ -290,12 +299,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     } else if (warp == 1) {
         // MMA issuer (leader)
         if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = (1u << 4) | ((updates(FORM) ? 1u : 0u) << 16) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
+            constexpr uint32_t idesc = (1u << 4) | ((updates(FORM) ? 1u : 0u) << 16) | ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             for (int u = first; u < p.units && ok; u += step) {
-                const Unit un = product_unit<FORM>(p, u);
+                const Unit un = product_unit<FORM, PN>(p, u);
                 if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag))
                     break;
                 tc_fence_after();
@@ -338,7 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         int acc = 0, block = 0;
         uint32_t acc_phase = 0;
         for (int u = first; u < p.units; u += step) {
-            const Unit un = product_unit<FORM>(p, u);
+            const Unit un = product_unit<FORM, PN>(p, u);
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PT + part * PART;
             const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
             const auto there = [&](int c) { return row0 < p.n && col0 + c * 32 < p.cols; }; // multiples of 32: a block is there or not
@@ -353,7 +362,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         rows[i] = *(const uint4 *)(from + (size_t)(4 * i) * p.cols);
                 }
             };
-            uint4 *const lows = p.lo + ((size_t)un.matrix * p.tiles + un.tile) * HALF_PIECES + lane_piece(row0 - un.row + lane, part * PART);
+            uint4 *const lows = p.lo + ((size_t)un.matrix * p.low_tiles + un.row / PT * p.low_cols + un.col / PT) * HALF_PIECES +
+                               lane_piece(row0 - un.row + lane, un.col % PT + part * PART);
             const auto fetch_low = [&](int c) {
                 if constexpr (RES == 2)
                     if (there(c)) {
@@ -388,7 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                             *(uint4 *)(handed + at * 128 + (((lane & 7) ^ (at & 7)) << 4)) = rows[i];
                         }
                         __syncwarp();
-                        if (c == 0)
+                        if (c == 0 && PART > 64)
                             fetch(1);
                     }
 #pragma unroll
@@ -467,7 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (c + 1 < PART / 32)
                         fetch_low(c + 1);
                 } else {
-                    const bool mirror = FORM != UPDATE && un.row != un.col;
+                    const bool mirror = FORM != UPDATE && un.col >= un.row + PT;
                     const int other = block == BLOCKS - 1 ? 0 : block + 1;
                     uint8_t *const first_block = blocks + block * BLOCK, *const second = blocks + other * BLOCK;
                     block = other == BLOCKS - 1 ? 0 : other + 1;
@@ -656,17 +666,17 @@ static int half_map(CUtensorMap *tm, const void *base, int64_t cols, int64_t row
     return r == CUDA_SUCCESS ? TS2_OK : fail(TS2_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
 }
 
-template <int FORM>
+template <int FORM, int PN = PT>
 static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, const CUtensorMap &C, const ProductArgs &p)
 {
     static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
     const unsigned bit = 1u << (c.device & 15);
     if (!(ready.load() & bit)) {
-        TS2_CUDA(cudaFuncSetAttribute((const void *)orth_product_kernel<FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        TS2_CUDA(cudaFuncSetAttribute((const void *)orth_product_kernel<FORM, PN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         ready.fetch_or(bit);
     }
     const int pairs = std::min(sm_count(c.device) / 2, p.units);
-    TS2_LAUNCH((orth_product_kernel<FORM>), 2 * pairs, THREADS, SMEM, c.stream, A, B, C, p);
+    TS2_LAUNCH((orth_product_kernel<FORM, PN>), 2 * pairs, THREADS, SMEM, c.stream, A, B, C, p);
     return TS2_OK;
 }
 
@@ -732,7 +742,7 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     else
         TS2_LAUNCH((orth_load_kernel<T, false>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lows, mt,
                    nt * mt);
-    CUtensorMap x_rows[2], x_cols[2], x_block[2], a_rows, a_block, b_rows, b_block;
+    CUtensorMap x_rows[2], x_cols[2], x_block[2], a_rows, a_half, a_block, b_rows, b_block; // x_cols, a_half: boxes of 64 rows x 64
     int rc = TS2_OK;
     for (int i = 0; i < 2 && rc == TS2_OK; ++i) {
         rc = half_map(&x_rows[i], hi[i], mp, np, batch, 64, 128);
@@ -741,7 +751,7 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
         if (rc == TS2_OK)
             rc = half_map(&x_block[i], hi[i], mp, np, batch, 32, 32);
     }
-    if (rc != TS2_OK || (rc = half_map(&a_rows, A, np, np, batch, 64, 128)) ||
+    if (rc != TS2_OK || (rc = half_map(&a_rows, A, np, np, batch, 64, 128)) || (rc = half_map(&a_half, A, np, np, batch, 64, 64)) ||
         (rc = half_map(&a_block, A, np, np, batch, 32, 32)) || (rc = half_map(&b_rows, B, np, np, batch, 64, 128)) ||
         (rc = half_map(&b_block, B, np, np, batch, 32, 32)))
         return rc;
@@ -750,11 +760,22 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     if (!p.status)
         return fail(TS2_ERR_CUDA, "no device status word");
     p.n = np;
-    p.lo = lows, p.diag = (float *)(sums + (size_t)batch * n_part);
+    p.lo = lows, p.low_tiles = nt * mt, p.low_cols = mt, p.diag = (float *)(sums + (size_t)batch * n_part);
     p.part = part;
-    const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &to, __half *dst) {
+    // Tiles of 256 x 128 where those of 256 x 256 would leave half of the device without any: half the products and half the epilogue
+    // each, and more SMs at work.  3 x 1000 x 333 166 -> 143 us, 400 x 500 167 -> 133, 4 x 130 x 140 139 -> 108; from 38 tiles on
+    // narrow ones would come in a second round.  Outputs of so few tiles that K is divided keep whole tiles.
+    const auto few = [&](int64_t tiles) { return 2 * tiles <= pairs; };
+    const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &in_half, const CUtensorMap &to, __half *dst) {
         p.cols = np, p.tiles = upper, p.col_tiles = 0;
         p.k_blocks = k / BK, p.splits = splits, p.kb_per_split = (int)ceil_div(p.k_blocks, splits), p.units = batch * upper * splits;
+        if (splits == 1 && few(batch * upper)) {
+            p.col_tiles = (int)ceil_div(np, 128), p.tiles = 0;
+            for (int r = 0; r < nt; ++r)
+                p.tiles += std::max(0, p.col_tiles - 2 * r);
+            p.units = batch * p.tiles;
+            return poly ? product<POLY, 128>(c, in, in_half, to, p) : product<SQUARE, 128>(c, in, in_half, to, p);
+        }
         if (splits == 1)
             return poly ? product<POLY>(c, in, in, to, p) : product<SQUARE>(c, in, in, to, p);
         if (int e = product<PARTIAL>(c, in, in, to, p))
@@ -765,10 +786,10 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     for (int k = 0; k < steps; ++k) {
         const int now = k & 1;
         p.alpha = SA / (SX * SX), p.beta = 0.f;
-        if ((rc = symmetric(false, mp, split1, x_rows[now], a_block, A)))
+        if ((rc = symmetric(false, mp, split1, x_rows[now], x_cols[now], a_block, A)))
             return rc;
         p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA, p.res = A;
-        if ((rc = symmetric(true, np, split2, a_rows, b_block, B)))
+        if ((rc = symmetric(true, np, split2, a_rows, a_half, b_block, B)))
             return rc;
         p.alpha = 1.f / SB, p.beta = coef[0], p.res = hi[now];
         p.cols = mp, p.tiles = nt * mt, p.col_tiles = mt, p.k_blocks = np / BK, p.splits = 1, p.kb_per_split = p.k_blocks, p.units = batch * nt * mt;
@@ -776,8 +797,15 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
             p.out = out, p.ld_out = ld_out, p.out_stride = out_stride, p.out_rows = rows, p.out_cols = cols, p.out_scale = out_scale / SX, p.tall = tall;
             p.vec_out = ((uintptr_t)out | (uintptr_t)(ld_out * 2) | (uintptr_t)(out_stride * 2)) % 16 == 0;
         }
-        if ((rc = k < steps - 1 ? product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], p)
-                                : product<LAST>(c, b_rows, x_cols[now], x_block[now ^ 1], p)))
+        if (few(p.units)) {
+            p.col_tiles = (int)ceil_div(mp, 128), p.tiles = nt * p.col_tiles, p.units = batch * p.tiles;
+            rc = k < steps - 1 ? product<UPDATE, 128>(c, b_rows, x_cols[now], x_block[now ^ 1], p)
+                               : product<LAST, 128>(c, b_rows, x_cols[now], x_block[now ^ 1], p);
+        } else {
+            rc = k < steps - 1 ? product<UPDATE>(c, b_rows, x_cols[now], x_block[now ^ 1], p)
+                               : product<LAST>(c, b_rows, x_cols[now], x_block[now ^ 1], p);
+        }
+        if (rc != TS2_OK)
             return rc;
     }
     return TS2_OK;

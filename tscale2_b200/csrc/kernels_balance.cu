@@ -38,7 +38,7 @@ struct alignas(VEC * sizeof(T)) Piece {
 // Columns of a lane: piece i holds columns (i G + lane of the group) VEC ...
 template <class T, int VEC, int G, int N>
 struct Row {
-    static constexpr int VALUES = VEC * N;
+    static constexpr int VALUES = VEC * N, PIECE = VEC % 4 ? 1 : 4; // PIECE: neighbouring columns that are 16 bytes of fp32
     float v[VALUES];
 
     static __device__ __forceinline__ int column(int i) { return ((i / VEC) * G + (int)(threadIdx.x & (G - 1))) * VEC + i % VEC; }
@@ -154,11 +154,15 @@ __device__ __forceinline__ int ld_int(uint32_t a)
     return v;
 }
 
-// an expert's part of the loss
-__device__ __forceinline__ double loss_term(double mean, int count, int tokens, int E, int selected)
-{
-    return tokens ? mean * count * E / ((double)tokens * selected) : 0.;
-}
+// 1 / N, and what sum_e C[e] P[e] is multiplied by: found while other things are on their way
+struct Unit {
+    double mean, loss;
+    __device__ __forceinline__ Unit(int tokens, int E, int selected)
+    {
+        mean = tokens ? 1. / tokens : 0.;
+        loss = mean * E / selected;
+    }
+};
 __device__ __forceinline__ double warp_sum(double v)
 {
 #pragma unroll
@@ -167,14 +171,16 @@ __device__ __forceinline__ double warp_sum(double v)
     return v;
 }
 
+// Two blocks an SM, but where a lane has more than 16 columns (65536 x 512 bf16 41 us; with one, and 32 clusters for which there is no room
+// at once, 69)
 template <class T, int VEC, int G, int N>
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS) balance_sums_kernel(const BalanceArgs p)
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS, VEC * N <= 16 ? 2 : 1) balance_sums_kernel(const BalanceArgs p)
 {
     grid_dep_wait();
     using R = Row<T, VEC, G, N>;
     constexpr int ROWS = 32 / G, WIDTH = VEC * G * N < MAX_EXPERTS ? VEC * G * N : MAX_EXPERTS; // columns there is room for
-    constexpr int PARTS = WIDTH <= 256 ? SUM_WARPS : 1; // warps that leave their sums side by side
-    __shared__ float sums[PARTS][WIDTH];
+    constexpr int PARTS = WIDTH <= 512 ? SUM_WARPS : SUM_WARPS / 2; // warps that leave their sums side by side
+    __shared__ __align__(16) float sums[PARTS][WIDTH];
     __shared__ int count[MAX_EXPERTS + 1];
     __shared__ double terms[CLUSTER], warp_terms[SUM_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.E;
@@ -240,27 +246,33 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS) b
 #pragma unroll
         for (int o = G; o < 32; o <<= 1)
             acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    if (PARTS > 1) {
+    const auto leave = [&](bool add) {
         if (lane < G)
 #pragma unroll
-            for (int i = 0; i < R::VALUES; ++i)
-                sums[warp % PARTS][R::column(i)] = acc[i];
+            for (int i = 0; i < R::VALUES; i += R::PIECE) {
+                float *to = &sums[warp % PARTS][R::column(i)];
+                if constexpr (R::PIECE == 4) {
+                    const float4 old = add ? *(const float4 *)to : make_float4(0.f, 0.f, 0.f, 0.f);
+                    *(float4 *)to = make_float4(old.x + acc[i], old.y + acc[i + 1], old.z + acc[i + 2], old.w + acc[i + 3]);
+                } else {
+                    *to = add ? *to + acc[i] : acc[i];
+                }
+            }
+    };
+    if (warp < PARTS)
+        leave(false);
+    __syncthreads();
+    if (PARTS < SUM_WARPS) {
+        if (warp >= PARTS)
+            leave(true);
         __syncthreads();
-        for (int e = threadIdx.x; e < E; e += SUM_THREADS) {
-            float sum = 0.f;
+    }
+    for (int e = threadIdx.x; e < E; e += SUM_THREADS) {
+        float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < PARTS; ++w)
-                sum += sums[w][e];
-            sums[0][e] = sum;
-        }
-    } else {
-        for (int w = 0; w < SUM_WARPS; ++w) { // warp by warp
-            if (warp == w && lane < G)
-#pragma unroll
-                for (int i = 0; i < R::VALUES; ++i)
-                    sums[0][R::column(i)] = w ? sums[0][R::column(i)] + acc[i] : acc[i];
-            __syncthreads();
-        }
+        for (int w = 0; w < PARTS; ++w)
+            sum += sums[w][e];
+        sums[0][e] = sum;
     }
     // every CTA joins the columns rank, rank + 8, .. of the cluster
     cluster_sync();
@@ -270,6 +282,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS) b
 #pragma unroll
     for (int r = 0; r < CLUSTER; ++r)
         tokens += ld_int(in_rank(&count[E], r));
+    const Unit unit(tokens, E, p.selected);
     double loss = 0.;
     const size_t cluster = blockIdx.x / CLUSTER;
     for (int e = (int)rank + CLUSTER * threadIdx.x; e < E; e += CLUSTER * SUM_THREADS) {
@@ -281,10 +294,10 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS) b
             n += ld_int(in_rank(&count[e], r));
         }
         if (alone) {
-            const double mean = tokens ? sum / tokens : 0.;
+            const double mean = sum * unit.mean;
             p.prob[e] = (float)mean;
             p.counts[e] = n;
-            loss += loss_term(mean, n, tokens, E, p.selected);
+            loss += mean * n;
         } else {
             p.part_prob[cluster * E + e] = (float)sum;
             p.part_count[cluster * (E + 1) + e] = n;
@@ -297,57 +310,64 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS) b
         if (lane == 0)
             warp_terms[warp] = loss;
         __syncthreads();
+        if (warp == 0)
+            loss = warp_sum(lane < SUM_WARPS ? warp_terms[lane] : 0.);
         if (threadIdx.x == 0) {
-            for (int w = 1; w < SUM_WARPS; ++w)
-                loss += warp_terms[w];
             asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_rank(&terms[rank], 0)), "d"(loss) : "memory");
         }
     }
     cluster_sync(); // nobody reads a CTA's shared memory any more; the terms of the loss are there
     if (alone && rank == 0 && threadIdx.x == 0) {
+#pragma unroll
         for (int r = 1; r < CLUSTER; ++r)
             loss += terms[r];
-        *p.loss = (float)loss;
+        *p.loss = (float)(loss * unit.loss);
     }
 }
 
-// one block: the clusters' sums, in their order; a warp a column, a lane a cluster
-__global__ void __launch_bounds__(1024) balance_finish_kernel(const BalanceArgs p, int clusters)
+// One block: the clusters' sums.  `parts` threads a column, a part of the clusters each; a thread's loads are on their way together and
+// a warp's are neighbours: 2 us behind a large launch (with a warp a column and a lane a cluster it grew to 20)
+__global__ void __launch_bounds__(1024) balance_finish_kernel(const BalanceArgs p, int clusters, int width, int parts)
 {
     grid_dep_wait();
-    __shared__ double terms[32];
-    const int E = p.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ double sums[1024], terms[32];
+    __shared__ int counts[1024];
+    const int E = p.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x % width, part = threadIdx.x / width;
     const int tokens = __reduce_add_sync(0xffffffffu, lane < clusters ? p.part_count[(size_t)lane * (E + 1) + E] : 0);
-    double loss = 0.;
-    for (int e0 = warp; e0 < E; e0 += 128) { // four columns' loads at a time
-        float part[4];
-        int count[4];
+    const Unit unit(tokens, E, p.selected);
+    double sum = 0.;
+    int n = 0;
+    for (int c = part; c < clusters; c += 8 * parts) {
+        float v[8];
+        int k[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = e0 + 32 * i;
-            const bool in = lane < clusters && e < E;
-            part[i] = in ? p.part_prob[(size_t)lane * E + e] : 0.f;
-            count[i] = in ? p.part_count[(size_t)lane * (E + 1) + e] : 0;
+        for (int i = 0; i < 8; ++i) {
+            const bool in = c + i * parts < clusters && e < E;
+            v[i] = in ? p.part_prob[(size_t)(c + i * parts) * E + e] : 0.f;
+            k[i] = in ? p.part_count[(size_t)(c + i * parts) * (E + 1) + e] : 0;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = e0 + 32 * i;
-            const double sum = warp_sum((double)part[i]), mean = tokens ? sum / tokens : 0.;
-            const int n = __reduce_add_sync(0xffffffffu, count[i]);
-            if (e >= E)
-                continue;
-            if (lane == 0)
-                p.prob[e] = (float)mean, p.counts[e] = n;
-            loss += loss_term(mean, n, tokens, E, p.selected);
-        }
+        for (int i = 0; i < 8; ++i)
+            sum += v[i], n += k[i];
     }
+    sums[threadIdx.x] = sum, counts[threadIdx.x] = n;
+    __syncthreads();
+    double loss = 0.;
+    if (threadIdx.x < E) { // part 0
+        for (int i = 1; i < parts; ++i)
+            sum += sums[i * width + e], n += counts[i * width + e];
+        const double mean = sum * unit.mean;
+        p.prob[e] = (float)mean, p.counts[e] = n;
+        loss = mean * n;
+    }
+    loss = warp_sum(loss);
     if (lane == 0)
         terms[warp] = loss;
     __syncthreads();
+    if (warp == 0)
+        loss = warp_sum(lane < (int)blockDim.x / 32 ? terms[lane] : 0.);
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 32; ++w)
-            loss += terms[w];
-        *p.loss = (float)loss;
+        *p.loss = (float)(loss * unit.loss);
         p.counts[E] = tokens;
     }
 }
@@ -406,14 +426,18 @@ template <class T, int VEC, int G, int N>
 static int launch(const Ctx &c, BalanceArgs &p, bool backward)
 {
     if (backward) {
-        const int rows = 32 / G * WARPS, cap = sm_count(c.device) * 4;
+        // blocks a device holds, each of which reads the counts first: 2 an SM where a lane has several pieces (16384 x 512 bf16 11.2 us, with 4
+        // 13.0), 4 where it has one (65536 x 128 10.9 us, with 2 12.6)
+        const int rows = 32 / G * WARPS, cap = sm_count(c.device) * (N > 1 ? 2 : 4);
         TS2_LAUNCH((balance_backward_kernel<T, VEC, G, N>), (unsigned)std::max<int64_t>(1, std::min<int64_t>(cap, ceil_div(p.T, rows))), THREADS, 0,
                    c.stream, p);
         return TS2_OK;
     }
-    // one cluster for up to four rounds of its warps, and then as many as the device holds at once
+    // One cluster for up to four rounds of its warps, and then as many as the device holds at once: a second launch is 2 us, a round half
+    // of one (x 64 bf16, us with one cluster and with several: 2048 rows, 4 rounds 6.4 and 6.7; 4096, 8 rounds 8.8 and 7.0; 2048 x 512,
+    // 16 rounds 24.1 and 12.0)
     const int64_t round = (int64_t)32 / G * SUM_WARPS, clusters_wanted = ceil_div(p.T, round * CLUSTER);
-    const int clusters = clusters_wanted <= 4 ? 1 : (int)std::min<int64_t>(clusters_wanted, MAX_CLUSTERS);
+    const int clusters = clusters_wanted <= 4 ? 1 : (int)std::min<int64_t>(clusters_wanted, VEC * N <= 16 ? MAX_CLUSTERS : MAX_CLUSTERS / 2);
     p.rows_per_block = ceil_div(ceil_div(p.T, (int64_t)clusters * CLUSTER), 32 / G) * (32 / G);
     if (clusters == 1) {
         TS2_LAUNCH((balance_sums_kernel<T, VEC, G, N>), CLUSTER, SUM_THREADS, 0, c.stream, p);
@@ -426,7 +450,8 @@ static int launch(const Ctx &c, BalanceArgs &p, bool backward)
     p.part_count = (int *)scratch + (size_t)clusters * p.E;
     const auto work = [&] {
         TS2_LAUNCH((balance_sums_kernel<T, VEC, G, N>), clusters * CLUSTER, SUM_THREADS, 0, c.stream, p);
-        TS2_LAUNCH(balance_finish_kernel, 1, 1024, 0, c.stream, p, clusters);
+        const int width = (int)ceil_div(p.E, 32) * 32, parts = std::min(8, 1024 / width);
+        TS2_LAUNCH(balance_finish_kernel, 1, width * parts, 0, c.stream, p, clusters, width, parts);
         return TS2_OK;
     };
     const int rc = work();

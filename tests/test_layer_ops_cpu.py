@@ -65,3 +65,12 @@ def test_balance_backward(lib, change):
                                     dict(out_ld=7), dict(g=P + 2), dict(out=P + 1), dict(g_stride=-1), dict(out_stride=63)])
 def test_orthogonalize(lib, change):
     refused(lib, "ts2_op_orthogonalize", ORTH, **change)
+
+
+# Singular values of G / |G| lie in [0, 1].  (4, 0, 0) takes 1 to 4 > 3.9; (12, -12, c): 12 s (1 - s^2) is 4.6 at s = 0.577 although it is 0 at 1, and
+# so is (12, -12, 1e-30), whose other extremum is at 1e15; (0, 32, 0): B = 32; (2, 0, 0) leaves the range in the second step; (-4, 0, 0) as (4, 0, 0)
+@pytest.mark.parametrize("coef,steps", [((4, 0, 0), 1), ((12, -12, 0), 1), ((12, -12, 1e-30), 1), ((12, -12, -1e-30), 2), ((0, 32, 0), 1), ((0, 0, -32), 1),
+                                        ((2, 0, 0), 2), ((-4, 0, 0), 1), ((NAN, 0, 0), 1), ((1, NAN, 0), 1), ((1, 0, NAN), 1),
+                                        ((float("inf"), 0, 0), 1), ((1, 3e38, -3e38), 1), ((1.05, 0, 0), 64)])
+def test_orthogonalize_refuses_coefficients_that_leave_the_range_of_fp16(lib, coef, steps):
+    refused(lib, "ts2_op_orthogonalize", ORTH, rc=capi.TS2_ERR_UNSUPPORTED, coef=(C.c_float * 3)(*coef), steps=steps)

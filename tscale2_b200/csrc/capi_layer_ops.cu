@@ -107,6 +107,8 @@ int ts2_op_orthogonalize(int device, void *stream, int type, const void *g, int6
         g_stride < 0 || !rows_ok(g, ld, batch, cols, es) || !rows_ok(out, out_ld, batch, cols, 2) ||
         (batch > 1 && out_stride < (rows - 1) * out_ld + cols))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_orthogonalize: bad arguments");
+    if (!orthogonalize_in_range(coef, steps))
+        return fail(TS2_ERR_UNSUPPORTED, "ts2_op_orthogonalize: the coefficients take singular values out of the range of fp16");
     TS2_ON_DEVICE(device);
     if (batch == 0)
         return TS2_OK;

@@ -242,6 +242,8 @@ int recurrence_forward(const Ctx &c, int type, const void *gate, int64_t gate_ld
 int recurrence_backward(const Ctx &c, int type, const void *gate, int64_t gate_ld, const void *x, int64_t x_ld, const void *h, int64_t h_ld,
                         int T, int D, int n_seq, const int *seq_ptr, const float *h0, const void *dh, int64_t dh_ld, const float *dh_last,
                         void *dgate, int64_t dgate_ld, void *dx, int64_t dx_ld, float *dh0);
+// whether the coefficients keep every singular value, and every product, in the range of the fp16 scaling
+bool orthogonalize_in_range(const float coef[3], int steps);
 int orthogonalize(const Ctx &c, int type, const void *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
                   float out_scale, void *out, int64_t ld_out, int64_t out_stride);
 

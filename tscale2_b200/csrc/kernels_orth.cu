@@ -8,7 +8,7 @@
 // that falls off as 1/k^2, 512 x 1024, coefficients 3.4445, -4.7750, 2.0315, 5 steps: relative error 2.0e-2 with X in fp16,
 // 1.8e-4 with X in two halves; flat spectra 2.0e-3 and 1.3e-3).  For the same reason the diagonal of B, which is its largest part, stays in fp32 beside the zeros
 // of the operand: X = (a + diagonal) X + B X (flat spectra 1.3e-3 -> 0.8e-3).  All fp16 values are scaled by powers of two that keep them
-// below 65504 for every X the coefficients can reach (orth_check).
+// below 65504 for every X the coefficients can reach (orthogonalize_in_range).
 #include "orth.cuh"
 #include "pair_ptx.cuh"
 #include <cuda.h>
@@ -611,22 +611,21 @@ __global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict_
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-// largest |a s + b s^3 + c s^5| (odd) or |b q + c q^2| over [0, top]: at the end or where the derivative is zero
+// largest |a s + b s^3 + c s^5| over [0, top]: at the end or where the derivative a + 3 b q + 5 c q^2, q = s^2, is zero
 static double poly_max(double a, double b, double c, double top)
 {
     const auto p = [&](double s) { return std::fabs(s * (a + s * s * (b + s * s * c))); };
     double most = p(top);
     const double disc = 9 * b * b - 20 * a * c;
     if (disc >= 0) {
-        const double root[3] = {c ? (-3 * b + std::sqrt(disc)) / (10 * c) : -1, c ? (-3 * b - std::sqrt(disc)) / (10 * c) : -1,
-                                b ? -a / (3 * b) : -1};
-        for (int i = c ? 0 : 2; i < (c ? 2 : 3); ++i)
-            if (root[i] > 0 && root[i] < top * top)
-                most = std::max(most, p(std::sqrt(root[i])));
+        const double t = -0.5 * (3 * b + std::copysign(std::sqrt(disc), b)); // no difference of near numbers, however small c is
+        for (const double q : {t / (5 * c), a / t})
+            if (q > 0 && q < top * top)
+                most = std::max(most, p(std::sqrt(q)));
     }
     return most;
 }
-static bool orth_check(const float coef[3], int steps)
+bool orthogonalize_in_range(const float coef[3], int steps)
 {
     double x = 1.;
     for (int k = 0; k < steps; ++k) {
@@ -814,8 +813,6 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
 int orthogonalize(const Ctx &c, int type, const void *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
                   float out_scale, void *out, int64_t ld_out, int64_t out_stride)
 {
-    if (!orth_check(coef, steps))
-        return fail(TS2_ERR_UNSUPPORTED, "orthogonalize: the coefficients take singular values beyond %g", (double)MAX_X);
     if (orth_chip_ranks(rows, cols))
         return orth_chip(c, type, g, ld, stride, batch, rows, cols, coef, steps, out_scale, out, ld_out, out_stride);
     __nv_bfloat16 *o = (__nv_bfloat16 *)out;

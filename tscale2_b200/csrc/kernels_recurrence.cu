@@ -106,8 +106,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
-// a = 1 / (1 + exp(-g)) and 1 - a, each to fp32's relative accuracy.  The exponent stops at 126, where a is 1e-38 and 1 - a is
-// 1: beyond it exp(-g) would be infinite and 1 - a = exp(-g) a not a number.  A NaN stays one.
+// a = 1 / (1 + exp(-g)) and 1 - a, both with a small relative error (the product with log2 e is rounded: |g| 2^-24, and the three
+// instructions' own) however near to one the other is.  The exponent stops at 126, where a is 1e-38 and 1 - a is 1: beyond it exp(-g)
+// would be infinite and 1 - a = exp(-g) a not a number.  A NaN stays one.
 __device__ __forceinline__ void decay(float2 g, float2 &a, float2 &keep)
 {
     float2 e = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));

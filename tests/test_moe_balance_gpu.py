@@ -106,6 +106,13 @@ def test_against_the_formula(kind, T, E, k, masked):
     verify(kind, logits, ids, mask, k, dloss=0.25 if kind == "f32" else 64.0 * T)
 
 
+@pytest.mark.parametrize("kind,T,E,k,masked", [("f32", 6000, 1000, 4, True), ("bf16", 5000, 1024, 8, False), ("f16", 9000, 512, 8, True),
+                                               ("bf16", 4000, 515, 3, True), ("f32", 3000, 64, 40, True), ("f16", 2500, 1, 1, True)])
+def test_rows_of_every_width_over_many_clusters(kind, T, E, k, masked):
+    logits, ids, mask = make(kind, T, E, k, masked, T + E)
+    verify(kind, logits, ids, mask, k, dloss=0.25 if kind == "f32" else 64.0 * T)
+
+
 @pytest.mark.parametrize("kind,pitch,offset", [("f32", 32, 0), ("f32", 36, 4), ("f32", 33, 1), ("f16", 40, 8), ("f16", 41, 0), ("bf16", 48, 3)])
 def test_pitches_and_offsets(kind, pitch, offset):
     logits, ids, mask = make(kind, 777, 32, 2, True, pitch)

@@ -412,7 +412,6 @@ __global__ void __launch_bounds__(THREADS, 2) recurrence_maps_kernel(const ScanA
     int begin, end;
     scan_range(p, begin, end);
     const int s_lo = segment_start(p, seg, begin, end), s_hi = segment_start(p, seg + 1, begin, end);
-    int lo = s_lo + (int)((long long)(s_hi - s_lo) * sub / p.subs), hi = s_lo + (int)((long long)(s_hi - s_lo) * (sub + 1) / p.subs);
     // where the nodes begin (backward: end) that matter to the segment, and whether that is a border
     int from = BACKWARD ? s_hi : s_lo;
     bool border = !p.ptr && s_lo < s_hi && (BACKWARD ? s_hi == end : s_lo == begin);
@@ -423,17 +422,12 @@ __global__ void __launch_bounds__(THREADS, 2) recurrence_maps_kernel(const ScanA
         if (border)
             from = v;
     }
+    // this block's part of them
+    const int all_lo = BACKWARD ? s_lo : from, need = BACKWARD ? from - s_lo : s_hi - from;
+    const int lo = all_lo + (int)((long long)need * sub / p.subs), hi = all_lo + (int)((long long)need * (sub + 1) / p.subs);
     int seq = -1; // of the border, if it is in this block's part
-    if (BACKWARD) {
-        if (border && from > lo && from <= hi)
-            seq = sequence_of(p.ptr, p.n_seq, from - 1);
-        hi = min(hi, from);
-    } else {
-        if (border && from >= lo && from < hi)
-            seq = sequence_of(p.ptr, p.n_seq, from);
-        lo = max(lo, from);
-    }
-    hi = max(hi, lo);
+    if (border && lo < hi && (BACKWARD ? from == hi : from == lo))
+        seq = sequence_of(p.ptr, p.n_seq, BACKWARD ? from - 1 : from);
     const int part = ceil_div_dev(hi - lo, WARPS * S) * S;
     // this warp's nodes, from the one that the recurrence reaches first
     const int first = BACKWARD ? hi - warp * part : lo + warp * part, n = max(0, min(part, BACKWARD ? first - lo : hi - first));

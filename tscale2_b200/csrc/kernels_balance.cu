@@ -11,6 +11,7 @@
 // launch and a large one leaves a partial result per cluster to a second.  All sums have a fixed order; counts are integers, so
 // that the order of their atomics does not matter.
 #include "kernels.cuh"
+#include "pair_ptx.cuh"
 #include <algorithm>
 
 namespace ts2 {
@@ -123,24 +124,9 @@ struct BalanceArgs {
     int add;
 };
 
-__device__ __forceinline__ unsigned cluster_rank()
-{
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // this CTA's shared-memory address `p`, in CTA `rank` of the cluster
 template <class V>
-__device__ __forceinline__ uint32_t in_rank(const V *p, unsigned rank)
-{
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    return a;
-}
+__device__ __forceinline__ uint32_t in_rank(const V *p, unsigned rank) { return map_to_rank(smem_u32(p), rank); }
 __device__ __forceinline__ float ld_float(uint32_t a)
 {
     float v;

@@ -381,6 +381,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < PART / 32; ++c) {
                 uint32_t r[32];
+                __syncwarp(); // lane 0 comes from its stores
                 tmem_ld32(taddr + c * 32, r);
                 tmem_ld_wait();
                 if (c == PART / 32 - 1) { // the accumulator is read: the next tile may have it

@@ -8,6 +8,7 @@
 // 128 x 4000 on a cluster of 16: 90.
 #include "kernels.cuh"
 #include "orth.cuh"
+#include "pair_ptx.cuh"
 #include <algorithm>
 
 namespace ts2 {
@@ -33,27 +34,11 @@ struct ChipArgs {
     int32_t *status;
 };
 
-__device__ __forceinline__ unsigned cluster_rank()
-{
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ unsigned cluster_size()
 {
     unsigned r;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_rank(uint32_t addr, unsigned rank)
-{
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    return a;
 }
 // 16-byte piece c (0 .. 15) of row r of 128 columns of fp16, as two swizzled blocks
 __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)((c >> 3) * BLK + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
@@ -96,7 +81,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 0) {
+    if (warp == 1) { // a warp that no branch has split
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
@@ -215,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         sum = 0.;
         for (unsigned r = 0; r < ranks; ++r) {
             double s;
-            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(s) : "r"(in_rank(smem_u32(sums + 8), r)) : "memory");
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(s) : "r"(map_to_rank(smem_u32(sums + 8), r)) : "memory");
             sum += s;
         }
     }
@@ -251,6 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         }
         mbar_wait(bar, phase, abort_flag);
         phase ^= 1;
+        __syncwarp(); // the lanes left the wait one by one; what reads tensor memory wants the warp
         tc_fence_after();
     };
     const uint32_t x_at = smem_u32(smem), a_at = smem_u32(smem + A_OFF), b_at = smem_u32(smem + B_OFF), work = tmem + WORK;
@@ -293,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                         for (int e = 0; e < 2; ++e)
                             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                                          : "=f"(f[k][e].x), "=f"(f[k][e].y), "=f"(f[k][e].z), "=f"(f[k][e].w)
-                                         : "r"(in_rank(at[e], k0 + k))
+                                         : "r"(map_to_rank(at[e], k0 + k))
                                          : "memory");
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
@@ -308,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                     w[e] = *(const uint32_t *)&h;
                 }
                 for (unsigned k = 0; k < ranks; ++k)
-                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(in_rank(a_at + piece(r, c), k)), "r"(w[0]), "r"(w[1]),
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(map_to_rank(a_at + piece(r, c), k)), "r"(w[0]), "r"(w[1]),
                                  "r"(w[2]), "r"(w[3])
                                  : "memory");
             }
@@ -415,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
     __syncthreads();
     if (ranks > 1)
         cluster_sync(); // nobody uses another CTA's shared memory any more
-    if (warp == 0)
+    if (warp == 1)
         tmem_dealloc(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag)
         atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);

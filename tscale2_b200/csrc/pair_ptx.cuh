@@ -1,5 +1,5 @@
 // PTX of a pair of CTAs (a cluster of two) that works on one tile: tcgen05 with cta_group::2, copies and arrivals on the leader's
-// barriers.  Shared by gemm_pair.cu and kernels_orth.cu.
+// barriers.  Shared by gemm_pair.cu and kernels_orth.cu; kernels_orth_chip.cu and kernels_balance.cu use what it has for clusters.
 #pragma once
 #include "common.cuh"
 
@@ -17,8 +17,17 @@ __device__ __forceinline__ uint32_t map_to_leader(uint32_t addr)
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
+// this CTA's shared-memory address in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// An aligned barrier wants whole warps: lanes that come from a branch or a loop of their own meet first.
 __device__ __forceinline__ void cluster_sync()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)

@@ -223,20 +223,29 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
 
     // ---- steps ----
     uint32_t phase = 0;
-    // the operands in shared memory are complete and the product's columns are free: one thread issues, all wait for the product
+    bool alive = true; // of the whole CTA: no wait has given up
+    // The operands in shared memory are complete and the product's columns are free: one thread issues, all wait for the product.
+    // After a wait that gave up nothing is multiplied any more, but the CTA keeps its appointments with the rest of the cluster.
     const auto product = [&](auto &&issue) {
         fence_proxy_async();
         tmem_st_wait();
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        if (threadIdx.x == 0) {
-            issue();
-            tc_commit(bar);
+        if (alive) {
+            if (threadIdx.x == 0) {
+                issue();
+                tc_commit(bar);
+            }
+            const bool done = mbar_wait(bar, phase, abort_flag);
+            if (!done && threadIdx.x == 0) { // what was issued may still end (a bounded wait): it uses shared and tensor memory
+                const long long t0 = clock64();
+                while (!mbar_try_wait(bar, phase) && clock64() - t0 < 1500000000ll) {
+                }
+            }
+            alive = __syncthreads_and(done); // warps are whole again, too: what reads tensor memory wants them so
+            phase ^= 1;
         }
-        mbar_wait(bar, phase, abort_flag);
-        phase ^= 1;
-        __syncwarp(); // the lanes left the wait one by one; what reads tensor memory wants the warp
         tc_fence_after();
     };
     const uint32_t x_at = smem_u32(smem), a_at = smem_u32(smem + A_OFF), b_at = smem_u32(smem + B_OFF), work = tmem + WORK;

@@ -1,11 +1,14 @@
 // Orthogonalised updates (kernels_orth.cu has the formula and its scaling) of matrices with at most 128 rows or columns, in one launch
-// and without memory in between: a cluster holds a matrix.  Each CTA has the 128 rows (padded with zeros) of up to 384 columns of X:
-// as fp32 in tensor memory, thread = row, and rounded to fp16 in shared memory as the operand of the products
+// and without memory in between: a cluster holds a matrix.  Each CTA has the 128 rows (padded with zeros) of up to 256 columns of X:
+// as fp32 in tensor memory, thread = row, and as two fp16 halves in shared memory, the operands of the products
 //     A = X X^T   (the CTAs' parts are added through distributed shared memory, each 128 / cluster rows for all)
-//     B = b A + c A A   (every CTA for itself)      X = a X + B X   (128 columns at a time; the diagonal of B in fp32)
-// A chain of small products: its latency is the bound, 5 us a step (a tenth of it tensor work), 10 us to bring G in and normalise it,
-// and with more than one CTA the exchange of A, 5 - 8 us a step.  128 x 256: 33 us, as 15 launches of kernels_orth.cu 127;
-// 128 x 4000 on a cluster of 16: 90.
+//     B = b A + c A A   (every CTA for itself, in the place of A)      X = a X + B X
+// Operands in one fp16 half each would take a third of the tensor work (128 x 256: 34 us instead of 53), but results of few directions or
+// few rows were up to 2e-2 off: the rounding of X meets the large entries of B, and what it leaves in directions that X does not have
+// grows by a factor a in every step.  With two halves every matrix is within 1e-4.
+// A chain of small products: its latency is the bound, 9 us a step (4 of them tensor work at two chunks of columns), 10 us to bring G in
+// and normalise it, and with more than one CTA the exchange of A, 5 - 8 us a step.  64 x 64: 38 us, 128 x 256: 53, 128 x 4000 on a cluster
+// of 16: 112.
 #include "kernels.cuh"
 #include "orth.cuh"
 #include "pair_ptx.cuh"
@@ -15,12 +18,15 @@ namespace ts2 {
 
 namespace {
 
-constexpr int THREADS = 256, MAX_CHUNKS = 3, MAX_CLUSTER = 16;
+constexpr int THREADS = 256, MAX_CHUNKS = 2, MAX_CLUSTER = 16;
 constexpr int BLK = 128 * 128;   // 128 rows x 64 columns of fp16, 128-byte swizzle
-constexpr int A_OFF = MAX_CHUNKS * 2 * BLK, B_OFF = A_OFF + 2 * BLK, STG_OFF = B_OFF + 2 * BLK, END_OFF = STG_OFF + 128 * 128 * 4;
-constexpr int SMEM = END_OFF + 128 + 512 + 1024;
-static_assert(SMEM <= 232448, "shared memory budget");
-constexpr uint32_t WORK = MAX_CHUNKS * 128; // tensor-memory columns of the product at hand; X's chunks lie before it
+constexpr int PART = 2 * BLK;    // 128 x 128 of fp16
+// X's chunks, high half and low half each; behind them A, then B, alike.  The staging area of 128 x 128 fp32 is the same memory: it
+// is used while there is neither (G on its way in, the CTAs' parts of A, the result on its way out).
+constexpr int A_OFF = MAX_CHUNKS * 2 * PART, END_OFF = A_OFF + 2 * PART;
+constexpr int SMEM = END_OFF + 128 + 1024;
+static_assert(SMEM <= 232448 && 2 * PART == 128 * 128 * 4, "shared memory budget");
+constexpr uint32_t WORK = MAX_CHUNKS * 128; // tensor-memory columns of the products at hand; X's chunks lie before them
 
 struct ChipArgs {
     const void *g;
@@ -47,18 +53,16 @@ __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)((c >
 // row, nor every eighth row, meet in a bank
 __device__ __forceinline__ int staged(int r, int c) { return r * 128 + (((c >> 2) ^ ((r ^ (r >> 3)) & 7)) << 2); }
 
-// 32 values as fp16 to the columns [32 j, +32) of the thread's row
-__device__ __forceinline__ void put_half(uint8_t *base, int row, int j, const float (&v)[32])
+// 32 values as two halves to the columns [32 j, +32) of the thread's row
+__device__ __forceinline__ void put_halves(uint8_t *base, int row, int j, const float (&v)[32])
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const __half2 h = sat_half2(v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
-            w[k] = *(const uint32_t *)&h;
-        }
-        *(uint4 *)(base + piece(row, 4 * j + i)) = make_uint4(w[0], w[1], w[2], w[3]);
+        const float e[8] = {v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3], v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]};
+        uint4 hi, lo;
+        orth_split8(e, hi, lo);
+        *(uint4 *)(base + piece(row, 4 * j + i)) = hi;
+        *(uint4 *)(base + PART + piece(row, 4 * j + i)) = lo;
     }
 }
 
@@ -67,12 +71,11 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
 {
     extern __shared__ uint8_t chip_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)chip_smem + 1023) & ~(uintptr_t)1023); // the same offset in every CTA of a cluster
-    float *stage = (float *)(smem + STG_OFF);
+    float *stage = (float *)(smem + A_OFF);
     uint64_t *bar_at = (uint64_t *)(smem + END_OFF);
     uint32_t *tmem_slot = (uint32_t *)(bar_at + 1);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     double *sums = (double *)(smem + END_OFF + 32); // a warp's, the CTA's
-    float *diag = (float *)(smem + END_OFF + 128);  // of B
     const uint32_t bar = smem_u32(bar_at);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
@@ -93,7 +96,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
     grid_dep_wait();
     const uint32_t tmem = *tmem_slot, lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64; // the thread's row, its half of 128 columns
     const int row = quarter * 32 + lane, matrix = blockIdx.x / ranks;
-    const int n = TALL ? p.cols : p.rows, m = TALL ? p.rows : p.cols, j0 = (int)rank * p.chunks * 128;
+    const int j0 = (int)rank * p.chunks * 128;
     const T *g = (const T *)p.g + matrix * p.stride;
     const auto load32 = [&](uint32_t column, float (&v)[32]) {
         uint32_t r[32];
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                 for (int i = 0; i < 32; ++i)
                     v[i] = small ? (float)(v[i] * scale) : v[i] * scale32;
                 store32(q * 128 + h * 32, v);
-                put_half(smem + q * 2 * BLK, row, half * 2 + h, v);
+                put_halves(smem + q * 2 * PART, row, half * 2 + h, v);
             }
     }
 
@@ -248,14 +251,23 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         }
         tc_fence_after();
     };
-    const uint32_t x_at = smem_u32(smem), a_at = smem_u32(smem + A_OFF), b_at = smem_u32(smem + B_OFF), work = tmem + WORK;
+    const uint32_t x_at = smem_u32(smem), a_at = smem_u32(smem + A_OFF), work = tmem + WORK;
     constexpr uint32_t IDESC = umma_idesc_f16(128, false, false), IDESC_MN = umma_idesc_f16(128, false, true);
+    // A product of operands in two halves: low times high, high times low, high times high (low times low is 2^-22 of it).  The small
+    // ones come first, while the sum that they are added to is small.
+    const auto halves = [&](auto &&one) {
+        one(PART, 0, true);
+        one(0, PART, false);
+        one(0, 0, false);
+    };
     for (int step = 0; step < p.steps; ++step) {
         product([&] { // A = X X^T
-            for (int b = 0; b < 2 * p.chunks; ++b) {
-                const uint64_t d = umma_smem_desc(x_at + b * BLK, 16, 1024);
-                umma_f16_x4(work, d, d, IDESC, b > 0, 2, 2);
-            }
+            halves([&](int left, int right, bool clear) {
+                for (int b = 0; b < 2 * p.chunks; ++b) {
+                    const uint32_t at = x_at + (b >> 1) * 2 * PART + (b & 1) * BLK;
+                    umma_f16_x4(work, umma_smem_desc(at + left, 16, 1024), umma_smem_desc(at + right, 16, 1024), IDESC, !clear || b > 0, 2, 2);
+                }
+            });
         });
         constexpr float ALPHA = ORTH_SA / (ORTH_SX * ORTH_SX);
         float w2[2][32];
@@ -268,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
             for (int i = 0; i < 32; ++i)
                 v[i] *= ALPHA;
             if (ranks == 1) {
-                put_half(smem + A_OFF, row, half * 2 + h, v);
+                put_halves(smem + A_OFF, row, half * 2 + h, v);
             } else {
                 stage32(half * 64 + h * 32, v);
             }
@@ -276,7 +288,12 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         if (ranks > 1) {
             cluster_sync();
             const int rows_each = 128 / (int)ranks;
-            for (int i = threadIdx.x; i < rows_each * 16; i += THREADS) {
+            uint4 hi[4], lo[4]; // this CTA's 8-column pieces of A: 2048 / ranks of them
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = threadIdx.x + q * THREADS;
+                if (i >= rows_each * 16)
+                    break;
                 const int r = (int)rank * rows_each + (i >> 4), c = i & 15;
                 const uint32_t at[2] = {smem_u32(stage + staged(r, c * 8)), smem_u32(stage + staged(r, c * 8 + 4))};
                 float v[8] = {};
@@ -296,72 +313,67 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                         for (int e = 0; e < 2; ++e)
                             v[4 * e] += f[k][e].x, v[4 * e + 1] += f[k][e].y, v[4 * e + 2] += f[k][e].z, v[4 * e + 3] += f[k][e].w;
                 }
-                uint32_t w[4];
+                orth_split8(v, hi[q], lo[q]);
+            }
+            cluster_sync(); // the parts have been read everywhere: A may take their place
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __half2 h = sat_half2(v[2 * e], v[2 * e + 1]);
-                    w[e] = *(const uint32_t *)&h;
-                }
-                for (unsigned k = 0; k < ranks; ++k)
-                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(map_to_rank(a_at + piece(r, c), k)), "r"(w[0]), "r"(w[1]),
-                                 "r"(w[2]), "r"(w[3])
+            for (int q = 0; q < 4; ++q) {
+                const int i = threadIdx.x + q * THREADS;
+                if (i >= rows_each * 16)
+                    break;
+                const uint32_t at = a_at + piece((int)rank * rows_each + (i >> 4), i & 15);
+                for (unsigned k = 0; k < ranks; ++k) {
+                    const uint32_t to = map_to_rank(at, k);
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi[q].x), "r"(hi[q].y), "r"(hi[q].z),
+                                 "r"(hi[q].w)
                                  : "memory");
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + PART), "r"(lo[q].x), "r"(lo[q].y), "r"(lo[q].z),
+                                 "r"(lo[q].w)
+                                 : "memory");
+                }
             }
             cluster_sync();
         }
         product([&] { // A A
-            for (int b = 0; b < 2; ++b) {
-                const uint64_t d = umma_smem_desc(a_at + b * BLK, 16, 1024);
-                umma_f16_x4(work, d, d, IDESC, b > 0, 2, 2);
-            }
+            halves([&](int left, int right, bool clear) {
+                for (int b = 0; b < 2; ++b)
+                    umma_f16_x4(work, umma_smem_desc(a_at + left + b * BLK, 16, 1024), umma_smem_desc(a_at + right + b * BLK, 16, 1024), IDESC,
+                                !clear || b > 0, 2, 2);
+            });
         });
         const float kb = ORTH_SB * p.b / ORTH_SA, kc = ORTH_SB * p.c / (ORTH_SA * ORTH_SA);
         load64(WORK, w2);
         tmem_ld_wait();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) { // a thread's values of B take the place of its values of A
             float(&v)[32] = w2[h];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint4 raw = *(const uint4 *)(smem + A_OFF + piece(row, (half * 2 + h) * 4 + i));
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                const uint8_t *at = smem + A_OFF + piece(row, (half * 2 + h) * 4 + i);
+                float f[8];
+                orth_join8(*(const uint4 *)at, *(const uint4 *)(at + PART), f);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 f = __half22float2(*(const __half2 *)&w[k]);
-                    v[8 * i + 2 * k] = fmaf(kb, f.x, kc * v[8 * i + 2 * k]);
-                    v[8 * i + 2 * k + 1] = fmaf(kb, f.y, kc * v[8 * i + 2 * k + 1]);
-                }
+                for (int k = 0; k < 8; ++k)
+                    v[8 * i + k] = fmaf(kb, f[k], kc * v[8 * i + k]);
             }
-            if (quarter == half * 2 + h) { // the warp's 32 x 32 on the diagonal
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (lane == i) {
-                        diag[row] = v[i] * (1.f / ORTH_SB);
-                        v[i] = 0.f;
-                    }
-            }
-            put_half(smem + B_OFF, row, half * 2 + h, v);
+            put_halves(smem + A_OFF, row, half * 2 + h, v);
         }
         const bool last = step == p.steps - 1;
-        // up to two chunks have tensor memory for their products at once
-        const bool together = p.chunks < MAX_CHUNKS;
-        for (int q = 0; q < p.chunks; ++q) {
-            const uint32_t at = together ? WORK - (p.chunks - 1 - q) * 128 : WORK;
-            if (q == 0 || !together)
-                product([&] { // B X, 128 columns a chunk
-                    for (int k = q; k < (together ? p.chunks : q + 1); ++k) {
-                        const uint64_t x = umma_smem_desc(x_at + k * 2 * BLK, BLK, 1024);
-                        for (int b = 0; b < 2; ++b)
-                            umma_f16_x4(tmem + at + (k - q) * 128, umma_smem_desc(b_at + b * BLK, 16, 1024), x + (uint64_t)(b * 4 * (16 * 128 >> 4)),
-                                        IDESC_MN, b > 0, 2, 16 * 128 >> 4);
-                    }
+        product([&] { // B X, 128 columns a chunk
+            for (int q = 0; q < p.chunks; ++q)
+                halves([&](int left, int right, bool clear) {
+                    const uint64_t x = umma_smem_desc(x_at + q * 2 * PART + right, BLK, 1024);
+                    for (int b = 0; b < 2; ++b)
+                        umma_f16_x4(work + q * 128, umma_smem_desc(a_at + left + b * BLK, 16, 1024), x + (uint64_t)(b * 4 * (16 * 128 >> 4)), IDESC_MN,
+                                    !clear || b > 0, 2, 16 * 128 >> 4);
                 });
-            else if (last)
+        });
+        for (int q = 0; q < p.chunks; ++q) {
+            if (last && q)
                 __syncthreads(); // the staging of the chunk before has been read
             float x2[2][32];
-            load64(at, w2);
+            load64(WORK + q * 128, w2);
             load64(q * 128, x2);
-            const float beta = p.a + diag[row];
             tmem_ld_wait();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -369,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                 const float(&x)[32] = x2[h];
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    v[i] = fmaf(beta, x[i], v[i] * (1.f / ORTH_SB));
+                    v[i] = fmaf(p.a, x[i], v[i] * (1.f / ORTH_SB));
                 if (last) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
@@ -377,7 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
                     stage32(half * 64 + h * 32, v);
                 } else {
                     store32(q * 128 + h * 32, v);
-                    put_half(smem + q * 2 * BLK, row, half * 2 + h, v);
+                    put_halves(smem + q * 2 * PART, row, half * 2 + h, v);
                 }
             }
             if (!last)
@@ -414,7 +426,6 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         tmem_dealloc(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag)
         atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);
-    (void)n, (void)m;
 }
 
 template <class T, bool TALL>
@@ -458,8 +469,8 @@ int orth_chip_ranks(int rows, int cols)
     if (std::min(rows, cols) > 128)
         return 0;
     const int64_t chunks = ceil_div(std::max(rows, cols), 128);
-    // as few as hold it: more CTAs with fewer chunks each save less than the exchange of A costs (100 x 384 in one 47 us, in two 55;
-    // 200 matrices of 128 x 300 117 and 194; only 100 x 700 gains, in four instead of two 77 -> 72)
+    // as few as hold it: more CTAs with fewer chunks each save less than the exchange of A costs (128 x 256 in one 53 us, 100 x 384 in
+    // two 76)
     for (int ranks = 1; ranks <= MAX_CLUSTER; ranks *= 2)
         if (chunks <= (int64_t)ranks * MAX_CHUNKS)
             return ranks;

@@ -566,9 +566,10 @@ int ts2_op_moe_balance_backward(int device, void *stream, int type, const void *
  * p(s) = coef[0] s + coef[1] s^3 + coef[2] s^5 (a host array), |G| the Frobenius norm: Newton-Schulz products that take the
  * singular values to about one.  g: [batch] matrices [rows][cols] of `type`, rows of ld elements, g_stride elements apart (may
  * be 0); out: bf16, alike (out_ld, out_stride); out may be g itself where type is TS2_OUT_BF16 and the pitches agree.  A zero
- * matrix gives zeros, one with a NaN or an infinity NaNs; the scale of g does not matter.  Products are fp16 with fp32 sums, the
- * iterate is held in 32 bits: for the usual coefficients (3.4445, -4.7750, 2.0315) and 5 steps the result is within 1.5e-3 (relative L2,
- * before its rounding to bf16) of the formula, 2.5e-3 for matrices of fewer than 24 rows or columns, whose few entries average less.  TS2_ERR_UNSUPPORTED for coefficients that can take a singular value beyond 3.9, or
+ * matrix gives zeros, one with a NaN or an infinity NaNs; the scale of g does not matter.  The iterate and the operands of all products
+ * are held as two fp16 halves each, sums are fp32: for the usual coefficients (3.4445, -4.7750, 2.0315) and 5 steps the result is within
+ * 1e-4 (relative L2, before its rounding to bf16) of the formula for matrices of up to 8192 rows and columns, of whatever rank and
+ * spectrum.  TS2_ERR_UNSUPPORTED for coefficients that can take a singular value beyond 3.9, or
  * |coef[1] s^2 + coef[2] s^4| beyond 31, which the fp16 scaling does not allow.  Up to 64 steps, 65535 matrices, 2^20 rows and columns. */
 int ts2_op_orthogonalize(int device, void *stream, int type, const void *g, int64_t ld, int64_t g_stride, int batch, int64_t rows, int64_t cols,
                          const float coef[3], int steps, float out_scale, void *out, int64_t out_ld, int64_t out_stride);

@@ -80,3 +80,26 @@ def test_types_of_matrices_that_a_cluster_holds(name, kind):
 @pytest.mark.parametrize("coef,steps", [(COEF, 1), (COEF, 2), ((1.875, -1.25, 0.375), 8), ((1.5, -0.5, 0.0), 12)])
 def test_other_coefficients_of_matrices_that_a_cluster_holds(coef, steps):
     check(falling(100, 300, 1), 3, coef=coef, steps=steps)
+
+
+# products through memory: whole and half tiles, divided K, rows that are not a tile, more of K than a cluster holds
+LARGE = {"130x140": (rank(130, 140, 130), 3), "rank 1 of 200x300": (rank(200, 300, 1), 2), "rank 4 of 700x260": (rank(700, 260, 4), 2),
+         "2 rows of 1000x400": (sparse(1000, 400, 2), 2), "1/k^2, 512x1024": (falling(512, 1024, 2), 1), "1/k, 300x2500": (falling(300, 2500, 1), 1),
+         "20x6300": (rank(20, 6300, 20), 2), "rank 1 of 7000x64": (rank(7000, 64, 1), 1), "rank 2 of 30 of 200x264": (rank(200, 264, 2), 30),
+         "1500x1100": (falling(1500, 1100, 0.5), 1)}
+
+
+@pytest.mark.parametrize("name", LARGE)
+def test_products_through_memory(name):
+    check(*LARGE[name])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("name", ["130x140", "rank 4 of 700x260"])
+def test_types_of_products_through_memory(name, kind):
+    check(*LARGE[name], kind=kind)
+
+
+@pytest.mark.parametrize("coef,steps", [(COEF, 1), (COEF, 2), ((1.875, -1.25, 0.375), 8), ((1.5, -0.5, 0.0), 12)])
+def test_other_coefficients_of_products_through_memory(coef, steps):
+    check(falling(300, 280, 1), 1, coef=coef, steps=steps)

@@ -3,12 +3,12 @@
 //     X = G / |G|;   `steps` times:  A = X X^T,  B = b A + c A A,  X = a X + B X
 // in the orientation with fewer rows than columns.  A zero matrix gives zeros.
 //
-// The products are fp16 with fp32 sums on the tensor cores.  X itself is kept in 32 bits, as two halves: small singular values
-// are carried by the term a X and grow by a factor a in every step, so one rounding of X to 16 bits grows with them (a spectrum
-// that falls off as 1/k^2, 512 x 1024, coefficients 3.4445, -4.7750, 2.0315, 5 steps: relative error 2.0e-2 with X in fp16,
-// 1.8e-4 with X in two halves; flat spectra 2.0e-3 and 1.3e-3).  For the same reason the diagonal of B, which is its largest part, stays in fp32 beside the zeros
-// of the operand: X = (a + diagonal) X + B X (flat spectra 1.3e-3 -> 0.8e-3).  All fp16 values are scaled by powers of two that keep them
-// below 65504 for every X the coefficients can reach (orthogonalize_in_range).
+// The products are fp16 with fp32 sums on the tensor cores, of operands in two halves: hi hi + hi lo + lo hi (lo lo would be 2^-22 of
+// it).  X, A and B are such pairs in memory, too.  One half would be a third of the tensor work (32 x 1024 x 1024: 1.07 ms), but small
+// singular values are carried by the term a X and grow by a factor a in every step, and so does what a rounding leaves in directions
+// that X does not have: with 16 bits of X results were 2e-2 off where the spectrum falls off as 1/k^2, with X in two halves and operands
+// of one 1e-3 for flat spectra, 6e-3 where two rows hold everything and up to 2e-2 for one direction.  All fp16 values are scaled by
+// powers of two that keep them below 65504 for every X the coefficients can reach (orthogonalize_in_range).
 #include "orth.cuh"
 #include "pair_ptx.cuh"
 #include <cuda.h>
@@ -18,23 +18,7 @@
 namespace ts2 {
 
 static constexpr float SX = ORTH_SX, SA = ORTH_SA, SB = ORTH_SB, MAX_X = ORTH_MAX_X, MAX_B = ORTH_MAX_B;
-static constexpr float LO = 2048.f; // the low half is stored times 2^11: its values are below 2^-11 of the high half's
-
-__device__ __forceinline__ void split(float x, __half &hi, __half &lo)
-{
-    hi = __low2half(sat_half2(x, x));
-    const float r = (x - __half2float(hi)) * LO;
-    lo = __low2half(sat_half2(r, r));
-}
-
 constexpr int PT = 256, BK = 64, HALF = 128 * 128; // HALF: a CTA's part of the first operand, one K block
-// Order of the low halves of a tile of 256 x 256: [CTA of the pair][epilogue warp][block of 32 columns][piece of 8][lane = row]
-constexpr int HALF_PIECES = PT * PT / 8;
-__device__ __forceinline__ int lane_piece(int row, int col) // of the piece at column col
-{
-    return ((((row >> 7) * 8 + (row >> 5 & 3) + 4 * (col >> 7)) * 4 + (col >> 5 & 3)) * 4 + (col >> 3 & 3)) * 32 + (row & 31);
-}
-
 // ---- G -> X ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ double warp_sum(double v)
 {
@@ -77,7 +61,7 @@ __global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g,
 // 64 x 64 of X [n][m] (padded to np x mp with zeros) from G, transposed where G has more rows than columns
 template <class T, bool TALL>
 __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, bool vec,
-                                                        const double *part, int n_part, int np, int mp, __half *hi, uint4 *lo, int col_tiles, int tiles)
+                                                        const double *part, int n_part, int np, int mp, __half *hi, __half *lo)
 {
     grid_dep_wait();
     __shared__ double norm;
@@ -118,16 +102,14 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int i = q + 32 * h;
-        alignas(16) __half hs[8], ls[8];
+        float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float x = TALL ? tile[c8 + j][i] : v[h][j];
-            split(small ? (float)(x * scale) : x * scale32, hs[j], ls[j]);
+            x[j] = TALL ? tile[c8 + j][i] : v[h][j];
+            x[j] = small ? (float)(x[j] * scale) : x[j] * scale32;
         }
         const size_t at = ((size_t)b * np + i0 + i) * mp + j0 + c8;
-        *(uint4 *)(hi + at) = *(uint4 *)hs;
-        const int row = i0 + i, col = j0 + c8;
-        lo[((size_t)b * tiles + (row / PT) * col_tiles + col / PT) * HALF_PIECES + lane_piece(row % PT, col % PT)] = *(uint4 *)ls;
+        orth_split8(x, *(uint4 *)(hi + at), *(uint4 *)(lo + at));
     }
 }
 
@@ -135,17 +117,19 @@ __global__ void __launch_bounds__(256) orth_load_kernel(const T *__restrict__ g,
 // Pairs of CTAs on tiles of 256 x 256 or 256 x 128 (as in gemm_pair.cu), one launch for a product of every matrix of the batch.
 //   SQUARE  A = X X^T     POLY  B = b A + c A A     both operands K-contiguous; symmetric, so only tiles on and above the diagonal are
 //                         computed, and what is above it leaves a second time as its transpose
-//   UPDATE  X = a X + B X   B is K-contiguous (it is its own transpose), X is contiguous along N; writes the high halves to a second
-//                         array, since other tiles still read them, and the low halves in place
+//   UPDATE  X = a X + B X   B is K-contiguous (it is its own transpose), X is contiguous along N; writes a second pair of arrays, since
+//                         other tiles still read the first
 //   LAST    UPDATE of the last step: writes the result
 //   PARTIAL a K range of SQUARE or POLY in fp32, for outputs of few tiles; orth_join_kernel adds the ranges
-// Residual inputs are read row by row and handed out to the threads, which have a row of 32 each, through shared memory; the low
-// halves, which nothing else reads, lie in the order of these threads (lane_piece).  Results leave as blocks of 32 x 32 by TMA.
+// A pair of arrays is one tensor of 2 x batch matrices, the low halves behind the high ones.  A slot of the ring holds the high or the low
+// halves of a K block; the products of a block begin with its first slot and free both.  Residual inputs are read row by row and
+// handed out to the threads, which have a row of 32 each, through shared memory; results leave from there as blocks of 32 x 32 by TMA.
 enum Form { SQUARE, POLY, UPDATE, PARTIAL, LAST };
 constexpr bool updates(int form) { return form == UPDATE || form == LAST; }
-constexpr int STAGES = 5, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS, BLOCKS = 2;
-// an epilogue warp's shared memory: two blocks of 32 x 32 on their way out, 32 x 64 of the residual input
-constexpr int BLOCK = 2048, WARP_BYTES = BLOCKS * BLOCK + 4096, STG_OFF = STAGES * 2 * HALF, BAR_OFF = STG_OFF + EPI_WARPS * WARP_BYTES,
+constexpr int STAGES = 5, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+// an epilogue warp's shared memory: blocks of 32 x 32, high and low halves of the residual input and then of the output, and of what is
+// mirrored
+constexpr int BLOCK = 2048, WARP_BYTES = 4 * BLOCK, STG_OFF = STAGES * 2 * HALF, BAR_OFF = STG_OFF + EPI_WARPS * WARP_BYTES,
               SMEM = BAR_OFF + 1024 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 
@@ -155,10 +139,9 @@ struct ProductArgs {
     int units, k_blocks, splits, kb_per_split;
     float alpha, beta; // POLY: alpha acc + beta A; UPDATE: alpha acc + beta X; else alpha acc
     float *part;       // PARTIAL: [matrix][tile][split][256][256]
-    const __half *res; // A, or the high halves of X
-    uint4 *lo;         // the low halves, [matrix][tile of 256 x 256 of X] in the order of lane_piece
-    int low_tiles, low_cols;
-    float *diag;       // [matrix][n]: the diagonal of B
+    const __half *res; // A, or X: the high halves, the low ones res_low elements behind them
+    size_t res_low;
+    int batch; // the low halves of matrix i are matrix batch + i of a pair
     // LAST
     __nv_bfloat16 *out;
     long long ld_out, out_stride;
@@ -167,7 +150,7 @@ struct ProductArgs {
     bool tall, vec_out;
     int32_t *status;
 };
-struct Unit {
+struct ProductUnit {
     int matrix, row, col, kb0, kb1, index;
 };
 // the r-th tile on or above the diagonal of a square of tiles, column by column
@@ -181,9 +164,9 @@ __device__ __forceinline__ void upper_tile(int r, int &row, int &col)
     row = r - col * (col + 1) / 2;
 }
 template <int FORM, int PN>
-__device__ __forceinline__ Unit product_unit(const ProductArgs &p, int u)
+__device__ __forceinline__ ProductUnit product_unit(const ProductArgs &p, int u)
 {
-    Unit t;
+    ProductUnit t;
     const int tile = u / p.splits, split = u - tile * p.splits;
     t.index = u;
     t.matrix = tile / p.tiles;
@@ -212,7 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         const ProductArgs p)
 {
     constexpr int STAGE = HALF + PN * 64, PART = PN / 2; // bytes; columns of an epilogue warp
-    constexpr int RES = FORM == POLY ? 1 : updates(FORM) ? 2 : 0; // residual arrays
+    constexpr bool RES = FORM == POLY || updates(FORM); // there is a residual input
     extern __shared__ uint8_t orth_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)orth_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
     uint64_t *bars = (uint64_t *)(smem + BAR_OFF);
@@ -256,9 +239,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             uint32_t phase = 0;
             bool ok = true;
             for (int u = first; u < p.units && ok; u += step) {
-                const Unit un = product_unit<FORM, PN>(p, u);
+                const ProductUnit un = product_unit<FORM, PN>(p, u);
                 const int am = un.row + (int)rank * 128, bn = un.col + (int)rank * (PN / 2);
-                for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                for (int i = 2 * un.kb0; i < 2 * un.kb1; ++i) { // the high, then the low halves of a K block
+                    const int kb = i >> 1, matrix = un.matrix + (i & 1 ? p.batch : 0);
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
                         ok = false;
                         break;
@@ -267,13 +251,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (rank == 0)
                         mbar_arrive_expect_tx(full0 + 8 * stage, 2 * STAGE);
                     const uint32_t sa = smem_u32(smem + stage * STAGE), sb = sa + HALF;
-                    tma_load_3d_pair(sa, &tmA, fb, kb * BK, am, un.matrix);
+                    tma_load_3d_pair(sa, &tmA, fb, kb * BK, am, matrix);
                     if constexpr (updates(FORM)) {
-                        tma_load_3d_pair(sb, &tmB, fb, bn, kb * BK, un.matrix);
+                        tma_load_3d_pair(sb, &tmB, fb, bn, kb * BK, matrix);
                         if (PN == PT)
-                            tma_load_3d_pair(sb + BK * 128, &tmB, fb, bn + 64, kb * BK, un.matrix);
+                            tma_load_3d_pair(sb + BK * 128, &tmB, fb, bn + 64, kb * BK, matrix);
                     } else {
-                        tma_load_3d_pair(sb, &tmB, fb, kb * BK, bn, un.matrix);
+                        tma_load_3d_pair(sb, &tmB, fb, kb * BK, bn, matrix);
                     }
                     ++issued;
                     if (++stage == STAGES) {
@@ -304,25 +288,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             for (int u = first; u < p.units && ok; u += step) {
-                const Unit un = product_unit<FORM, PN>(p, u);
+                const ProductUnit un = product_unit<FORM, PN>(p, u);
                 if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag))
                     break;
                 tc_fence_after();
                 const uint32_t tmem_d = tmem_base + acc * PT;
-                for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                const auto multiply = [&](int left, int right, bool clear) { // of the operands in these slots
+                    const uint32_t a = smem_u32(smem + left * STAGE), b = smem_u32(smem + right * STAGE) + HALF;
+                    const uint64_t adesc = umma_smem_desc(a, 16, 1024), bdesc = umma_smem_desc(b, updates(FORM) ? BK * 128 : 16, 1024);
+                    constexpr uint64_t a_step = 2, b_step = updates(FORM) ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_pair<1>(tmem_d, adesc + k * a_step, bdesc + k * b_step, idesc, !clear || k > 0 ? 1u : 0u);
+                };
+                int high = 0; // the slot of the block's high halves
+                for (int i = 2 * un.kb0; i < 2 * un.kb1; ++i) {
                     if (!mbar_wait(full0 + 8 * stage, phase, abort_flag)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + stage * STAGE);
-                    const uint64_t adesc = umma_smem_desc(sa, 16, 1024);
-                    const uint64_t bdesc = umma_smem_desc(sa + HALF, updates(FORM) ? BK * 128 : 16, 1024);
-                    constexpr uint64_t a_step = 2, b_step = updates(FORM) ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_pair<1>(tmem_d, adesc + k * a_step, bdesc + k * b_step, idesc, (kb > un.kb0 || k > 0) ? 1u : 0u);
-                    commit_both(empty0 + 8 * stage);
+                    if (i & 1) {
+                        multiply(high, stage, false);
+                        multiply(stage, high, false);
+                        commit_both(empty0 + 8 * high);
+                        commit_both(empty0 + 8 * stage);
+                    } else {
+                        multiply(stage, stage, i == 2 * un.kb0);
+                        high = stage;
+                    }
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1;
@@ -340,45 +334,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
         }
     } else {
-        // epilogue: a warp takes 32 rows x 64 columns in two blocks of 32 x 32, thread = row
+        // epilogue: a warp takes 32 rows x PART columns in blocks of 32 x 32, thread = row
         const int quarter = warp & 3, ew = warp - 2, part = ew >> 2;
-        uint8_t *const blocks = smem + STG_OFF + ew * WARP_BYTES, *const handed = blocks + BLOCKS * BLOCK; // in turn, a store's each
+        uint8_t *const high = smem + STG_OFF + ew * WARP_BYTES, *const low = high + BLOCK, *const mirrored = low + BLOCK;
         const int sw = (lane >> 1) & 3; // the 64-byte swizzle of the thread's row
-        int acc = 0, block = 0;
+        uint32_t column[4];             // of the thread in a mirrored row; the swizzle of rows 8 i + 2 j and the one behind is j
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            column[j] = smem_u32(mirrored) + (((lane >> 3) ^ j) << 4) + (lane & 7) * 2;
+        int acc = 0;
         uint32_t acc_phase = 0;
         for (int u = first; u < p.units; u += step) {
-            const Unit un = product_unit<FORM, PN>(p, u);
+            const ProductUnit un = product_unit<FORM, PN>(p, u);
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PT + part * PART;
             const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
             const auto there = [&](int c) { return row0 < p.n && col0 + c * 32 < p.cols; }; // multiples of 32: a block is there or not
-            uint4 rows[8], xs[4], ls[4]; // of 32 rows x 64: 8 lanes a row; of the block at hand: the thread's row
-            const auto fetch = [&](int h) {
-                if constexpr (RES > 0) {
-                    if (!there(2 * h))
+            uint4 rows[2][4]; // of the next block of the residual input, high and low halves: 4 lanes a row, 8 rows at a time
+            const auto fetch = [&](int c) {
+                if constexpr (RES) {
+                    if (!there(c))
                         return;
-                    const __half *from = p.res + ((size_t)un.matrix * p.n + row0 + (lane >> 3)) * p.cols + col0 + h * 64 + (lane & 7) * 8;
+                    const __half *from = p.res + ((size_t)un.matrix * p.n + row0 + (lane >> 2)) * p.cols + col0 + c * 32 + (lane & 3) * 8;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        rows[i] = *(const uint4 *)(from + (size_t)(4 * i) * p.cols);
+                    for (int i = 0; i < 4; ++i) {
+                        rows[0][i] = *(const uint4 *)(from + (size_t)(8 * i) * p.cols);
+                        rows[1][i] = *(const uint4 *)(from + p.res_low + (size_t)(8 * i) * p.cols);
+                    }
                 }
             };
-            uint4 *const lows = p.lo + ((size_t)un.matrix * p.low_tiles + un.row / PT * p.low_cols + un.col / PT) * HALF_PIECES +
-                               lane_piece(row0 - un.row + lane, un.col % PT + part * PART);
-            const auto fetch_low = [&](int c) {
-                if constexpr (RES == 2)
-                    if (there(c)) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            ls[i] = lows[(c * 4 + i) * 32];
-                    }
-            };
             fetch(0);
-            fetch_low(0);
-            const float beta = p.beta + (RES == 2 && there(0) ? p.diag[(size_t)un.matrix * p.n + row0 + lane] : 0.f);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag)))
                 break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < PART / 32; ++c) {
                 uint32_t r[32];
                 __syncwarp(); // lane 0 comes from its stores
@@ -390,57 +378,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (lane == 0)
                         mbar_arrive_cluster(map_to_leader(tempty0 + 8 * acc));
                 }
-                if constexpr (RES > 0) {
-                    if (!(c & 1)) {
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int at = i * 4 + (lane >> 3);
-                            *(uint4 *)(handed + at * 128 + (((lane & 7) ^ (at & 7)) << 4)) = rows[i];
-                        }
-                        __syncwarp();
-                        if (c == 0 && PART > 64)
-                            fetch(1);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        xs[i] = *(const uint4 *)(handed + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
+                if constexpr (FORM != PARTIAL && FORM != LAST) {
+                    if (lane == 0)
+                        bulk_wait_read<0>(); // the stores of the block before have read what lies here
+                    __syncwarp();
                 }
+                if constexpr (RES) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = (8 * i + (lane >> 2)) * 64 + (((lane & 3) ^ (lane >> 3 & 3)) << 4);
+                        *(uint4 *)(high + at) = rows[0][i];
+                        *(uint4 *)(low + at) = rows[1][i];
+                    }
+                    __syncwarp();
+                    if (c + 1 < PART / 32)
+                        fetch(c + 1);
+                }
+                // 8 columns of the thread's row: alpha times the accumulator, and beta times the residual input
+                const auto eight = [&](int i, float (&v)[8]) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        v[j] = p.alpha * __uint_as_float(r[8 * i + j]);
+                    if constexpr (RES) {
+                        const int at = lane * 64 + ((i ^ sw) << 4);
+                        float x[8];
+                        orth_join8(*(const uint4 *)(high + at), *(const uint4 *)(low + at), x);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            v[j] = fmaf(p.beta, x[j], v[j]);
+                    }
+                };
                 const int col = col0 + c * 32;
                 if constexpr (FORM == PARTIAL) {
                     // through shared memory, so that 8 lanes write 128 bytes of a row
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        *(uint4 *)(handed + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                        *(uint4 *)(high + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
                     __syncwarp();
                     float *to = p.part + ((size_t)un.index * PT + (row0 - un.row)) * PT + (col - un.col);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int at = i * 4 + (lane >> 3), q = lane & 7;
-                        *(uint4 *)(to + (size_t)at * PT + q * 4) = *(const uint4 *)(handed + at * 128 + ((q ^ (at & 7)) << 4));
+                        *(uint4 *)(to + (size_t)at * PT + q * 4) = *(const uint4 *)(high + at * 128 + ((q ^ (at & 7)) << 4));
                     }
                 } else if constexpr (FORM == LAST) {
                     const int i0 = row0 + lane; // X's row: (tall) a column of the result, 32 neighbours a store
                     __nv_bfloat16 *out = p.out + un.matrix * p.out_stride;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { // 8 columns
-                        const uint32_t xw[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w}, lw[4] = {ls[i].x, ls[i].y, ls[i].z, ls[i].w};
+                    for (int i = 0; i < 4; ++i) {
+                        float v[8];
+                        eight(i, v);
                         __nv_bfloat162 o[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 x = __half22float2(*(const __half2 *)&xw[j]), l = __half22float2(*(const __half2 *)&lw[j]);
-                            const float v0 = fmaf(beta, fmaf(l.x, 1.f / LO, x.x), p.alpha * __uint_as_float(r[8 * i + 2 * j]));
-                            const float v1 = fmaf(beta, fmaf(l.y, 1.f / LO, x.y), p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]));
-                            o[j] = __floats2bfloat162_rn(v0 * p.out_scale, v1 * p.out_scale);
-                        }
+                        for (int j = 0; j < 4; ++j)
+                            o[j] = __floats2bfloat162_rn(v[2 * j] * p.out_scale, v[2 * j + 1] * p.out_scale);
                         if (p.tall) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
                                 if (i0 < p.out_cols && col + 8 * i + j < p.out_rows)
                                     out[(long long)(col + 8 * i + j) * p.ld_out + i0] = j & 1 ? __high2bfloat16(o[j / 2]) : __low2bfloat16(o[j / 2]);
                         } else {
-                            *(uint4 *)(blocks + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4)) =
+                            *(uint4 *)(mirrored + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4)) =
                                 make_uint4(*(uint32_t *)&o[0], *(uint32_t *)&o[1], *(uint32_t *)&o[2], *(uint32_t *)&o[3]);
                         }
                     }
@@ -451,7 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const int at = i * 4 + (lane >> 3), q = lane & 7;
-                                const uint4 eight = *(const uint4 *)(blocks + at * 128 + ((q ^ (at & 7)) << 4));
+                                const uint4 eight = *(const uint4 *)(mirrored + at * 128 + ((q ^ (at & 7)) << 4));
                                 __nv_bfloat16 *to = out + (long long)(row0 + at) * p.ld_out + left + q * 8;
                                 if (row0 + at >= p.out_rows)
                                     continue;
@@ -470,70 +469,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                     const int k = h * 32 + lane;
                                     if (k < right)
                                         out[(long long)(row0 + at) * p.ld_out + left + k] =
-                                            *(const __nv_bfloat16 *)(blocks + at * 128 + (((k >> 3) ^ (at & 7)) << 4) + (k & 7) * 2);
+                                            *(const __nv_bfloat16 *)(mirrored + at * 128 + (((k >> 3) ^ (at & 7)) << 4) + (k & 7) * 2);
                                 }
                         }
                         __syncwarp();
                     }
-                    if (c + 1 < PART / 32)
-                        fetch_low(c + 1);
                 } else {
                     const bool mirror = FORM != UPDATE && un.col >= un.row + PT;
-                    const int other = block == BLOCKS - 1 ? 0 : block + 1;
-                    uint8_t *const first_block = blocks + block * BLOCK, *const second = blocks + other * BLOCK;
-                    block = other == BLOCKS - 1 ? 0 : other + 1;
-                    if (lane == 0)
-                        bulk_wait_read<BLOCKS - 2>(); // the stores that last used the two blocks have read them
-                    __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { // 8 columns
-                        uint32_t out[4], low[4];
-                        const uint32_t xw[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w}, lw[4] = {ls[i].x, ls[i].y, ls[i].z, ls[i].w};
+                    for (int i = 0; i < 4; ++i) {
+                        float v[8];
+                        eight(i, v);
+                        uint4 h, l;
+                        orth_split8(v, h, l);
+                        const int at = lane * 64 + ((i ^ sw) << 4); // in the place of the thread's residual input
+                        *(uint4 *)(high + at) = h;
+                        *(uint4 *)(low + at) = l;
+                        if (mirror) {
+                            // element (column, row) of the transpose: a column's 32 rows are the 64 bytes of one row there
+                            const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float v0 = p.alpha * __uint_as_float(r[8 * i + 2 * j]), v1 = p.alpha * __uint_as_float(r[8 * i + 2 * j + 1]);
-                            if constexpr (RES > 0) {
-                                float2 x = __half22float2(*(const __half2 *)&xw[j]);
-                                if constexpr (RES == 2) {
-                                    const float2 l = __half22float2(*(const __half2 *)&lw[j]);
-                                    x.x = fmaf(l.x, 1.f / LO, x.x), x.y = fmaf(l.y, 1.f / LO, x.y);
-                                }
-                                v0 = fmaf(beta, x.x, v0), v1 = fmaf(beta, x.y, v1);
-                            }
-                            if constexpr (FORM == POLY)
-                                if (row0 == col && lane >> 1 == 4 * i + j) { // on the diagonal
-                                    if (there(c))
-                                        p.diag[(size_t)un.matrix * p.n + row0 + lane] = (lane & 1 ? v1 : v0) * (1.f / SB);
-                                    (lane & 1 ? v1 : v0) = 0.f;
-                                }
-                            const __half2 h = sat_half2(v0, v1);
-                            out[j] = *(const uint32_t *)&h;
-                            if constexpr (FORM == UPDATE) {
-                                const float2 b = __half22float2(h);
-                                const __half2 l = sat_half2((v0 - b.x) * LO, (v1 - b.y) * LO);
-                                low[j] = *(const uint32_t *)&l;
-                            } else if (mirror) {
-                                // element (column, row) of the transpose: a column's 32 rows are the 64 bytes of one row there
-                                const int k = 8 * i + 2 * j;
-                                *(__half *)(second + k * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __low2half(h);
-                                *(__half *)(second + (k + 1) * 64 + (((lane >> 3) ^ ((k >> 1) & 3)) << 4) + (lane & 7) * 2) = __high2half(h);
+                            for (int j = 0; j < 8; ++j) {
+                                const uint32_t to = column[j >> 1] + (8 * i + j) * 64;
+                                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"((uint16_t)(hw[j >> 1] >> 16 * (j & 1))) : "memory");
+                                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + BLOCK), "h"((uint16_t)(lw[j >> 1] >> 16 * (j & 1))) : "memory");
                             }
                         }
-                        *(uint4 *)(first_block + lane * 64 + ((i ^ sw) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-                        if constexpr (FORM == UPDATE)
-                            if (there(c))
-                                lows[(c * 4 + i) * 32] = make_uint4(low[0], low[1], low[2], low[3]);
                     }
-                    if (c + 1 < PART / 32)
-                        fetch_low(c + 1);
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        if (there(c))
-                            tma_store_3d(&tmC, smem_u32(first_block), col, row0, un.matrix);
-                        bulk_commit();
-                        if (there(c) && mirror)
-                            tma_store_3d(&tmC, smem_u32(second), row0, col, un.matrix);
+                        if (there(c)) {
+                            tma_store_3d(&tmC, smem_u32(high), col, row0, un.matrix);
+                            tma_store_3d(&tmC, smem_u32(low), col, row0, un.matrix + p.batch);
+                            if (mirror) {
+                                tma_store_3d(&tmC, smem_u32(mirrored), row0, col, un.matrix);
+                                tma_store_3d(&tmC, smem_u32(mirrored + BLOCK), row0, col, un.matrix + p.batch);
+                            }
+                        }
                         bulk_commit();
                     }
                 }
@@ -555,7 +528,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 }
 
 // The K ranges of SQUARE or (with a) POLY added in their order; 64 x 64 of a tile per block
-__global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict__ part, const ProductArgs p, const __half *__restrict__ a, __half *out)
+__global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict__ part, const ProductArgs p, bool poly, __half *out, size_t out_low)
 {
     grid_dep_wait();
     __shared__ float tile[64][65];
@@ -569,8 +542,7 @@ __global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict_
         return;
     part += ((size_t)blockIdx.z * p.tiles + blockIdx.y) * p.splits * PT * PT;
     out += (size_t)blockIdx.z * p.n * p.n;
-    if (a)
-        a += (size_t)blockIdx.z * p.n * p.n;
+    const __half *a = p.res + (size_t)blockIdx.z * p.n * p.n; // poly
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int i = q + 32 * h;
@@ -581,21 +553,15 @@ __global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict_
             sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w, sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
         }
         const size_t at = (size_t)(row + i) * p.n + col + c8;
-        uint4 old = make_uint4(0, 0, 0, 0);
-        if (a)
-            old = *(const uint4 *)(a + at);
-        alignas(16) __half o[8];
+        float old[8] = {};
+        if (poly)
+            orth_join8(*(const uint4 *)(a + at), *(const uint4 *)(a + p.res_low + at), old);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float v = a ? fmaf(p.beta, __half2float(((const __half *)&old)[j]), p.alpha * sum[j]) : p.alpha * sum[j];
-            if (a && row + i == col + c8 + j) {
-                p.diag[(size_t)blockIdx.z * p.n + row + i] = v * (1.f / SB);
-                v = 0.f;
-            }
-            tile[i][c8 + j] = v;
-            o[j] = __low2half(sat_half2(v, v));
+            sum[j] = fmaf(p.beta, old[j], p.alpha * sum[j]);
+            tile[i][c8 + j] = sum[j];
         }
-        *(uint4 *)(out + at) = *(uint4 *)o;
+        orth_split8(sum, *(uint4 *)(out + at), *(uint4 *)(out + out_low + at));
     }
     if (!mirror)
         return;
@@ -603,11 +569,12 @@ __global__ void __launch_bounds__(256) orth_join_kernel(const float *__restrict_
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int i = q + 32 * h;
-        alignas(16) __half o[8];
+        float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            o[j] = __low2half(sat_half2(tile[c8 + j][i], 0.f));
-        *(uint4 *)(out + (size_t)(col + i) * p.n + row + c8) = *(uint4 *)o;
+            v[j] = tile[c8 + j][i];
+        const size_t at = (size_t)(col + i) * p.n + row + c8;
+        orth_split8(v, *(uint4 *)(out + at), *(uint4 *)(out + out_low + at));
     }
 }
 
@@ -680,18 +647,18 @@ static int product(const Ctx &c, const CUtensorMap &A, const CUtensorMap &B, con
     return TS2_OK;
 }
 
-// K ranges of a symmetric product: the number with the least estimated time, in K blocks of a tile (0.27 us each).  A tile costs 4
-// more, joining the ranges a launch (10) and its bytes.
+// K ranges of a symmetric product: the number with the least estimated time, in K blocks of a whole tile (0.8 us each).  Halves of few tiles
+// (see `few`) take 0.9 a block; ranges leave fp32 and are joined by another launch, 2.5 and their bytes more than such an epilogue.
+// SQUARE, us of a call with whole tiles, halves, 2 and 4 ranges: 1024 x 1024 332, 306, 292, 278; 2000 x 2000 572, 539, 513, 526; 512 x 512
+// 235, 212, 209, 203; 3 x 1000 x 333 246, 233, 217, 204; SQUARE and POLY of 3000 x 3001 whole 1500, 2 ranges 1413.
 static int choose_splits(int pairs, int64_t tiles, int k_blocks)
 {
-    double best = 1e30;
+    double best = 2 * tiles <= pairs ? 0.9 * k_blocks + 1 : (double)ceil_div(tiles, pairs) * (k_blocks + 1) + 2;
     int splits = 1;
-    for (int s = 1; s <= 64 && s <= k_blocks; ++s) {
+    for (int s = 2; s <= 64 && s <= k_blocks; ++s) {
         const int per = (int)ceil_div(k_blocks, s), used = (int)ceil_div(k_blocks, per);
-        if (used != s)
-            continue;
-        const double cost = (double)ceil_div(tiles * s, pairs) * (per + 4) + (s > 1 ? 10 + 0.3 * tiles * s : 0.);
-        if (cost < best)
+        const double cost = (double)ceil_div(tiles * s, pairs) * (per + 1) + 3.5 + 0.1 * tiles * s + 0.1 * s;
+        if (used == s && cost < best)
             best = cost, splits = s;
     }
     return splits;
@@ -724,47 +691,44 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
     const int split1 = choose_splits(pairs, (int64_t)batch * upper, mp / BK), split2 = choose_splits(pairs, (int64_t)batch * upper, np / BK);
     const int most = std::max(split1, split2);
     const size_t part_bytes = most > 1 ? (size_t)batch * upper * most * PT * PT * 4 : 0;
-    const size_t low_bytes = (size_t)batch * nt * mt * HALF_PIECES * 16;
-    Scratch s(c, part_bytes + low_bytes + x * 4 + a * 4 + (size_t)batch * n_part * 8 + (size_t)batch * np * 4);
+    Scratch s(c, part_bytes + x * 8 + a * 8 + (size_t)batch * n_part * 8);
     if (s.rc != TS2_OK)
         return s.rc;
+    // pairs: the low halves behind the high ones
     float *part = (float *)s.p;
-    uint4 *lows = (uint4 *)((uint8_t *)s.p + part_bytes);
-    __half *hi[2] = {(__half *)((uint8_t *)lows + low_bytes), (__half *)((uint8_t *)lows + low_bytes) + x}, *A = hi[1] + x, *B = A + a;
-    double *sums = (double *)(B + a);
+    __half *X[2] = {(__half *)((uint8_t *)s.p + part_bytes), (__half *)((uint8_t *)s.p + part_bytes) + 2 * x}, *A = X[1] + 2 * x, *B = A + 2 * a;
+    double *sums = (double *)(B + 2 * a);
 
     const bool vec = ((uintptr_t)g | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(stride * sizeof(T))) % 16 == 0;
     TS2_LAUNCH((orth_sum2_kernel<T>), dim3(n_part, batch), 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums);
     const dim3 blocks(mp / 64, np / 64, batch);
     if (tall)
-        TS2_LAUNCH((orth_load_kernel<T, true>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lows, mt,
-                   nt * mt);
+        TS2_LAUNCH((orth_load_kernel<T, true>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, X[0], X[0] + x);
     else
-        TS2_LAUNCH((orth_load_kernel<T, false>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, hi[0], lows, mt,
-                   nt * mt);
+        TS2_LAUNCH((orth_load_kernel<T, false>), blocks, 256, 0, c.stream, g, ld, stride, rows, cols, vec, sums, n_part, np, mp, X[0], X[0] + x);
     CUtensorMap x_rows[2], x_cols[2], x_block[2], a_rows, a_half, a_block, b_rows, b_block; // x_cols, a_half: boxes of 64 rows x 64
     int rc = TS2_OK;
     for (int i = 0; i < 2 && rc == TS2_OK; ++i) {
-        rc = half_map(&x_rows[i], hi[i], mp, np, batch, 64, 128);
+        rc = half_map(&x_rows[i], X[i], mp, np, 2 * batch, 64, 128);
         if (rc == TS2_OK)
-            rc = half_map(&x_cols[i], hi[i], mp, np, batch, 64, 64);
+            rc = half_map(&x_cols[i], X[i], mp, np, 2 * batch, 64, 64);
         if (rc == TS2_OK)
-            rc = half_map(&x_block[i], hi[i], mp, np, batch, 32, 32);
+            rc = half_map(&x_block[i], X[i], mp, np, 2 * batch, 32, 32);
     }
-    if (rc != TS2_OK || (rc = half_map(&a_rows, A, np, np, batch, 64, 128)) || (rc = half_map(&a_half, A, np, np, batch, 64, 64)) ||
-        (rc = half_map(&a_block, A, np, np, batch, 32, 32)) || (rc = half_map(&b_rows, B, np, np, batch, 64, 128)) ||
-        (rc = half_map(&b_block, B, np, np, batch, 32, 32)))
+    if (rc != TS2_OK || (rc = half_map(&a_rows, A, np, np, 2 * batch, 64, 128)) || (rc = half_map(&a_half, A, np, np, 2 * batch, 64, 64)) ||
+        (rc = half_map(&a_block, A, np, np, 2 * batch, 32, 32)) || (rc = half_map(&b_rows, B, np, np, 2 * batch, 64, 128)) ||
+        (rc = half_map(&b_block, B, np, np, 2 * batch, 32, 32)))
         return rc;
     ProductArgs p = {};
     p.status = device_status_word(c.device);
     if (!p.status)
         return fail(TS2_ERR_CUDA, "no device status word");
     p.n = np;
-    p.lo = lows, p.low_tiles = nt * mt, p.low_cols = mt, p.diag = (float *)(sums + (size_t)batch * n_part);
+    p.batch = batch;
     p.part = part;
     // Tiles of 256 x 128 where those of 256 x 256 would leave half of the device without any: half the products and half the epilogue
-    // each, and more SMs at work.  3 x 1000 x 333 166 -> 143 us, 400 x 500 167 -> 133, 4 x 130 x 140 139 -> 108; from 38 tiles on
-    // narrow ones would come in a second round.  Outputs of so few tiles that K is divided keep whole tiles.
+    // each, and more SMs at work.  4 x 130 x 140 184 -> 144 us, 8 x 200 x 264 207 -> 159, 400 x 500 262 -> 207; from 38 tiles on narrow
+    // ones would come in a second round.  Outputs of so few tiles that K is divided keep whole tiles.
     const auto few = [&](int64_t tiles) { return 2 * tiles <= pairs; };
     const auto symmetric = [&](bool poly, int k, int splits, const CUtensorMap &in, const CUtensorMap &in_half, const CUtensorMap &to, __half *dst) {
         p.cols = np, p.tiles = upper, p.col_tiles = 0;
@@ -780,7 +744,7 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
             return poly ? product<POLY>(c, in, in, to, p) : product<SQUARE>(c, in, in, to, p);
         if (int e = product<PARTIAL>(c, in, in, to, p))
             return e;
-        TS2_LAUNCH(orth_join_kernel, dim3(16, upper, batch), 256, 0, c.stream, part, p, poly ? A : (const __half *)nullptr, dst);
+        TS2_LAUNCH(orth_join_kernel, dim3(16, upper, batch), 256, 0, c.stream, part, p, poly, dst, a);
         return TS2_OK;
     };
     for (int k = 0; k < steps; ++k) {
@@ -788,10 +752,10 @@ static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t str
         p.alpha = SA / (SX * SX), p.beta = 0.f;
         if ((rc = symmetric(false, mp, split1, x_rows[now], x_cols[now], a_block, A)))
             return rc;
-        p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA, p.res = A;
+        p.alpha = SB * coef[2] / (SA * SA), p.beta = SB * coef[1] / SA, p.res = A, p.res_low = a;
         if ((rc = symmetric(true, np, split2, a_rows, a_half, b_block, B)))
             return rc;
-        p.alpha = 1.f / SB, p.beta = coef[0], p.res = hi[now];
+        p.alpha = 1.f / SB, p.beta = coef[0], p.res = X[now], p.res_low = x;
         p.cols = mp, p.tiles = nt * mt, p.col_tiles = mt, p.k_blocks = np / BK, p.splits = 1, p.kb_per_split = p.k_blocks, p.units = batch * nt * mt;
         if (k == steps - 1) {
             p.out = out, p.ld_out = ld_out, p.out_stride = out_stride, p.out_rows = rows, p.out_cols = cols, p.out_scale = out_scale / SX, p.tall = tall;

@@ -82,6 +82,8 @@ int ts2_op_moe_balance_forward(int device, void *stream, int type, const void *l
         !rows_ok(logits, ld, T, expert_count, es) || (!ids && T) || !floats_ok(ids) || !counts || !prob || !loss || !floats_ok(counts) ||
         !floats_ok(prob) || !floats_ok(loss))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_moe_balance_forward: bad arguments");
+    if (expert_count > MOE_BALANCE_MAX_EXPERTS)
+        return fail(TS2_ERR_UNSUPPORTED, "ts2_op_moe_balance_forward: at most %d experts (got %d)", MOE_BALANCE_MAX_EXPERTS, expert_count);
     TS2_ON_DEVICE(device);
     return moe_balance_forward(layer_ctx(device, stream), type, logits, ld, T, expert_count, selected, ids, token_mask, counts, prob, loss);
 }
@@ -94,6 +96,8 @@ int ts2_op_moe_balance_backward(int device, void *stream, int type, const void *
     if (!es || T < 0 || T > 1 << 30 || expert_count < 1 || selected < 1 || selected > expert_count || !rows_ok(logits, ld, T, expert_count, es) || !counts ||
         !floats_ok(counts) || !floats_ok(dloss) || !rows_ok(dlogits, dlogits_ld, T, expert_count, es))
         return fail(TS2_ERR_INVALID_ARG, "ts2_op_moe_balance_backward: bad arguments");
+    if (expert_count > MOE_BALANCE_MAX_EXPERTS)
+        return fail(TS2_ERR_UNSUPPORTED, "ts2_op_moe_balance_backward: at most %d experts (got %d)", MOE_BALANCE_MAX_EXPERTS, expert_count);
     TS2_ON_DEVICE(device);
     return moe_balance_backward(layer_ctx(device, stream), type, logits, ld, T, expert_count, selected, token_mask, counts, dloss, scale, dlogits,
                                 dlogits_ld, add != 0);

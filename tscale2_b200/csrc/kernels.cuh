@@ -233,6 +233,7 @@ int moe_router_backward(const Ctx &c, const float *dmoe_part, int tiles, const i
 
 // ---- kernels_balance.cu, kernels_recurrence.cu, kernels_orth.cu ---------------------
 // what the ts2_op_* calls of the same names do (include/ts2_b200.h); type: TS2_OUT_F32, TS2_OUT_F16 or TS2_OUT_BF16
+constexpr int MOE_BALANCE_MAX_EXPERTS = 1024;
 int moe_balance_forward(const Ctx &c, int type, const void *logits, int64_t ld, int64_t T, int E, int selected, const int *ids,
                         const uint8_t *mask, int *counts, float *prob, float *loss);
 int moe_balance_backward(const Ctx &c, int type, const void *logits, int64_t ld, int64_t T, int E, int selected, const uint8_t *mask,

@@ -18,7 +18,7 @@ namespace ts2 {
 
 static constexpr int THREADS = 256, WARPS = THREADS / 32;                // backward
 static constexpr int SUM_THREADS = 512, SUM_WARPS = SUM_THREADS / 32;    // forward
-static constexpr int MAX_EXPERTS = 1024, CLUSTER = 8, MAX_CLUSTERS = 32;
+static constexpr int MAX_EXPERTS = MOE_BALANCE_MAX_EXPERTS, CLUSTER = 8, MAX_CLUSTERS = 32;
 
 template <class T>
 __device__ __forceinline__ float widen(T v) { return (float)v; }
@@ -484,8 +484,6 @@ static int by_type(const Ctx &c, BalanceArgs &p, bool backward)
 
 static int run(const Ctx &c, int type, BalanceArgs &p, bool backward)
 {
-    if (p.E < 1 || p.E > MAX_EXPERTS)
-        return fail(TS2_ERR_UNSUPPORTED, "moe balance: need 1 <= experts <= %d (got %d)", MAX_EXPERTS, p.E);
     switch (type) {
     case TS2_OUT_F32: return by_type<float>(c, p, backward);
     case TS2_OUT_F16: return by_type<__half>(c, p, backward);

@@ -346,6 +346,13 @@ __device__ __forceinline__ __half2 sat_half2(float lo, float hi)
     return *(__half2 *)&r;
 }
 
+__device__ __forceinline__ double warp_sum(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll

@@ -141,21 +141,14 @@ __device__ __forceinline__ int ld_int(uint32_t a)
 }
 
 // 1 / N, and what sum_e C[e] P[e] is multiplied by: found while other things are on their way
-struct Unit {
+struct BalanceUnit {
     double mean, loss;
-    __device__ __forceinline__ Unit(int tokens, int E, int selected)
+    __device__ __forceinline__ BalanceUnit(int tokens, int E, int selected)
     {
         mean = tokens ? 1. / tokens : 0.;
         loss = mean * E / selected;
     }
 };
-__device__ __forceinline__ double warp_sum(double v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
 
 // Two blocks an SM, but where a lane has more than 16 columns (65536 x 512 bf16 41 us; with one, and 32 clusters for which there is no room
 // at once, 69)
@@ -268,7 +261,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS, V
 #pragma unroll
     for (int r = 0; r < CLUSTER; ++r)
         tokens += ld_int(in_rank(&count[E], r));
-    const Unit unit(tokens, E, p.selected);
+    const BalanceUnit unit(tokens, E, p.selected);
     double loss = 0.;
     const size_t cluster = blockIdx.x / CLUSTER;
     for (int e = (int)rank + CLUSTER * threadIdx.x; e < E; e += CLUSTER * SUM_THREADS) {
@@ -320,7 +313,7 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const BalanceArgs 
     __shared__ int counts[1024];
     const int E = p.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x % width, part = threadIdx.x / width;
     const int tokens = __reduce_add_sync(0xffffffffu, lane < clusters ? p.part_count[(size_t)lane * (E + 1) + E] : 0);
-    const Unit unit(tokens, E, p.selected);
+    const BalanceUnit unit(tokens, E, p.selected);
     double sum = 0.;
     int n = 0;
     for (int c = part; c < clusters; c += 8 * parts) {

@@ -20,14 +20,6 @@ namespace ts2 {
 static constexpr float SX = ORTH_SX, SA = ORTH_SA, SB = ORTH_SB, MAX_X = ORTH_MAX_X, MAX_B = ORTH_MAX_B;
 constexpr int PT = 256, BK = 64, HALF = 128 * 128; // HALF: a CTA's part of the first operand, one K block
 // ---- G -> X ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ double warp_sum(double v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // partial sums of squares in fp64: no input over- or underflows, and nothing is lost over 2^40 terms
 template <class T>
 __global__ void __launch_bounds__(256) orth_sum2_kernel(const T *__restrict__ g, long long ld, long long stride, int rows, int cols, bool vec,

@@ -182,9 +182,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
         __syncthreads();
     }
     tmem_st_wait();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum = warp_sum(sum);
     if (lane == 0)
         sums[warp] = sum;
     __syncthreads();

@@ -71,16 +71,10 @@ __device__ __forceinline__ void commit_own(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// 3-D forms of the tiled copies: a load that completes on a barrier of either CTA, a load of this CTA's own, a store (clipped)
+// 3-D forms of the tiled copies: a load that completes on a barrier of either CTA, a store (clipped)
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2)
 {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-                 "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2)
-{
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
                  "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
 }

@@ -103,3 +103,20 @@ def test_types_of_products_through_memory(name, kind):
 @pytest.mark.parametrize("coef,steps", [(COEF, 1), (COEF, 2), ((1.875, -1.25, 0.375), 8), ((1.5, -0.5, 0.0), 12)])
 def test_other_coefficients_of_products_through_memory(coef, steps):
     check(falling(300, 280, 1), 1, coef=coef, steps=steps)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 8192, 1100), (2, 2100, 8192)])
+def test_long_sums(batch, rows, cols):
+    """K of 8192, in ranges and in one piece; the formula in float64 on the device"""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    g = torch.randn((batch, rows, cols), device="cuda", generator=gen) + 0.1 * torch.randn((batch, rows, 8), device="cuda", generator=gen) @ \
+        torch.randn((batch, 8, cols), device="cuda", generator=gen)
+    x = g.double()
+    x /= torch.linalg.matrix_norm(x)[:, None, None]
+    x = x.transpose(1, 2) if rows > cols else x
+    for _ in range(5):
+        a = x @ x.transpose(1, 2)
+        x = COEF[0] * x + (COEF[1] * a + COEF[2] * a @ a) @ x
+    x = (x.transpose(1, 2) if rows > cols else x).cpu().numpy()
+    assert error(run("f32", g.cpu().numpy()), x) <= LIMIT

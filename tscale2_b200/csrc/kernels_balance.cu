@@ -151,7 +151,7 @@ struct BalanceUnit {
 };
 
 // Two blocks an SM, but where a lane has more than 16 columns (65536 x 512 bf16 41 us; with one, and 32 clusters for which there is no room
-// at once, 69)
+// at once, 69).  That spills 48 bytes a thread for 512 columns of 16 bits, and 32 single columns a lane (1024 without alignment) 148.
 template <class T, int VEC, int G, int N>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SUM_THREADS, VEC * N <= 16 ? 2 : 1) balance_sums_kernel(const BalanceArgs p)
 {

@@ -98,8 +98,10 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
     const int row = quarter * 32 + lane, matrix = blockIdx.x / ranks;
     const int j0 = (int)rank * p.chunks * 128;
     const T *g = (const T *)p.g + matrix * p.stride;
+    // (accesses of tensor memory are a warp's: lanes that come from branches of their own meet first)
     const auto load32 = [&](uint32_t column, float (&v)[32]) {
         uint32_t r[32];
+        __syncwarp();
         tmem_ld32(lane_base + column, r);
         tmem_ld_wait();
 #pragma unroll
@@ -108,6 +110,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
     };
     const auto load64 = [&](uint32_t column, float (&v)[2][32]) { // the thread's half of 128 columns; tmem_ld_wait is the caller's
         uint32_t(&r)[2][32] = (uint32_t(&)[2][32])v;
+        __syncwarp();
         tmem_ld32(lane_base + column, r[0]);
         tmem_ld32(lane_base + column + 32, r[1]);
     };
@@ -116,6 +119,7 @@ __global__ void __launch_bounds__(THREADS, 1) orth_chip_kernel(const ChipArgs p)
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             r[i] = __float_as_uint(v[i]);
+        __syncwarp();
         tmem_st32(lane_base + column, r);
     };
 

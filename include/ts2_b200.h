@@ -574,6 +574,75 @@ int ts2_op_moe_balance_backward(int device, void *stream, int type, const void *
 int ts2_op_orthogonalize(int device, void *stream, int type, const void *g, int64_t ld, int64_t g_stride, int batch, int64_t rows, int64_t cols,
                          const float coef[3], int steps, float out_scale, void *out, int64_t out_ld, int64_t out_stride);
 
+/* A dense layer: z = x W^T + bias, y = act(z) + residual, in one pass over the product.  x [T][in_dim], w [out_dim][in_dim], residual
+ * (optional), y and z (optional: what the backward pass needs of a layer with an activation) [T][out_dim], all of `type`
+ * (TS2_OUT_F16 or TS2_OUT_BF16), rows of *_ld elements; bias (optional) fp32 [out_dim].  Sums, bias, activation and residual are fp32,
+ * y and z are rounded once.  residual may be y itself (same pitch): y += act(z).  A few tokens, the step of a generation, take a form
+ * that is bound by reading W.  T up to 2^30, in_dim and out_dim up to 2^20. */
+#define TS2_ACT_NONE 0
+#define TS2_ACT_RELU 1
+#define TS2_ACT_GELU 2 /* z Phi(z), Phi of the error function */
+#define TS2_ACT_SILU 3 /* z / (1 + exp(-z)) */
+int ts2_op_linear_forward(int device, void *stream, int type, int act, int64_t T, int64_t in_dim, int64_t out_dim, const void *x, int64_t x_ld,
+                          const void *w, int64_t w_ld, const float *bias, const void *residual, int64_t residual_ld, void *y, int64_t y_ld, void *z,
+                          int64_t z_ld);
+/* Its backward pass: dz = dy act'(z), dx = dz W, dw = dz^T x, dbias = sum_t dz; the gradient of the residual is dy.  Each of dx, dw and dbias
+ * may be null.  z: what the forward call left; not read where act is TS2_ACT_NONE.  x is read for dw only, w for dx only.  dx [T][in_dim] of `type`; dw
+ * [out_dim][in_dim] of dw_kind: `type`, TS2_OUT_F32 or TS2_OUT_F32_ADD (dw +=); dbias fp32 [out_dim].  With an activation dz is rounded to
+ * `type` for the two products (not for dbias).  T = 0 gives zeros.  All are gradients of the same sign. */
+int ts2_op_linear_backward(int device, void *stream, int type, int act, int64_t T, int64_t in_dim, int64_t out_dim, const void *dy, int64_t dy_ld,
+                           const void *z, int64_t z_ld, const void *x, int64_t x_ld, const void *w, int64_t w_ld, void *dx, int64_t dx_ld,
+                           int dw_kind, void *dw, int64_t dw_ld, float *dbias);
+
+/* Choice of experts from a router's logits, on the device and with a gradient (ts2_moe_route is the reference's rule on host arrays).  Per token
+ *     score[e] = softmax(logits)[e] or 1 / (1 + exp(-logits[e])),   key[e] = score[e] + bias[e]
+ * bias fp32 [expert_count] (optional) moves the choice and not the weights.  With groups > 1 the experts are that many groups of neighbours
+ * (groups divides expert_count); a group's rank is the sum of its group_top (1 or 2) largest keys, and only experts of the groups_kept first groups
+ * can be chosen; up to 32 groups.  ids [T][selected]: the largest keys, descending; the lower index first among equal ones, of groups too.  Keys that differ
+ * are told apart as in fp64, without a bias by the logits themselves.  weights fp32 [T][selected]: scale * score, with
+ * renormalize scale * score / sum of the token's chosen scores.
+ * An expert whose logit is -inf or whose key is -inf or NaN is not chosen, and does not count in its group (a NaN or +inf logit takes out a whole softmax row);
+ * where too few are left, ids ends with -1, weights with 0.  Tokens with a zero byte in token_mask [T] (optional) have ids -1 and weights 0, whatever
+ * their logits are.  expert_count up to 1024, selected up to 32 and to the experts of groups_kept groups, T up to 2^30. */
+#define TS2_SCORE_SOFTMAX 0
+#define TS2_SCORE_SIGMOID 1
+int ts2_op_moe_route_forward(int device, void *stream, int type, int score, const void *logits, int64_t ld, int64_t T, int expert_count, int selected,
+                             const float *bias, int groups, int groups_kept, int group_top, int renormalize, float scale, const uint8_t *token_mask,
+                             int32_t *ids, float *weights);
+/* dlogits (+)= the gradient of those weights: dweights fp32 [T][selected] -> dlogits [T][expert_count] of `type`, rows of dlogits_ld elements.  ids
+ * of the forward call (an id outside [0, expert_count) is a choice not made, and its dweights are not read); tokens that do not count get zeros.  add: dlogits += instead
+ * of =, for the sum with the gradient of ts2_op_moe_balance_backward. */
+int ts2_op_moe_route_backward(int device, void *stream, int type, int score, const void *logits, int64_t ld, int64_t T, int expert_count, int selected,
+                              int renormalize, float scale, const uint8_t *token_mask, const int32_t *ids, const float *dweights, void *dlogits,
+                              int64_t dlogits_ld, int add);
+
+/* One AdamW step of many tensors: with g = fp32(grad * grad_scale) (times *grad_scale_dev, optional, fp32 on the device: unscaling or clipping
+ * that the host does not know yet), r = rate * the tensor's rate and k = step >= 1
+ *     m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+ *     param = param (1 - r decay) - r m / (1 - beta1^k) / (sqrt(v / (1 - beta2^k)) + eps)
+ * tensors: a host array, read before the call returns.  param fp32; grad of grad_type (TS2_OUT_F32, _F16 or _BF16); copy: param rounded to copy_type
+ * (TS2_OUT_F16 or TS2_OUT_BF16), or null; TS2_OUT_F32: no tensor has one.  An ascent direction, as the engine's gradients are, takes a negative
+ * grad_scale.  A captured call repeats its step.
+ * state_bits 32: m, v fp32.  state_bits 8: m, v bytes in e4m3 (v without a sign) and for every 32 neighbours, counted from the tensor's
+ * first element, a power of two 2^(byte - 127) in m_scale and v_scale [ceil(n / 32)]; all bytes zero are zero moments.  The power is that of the largest
+ * magnitude M of the 32, 2^(floor(log2 M) - 7).  A value is rounded to one of its two neighbours so that its expectation is itself: to
+ * step * floor(|value| / step + u); a v that is not zero stays at or above the smallest step.  u of element j of tensor i: the upper (m) or lower (v)
+ * 16 bits of h / 2^16, h = mix32(j * 0x9E3779B1 + key), key = the lower 32 bits of mix64(mix64(seed + step) ^ i); mix32: the finaliser of
+ * MurmurHash3, mix64: SplitMix64's next output for that state.  Moments are summed in fp64 there, so that nothing but u decides.  A NaN or
+ * an infinity in a gradient makes the moments of its 32 neighbours NaN from the next step on.
+ * n up to 2^40 elements and 2^40 in all, beta1 and beta2 in [0, 1), eps > 0, up to 2^20 tensors; tensors may not overlap. */
+typedef struct ts2_adamw_tensor {
+    float *param;
+    const void *grad;
+    void *m, *v;
+    uint8_t *m_scale, *v_scale; /* state_bits 8 */
+    void *copy;
+    int64_t n;
+    float rate, decay;
+} ts2_adamw_tensor;
+int ts2_op_adamw(int device, void *stream, int grad_type, int state_bits, int copy_type, const ts2_adamw_tensor *tensors, int n_tensors, float rate,
+                 float beta1, float beta2, float eps, int64_t step, float grad_scale, const float *grad_scale_dev, uint64_t seed);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,8 @@ LABEL_NEGATIVE, LABEL_MASK = 0x80000000, 0x7FFFFFFF
 PARAM_WEIGHTS, PARAM_MOMENTUM, PARAM_GRADIENT = 0, 1, 2
 OUT_F32, OUT_F32_ADD, OUT_F16, OUT_BF16 = 0, 1, 2, 3
 COMM_ID_BYTES = 128
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 
 class LayerParams(C.Structure):
@@ -54,6 +56,11 @@ class BatchNodes(C.Structure):
 class TrainingStep(C.Structure):
     _fields_ = [("rate", C.c_float), ("l2reg", C.c_float), ("beta1", C.c_float), ("weight0", C.c_float),
                 ("weight1", C.c_float), ("disp_decay", C.c_float)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("copy", C.c_void_p), ("n", C.c_int64), ("rate", C.c_float), ("decay", C.c_float)]
 
 
 class Ts2Error(RuntimeError):
@@ -168,6 +175,11 @@ def _declare(lib):
         "ts2_op_moe_balance_forward": (i32, [i32, vp, i32, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp]),
         "ts2_op_moe_balance_backward": (i32, [i32, vp, i32, vp, i64, i64, i32, i32, vp, vp, vp, f32, vp, i64, i32]),
         "ts2_op_orthogonalize": (i32, [i32, vp, i32, vp, i64, i64, i32, i64, i64, P(f32), i32, f32, vp, i64, i64]),
+        "ts2_op_linear_forward": (i32, [i32, vp, i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64]),
+        "ts2_op_linear_backward": (i32, [i32, vp, i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, i64, vp]),
+        "ts2_op_moe_route_forward": (i32, [i32, vp, i32, i32, vp, i64, i64, i32, i32, vp, i32, i32, i32, i32, f32, vp, vp, vp]),
+        "ts2_op_moe_route_backward": (i32, [i32, vp, i32, i32, vp, i64, i64, i32, i32, i32, f32, vp, vp, vp, vp, i64, i32]),
+        "ts2_op_adamw": (i32, [i32, vp, i32, i32, i32, vp, i32, f32, f32, f32, f32, i64, f32, vp, C.c_uint64]),
         "ts2_gemm_dw": (i32, [i32, vp, i32, i32, i64, i64, i64, vp, vp, vp, f32, vp, C.c_size_t]),
     }
     missing = []

@@ -16,6 +16,21 @@ struct Ctx {
     float s_act = 16.f; // quantization scale of normalized activations (1 for fp16)
 };
 
+// scratch of a call, given back when the call returns (stream-ordered)
+struct Scratch {
+    void *p = nullptr;
+    cudaStream_t stream;
+    int rc;
+    Scratch(const Ctx &c, size_t bytes) : stream(c.stream) { rc = bytes ? scratch_alloc(c.device, bytes, c.stream, &p) : (int)TS2_OK; }
+    ~Scratch()
+    {
+        if (p)
+            scratch_free(stream, p);
+    }
+    Scratch(const Scratch &) = delete;
+    Scratch &operator=(const Scratch &) = delete;
+};
+
 // ---- kernels_batch.cu: batch preparation on the device -------------------------------
 // codes of the batch status record {code, where, detail, detail}; 0 = the batch was well formed
 enum {
@@ -247,6 +262,32 @@ int recurrence_backward(const Ctx &c, int type, const void *gate, int64_t gate_l
 bool orthogonalize_in_range(const float coef[3], int steps);
 int orthogonalize(const Ctx &c, int type, const void *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
                   float out_scale, void *out, int64_t ld_out, int64_t out_stride);
+
+// ---- kernels_linear.cu, kernels_route.cu, kernels_adamw.cu ---------------------------
+// what ts2_op_linear_*, ts2_op_moe_route_* and ts2_op_adamw do (include/ts2_b200.h)
+struct LinearShape {
+    int64_t T;
+    int in, out;
+    int type, act; // TS2_OUT_F16 or TS2_OUT_BF16; TS2_ACT_*
+};
+int linear_forward(const Ctx &c, const LinearShape &s, const void *x, int64_t x_ld, const void *w, int64_t w_ld, const float *bias,
+                   const void *residual, int64_t residual_ld, void *y, int64_t y_ld, void *z, int64_t z_ld);
+int linear_backward(const Ctx &c, const LinearShape &s, const void *dy, int64_t dy_ld, const void *z, int64_t z_ld, const void *x, int64_t x_ld,
+                    const void *w, int64_t w_ld, void *dx, int64_t dx_ld, int dw_kind, void *dw, int64_t dw_ld, float *dbias);
+constexpr int MOE_ROUTE_MAX_EXPERTS = 1024, MOE_ROUTE_MAX_SELECTED = 32, MOE_ROUTE_MAX_GROUPS = 32;
+struct RouteShape {
+    int type, score; // TS2_OUT_F32, _F16, _BF16; TS2_SCORE_*
+    int64_t T;
+    int E, selected;
+    bool renormalize;
+    float scale;
+};
+int moe_route_forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const float *bias, int groups, int groups_kept, int group_top,
+                      const uint8_t *mask, int *ids, float *weights);
+int moe_route_backward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const uint8_t *mask, const int *ids, const float *dweights,
+                       void *dlogits, int64_t dlogits_ld, bool add);
+int adamw(const Ctx &c, int grad_type, int state_bits, int copy_type, const ts2_adamw_tensor *tensors, int n, float rate, float beta1, float beta2,
+          float eps, int64_t step, float grad_scale, const float *grad_scale_dev, uint64_t seed);
 
 // ---- kernels_opt.cu ----------------------------------------------------------------
 // ---- flat, sharded optimizer + requantiser (kernels_opt.cu) -------------------------

@@ -10,6 +10,7 @@
 // block's rows are done; the blocks of a cluster join theirs through distributed shared memory, so that a small call is one
 // launch and a large one leaves a partial result per cluster to a second.  All sums have a fixed order; counts are integers, so
 // that the order of their atomics does not matter.
+#include "elem_types.cuh"
 #include "kernels.cuh"
 #include "pair_ptx.cuh"
 #include <algorithm>
@@ -19,22 +20,6 @@ namespace ts2 {
 static constexpr int THREADS = 256, WARPS = THREADS / 32;                // backward
 static constexpr int SUM_THREADS = 512, SUM_WARPS = SUM_THREADS / 32;    // forward
 static constexpr int MAX_EXPERTS = MOE_BALANCE_MAX_EXPERTS, CLUSTER = 8, MAX_CLUSTERS = 32;
-
-template <class T>
-__device__ __forceinline__ float widen(T v) { return (float)v; }
-template <class T>
-__device__ __forceinline__ T narrow(float v);
-template <>
-__device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half narrow<__half>(float v) { return __low2half(sat_half2(v, v)); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-template <class T, int VEC>
-struct alignas(VEC * sizeof(T)) Piece {
-    T v[VEC];
-};
 
 // Columns of a lane: piece i holds columns (i G + lane of the group) VEC ...
 template <class T, int VEC, int G, int N>

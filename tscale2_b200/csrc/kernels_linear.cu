@@ -1,0 +1,823 @@
+// A dense layer, z = x W^T + bias, y = act(z) + residual, and its backward pass: dz = dy act'(z), dx = dz W, dw = dz^T x, dbias = sum_t dz.
+//
+// The three products are one kernel: pairs of CTAs (tcgen05 with cta_group::2) on tiles of 256 x 256 or 256 x 128 of the output, operands by TMA from where they
+// lie, either contiguous along K (x, W and dz in the forward product and dx) or along the output's rows or columns (W in dx; dz and x in
+// dw).  fp16 or bf16 operands, fp32 sums in tensor memory, two accumulators so that a tile's epilogue runs beside the next tile's products.  The
+// epilogue adds the bias, takes the activation and adds the residual in fp32, rounds once, and sends blocks of 32 rows x 128 bytes by TMA.
+// Large products are bound by the tensor pipe (under the part's power limit), small ones by the latency of a launch and the first loads.  Outputs of few tiles are
+// divided along K: partial tiles in fp32, added in their order by a second launch that runs the epilogue.
+// Rows that TMA cannot address (a base or a pitch that is no multiple of 16 bytes) are copied to a pitch that it can.
+#include "elem_types.cuh"
+#include "kernels.cuh"
+#include "pair_ptx.cuh"
+#include <cuda.h>
+#include <algorithm>
+
+namespace ts2 {
+
+namespace {
+
+constexpr int PM = 256, BK = 64, HALF = 128 * BK * 2; // HALF: a CTA's 128 rows of an operand, one K block, bytes
+constexpr int STAGES = 4, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int BLOCK = 4096, SLOTS = 3; // an epilogue warp's blocks of 32 rows x 128 bytes on their way out
+constexpr int STG_OFF = STAGES * 2 * HALF, BAR_OFF = STG_OFF + EPI_WARPS * SLOTS * BLOCK, SMEM = BAR_OFF + 256 + 1024;
+static_assert(SMEM <= 232448, "shared memory budget");
+enum { KIND_PARTIAL = 16 }; // beside TS2_OUT_*: fp32 partial tiles
+
+struct LinearArgs {
+    int m, n; // rows and columns of the output
+    int m_tiles, n_tiles, units, k_blocks, splits, kb_per_split;
+    int kind, act;
+    const float *bias;
+    const void *res;
+    int64_t res_ld;
+    void *y, *z;
+    int64_t y_ld, z_ld;
+    bool y_tma, z_tma, res_vec, bias_vec; // what 16-byte accesses can reach
+    bool ends_whole;                      // a row of y and z is a multiple of 16 bytes
+    float *part;
+    int32_t *status;
+};
+struct Unit {
+    int row, col, kb0, kb1;
+};
+// Units go through the output in bands of 8 rows of tiles, column by column, so that the tiles at work at a time share rows and columns of the operands in
+// the L2; the K ranges of a tile are neighbours.
+template <int PN>
+__device__ __forceinline__ Unit unit_of(const LinearArgs &p, int u)
+{
+    const int tile = u / p.splits, split = u - tile * p.splits, band = tile / (8 * p.n_tiles), rest = tile - band * 8 * p.n_tiles;
+    const int high = min(8, p.m_tiles - band * 8), col = rest / high;
+    Unit t;
+    t.row = (band * 8 + rest - col * high) * PM;
+    t.col = col * PN;
+    t.kb0 = split * p.kb_per_split;
+    t.kb1 = min(p.k_blocks, t.kb0 + p.kb_per_split);
+    return t;
+}
+
+// ---- activations ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// 1 - Phi(|z|) and exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun for the error function (absolute error below 1.5e-7): a third of the instructions of
+// erff, and far below the rounding of a 16-bit result
+__device__ __forceinline__ float normal_tail(float z, float &e)
+{
+    const float a = fabsf(z), t = rcp(fmaf(a, 0.3275911f * 0.70710678f, 1.f));
+    e = ex2(z * z * -0.72134752f);
+    return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f) * e;
+}
+template <int ACT>
+__device__ __forceinline__ float activation(float z)
+{
+    if (ACT == TS2_ACT_RELU)
+        return z < 0.f ? 0.f : z; // a NaN stays one
+    if (ACT == TS2_ACT_GELU) {
+        float e;
+        return fmaf(-fminf(fabsf(z), 64.f), normal_tail(z, e), z < 0.f ? 0.f : z); // z Phi(z) = max(z, 0) - |z| (1 - Phi(|z|))
+    }
+    if (ACT == TS2_ACT_SILU)
+        return z * rcp(1.f + ex2(z * -1.44269504f));
+    return z;
+}
+template <int ACT>
+__device__ __forceinline__ float activation_slope(float z)
+{
+    if (ACT == TS2_ACT_RELU)
+        return z > 0.f ? 1.f : 0.f;
+    if (ACT == TS2_ACT_GELU) {
+        float e;
+        const float tail = normal_tail(z, e);
+        return fmaf(fminf(fmaxf(z, -64.f), 64.f) * 0.39894228f, e, z < 0.f ? tail : 1.f - tail);
+    }
+    if (ACT == TS2_ACT_SILU) {
+        const float s = rcp(1.f + ex2(z * -1.44269504f));
+        return s * fmaf(z, 1.f - s, 1.f);
+    }
+    return 1.f;
+}
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N])
+{
+    switch (act) {
+    case TS2_ACT_RELU:
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = activation<TS2_ACT_RELU>(v[i]);
+        break;
+    case TS2_ACT_GELU:
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = activation<TS2_ACT_GELU>(v[i]);
+        break;
+    case TS2_ACT_SILU:
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = activation<TS2_ACT_SILU>(v[i]);
+        break;
+    default: break;
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    if (BF16) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+        return *(const uint32_t *)&r;
+    }
+    const __half2 r = sat_half2(lo, hi);
+    return *(const uint32_t *)&r;
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v)
+{
+    return BF16 ? __bfloat1622float2(*(const __nv_bfloat162 *)&v) : __half22float2(*(const __half2 *)&v);
+}
+template <bool BF16>
+__device__ __forceinline__ float widen16(uint16_t v)
+{
+    return unpack2<BF16>(v).x;
+}
+
+__device__ __forceinline__ void tma_add_2d(const void *tmap, uint32_t src, int c0, int c1)
+{
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src), "r"(c0), "r"(c1)
+                 : "memory");
+}
+
+// ---- the product ----------------------------------------------------------------------------------------------------------
+// A_MN, B_MN: that operand is contiguous along the output's rows (columns) instead of along K.  tmA, tmB: boxes of 64 along K x 128 (B of PN = 128: 64)
+// rows, or of 64 rows or columns x 64 along K; tmY, tmZ: blocks of 32 rows x 128 bytes; all 128-byte swizzle
+template <bool A_MN, bool B_MN, int PN, bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    linear_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
+                          const __grid_constant__ CUtensorMap tmZ, const LinearArgs p)
+{
+    constexpr int PART = PN / 2, STAGE = HALF + PART * BK * 2;
+    extern __shared__ uint8_t linear_smem[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)linear_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
+    uint64_t *bars = (uint64_t *)(smem + BAR_OFF);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), tfull0 = smem_u32(bars + 2 * STAGES),
+                   tempty0 = smem_u32(bars + 2 * STAGES + 2), drain = smem_u32(bars + 2 * STAGES + 4);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 5);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull0 + 8 * a, 1);
+            mbar_init(tempty0 + 8 * a, 2 * EPI_WARPS); // the leader's counts the epilogue warps of both CTAs
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmA);
+        prefetch_tmap(&tmB);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); // both CTAs' barriers exist
+    tc_fence_after();
+    grid_dep_wait();
+    const uint32_t tmem_base = *tmem_slot;
+    const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+
+    if (warp == 0) {
+        // TMA producer of the CTA's halves; all copies of a stage complete on the leader's barrier
+        if (lane == 0) {
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int u = first; u < p.units && ok; u += step) {
+                const Unit un = unit_of<PN>(p, u);
+                const int am = un.row + (int)rank * 128, bn = un.col + (int)rank * PART;
+                for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = map_to_leader(full0 + 8 * stage);
+                    if (rank == 0)
+                        mbar_arrive_expect_tx(full0 + 8 * stage, 2 * STAGE);
+                    const uint32_t sa = smem_u32(smem + stage * STAGE), sb = sa + HALF;
+                    if constexpr (A_MN) {
+                        tma_load_2d_pair(sa, &tmA, fb, am, kb * BK);
+                        tma_load_2d_pair(sa + BK * 128, &tmA, fb, am + 64, kb * BK);
+                    } else {
+                        tma_load_2d_pair(sa, &tmA, fb, kb * BK, am);
+                    }
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < PART / 64; ++j)
+                            tma_load_2d_pair(sb + j * BK * 128, &tmB, fb, bn + 64 * j, kb * BK);
+                    } else {
+                        tma_load_2d_pair(sb, &tmB, fb, kb * BK, bn);
+                    }
+                    ++issued;
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok && rank == 0) { // copies in flight land (a bounded wait) before the CTA may leave
+                int s = stage;
+                uint32_t ph = phase;
+                for (int i = 0; i < min(issued, STAGES); ++i) {
+                    if (--s < 0) {
+                        s = STAGES - 1;
+                        ph ^= 1;
+                    }
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(full0 + 8 * s, ph) && clock64() - t0 < 200000000ll) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // MMA issuer (leader)
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                                       ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int u = first; u < p.units && ok; u += step) {
+                const Unit un = unit_of<PN>(p, u);
+                if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag))
+                    break;
+                tc_fence_after();
+                const uint32_t tmem_d = tmem_base + acc * PN;
+                for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                    if (!mbar_wait(full0 + 8 * stage, phase, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + stage * STAGE), b = a + HALF;
+                    const uint64_t adesc = umma_smem_desc(a, A_MN ? BK * 128 : 16, 1024), bdesc = umma_smem_desc(b, B_MN ? BK * 128 : 16, 1024);
+                    constexpr uint64_t a_step = A_MN ? (16 * 128) >> 4 : 2, b_step = B_MN ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_pair<1>(tmem_d, adesc + k * a_step, bdesc + k * b_step, idesc, kb > un.kb0 || k > 0 ? 1u : 0u);
+                    commit_both(empty0 + 8 * stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (ok)
+                    commit_both(tfull0 + 8 * acc);
+                acc ^= 1;
+                if (acc == 0)
+                    acc_phase ^= 1;
+            }
+            commit_own(drain); // every MMA issued so far has completed once this arrives
+            const long long t0 = clock64();
+            while (!mbar_try_wait(drain, 0) && clock64() - t0 < 1500000000ll) {
+            }
+        }
+    } else {
+        // epilogue: a warp takes 32 rows x PART columns, 32 columns at a time, thread = row
+        const int quarter = warp & 3, ew = warp - 2, part = ew >> 2;
+        uint8_t *const slots = smem + STG_OFF + ew * SLOTS * BLOCK;
+        int slot = 0, acc = 0;
+        uint32_t acc_phase = 0;
+        // the next block; the store that last used it, three blocks before, has read it (a block for z is taken while y's has not left)
+        const auto take = [&](bool second) {
+            uint8_t *b = slots + slot * BLOCK;
+            slot = slot == SLOTS - 1 ? 0 : slot + 1;
+            if (lane == 0) {
+                if (second)
+                    bulk_wait_read<SLOTS - 2>();
+                else
+                    bulk_wait_read<SLOTS - 1>();
+            }
+            __syncwarp();
+            return b;
+        };
+        const auto piece = [&](uint8_t *block, int row, int q) { return (uint4 *)(block + row * 128 + ((q ^ (row & 7)) << 4)); };
+        const bool halves = p.kind == TS2_OUT_F16 || p.kind == TS2_OUT_BF16;
+        for (int u = first; u < p.units; u += step) {
+            const Unit un = unit_of<PN>(p, u);
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PN + part * PART;
+            const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
+            uint4 rows[4]; // of the next 32 columns of the residual: 4 lanes a row, 8 rows at a time
+            const auto fetch = [&](int col) {
+                if (!p.res || col >= p.n)
+                    return;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = row0 + 8 * i + (lane >> 2), at = col + (lane & 3) * 8;
+                    const uint16_t *from = (const uint16_t *)p.res + row * p.res_ld + at;
+                    rows[i] = make_uint4(0, 0, 0, 0);
+                    if (row >= p.m)
+                        continue;
+                    if (p.res_vec && at + 8 <= p.n) {
+                        rows[i] = *(const uint4 *)from;
+                    } else {
+                        uint32_t w[4] = {};
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            w[k >> 1] |= at + k < p.n ? (uint32_t)from[k] << (16 * (k & 1)) : 0u;
+                        rows[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            };
+            fetch(col0);
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag)))
+                break;
+            tc_fence_after();
+            uint8_t *yb = nullptr, *zb = nullptr;
+#pragma unroll 1
+            for (int c = 0; c < PART / 32; ++c) {
+                const int col = col0 + c * 32, half = c & 1; // 16-bit results fill half of a block's rows
+                uint32_t r[32];
+                __syncwarp(); // lane 0 comes from its stores
+                tmem_ld32(taddr + c * 32, r);
+                tmem_ld_wait();
+                if (c == PART / 32 - 1) { // the accumulator is read: the next tile may have it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive_cluster(map_to_leader(tempty0 + 8 * acc));
+                }
+                if (row0 >= p.m || col0 >= p.n)
+                    continue;
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    v[i] = __uint_as_float(r[i]);
+                if (!halves) {
+                    yb = take(false);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        *piece(yb, lane, q) = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+                } else {
+                    if (!half) {
+                        yb = take(false);
+                        if (p.z)
+                            zb = take(true);
+                    }
+                    if (p.res) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *piece(yb, 8 * i + (lane >> 2), 4 * half + (lane & 3)) = rows[i];
+                        __syncwarp();
+                        if (c + 1 < PART / 32)
+                            fetch(col + 32);
+                    }
+                    if (p.bias) {
+                        if (p.bias_vec && col + 32 <= p.n) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 b = *(const float4 *)(p.bias + col + 4 * i);
+                                v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (col + i < p.n)
+                                    v[i] += p.bias[col + i];
+                        }
+                    }
+                    if (p.z) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            *piece(zb, lane, 4 * half + q) = make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
+                                                                        pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7]));
+                    }
+                    activate(p.act, v);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint4 *at = piece(yb, lane, 4 * half + q);
+                        if (p.res) {
+                            const uint4 raw = *at;
+                            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 f = unpack2<BF16>(w[k]);
+                                v[8 * q + 2 * k] += f.x, v[8 * q + 2 * k + 1] += f.y;
+                            }
+                        }
+                        *at = make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
+                                         pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7]));
+                    }
+                    if (!half)
+                        continue;
+                }
+                const int left = halves ? col - 32 : col; // of the block
+                // a store by TMA is cut off at the last 16 bytes that hold some of the row, not at its last element
+                const bool whole = p.ends_whole || left + (halves ? 64 : 32) <= p.n, y_tma = p.y_tma && whole, z_tma = p.z_tma && whole;
+                fence_proxy_async();
+                __syncwarp();
+                if (y_tma && lane == 0 && left < p.n) {
+                    if (p.kind == KIND_PARTIAL)
+                        tma_store_2d(&tmY, smem_u32(yb), left - un.col, u * PM + row0 - un.row);
+                    else if (p.kind == TS2_OUT_F32_ADD)
+                        tma_add_2d(&tmY, smem_u32(yb), left, row0);
+                    else
+                        tma_store_2d(&tmY, smem_u32(yb), left, row0);
+                }
+                if (lane == 0)
+                    bulk_commit(); // a group for every block taken, with or without a store
+                if (halves && p.z) {
+                    if (z_tma && lane == 0 && left < p.n)
+                        tma_store_2d(&tmZ, smem_u32(zb), left, row0);
+                    if (lane == 0)
+                        bulk_commit();
+                }
+                // rows that TMA cannot address: neighbours by neighbours
+                const auto by_rows = [&](const uint8_t *block, uint16_t *to, int64_t ld) {
+                    for (int i = 0; i < 32 && row0 + i < p.m; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int k = h * 32 + lane;
+                            if (left + k < p.n)
+                                to[(row0 + i) * ld + left + k] = *(const uint16_t *)(block + i * 128 + (((k >> 3) ^ (i & 7)) << 4) + (k & 7) * 2);
+                        }
+                };
+                if (!y_tma) {
+                    if (halves) {
+                        by_rows(yb, (uint16_t *)p.y, p.y_ld);
+                    } else {
+                        for (int i = 0; i < 32 && row0 + i < p.m; ++i)
+                            if (left + lane < p.n) {
+                                float *to = (float *)p.y + (row0 + i) * p.y_ld + left + lane;
+                                const float now = *(const float *)(yb + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4);
+                                *to = p.kind == TS2_OUT_F32_ADD ? *to + now : now;
+                            }
+                    }
+                }
+                if (halves && p.z && !z_tma)
+                    by_rows(zb, (uint16_t *)p.z, p.z_ld);
+                __syncwarp();
+            }
+            acc ^= 1;
+            if (acc == 0)
+                acc_phase ^= 1;
+        }
+        if (lane == 0)
+            bulk_wait_read<0>(); // the blocks must outlive the stores that read them
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); // nothing of the peer refers to this CTA any more
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    if (threadIdx.x == 0 && *abort_flag)
+        atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);
+}
+
+// The K ranges of a product added in their order, and its epilogue: 4 columns a thread
+template <int PN, bool BF16>
+__global__ void __launch_bounds__(256) linear_join_kernel(const LinearArgs p, int kind)
+{
+    grid_dep_wait();
+    const int quads = (p.n + 3) / 4;
+    const int64_t total = (int64_t)p.m * quads;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int row = (int)(i / quads), col = (int)(i - (int64_t)row * quads) * 4;
+        const int band = row / (8 * PM), high = min(8, p.m_tiles - band * 8);
+        const int tile = band * 8 * p.n_tiles + col / PN * high + row / PM - band * 8;
+        const float *from = p.part + ((int64_t)tile * p.splits * PM + row % PM) * PN + col % PN;
+        float v[4] = {};
+        for (int s = 0; s < p.splits; ++s) {
+            const float4 x = *(const float4 *)(from + (int64_t)s * PM * PN);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        if (kind == TS2_OUT_F32 || kind == TS2_OUT_F32_ADD) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (col + k < p.n) {
+                    float *to = (float *)p.y + row * p.y_ld + col + k;
+                    *to = kind == TS2_OUT_F32_ADD ? *to + v[k] : v[k];
+                }
+            continue;
+        }
+        const auto store = [&](void *base, int64_t ld, bool vec) {
+            const uint32_t a = pack2<BF16>(v[0], v[1]), b = pack2<BF16>(v[2], v[3]);
+            uint16_t *to = (uint16_t *)base + row * ld + col;
+            if (vec && col + 4 <= p.n) {
+                *(uint2 *)to = make_uint2(a, b);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (col + k < p.n)
+                        to[k] = (uint16_t)((k & 2 ? b : a) >> (16 * (k & 1)));
+            }
+        };
+        if (p.bias) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (col + k < p.n)
+                    v[k] += p.bias[col + k];
+        }
+        if (p.z)
+            store(p.z, p.z_ld, p.z_tma);
+        activate(p.act, v);
+        if (p.res) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (col + k < p.n)
+                    v[k] += widen16<BF16>(((const uint16_t *)p.res)[row * p.res_ld + col + k]);
+        }
+        store(p.y, p.y_ld, p.y_tma);
+    }
+}
+
+// ---- dz and its column sums ------------------------------------------------------------------------------------------------
+// A block takes 128 columns and rows b, b + blocks, ... of 16: dz = dy act'(z) rounded to 16 bits (dz null: not wanted), and the sums of the unrounded
+// dz over its rows (sums null: not wanted).  Bound by reading dy and z.
+template <int ACT, bool BF16>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restrict__ dy, int64_t dy_ld, const uint16_t *__restrict__ z, int64_t z_ld,
+                                                        int64_t T, int n, bool vec, uint16_t *dz, int64_t dz_ld, float *sums)
+{
+    grid_dep_wait();
+    __shared__ float part[16][132];
+    const int c8 = (threadIdx.x & 15) * 8, col = blockIdx.x * 128 + c8, line = threadIdx.x >> 4;
+    float acc[8] = {};
+    const auto read = [&](const uint16_t *row, uint4 &raw) {
+        if (vec && col + 8 <= n) {
+            raw = *(const uint4 *)(row + col);
+        } else {
+            uint32_t w[4] = {};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                w[k >> 1] |= col + k < n ? (uint32_t)row[col + k] << (16 * (k & 1)) : 0u;
+            raw = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    };
+#pragma unroll 2
+    for (int64_t t = (int64_t)blockIdx.y * 16 + line; t < T; t += (int64_t)gridDim.y * 16) {
+        uint4 a, b = make_uint4(0, 0, 0, 0);
+        read(dy + t * dy_ld, a);
+        if (ACT != TS2_ACT_NONE)
+            read(z + t * z_ld, b);
+        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float2 d = unpack2<BF16>(aw[k]);
+            const float2 s = unpack2<BF16>(bw[k]);
+            if (ACT != TS2_ACT_NONE)
+                d.x *= activation_slope<ACT>(s.x), d.y *= activation_slope<ACT>(s.y);
+            acc[2 * k] += d.x, acc[2 * k + 1] += d.y;
+            o[k] = pack2<BF16>(d.x, d.y);
+        }
+        if (dz && col < n)
+            *(uint4 *)(dz + t * dz_ld + col) = make_uint4(o[0], o[1], o[2], o[3]); // the pitch is a multiple of 8
+    }
+    if (!sums)
+        return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        part[line][c8 + k] = acc[k];
+    __syncthreads();
+    if (threadIdx.x < 128 && blockIdx.x * 128 + threadIdx.x < n) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            s += part[i][threadIdx.x];
+        sums[(int64_t)blockIdx.y * n + blockIdx.x * 128 + threadIdx.x] = s;
+    }
+}
+__global__ void __launch_bounds__(128) linear_sum_kernel(const float *__restrict__ sums, int n, int blocks, float *out)
+{
+    grid_dep_wait();
+    const int col = blockIdx.x * 128 + threadIdx.x;
+    if (col >= n)
+        return;
+    float s = 0.f;
+    for (int b = 0; b < blocks; ++b)
+        s += sums[(int64_t)b * n + col];
+    out[col] = s;
+}
+// rows of 16-bit elements to a pitch that TMA can address
+__global__ void __launch_bounds__(256) linear_pitch_kernel(const uint16_t *__restrict__ from, int64_t from_ld, uint16_t *to, int64_t to_ld, int64_t rows, int cols)
+{
+    grid_dep_wait();
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8)
+        for (int c = threadIdx.x & 31; c < cols; c += 32)
+            to[r * to_ld + c] = from[r * from_ld + c];
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// [rows][cols] of 2- or 4-byte elements; boxes of 128 bytes x `high` rows, 128-byte swizzle
+int linear_map(CUtensorMap *tm, const void *base, int size, int64_t cols, int64_t rows, int64_t ld, int high)
+{
+    static const EncodeTiledFn encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return (EncodeTiledFn)f;
+    }();
+    if (!encode)
+        return fail(TS2_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(ld * size)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)high}, estr[2] = {1, 1};
+    const CUresult r = encode(tm, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(base), dims, strides,
+                              box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? TS2_OK : fail(TS2_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+}
+bool tma_ok(const void *base, int64_t ld, int size) { return (uintptr_t)base % 16 == 0 && ld * size % 16 == 0; }
+
+// an operand: rows of 16-bit elements, where they lie or copied to a pitch that TMA can address
+struct Operand {
+    const void *p;
+    int64_t rows, ld;
+    int cols;
+    Scratch copy;
+    int rc = TS2_OK;
+    Operand(const Ctx &c, const void *from, int64_t from_ld, int64_t rows_, int cols_)
+        : p(from), rows(rows_), ld(from_ld), cols(cols_), copy(c, tma_ok(from, from_ld, 2) ? 0 : (size_t)rows_ * ceil_div(cols_, 8) * 16)
+    {
+        if (tma_ok(from, from_ld, 2))
+            return;
+        rc = copy.rc;
+        if (rc == TS2_OK) {
+            p = copy.p, ld = ceil_div(cols, 8) * 8;
+            rc = [&] {
+                TS2_LAUNCH(linear_pitch_kernel, (int)std::min<int64_t>(ceil_div(rows, 8), 8 * sm_count(c.device)), 256, 0, c.stream,
+                           (const uint16_t *)from, from_ld, (uint16_t *)copy.p, ld, rows, cols);
+                return (int)TS2_OK;
+            }();
+        }
+    }
+};
+
+// K ranges of a product, see below
+int choose_splits(int pairs, int64_t tiles, int k_blocks)
+{
+    double best = (double)ceil_div(tiles, pairs) * (k_blocks + 4);
+    int splits = 1;
+    for (int s = 2; s <= 64 && s <= k_blocks; ++s) {
+        const int per = (int)ceil_div(k_blocks, s), used = (int)ceil_div(k_blocks, per);
+        const double cost = (double)ceil_div(tiles * s, pairs) * (per + 4) + 10 + 0.1 * tiles * s;
+        if (used == s && cost < best)
+            best = cost, splits = s;
+    }
+    return splits;
+}
+
+template <bool A_MN, bool B_MN, int PN, bool BF16>
+int product(const Ctx &c, const Operand &a, const Operand &b, int64_t K, LinearArgs p)
+{
+    static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
+    const unsigned bit = 1u << (c.device & 15);
+    if (!(ready.load() & bit)) {
+        TS2_CUDA(cudaFuncSetAttribute((const void *)linear_product_kernel<A_MN, B_MN, PN, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        ready.fetch_or(bit);
+    }
+    const int pairs = sm_count(c.device) / 2, kind = p.kind;
+    p.m_tiles = (int)ceil_div(p.m, PM), p.n_tiles = (int)ceil_div(p.n, PN), p.k_blocks = (int)ceil_div(K, BK);
+    p.splits = choose_splits(pairs, (int64_t)p.m_tiles * p.n_tiles, p.k_blocks);
+    p.kb_per_split = (int)ceil_div(p.k_blocks, p.splits), p.units = p.m_tiles * p.n_tiles * p.splits;
+    p.status = device_status_word(c.device);
+    if (!p.status)
+        return fail(TS2_ERR_CUDA, "no device status word");
+    const int size = kind == TS2_OUT_F32 || kind == TS2_OUT_F32_ADD ? 4 : 2;
+    p.y_tma = tma_ok(p.y, p.y_ld, size), p.z_tma = tma_ok(p.z, p.z_ld, 2), p.res_vec = tma_ok(p.res, p.res_ld, 2), p.bias_vec = (uintptr_t)p.bias % 16 == 0;
+    p.ends_whole = p.n * size % 16 == 0;
+    Scratch part(c, p.splits > 1 ? (size_t)p.units * PM * PN * 4 : 0);
+    if (part.rc != TS2_OK)
+        return part.rc;
+    CUtensorMap ta, tb, ty = {}, tz = {};
+    int rc = linear_map(&ta, a.p, 2, a.cols, a.rows, a.ld, A_MN ? BK : 128);
+    if (rc == TS2_OK)
+        rc = linear_map(&tb, b.p, 2, b.cols, b.rows, b.ld, B_MN ? BK : PN / 2);
+    LinearArgs q = p; // of the product
+    if (p.splits > 1) {
+        q.kind = KIND_PARTIAL, q.y_tma = q.ends_whole = true, q.res = nullptr, q.z = nullptr, q.bias = nullptr, p.part = (float *)part.p;
+        if (rc == TS2_OK)
+            rc = linear_map(&ty, part.p, 4, PN, (int64_t)p.units * PM, PN, 32);
+    } else {
+        if (rc == TS2_OK && p.y_tma)
+            rc = linear_map(&ty, p.y, size, p.n, p.m, p.y_ld, 32);
+        if (rc == TS2_OK && p.z && p.z_tma)
+            rc = linear_map(&tz, p.z, 2, p.n, p.m, p.z_ld, 32);
+    }
+    if (rc != TS2_OK)
+        return rc;
+    TS2_LAUNCH((linear_product_kernel<A_MN, B_MN, PN, BF16>), 2 * std::min(pairs, p.units), THREADS, SMEM, c.stream, ta, tb, ty, tz, q);
+    if (p.splits > 1)
+        TS2_LAUNCH((linear_join_kernel<PN, BF16>), (int)std::min<int64_t>(ceil_div((int64_t)p.m * ceil_div(p.n, 4), 256), 8 * sm_count(c.device)), 256, 0,
+                   c.stream, p, kind);
+    return TS2_OK;
+}
+template <bool A_MN, bool B_MN>
+int product(const Ctx &c, bool bf16, const Operand &a, const Operand &b, int64_t K, const LinearArgs &p)
+{
+    // tiles of 256 x 128 where those of 256 x 256 would leave half of the device idle
+    const bool few = 2 * ceil_div(p.m, PM) * ceil_div(p.n, 256) <= sm_count(c.device) / 2;
+    if (few)
+        return bf16 ? product<A_MN, B_MN, 128, true>(c, a, b, K, p) : product<A_MN, B_MN, 128, false>(c, a, b, K, p);
+    return bf16 ? product<A_MN, B_MN, 256, true>(c, a, b, K, p) : product<A_MN, B_MN, 256, false>(c, a, b, K, p);
+}
+
+} // namespace
+
+int linear_forward(const Ctx &c, const LinearShape &s, const void *x, int64_t x_ld, const void *w, int64_t w_ld, const float *bias, const void *residual,
+                   int64_t residual_ld, void *y, int64_t y_ld, void *z, int64_t z_ld)
+{
+    if (s.T == 0)
+        return TS2_OK;
+    const Operand a(c, x, x_ld, s.T, s.in), b(c, w, w_ld, s.out, s.in);
+    if (a.rc != TS2_OK || b.rc != TS2_OK)
+        return a.rc != TS2_OK ? a.rc : b.rc;
+    LinearArgs p = {};
+    p.m = (int)s.T, p.n = s.out, p.kind = s.type, p.act = s.act, p.bias = bias;
+    p.res = residual, p.res_ld = residual_ld, p.y = y, p.y_ld = y_ld, p.z = z, p.z_ld = z_ld;
+    return product<false, false>(c, s.type == TS2_OUT_BF16, a, b, s.in, p);
+}
+
+template <int ACT, bool BF16>
+static int dz_of(const Ctx &c, const LinearShape &s, const void *dy, int64_t dy_ld, const void *z, int64_t z_ld, void *dz, int64_t dz_ld, float *sums,
+                 int blocks, float *dbias)
+{
+    const bool vec = tma_ok(dy, dy_ld, 2) && (ACT == TS2_ACT_NONE || tma_ok(z, z_ld, 2));
+    TS2_LAUNCH((linear_dz_kernel<ACT, BF16>), dim3((int)ceil_div(s.out, 128), blocks), 256, 0, c.stream, (const uint16_t *)dy, dy_ld, (const uint16_t *)z, z_ld,
+               s.T, s.out, vec, (uint16_t *)dz, dz_ld, sums);
+    if (dbias)
+        TS2_LAUNCH(linear_sum_kernel, (int)ceil_div(s.out, 128), 128, 0, c.stream, sums, s.out, blocks, dbias);
+    return TS2_OK;
+}
+
+int linear_backward(const Ctx &c, const LinearShape &s, const void *dy, int64_t dy_ld, const void *z, int64_t z_ld, const void *x, int64_t x_ld,
+                    const void *w, int64_t w_ld, void *dx, int64_t dx_ld, int dw_kind, void *dw, int64_t dw_ld, float *dbias)
+{
+    const bool bf16 = s.type == TS2_OUT_BF16, products = dx || dw;
+    if (s.T == 0) {
+        if (dw && dw_kind != TS2_OUT_F32_ADD) {
+            const size_t size = dw_kind == TS2_OUT_F32 ? 4 : 2;
+            TS2_CUDA(cudaMemset2DAsync(dw, dw_ld * size, 0, s.in * size, s.out, c.stream));
+        }
+        if (dbias)
+            TS2_CUDA(cudaMemsetAsync(dbias, 0, (size_t)s.out * 4, c.stream));
+        return TS2_OK;
+    }
+    // dz where it differs from dy, and the sums of its columns
+    const bool own_dz = s.act != TS2_ACT_NONE && products;
+    const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.T, 64), 8 * sm_count(c.device) / ceil_div(s.out, 128)));
+    const int64_t dz_ld = ceil_div(s.out, 8) * 8;
+    const Scratch dz(c, own_dz ? (size_t)s.T * dz_ld * 2 : 0), sums(c, dbias ? (size_t)blocks * s.out * 4 : 0);
+    if (dz.rc != TS2_OK || sums.rc != TS2_OK)
+        return dz.rc != TS2_OK ? dz.rc : sums.rc;
+    if (own_dz || dbias) {
+        using F = int (*)(const Ctx &, const LinearShape &, const void *, int64_t, const void *, int64_t, void *, int64_t, float *, int, float *);
+        static const F forms[4][2] = {{dz_of<TS2_ACT_NONE, false>, dz_of<TS2_ACT_NONE, true>},
+                                      {dz_of<TS2_ACT_RELU, false>, dz_of<TS2_ACT_RELU, true>},
+                                      {dz_of<TS2_ACT_GELU, false>, dz_of<TS2_ACT_GELU, true>},
+                                      {dz_of<TS2_ACT_SILU, false>, dz_of<TS2_ACT_SILU, true>}};
+        if (const int rc = forms[s.act][bf16](c, s, dy, dy_ld, z, z_ld, dz.p, dz_ld, (float *)sums.p, blocks, dbias))
+            return rc;
+    }
+    if (!products)
+        return TS2_OK;
+    const Operand d(c, own_dz ? dz.p : dy, own_dz ? dz_ld : dy_ld, s.T, s.out);
+    if (d.rc != TS2_OK)
+        return d.rc;
+    if (dx) {
+        const Operand b(c, w, w_ld, s.out, s.in);
+        if (b.rc != TS2_OK)
+            return b.rc;
+        LinearArgs p = {};
+        p.m = (int)s.T, p.n = s.in, p.kind = s.type, p.y = dx, p.y_ld = dx_ld;
+        if (const int rc = product<false, true>(c, bf16, d, b, s.out, p))
+            return rc;
+    }
+    if (dw) {
+        const Operand b(c, x, x_ld, s.T, s.in);
+        if (b.rc != TS2_OK)
+            return b.rc;
+        LinearArgs p = {};
+        p.m = s.out, p.n = s.in, p.kind = dw_kind, p.y = dw, p.y_ld = dw_ld;
+        if (const int rc = product<true, true>(c, bf16, d, b, s.T, p))
+            return rc;
+    }
+    return TS2_OK;
+}
+
+} // namespace ts2

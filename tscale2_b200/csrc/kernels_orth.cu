@@ -656,20 +656,6 @@ static int choose_splits(int pairs, int64_t tiles, int k_blocks)
     return splits;
 }
 
-struct Scratch {
-    void *p = nullptr;
-    cudaStream_t stream;
-    int rc;
-    Scratch(const Ctx &c, size_t bytes) : stream(c.stream) { rc = scratch_alloc(c.device, bytes, c.stream, &p); }
-    ~Scratch()
-    {
-        if (p)
-            scratch_free(stream, p);
-    }
-    Scratch(const Scratch &) = delete;
-    Scratch &operator=(const Scratch &) = delete;
-};
-
 template <class T>
 static int orthogonalize_typed(const Ctx &c, const T *g, int64_t ld, int64_t stride, int batch, int rows, int cols, const float coef[3], int steps,
                                float out_scale, __nv_bfloat16 *out, int64_t ld_out, int64_t out_stride)

@@ -6,14 +6,21 @@
 //     softmax, renormalised  dl[e] = scale w[e] (d[e] - sum_j d[j] w[j])            for chosen e
 //     sigmoid              dl[e] = scale d[e] s[e] (1 - s[e])
 //     sigmoid, renormalised  dl[e] = scale w[e] (1 - s[e]) (d[e] - sum_j d[j] w[j])
-// A warp takes a row.
+//
+// A warp takes 8 rows.  They come in a row at a time in pieces of 8 columns a lane, and their keys and every piece's largest key go to shared memory.  Then
+// four lanes have a row, each the largest keys of every fourth piece in registers: a choice is a maximum over those and over the four lanes, and only the piece
+// that it came from is looked at again.
+//
+// Keys are fp32 first.  They order as exact ones would where they differ by more than fp32 can be wrong, so a row in which two choices, the last choice and the
+// next key, or two groups at the border are nearer than that is done once more in fp64 by the whole warp.  Without a bias (and with groups ranked by one key)
+// the logits themselves are the keys, and exact.
 #include "elem_types.cuh"
 #include "kernels.cuh"
 #include <algorithm>
 
 namespace ts2 {
 
-static constexpr int WARPS = 8, THREADS = 32 * WARPS;
+static constexpr int THREADS = 128;
 static constexpr unsigned FULL = 0xffffffffu;
 
 __device__ __forceinline__ double warp_max(double v)
@@ -58,175 +65,604 @@ __device__ __forceinline__ float choice_weight(bool softmax, bool renormalize, b
     return sum > 0.f ? w / sum : 0.f;
 }
 
+struct Choice { // what the forward pass needs beside a RouteShape
+    const float *bias;
+    int groups, kept, group_top;
+};
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// One row by the whole warp, its keys in fp64: any row, and slow
 template <class T>
-__global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restrict__ logits, int64_t ld, RouteShape p, const float *__restrict__ bias,
-                                                                int groups, int kept, int group_top, const uint8_t *__restrict__ mask, int *ids, float *weights)
+__device__ __noinline__ void route_row_exactly(const T *__restrict__ row, const RouteShape &p, const Choice &c, double *key, int *ids, float *weights)
+{
+    const int lane = threadIdx.x & 31, E = p.E, per = E / c.groups;
+    const bool softmax = p.score == TS2_SCORE_SOFTMAX;
+    float top = -INFINITY, sum = 0.f;
+    double sum64 = 0.;
+    bool bad = false;
+    if (softmax) {
+        for (int e = lane; e < E; e += 32) {
+            const float l = widen(row[e]);
+            bad |= !(l < INFINITY);
+            top = fmaxf(top, l);
+        }
+        bad = __any_sync(FULL, bad);
+        top = warp_max(top);
+        if (top == -INFINITY)
+            top = 0.f;
+        for (int e = lane; e < E; e += 32)
+            sum64 += exp((double)widen(row[e]) - (double)top);
+        sum64 = warp_sum(sum64);
+        sum = (float)sum64;
+    }
+    for (int e = lane; e < E; e += 32) {
+        const double l = widen(row[e]);
+        double k = softmax ? exp(l - (double)top) / sum64 : 1. / (1. + exp(-l));
+        if (c.bias)
+            k += c.bias[e];
+        key[e] = bad || l == -INFINITY || !(k == k) ? -INFINITY : k;
+    }
+    __syncwarp();
+    unsigned keep = FULL; // groups that experts are taken from
+    if (c.groups > 1) {
+        double best = -INFINITY, second = -INFINITY;
+        if (lane < c.groups)
+            for (int e = lane * per; e < (lane + 1) * per; ++e) {
+                second = fmax(second, fmin(best, key[e]));
+                best = fmax(best, key[e]);
+            }
+        double rank = c.group_top == 2 ? best + second : best;
+        if (!(rank == rank))
+            rank = -INFINITY;
+        keep = 0;
+        for (int k = 0; k < c.kept; ++k) {
+            const int g = warp_best(rank, lane);
+            if (g < 0)
+                break;
+            keep |= 1u << g;
+            if (lane == g)
+                rank = -INFINITY;
+        }
+    }
+    __syncwarp();
+    for (int e = lane; e < E; e += 32) {
+        if (!(keep >> (c.groups > 1 ? e / per : 0) & 1))
+            key[e] = -INFINITY;
+        else if (!c.bias && key[e] > -INFINITY)
+            key[e] = widen(row[e]);
+    }
+    __syncwarp();
+    int id = -1; // lane j: choice j
+    for (int j = 0; j < p.selected; ++j) {
+        double best = -INFINITY;
+        int at = E;
+        for (int e = lane; e < E; e += 32)
+            if (key[e] > best)
+                best = key[e], at = e;
+        at = warp_best(best, at);
+        if (at < 0)
+            break;
+        if (lane == j)
+            id = at;
+        __syncwarp();
+        if (lane == 0)
+            key[at] = -INFINITY;
+        __syncwarp();
+    }
+    float s;
+    const float w = choice_weight(softmax, p.renormalize, id >= 0, id >= 0 ? widen(row[id]) : 0.f, top, sum, s);
+    if (lane < p.selected) {
+        ids[lane] = id;
+        weights[lane] = p.scale * w;
+    }
+    __syncwarp();
+}
+
+// Shared memory of a warp, in 4-byte words: keys of ROWS rows (a pitch that keeps the rows' pieces in different banks), the largest and the second key of
+// their pieces, the groups' ranks, choices and what they weigh, and of the softmax the row's maximum and its sum's reciprocal.
+static constexpr int ROWS = 8, SLOTS = MOE_ROUTE_MAX_SELECTED + 1;
+__host__ __device__ constexpr int key_pitch(int pieces) { return (pieces + 3) / 4 * 32 + 4; }
+__host__ __device__ constexpr int warp_words(int pieces) { return ROWS * (key_pitch(pieces) + 2 * (pieces | 1) + 33 + 2 * SLOTS + 2); }
+
+// eight neighbours from column e on, -inf behind the last one
+template <class T>
+__device__ __forceinline__ void load8(const T *row, int e, int E, bool vec, float (&v)[8])
+{
+    if (vec && e + 8 <= E) {
+        constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8 / PER; ++i) {
+            const Piece<T, PER> q = *(const Piece<T, PER> *)(row + e + i * PER);
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                v[i * PER + j] = widen(q.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = e + i < E ? widen(row[e + i]) : -INFINITY;
+    }
+}
+// over the `width` neighbouring lanes that share a row
+__device__ __forceinline__ float max_over(float v, int width)
+{
+    for (int o = width / 2; o > 0; o >>= 1)
+        v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+    return v;
+}
+__device__ __forceinline__ float sum_over(float v, int width)
+{
+    for (int o = width / 2; o > 0; o >>= 1)
+        v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+__device__ __forceinline__ float max8(const float (&v)[8])
+{
+    return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+}
+
+// NB: pieces of 8 columns that each of the four lanes of a row has (E <= 32 NB)
+template <class T, int NB>
+__global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p, const Choice c,
+                                                                     const uint8_t *__restrict__ mask, int *ids, float *weights)
 {
     grid_dep_wait();
-    extern __shared__ double route_keys[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, per = E / groups;
-    double *key = route_keys + warp * E;
-    const bool softmax = p.score == TS2_SCORE_SOFTMAX;
-    for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < p.T; t += (int64_t)gridDim.x * WARPS) {
-        const T *row = logits + t * ld;
-        const bool on = !mask || mask[t];
-        float top = -INFINITY, sum = 1.f;
-        double top64 = 0., sum64 = 1.;
-        bool bad = false;
-        if (softmax) {
-            sum = 0.f, sum64 = 0.;
-            for (int c = lane; c < E; c += 32) {
-                const float l = widen(row[c]);
-                bad |= !(l < INFINITY);
-                top = fmaxf(top, l);
-            }
-            top = warp_max(top);
-            if (top == -INFINITY)
-                top = 0.f;
-            top64 = top;
-            for (int c = lane; c < E; c += 32) {
-                const float l = widen(row[c]);
-                sum += expf(l - top);
-                sum64 += exp((double)l - top64);
-            }
-            sum = warp_sum(sum), sum64 = warp_sum(sum64);
-            bad = __any_sync(FULL, bad);
+    constexpr int HELD = (NB + 7) / 8; // pieces a lane has of a row that comes in
+    extern __shared__ __align__(16) float route_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, pieces = (E + 7) / 8, per = E / c.groups;
+    const int pitch = key_pitch(pieces), piece_pitch = pieces | 1;
+    float *keys = route_smem + warp * warp_words(pieces), *first = keys + ROWS * pitch, *second = first + ROWS * piece_pitch,
+          *ranks = second + ROWS * piece_pitch, *chosen = ranks + ROWS * 33, *row_max = chosen + ROWS * SLOTS, *row_inv = row_max + ROWS;
+    int *chosen_id = (int *)(row_inv + ROWS);
+    const int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * ROWS;
+    if (t0 >= p.T)
+        return;
+    const bool softmax = p.score == TS2_SCORE_SOFTMAX, by_logit = !c.bias && (c.groups == 1 || c.group_top == 1), stats = softmax && !(by_logit && p.renormalize);
+    int width = 1; // lanes that share a row
+    while (width < pieces && width < 32)
+        width *= 2;
+
+    // rows come in
+#pragma unroll 1
+    for (int pass = 0; pass < ROWS * width / 32 || pass == 0; ++pass) {
+        const int r = pass * (32 / width) + lane / width, at = lane & (width - 1);
+        const int64_t t = t0 + r;
+        const bool on = r < ROWS && t < p.T && (!mask || mask[t]);
+        float v[HELD][8];
+        float top = -INFINITY, sum = 0.f;
+        bool bad = !on;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (on && at + 32 * h < pieces)
+                load8(logits + t * ld, (at + 32 * h) * 8, E, vec, v[h]);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[h][i] = -INFINITY;
+            top = fmaxf(top, max8(v[h]));
         }
-        const auto out = [&](float l) { return bad || !on || l == -INFINITY || !(l == l); };
-        for (int c = lane; c < E; c += 32) {
-            const float l = widen(row[c]);
-            double k = softmax ? exp((double)l - top64) / sum64 : 1. / (1. + exp(-(double)l));
-            if (bias)
-                k += bias[c];
-            key[c] = out(l) || !(k == k) ? -INFINITY : k;
+        if (stats) {
+            top = max_over(top, width);
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sum += ex2((v[h][i] - ref) * 1.44269504f); // a NaN, and infinity minus itself, end here
+            sum = sum_over(sum, width);
+            bad |= !(sum == sum);
+            if (r < ROWS && at == 0)
+                row_max[r] = ref, row_inv[r] = 1.f / sum;
+            top = ref;
+        } else if (softmax) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    bad |= !(v[h][i] < INFINITY);
+            bad = max_over(bad ? 1.f : 0.f, width) > 0.f;
         }
-        __syncwarp();
-        unsigned keep = FULL; // groups that experts are taken from
-        if (groups > 1) {
-            double best = -INFINITY, second = -INFINITY;
-            if (lane < groups)
-                for (int c = lane * per; c < (lane + 1) * per; ++c) {
-                    second = fmax(second, fmin(best, key[c]));
-                    best = fmax(best, key[c]);
+        const float inv = stats ? 1.f / sum : 1.f;
+        if (r >= ROWS)
+            continue;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const int piece = at + 32 * h;
+            if (piece >= pieces)
+                continue;
+            float k[8];
+            if (by_logit) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    k[i] = fmaxf(v[h][i], -INFINITY); // a NaN is none
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float l = v[h][i];
+                    float s = softmax ? ex2((l - top) * 1.44269504f) * inv : rcp(1.f + ex2(l * -1.44269504f));
+                    if (c.bias)
+                        s += piece * 8 + i < E ? c.bias[piece * 8 + i] : 0.f;
+                    k[i] = l == -INFINITY ? -INFINITY : fmaxf(s, -INFINITY);
                 }
-            double rank = group_top == 2 ? best + second : best;
-            if (!(rank == rank))
-                rank = -INFINITY;
-            keep = 0;
-            for (int k = 0; k < kept; ++k) {
-                const int g = warp_best(rank, lane);
-                if (g < 0)
-                    break;
-                keep |= 1u << g;
-                if (lane == g)
-                    rank = -INFINITY;
+            }
+            if (bad)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    k[i] = -INFINITY;
+            float4 *to = (float4 *)(keys + r * pitch + piece * 8);
+            to[0] = make_float4(k[0], k[1], k[2], k[3]);
+            to[1] = make_float4(k[4], k[5], k[6], k[7]);
+            if (c.groups > 1 && c.group_top == 2) {
+                float best = k[0], next = -INFINITY;
+#pragma unroll
+                for (int i = 1; i < 8; ++i) {
+                    next = fmaxf(next, fminf(best, k[i]));
+                    best = fmaxf(best, k[i]);
+                }
+                first[r * piece_pitch + piece] = best, second[r * piece_pitch + piece] = next;
+            } else {
+                first[r * piece_pitch + piece] = max8(k);
             }
         }
-        __syncwarp();
-        for (int c = lane; c < E; c += 32) {
-            if (!(keep >> (groups > 1 ? c / per : 0) & 1))
-                key[c] = -INFINITY;
-            else if (!bias && key[c] > -INFINITY)
-                key[c] = widen(row[c]);
+    }
+    __syncwarp();
+
+    // four lanes a row from here on
+    const int r = lane >> 2, l = lane & 3;
+    const int64_t t = t0 + r;
+    float *my_keys = keys + r * pitch, *my_first = first + r * piece_pitch, *my_second = second + r * piece_pitch, *my_ranks = ranks + r * 33,
+          *my_chosen = chosen + r * SLOTS;
+    int *my_id = chosen_id + r * SLOTS;
+    const float unit = !by_logit && softmax ? row_inv[r] * 0x1p-18f : 0x1p-19f; // two scores are off by less together
+    const auto near = [&](float a, float b, float times) { return !(a - b > times * (unit + 0x1p-22f * (fabsf(a) + fabsf(b)))); };
+    bool unsure = false;
+    if (c.groups > 1) {
+        const bool aligned = per % 8 == 0; // a group is whole pieces
+        for (int g = l; g < c.groups; g += 4) {
+            float best = -INFINITY, next = -INFINITY;
+            const auto take = [&](float k) {
+                next = fmaxf(next, fminf(best, k));
+                best = fmaxf(best, k);
+            };
+            if (aligned) {
+                for (int i = g * (per / 8); i < (g + 1) * (per / 8); ++i) {
+                    if (c.group_top == 2)
+                        next = fmaxf(next, my_second[i]);
+                    take(my_first[i]);
+                }
+            } else {
+                for (int e = g * per; e < (g + 1) * per; ++e)
+                    take(my_keys[e]);
+            }
+            my_ranks[g] = c.group_top == 2 ? fmaxf(best + next, -INFINITY) : best;
         }
         __syncwarp();
-        int id = -1; // lane j: choice j
-        for (int j = 0; j < p.selected; ++j) {
-            double best = -INFINITY;
-            int at = E;
-            for (int c = lane; c < E; c += 32)
-                if (key[c] > best)
-                    best = key[c], at = c;
-            at = warp_best(best, at);
-            if (at < 0)
-                break;
-            if (lane == j)
-                id = at;
+        float worst_kept = INFINITY, best_left = -INFINITY;
+        for (int g = l; g < c.groups; g += 4) {
+            const float mine = my_ranks[g];
+            int before = 0;
+            for (int h = 0; h < c.groups; ++h)
+                before += my_ranks[h] > mine || (my_ranks[h] == mine && h < g) ? 1 : 0;
+            if (before < c.kept && mine > -INFINITY) {
+                worst_kept = fminf(worst_kept, mine);
+                continue;
+            }
+            best_left = fmaxf(best_left, mine);
+            if (aligned)
+                for (int i = g * (per / 8); i < (g + 1) * (per / 8); ++i)
+                    my_first[i] = -INFINITY;
+            else
+                for (int e = g * per; e < (g + 1) * per; ++e)
+                    my_keys[e] = -INFINITY;
+        }
+        worst_kept = fminf(worst_kept, __shfl_xor_sync(FULL, worst_kept, 1)), best_left = fmaxf(best_left, __shfl_xor_sync(FULL, best_left, 1));
+        worst_kept = fminf(worst_kept, __shfl_xor_sync(FULL, worst_kept, 2)), best_left = fmaxf(best_left, __shfl_xor_sync(FULL, best_left, 2));
+        unsure = !by_logit && best_left > -INFINITY && near(worst_kept, best_left, 2.f);
+        __syncwarp();
+        if (!aligned) { // what the pieces hold now
+            for (int i = l; i < pieces; i += 4) {
+                float best = -INFINITY;
+                for (int e = i * 8; e < min(E, i * 8 + 8); ++e)
+                    best = fmaxf(best, my_keys[e]);
+                my_first[i] = best;
+            }
             __syncwarp();
-            if (lane == 0)
-                key[at] = -INFINITY;
-            __syncwarp();
         }
-        float s;
-        const float w = choice_weight(softmax, p.renormalize, id >= 0, id >= 0 ? widen(row[id]) : 0.f, top, sum, s);
-        if (lane < p.selected) {
-            ids[t * p.selected + lane] = id;
-            weights[t * p.selected + lane] = p.scale * w;
+    }
+    float held[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+        held[i] = i * 4 + l < pieces ? my_first[i * 4 + l] : -INFINITY;
+    const int rounds = p.selected + (by_logit ? 0 : 1); // the first key that is not chosen, for its distance
+#pragma unroll 1
+    for (int j = 0; j < rounds; ++j) {
+        float best = held[0];
+#pragma unroll
+        for (int i = 1; i < NB; ++i)
+            best = fmaxf(best, held[i]);
+        best = fmaxf(best, __shfl_xor_sync(FULL, best, 1));
+        best = fmaxf(best, __shfl_xor_sync(FULL, best, 2));
+        int piece = 1 << 20; // the first one with this key
+#pragma unroll
+        for (int i = NB - 1; i >= 0; --i)
+            piece = held[i] == best ? i * 4 + l : piece;
+        int lowest = min(piece, __shfl_xor_sync(FULL, piece, 1));
+        lowest = min(lowest, __shfl_xor_sync(FULL, lowest, 2));
+        if (best == -INFINITY) {
+            if (l == 0)
+                my_id[j] = -1, my_chosen[j] = -INFINITY;
+        } else if (piece == lowest) { // this lane's: nobody else looks at the piece
+            const float4 a = *(const float4 *)(my_keys + piece * 8), b = *(const float4 *)(my_keys + piece * 8 + 4);
+            const float k[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            int i0 = 0;
+#pragma unroll
+            for (int i = 7; i >= 0; --i)
+                i0 = k[i] == best ? i : i0;
+            float rest = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                rest = fmaxf(rest, i == i0 ? -INFINITY : k[i]);
+            my_keys[piece * 8 + i0] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                held[i] = i * 4 + l == piece ? rest : held[i];
+            my_id[j] = piece * 8 + i0, my_chosen[j] = best;
         }
+    }
+    __syncwarp();
+
+    // weights: a lane has every fourth choice
+    const bool here = t < p.T;
+    const T *row = logits + t * ld;
+    const auto logit = [&](int id) { return widen(row[id]); };
+    float top = -INFINITY, total = 0.f;
+    for (int j = l; j < p.selected && here; j += 4) {
+        const int id = my_id[j];
+        if (id < 0)
+            continue;
+        const float v = logit(id);
+        top = fmaxf(top, softmax ? v : fminf(v, 0.f));
+        if (!by_logit) {
+            const int next = my_id[j + 1];
+            if (next >= 0 && near(my_chosen[j], my_chosen[j + 1], 1.f)) // equal logits and biases are equal keys, whose order is known
+                unsure |= j == p.selected - 1 || v != logit(next) || (c.bias && c.bias[id] != c.bias[next]);
+        }
+    }
+    top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+    __syncwarp(); // the keys have been compared
+    const float ref = p.renormalize ? top : softmax ? row_max[r] : 0.f;
+    for (int j = l; j < p.selected && here; j += 4) {
+        const int id = my_id[j];
+        float w = 0.f;
+        if (id >= 0) {
+            const float v = logit(id);
+            // sigmoid(v) = exp(min(v, 0)) / (1 + exp(-|v|)): nothing underflows that matters to a quotient
+            w = softmax ? expf(v - ref) : expf(fminf(v, 0.f) - ref) / (1.f + expf(-fabsf(v)));
+        }
+        my_chosen[j] = w;
+        total += w;
+    }
+    total += __shfl_xor_sync(FULL, total, 1);
+    total += __shfl_xor_sync(FULL, total, 2);
+    const float factor = p.renormalize ? (total > 0.f ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f;
+    for (int j = l; j < p.selected && here; j += 4) {
+        const int id = my_id[j];
+        ids[t * p.selected + j] = id;
+        weights[t * p.selected + j] = id < 0 ? 0.f : p.scale * (my_chosen[j] * factor);
+    }
+    unsigned again = __ballot_sync(FULL, unsure && here);
+    while (again) {
+        const int i = (__ffs(again) - 1) >> 2;
+        again &= ~(15u << (4 * i));
         __syncwarp();
+        route_row_exactly(logits + (t0 + i) * ld, p, c, (double *)keys, ids + (t0 + i) * p.selected, weights + (t0 + i) * p.selected);
     }
 }
 
+// Gradients of a warp's 8 rows are put together in shared memory, zeros but for the choices, and leave a row at a time in pieces of 8 columns a lane; with a softmax
+// over all experts every column has its share.
+__host__ __device__ constexpr int backward_words(int pieces) { return ROWS * (key_pitch(pieces) + 3); }
 template <class T>
-__global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__restrict__ logits, int64_t ld, RouteShape p, const uint8_t *__restrict__ mask,
-                                                                 const int *__restrict__ ids, const float *__restrict__ dweights, T *dlogits, int64_t ld_d, bool add)
+__global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p,
+                                                                      const uint8_t *__restrict__ mask, const int *__restrict__ ids,
+                                                                      const float *__restrict__ dweights, T *dlogits, int64_t ld_d, bool vec_d, bool add)
 {
     grid_dep_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
+    extern __shared__ __align__(16) float route_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, pieces = (E + 7) / 8, pitch = key_pitch(pieces);
+    float *grads = route_smem + warp * backward_words(pieces), *row_max = grads + ROWS * pitch, *row_inv = row_max + ROWS, *row_dot = row_inv + ROWS;
+    const int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * ROWS;
+    if (t0 >= p.T)
+        return;
     const bool softmax = p.score == TS2_SCORE_SOFTMAX, dense = softmax && !p.renormalize;
-    for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < p.T; t += (int64_t)gridDim.x * WARPS) {
-        const T *row = logits + t * ld;
-        const bool on = !mask || mask[t];
-        const int id = on && lane < p.selected ? ids[t * p.selected + lane] : -1;
-        const bool made = id >= 0 && id < E;
-        const float d = made ? dweights[t * p.selected + lane] : 0.f;
-        const bool any = __any_sync(FULL, made);
-        float top = -INFINITY, sum = 0.f;
-        if (dense && any) {
-            for (int c = lane; c < E; c += 32)
-                top = fmaxf(top, widen(row[c]));
-            top = warp_max(top);
-            if (top == -INFINITY)
-                top = 0.f;
-            for (int c = lane; c < E; c += 32)
-                sum += expf(widen(row[c]) - top);
-            sum = warp_sum(sum);
-        }
-        float s;
-        const float w = choice_weight(softmax, p.renormalize, made, made ? widen(row[id]) : 0.f, top, sum, s);
-        const float dot = warp_sum(d * w);
-        float g = d * w; // of the choice's logit, over scale
-        if (p.renormalize)
-            g = w * (d - dot) * (softmax ? 1.f : 1.f - s);
-        else if (!softmax)
-            g *= 1.f - s;
-        for (int c = lane; c < (E + 31) / 32 * 32; c += 32) {
-            float v = 0.f;
-            for (int j = 0; j < p.selected; ++j) {
-                const int e = __shfl_sync(FULL, made ? id : -1, j);
-                const float x = __shfl_sync(FULL, g, j);
-                v += e == c ? x : 0.f;
+    int width = 1; // lanes that share a row
+    while (width < pieces && width < 32)
+        width *= 2;
+    const int passes = max(1, ROWS * width / 32), at = lane & (width - 1), sub = lane / width;
+
+    if (dense)
+#pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass) {
+            const int r = pass * (32 / width) + sub;
+            const bool on = r < ROWS && t0 + r < p.T && (!mask || mask[t0 + r]);
+            float top = -INFINITY, sum = 0.f;
+            for (int i = at; i < pieces && on; i += width) {
+                float v[8];
+                load8(logits + (t0 + r) * ld, i * 8, E, vec, v);
+                // of what has come so far
+                const float now = fmaxf(top, max8(v)), ref = now == -INFINITY ? 0.f : now;
+                sum *= ex2((top - ref) * 1.44269504f);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    sum += ex2((v[k] - ref) * 1.44269504f);
+                top = now;
             }
-            if (c >= E)
-                continue;
-            if (dense && any)
-                v -= dot * (expf(widen(row[c]) - top) / sum);
-            v *= p.scale;
-            T *to = dlogits + t * ld_d + c;
-            *to = narrow<T>(add ? widen(*to) + v : v);
+            const float all = max_over(top, width), ref = all == -INFINITY ? 0.f : all;
+            sum = sum_over(sum * ex2((top - ref) * 1.44269504f), width);
+            if (r < ROWS && at == 0)
+                row_max[r] = ref, row_inv[r] = 1.f / sum;
         }
-        __syncwarp();
+    for (int i = lane; i < ROWS * pitch / 4; i += 32)
+        ((float4 *)grads)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncwarp();
+
+    { // the gradients of the choices' logits over scale; four lanes a row, every fourth choice each
+        const int r = lane >> 2, l = lane & 3;
+        const int64_t t = t0 + r;
+        const bool here = t < p.T && (!mask || mask[t]);
+        const T *row = logits + t * ld;
+        const int *my_ids = ids + t * p.selected;
+        const float *my_d = dweights + t * p.selected;
+        const auto choice = [&](int j) {
+            const int id = here && j < p.selected ? my_ids[j] : -1;
+            return id < E ? id : -1;
+        };
+        float top = -INFINITY;
+        if (p.renormalize)
+            for (int j = l; j < p.selected; j += 4) {
+                const int id = choice(j);
+                if (id >= 0) {
+                    const float v = widen(row[id]);
+                    top = fmaxf(top, softmax ? v : fminf(v, 0.f));
+                }
+            }
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        const float ref = p.renormalize ? top : softmax ? row_max[r] : 0.f;
+        const auto weight = [&](float v) { return softmax ? expf(v - ref) : expf(fminf(v, 0.f) - ref) / (1.f + expf(-fabsf(v))); };
+        float total = 0.f, dot = 0.f;
+        for (int j = l; j < p.selected; j += 4) {
+            const int id = choice(j);
+            if (id >= 0) {
+                const float w = weight(widen(row[id]));
+                total += w, dot += w * my_d[j];
+            }
+        }
+        total += __shfl_xor_sync(FULL, total, 1), dot += __shfl_xor_sync(FULL, dot, 1);
+        total += __shfl_xor_sync(FULL, total, 2), dot += __shfl_xor_sync(FULL, dot, 2);
+        const float factor = p.renormalize ? (total > 0.f ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f;
+        const bool any = total > 0.f; // a choice was made (or weighs nothing)
+        dot *= any ? factor : 0.f;
+        if (l == 0)
+            row_dot[r] = any ? dot : 0.f;
+#pragma unroll 1
+        for (int j0 = 0; j0 < p.selected; j0 += 4) {
+            const int id = choice(j0 + l);
+            float g = 0.f;
+            if (id >= 0) {
+                const float v = widen(row[id]), w = weight(v) * factor, d = my_d[j0 + l];
+                // 1 - sigmoid(v) = sigmoid(-v), without cancellation
+                const float rest = softmax ? 1.f : (v > 0.f ? expf(-v) : 1.f) / (1.f + expf(-fabsf(v)));
+                g = (p.renormalize ? w * (d - dot) : w * d) * rest;
+            }
+            // one of the four after the other: a caller's ids may name an expert twice
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (l == k && id >= 0)
+                    grads[r * pitch + id] += g;
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
+        const int r = pass * (32 / width) + sub;
+        const int64_t t = t0 + r;
+        if (r >= ROWS || t >= p.T)
+            continue;
+        const float dot = dense ? row_dot[r] : 0.f, ref = dense ? row_max[r] : 0.f, share = dense && dot != 0.f ? dot * row_inv[r] : 0.f;
+        for (int i = at; i < pieces; i += width) {
+            const float4 a = *(const float4 *)(grads + r * pitch + i * 8), b = *(const float4 *)(grads + r * pitch + i * 8 + 4);
+            float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            if (share != 0.f) {
+                float x[8];
+                load8(logits + t * ld, i * 8, E, vec, x);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    v[k] = fmaf(-share, ex2((x[k] - ref) * 1.44269504f), v[k]);
+            }
+            T *to = dlogits + t * ld_d + i * 8;
+            const bool whole = vec_d && i * 8 + 8 <= E;
+            constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+            for (int h = 0; h < 8 / PER; ++h) {
+                Piece<T, PER> q;
+                if (add) {
+                    if (whole)
+                        q = *(const Piece<T, PER> *)(to + h * PER);
+                    else
+#pragma unroll
+                        for (int k = 0; k < PER; ++k)
+                            if (i * 8 + h * PER + k < E)
+                                q.v[k] = to[h * PER + k];
+                }
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    q.v[k] = narrow<T>(add ? fmaf(p.scale, v[h * PER + k], widen(q.v[k])) : p.scale * v[h * PER + k]);
+                if (whole)
+                    *(Piece<T, PER> *)(to + h * PER) = q;
+                else
+#pragma unroll
+                    for (int k = 0; k < PER; ++k)
+                        if (i * 8 + h * PER + k < E)
+                            to[h * PER + k] = q.v[k];
+            }
+        }
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-static int blocks_for(const Ctx &c, int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(T, WARPS), 8 * sm_count(c.device))); }
-
-template <class T>
-static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const float *bias, int groups, int kept, int group_top,
-                   const uint8_t *mask, int *ids, float *weights)
+template <class T, int NB>
+static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const Choice &choice, const uint8_t *mask, int *ids, float *weights)
 {
-    const size_t smem = (size_t)WARPS * s.E * 8;
-    TS2_CUDA(cudaFuncSetAttribute((const void *)route_forward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * MOE_ROUTE_MAX_EXPERTS * 8));
-    TS2_LAUNCH((route_forward_kernel<T>), blocks_for(c, s.T), THREADS, smem, c.stream, (const T *)logits, ld, s, bias, groups, kept, group_top, mask, ids,
-               weights);
+    const int warps = THREADS / 32;
+    static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
+    const unsigned bit = 1u << (c.device & 15);
+    if (!(ready.load() & bit)) {
+        TS2_CUDA(cudaFuncSetAttribute((const void *)route_forward_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, warps * warp_words(4 * NB) * 4));
+        ready.fetch_or(bit);
+    }
+    const bool vec = (uintptr_t)logits % 16 == 0 && ld * sizeof(T) % 16 == 0;
+    TS2_LAUNCH((route_forward_kernel<T, NB>), (unsigned)ceil_div(s.T, warps * ROWS), THREADS, (size_t)warps * warp_words((s.E + 7) / 8) * 4, c.stream,
+               (const T *)logits, ld, vec, s, choice, mask, ids, weights);
     return TS2_OK;
+}
+template <class T>
+static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const Choice &choice, const uint8_t *mask, int *ids, float *weights)
+{
+    const auto f = s.E <= 32 ? forward<T, 1> : s.E <= 64 ? forward<T, 2> : s.E <= 128 ? forward<T, 4> : s.E <= 256 ? forward<T, 8> : s.E <= 512 ? forward<T, 16>
+                                                                                                                                     : forward<T, 32>;
+    return f(c, s, logits, ld, choice, mask, ids, weights);
 }
 template <class T>
 static int backward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const uint8_t *mask, const int *ids, const float *dweights,
                     void *dlogits, int64_t ld_d, bool add)
 {
-    TS2_LAUNCH((route_backward_kernel<T>), blocks_for(c, s.T), THREADS, 0, c.stream, (const T *)logits, ld, s, mask, ids, dweights, (T *)dlogits, ld_d, add);
+    const int warps = THREADS / 32;
+    static std::atomic<unsigned> ready{0}; // as above
+    const unsigned bit = 1u << (c.device & 15);
+    if (!(ready.load() & bit)) {
+        TS2_CUDA(cudaFuncSetAttribute((const void *)route_backward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      warps * backward_words(MOE_ROUTE_MAX_EXPERTS / 8) * 4));
+        ready.fetch_or(bit);
+    }
+    const auto aligned = [](const void *p, int64_t pitch) { return (uintptr_t)p % 16 == 0 && pitch * sizeof(T) % 16 == 0; };
+    TS2_LAUNCH((route_backward_kernel<T>), (unsigned)ceil_div(s.T, warps * ROWS), THREADS, (size_t)warps * backward_words((s.E + 7) / 8) * 4, c.stream,
+               (const T *)logits, ld, aligned(logits, ld), s, mask, ids, dweights, (T *)dlogits, ld_d, aligned(dlogits, ld_d), add);
     return TS2_OK;
 }
 
@@ -236,7 +672,7 @@ int moe_route_forward(const Ctx &c, const RouteShape &s, const void *logits, int
     if (s.T == 0)
         return TS2_OK;
     const auto f = s.type == TS2_OUT_F32 ? forward<float> : s.type == TS2_OUT_F16 ? forward<__half> : forward<__nv_bfloat16>;
-    return f(c, s, logits, ld, bias, groups, groups_kept, group_top, mask, ids, weights);
+    return f(c, s, logits, ld, {bias, groups, groups_kept, group_top}, mask, ids, weights);
 }
 int moe_route_backward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const uint8_t *mask, const int *ids, const float *dweights,
                        void *dlogits, int64_t dlogits_ld, bool add)

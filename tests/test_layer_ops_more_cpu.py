@@ -78,7 +78,7 @@ def adamw_args(n=2, **change):
 
 @pytest.mark.parametrize("change", [dict(grad_type=1), dict(bits=16), dict(bits=0), dict(copy_type=1), dict(copy_type=F32), dict(tensors=None), dict(n=-1),
                                     dict(rate=NAN), dict(rate=INF), dict(beta1=1.0), dict(beta1=-0.1), dict(beta1=NAN), dict(beta2=1.0), dict(beta2=NAN),
-                                    dict(eps=0.0), dict(eps=-1.0), dict(eps=NAN), dict(eps=INF), dict(step=0), dict(step=-3), dict(scale=NAN),
+                                    dict(eps=0.0), dict(eps=1e-39), dict(eps=-1.0), dict(eps=NAN), dict(eps=INF), dict(step=0), dict(step=-3), dict(scale=NAN),
                                     dict(scale_dev=P + 2)] +
                          [dict(tensor=t) for t in (dict(param=None), dict(grad=None), dict(m=None), dict(v=None), dict(m_scale=None), dict(v_scale=None),
                                                    dict(param=P + 2), dict(grad=P + 1), dict(copy=P + 1), dict(n=-1), dict(n=(1 << 40) + 1), dict(n=1 << 40),

@@ -202,7 +202,7 @@ int ts2_op_adamw(int device, void *stream, int grad_type, int state_bits, int co
 {
     const auto finite = [](float v) { return v - v == 0.f; };
     bool ok = type_size(grad_type) && (state_bits == 32 || state_bits == 8) && type_size(copy_type) && n_tensors >= 0 && n_tensors <= 1 << 20 &&
-              (tensors || !n_tensors) && finite(rate) && beta1 >= 0.f && beta1 < 1.f && beta2 >= 0.f && beta2 < 1.f && eps > 0.f && finite(eps) && step >= 1 &&
+              (tensors || !n_tensors) && finite(rate) && beta1 >= 0.f && beta1 < 1.f && beta2 >= 0.f && beta2 < 1.f && eps >= 0x1p-126f && finite(eps) && step >= 1 &&
               finite(grad_scale) && floats_ok(grad_scale_dev);
     int64_t total = 0;
     for (int i = 0; ok && i < n_tensors; ++i) {

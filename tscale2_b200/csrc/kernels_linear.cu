@@ -544,6 +544,119 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const LinearArgs p, in
     }
 }
 
+// ---- a few tokens --------------------------------------------------------------------------------------------------------
+// Bound by reading W once.  A CTA takes 16 rows of W; its 8 warps, and those of the up to 8 CTAs of a cluster where W has few rows, divide K.  A lane reads 8
+// neighbours of two rows of W and of the tokens' x; four lanes' pieces are 32 of K, and as both operands come in the same order they are the fragments of two
+// m16n8k16 products as they lie in the registers.  Sums are added in the order of the warps and CTAs.
+constexpr int FEW_WARPS = 8, FEW_BATCH = 4; // FEW_BATCH: blocks of 32 of K on their way at a time
+struct FewArgs {
+    int T, n, m; // tokens, columns of x and W, rows of W
+    const uint16_t *x, *w, *res;
+    int64_t x_ld, w_ld, res_ld, y_ld, z_ld;
+    const float *bias;
+    uint16_t *y, *z;
+    int act, ranks;
+};
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 neighbours of a row from column k on, zeros behind the last one and where the row is not there
+template <bool VEC>
+__device__ __forceinline__ uint4 eight_of(const uint16_t *row, int k, int n, bool there)
+{
+    if (VEC && there && k + 8 <= n)
+        return *(const uint4 *)(row + k);
+    uint32_t v[4] = {};
+    if (there)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i >> 1] |= k + i < n ? (uint32_t)row[k + i] << (16 * (i & 1)) : 0u;
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// NT: tokens in eights
+template <int NT, bool BF16, bool VEC>
+__global__ void __launch_bounds__(32 * FEW_WARPS) linear_few_kernel(const FewArgs p)
+{
+    __shared__ float part[FEW_WARPS][8 * NT][17], sums[8 * NT][17];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const uint32_t rank = p.ranks > 1 ? cluster_rank() : 0;
+    const int row0 = (int)(blockIdx.x / p.ranks) * 16, blocks = (p.n + 31) / 32, workers = p.ranks * FEW_WARPS, mine = (int)rank * FEW_WARPS + warp;
+    const int kb0 = (int)((int64_t)blocks * mine / workers), kb1 = (int)((int64_t)blocks * (mine + 1) / workers);
+    grid_dep_wait();
+    const uint16_t *wa = p.w + (int64_t)(row0 + g) * p.w_ld, *wb = wa + 8 * p.w_ld;
+    const bool a_there = row0 + g < p.m, b_there = row0 + g + 8 < p.m;
+    float c[NT][4] = {};
+#pragma unroll 1
+    for (int kb = kb0; kb < kb1; kb += FEW_BATCH) {
+        uint4 a[FEW_BATCH], b[FEW_BATCH], x[FEW_BATCH][NT];
+#pragma unroll
+        for (int i = 0; i < FEW_BATCH; ++i) {
+            const int k = (kb + i) * 32 + q * 8;
+            const bool in = kb + i < kb1;
+            a[i] = eight_of<VEC>(wa, k, p.n, in && a_there);
+            b[i] = eight_of<VEC>(wb, k, p.n, in && b_there);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                x[i][t] = eight_of<VEC>(p.x + (int64_t)(8 * t + g) * p.x_ld, k, p.n, in && 8 * t + g < p.T);
+        }
+#pragma unroll
+        for (int i = 0; i < FEW_BATCH; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                mma16<BF16>(c[t], a[i].x, b[i].x, a[i].y, b[i].y, x[i][t].x, x[i][t].y);
+                mma16<BF16>(c[t], a[i].z, b[i].z, a[i].w, b[i].w, x[i][t].z, x[i][t].w);
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        part[warp][8 * t + 2 * q][g] = c[t][0], part[warp][8 * t + 2 * q + 1][g] = c[t][1];
+        part[warp][8 * t + 2 * q][g + 8] = c[t][2], part[warp][8 * t + 2 * q + 1][g + 8] = c[t][3];
+    }
+    __syncthreads();
+    const int row = threadIdx.x & 15;
+    for (int t = threadIdx.x >> 4; t < 8 * NT; t += 2 * FEW_WARPS) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < FEW_WARPS; ++k)
+            s += part[k][t][row];
+        sums[t][row] = s;
+    }
+    if (p.ranks > 1)
+        cluster_sync(); // every CTA's sums are there
+    if (rank == 0) {
+        for (int t = threadIdx.x >> 4; t < p.T; t += 2 * FEW_WARPS) {
+            float v[1] = {sums[t][row]}; // this thread's own, the other CTAs' by their order
+            for (int k = 1; k < p.ranks; ++k) {
+                float other;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(map_to_rank(smem_u32(&sums[t][row]), k)) : "memory");
+                v[0] += other;
+            }
+            const int at = row0 + row;
+            if (at >= p.m)
+                continue;
+            if (p.bias)
+                v[0] += p.bias[at];
+            if (p.z)
+                p.z[t * p.z_ld + at] = (uint16_t)pack2<BF16>(v[0], 0.f);
+            activate(p.act, v);
+            if (p.res)
+                v[0] += widen16<BF16>(p.res[t * p.res_ld + at]);
+            p.y[t * p.y_ld + at] = (uint16_t)pack2<BF16>(v[0], 0.f);
+        }
+    }
+    if (p.ranks > 1)
+        cluster_sync(); // nobody reads this CTA's sums any more
+}
+
 // ---- dz and its column sums ------------------------------------------------------------------------------------------------
 // A block takes 128 columns and rows b, b + blocks, ... of 16: dz = dy act'(z) rounded to 16 bits (dz null: not wanted), and the sums of the unrounded
 // dz over its rows (sums null: not wanted).  Bound by reading dy and z.
@@ -737,6 +850,35 @@ int product(const Ctx &c, bool bf16, const Operand &a, const Operand &b, int64_t
     return bf16 ? product<A_MN, B_MN, 256, true>(c, a, b, K, p) : product<A_MN, B_MN, 256, false>(c, a, b, K, p);
 }
 
+// tokens that take the form for a few
+constexpr int FEW_TOKENS = 16;
+template <int NT, bool BF16, bool VEC>
+int few(const Ctx &c, const FewArgs &p)
+{
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.ranks, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ceil_div(p.m, 16) * p.ranks));
+    cfg.blockDim = 32 * FEW_WARPS;
+    cfg.stream = c.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.ranks > 1 ? 2 : 1;
+    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+    if (const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_few_kernel<NT, BF16, VEC>, p); e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(TS2_ERR_CUDA, "kernel launch failed: %s (%s:%d)", cudaGetErrorString(e), __FILE__, __LINE__);
+    }
+    return TS2_OK;
+}
+template <int NT>
+int few(const Ctx &c, bool bf16, bool vec, const FewArgs &p)
+{
+    return bf16 ? vec ? few<NT, true, true>(c, p) : few<NT, true, false>(c, p) : vec ? few<NT, false, true>(c, p) : few<NT, false, false>(c, p);
+}
+
 } // namespace
 
 int linear_forward(const Ctx &c, const LinearShape &s, const void *x, int64_t x_ld, const void *w, int64_t w_ld, const float *bias, const void *residual,
@@ -744,6 +886,15 @@ int linear_forward(const Ctx &c, const LinearShape &s, const void *x, int64_t x_
 {
     if (s.T == 0)
         return TS2_OK;
+    if (s.T <= FEW_TOKENS) {
+        FewArgs f = {(int)s.T, s.in, s.out, (const uint16_t *)x, (const uint16_t *)w, (const uint16_t *)residual, x_ld, w_ld, residual_ld, y_ld, z_ld, bias,
+                     (uint16_t *)y, (uint16_t *)z, s.act, 1};
+        // CTAs for two an SM, each warp with a batch of K at least
+        while (f.ranks < 8 && ceil_div(s.out, 16) * f.ranks < 2 * sm_count(c.device) && s.in >= 2 * f.ranks * FEW_WARPS * FEW_BATCH * 32)
+            f.ranks *= 2;
+        const bool vec = tma_ok(x, x_ld, 2) && tma_ok(w, w_ld, 2);
+        return s.T <= 8 ? few<1>(c, s.type == TS2_OUT_BF16, vec, f) : few<2>(c, s.type == TS2_OUT_BF16, vec, f);
+    }
     const Operand a(c, x, x_ld, s.T, s.in), b(c, w, w_ld, s.out, s.in);
     if (a.rc != TS2_OK || b.rc != TS2_OK)
         return a.rc != TS2_OK ? a.rc : b.rc;

@@ -584,7 +584,7 @@ __device__ __forceinline__ uint4 eight_of(const uint16_t *row, int k, int n, boo
 }
 // NT: tokens in eights
 template <int NT, bool BF16, bool VEC>
-__global__ void __launch_bounds__(32 * FEW_WARPS) linear_few_kernel(const FewArgs p)
+__global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 4 : 1) linear_few_kernel(const FewArgs p)
 {
     __shared__ float part[FEW_WARPS][8 * NT][17], sums[8 * NT][17];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;

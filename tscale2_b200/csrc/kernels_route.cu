@@ -17,6 +17,7 @@
 #include "elem_types.cuh"
 #include "kernels.cuh"
 #include <algorithm>
+#include <type_traits>
 
 namespace ts2 {
 
@@ -173,26 +174,51 @@ __device__ __noinline__ void route_row_exactly(const T *__restrict__ row, const 
 // their pieces, the groups' ranks, choices and what they weigh, and of the softmax the row's maximum and its sum's reciprocal.
 static constexpr int ROWS = 8, SLOTS = MOE_ROUTE_MAX_SELECTED + 1;
 __host__ __device__ constexpr int key_pitch(int pieces) { return (pieces + 3) / 4 * 32 + 4; }
-__host__ __device__ constexpr int warp_words(int pieces) { return ROWS * (key_pitch(pieces) + 2 * (pieces | 1) + 33 + 2 * SLOTS + 2); }
+__host__ __device__ constexpr int piece_pitch(int held) { return held * 4 + 4; } // held: pieces of each of a row's four lanes
+__host__ __device__ constexpr int warp_words(int pieces, int held, bool second, int groups, int selected)
+{
+    return ROWS * (key_pitch(pieces) + piece_pitch(held) * (second ? 2 : 1) + (groups > 1 ? groups : 0) + 2 * (selected + 1) + 2) + 4;
+}
 
-// eight neighbours from column e on, -inf behind the last one
+// eight neighbours from column e on as they lie in memory, -inf behind the last one and where there is nothing to read
+template <class T>
+struct Eight {
+    static constexpr int PER = 16 / sizeof(T);
+    Piece<T, PER> q[8 / PER];
+    __device__ __forceinline__ void load(const T *row, int e, int E, bool vec, bool there)
+    {
+        if (vec && there && e + 8 <= E) {
+#pragma unroll
+            for (int i = 0; i < 8 / PER; ++i)
+                q[i] = *(const Piece<T, PER> *)(row + e + i * PER);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                q[i / PER].v[i % PER] = there && e + i < E ? row[e + i] : narrow_infinity();
+        }
+    }
+    static __device__ __forceinline__ T narrow_infinity()
+    {
+        if constexpr (sizeof(T) == 4)
+            return -INFINITY;
+        else if constexpr (std::is_same<T, __half>::value)
+            return __ushort_as_half(0xfc00);
+        else
+            return __ushort_as_bfloat16(0xff80);
+    }
+    __device__ __forceinline__ void widen_to(float (&v)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = widen(q[i / PER].v[i % PER]);
+    }
+};
 template <class T>
 __device__ __forceinline__ void load8(const T *row, int e, int E, bool vec, float (&v)[8])
 {
-    if (vec && e + 8 <= E) {
-        constexpr int PER = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 8 / PER; ++i) {
-            const Piece<T, PER> q = *(const Piece<T, PER> *)(row + e + i * PER);
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                v[i * PER + j] = widen(q.v[j]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = e + i < E ? widen(row[e + i]) : -INFINITY;
-    }
+    Eight<T> q;
+    q.load(row, e, E, vec, true);
+    q.widen_to(v);
 }
 // over the `width` neighbouring lanes that share a row
 __device__ __forceinline__ float max_over(float v, int width)
@@ -212,107 +238,150 @@ __device__ __forceinline__ float max8(const float (&v)[8])
     return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
 }
 
+// the largest and the second of eight
+__device__ __forceinline__ void two_of(const float (&v)[8], float &best, float &next)
+{
+    float a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        a[i] = fmaxf(v[2 * i], v[2 * i + 1]), b[i] = fminf(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        b[i] = fmaxf(fminf(a[i], a[i + 1]), fmaxf(b[i], b[i + 1]));
+        a[i] = fmaxf(a[i], a[i + 1]);
+    }
+    best = fmaxf(a[0], a[2]), next = fmaxf(fminf(a[0], a[2]), fmaxf(b[0], b[2]));
+}
+
 // NB: pieces of 8 columns that each of the four lanes of a row has (E <= 32 NB)
 template <class T, int NB>
 __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p, const Choice c,
-                                                                     const uint8_t *__restrict__ mask, int *ids, float *weights)
+                                                                const uint8_t *__restrict__ mask, int *ids, float *weights)
 {
     grid_dep_wait();
-    constexpr int HELD = (NB + 7) / 8; // pieces a lane has of a row that comes in
+    // WIDTH: lanes that share a row while it comes in, HELD pieces each, STEP passes at a time
+    constexpr int WIDTH = NB >= 8 ? 32 : 4 * NB, HELD = NB > 8 ? NB / 8 : 1, PASSES = ROWS * WIDTH / 32, STEP = PASSES < 8 / HELD ? PASSES : 8 / HELD;
     extern __shared__ __align__(16) float route_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, pieces = (E + 7) / 8, per = E / c.groups;
-    const int pitch = key_pitch(pieces), piece_pitch = pieces | 1;
-    float *keys = route_smem + warp * warp_words(pieces), *first = keys + ROWS * pitch, *second = first + ROWS * piece_pitch,
-          *ranks = second + ROWS * piece_pitch, *chosen = ranks + ROWS * 33, *row_max = chosen + ROWS * SLOTS, *row_inv = row_max + ROWS;
+    const bool two = c.groups > 1 && c.group_top == 2;
+    constexpr int pp = piece_pitch(NB);
+    const int pitch = key_pitch(pieces), slots = p.selected + 1;
+    float *keys = route_smem + warp * warp_words(pieces, NB, two, c.groups, p.selected), *first = keys + ROWS * pitch, *second = first + ROWS * pp,
+          *ranks = second + (two ? ROWS * pp : 0), *chosen = ranks + (c.groups > 1 ? ROWS * c.groups : 0), *row_max = chosen + ROWS * slots,
+          *row_inv = row_max + ROWS;
     int *chosen_id = (int *)(row_inv + ROWS);
     const int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * ROWS;
     if (t0 >= p.T)
         return;
     const bool softmax = p.score == TS2_SCORE_SOFTMAX, by_logit = !c.bias && (c.groups == 1 || c.group_top == 1), stats = softmax && !(by_logit && p.renormalize);
-    int width = 1; // lanes that share a row
-    while (width < pieces && width < 32)
-        width *= 2;
+    const int at = lane & (WIDTH - 1), sub = lane / WIDTH;
+    float bias[HELD][8]; // of the lane's columns
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = (at + 32 * h) * 8 + i;
+            bias[h][i] = c.bias && e < E ? c.bias[e] : 0.f;
+        }
+    // a piece's place among the largest keys: neighbours of a lane of the four side by side
+    const auto place = [&](int piece) { return (piece & 3) * NB + (piece >> 2); };
 
     // rows come in
 #pragma unroll 1
-    for (int pass = 0; pass < ROWS * width / 32 || pass == 0; ++pass) {
-        const int r = pass * (32 / width) + lane / width, at = lane & (width - 1);
-        const int64_t t = t0 + r;
-        const bool on = r < ROWS && t < p.T && (!mask || mask[t]);
-        float v[HELD][8];
-        float top = -INFINITY, sum = 0.f;
-        bool bad = !on;
+    for (int pass0 = 0; pass0 < PASSES; pass0 += STEP) {
+        Eight<T> raw[STEP][HELD];
+        bool on[STEP];
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            if (on && at + 32 * h < pieces)
-                load8(logits + t * ld, (at + 32 * h) * 8, E, vec, v[h]);
-            else
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[h][i] = -INFINITY;
-            top = fmaxf(top, max8(v[h]));
-        }
-        if (stats) {
-            top = max_over(top, width);
-            const float ref = top == -INFINITY ? 0.f : top;
+        for (int s = 0; s < STEP; ++s) {
+            const int64_t t = t0 + (pass0 + s) * (32 / WIDTH) + sub;
+            on[s] = t < p.T && (!mask || mask[t]);
 #pragma unroll
             for (int h = 0; h < HELD; ++h)
+                raw[s][h].load(logits + t * ld, (at + 32 * h) * 8, E, vec, on[s] && at + 32 * h < pieces);
+        }
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    sum += ex2((v[h][i] - ref) * 1.44269504f); // a NaN, and infinity minus itself, end here
-            sum = sum_over(sum, width);
-            bad |= !(sum == sum);
-            if (r < ROWS && at == 0)
-                row_max[r] = ref, row_inv[r] = 1.f / sum;
-            top = ref;
-        } else if (softmax) {
+        for (int s = 0; s < STEP; ++s) {
+            const int r = (pass0 + s) * (32 / WIDTH) + sub;
+            float v[HELD][8];
+            float top = 0.f, inv = 1.f;
+            bool bad = !on[s];
 #pragma unroll
             for (int h = 0; h < HELD; ++h)
+                raw[s][h].widen_to(v[h]);
+            if (stats) {
+                top = max8(v[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    bad |= !(v[h][i] < INFINITY);
-            bad = max_over(bad ? 1.f : 0.f, width) > 0.f;
-        }
-        const float inv = stats ? 1.f / sum : 1.f;
-        if (r >= ROWS)
-            continue;
+                for (int h = 1; h < HELD; ++h)
+                    top = fmaxf(top, max8(v[h]));
+                top = max_over(top, WIDTH);
+                top = top == -INFINITY ? 0.f : top;
+                float sum = 0.f;
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            const int piece = at + 32 * h;
-            if (piece >= pieces)
-                continue;
-            float k[8];
-            if (by_logit) {
+                for (int h = 0; h < HELD; ++h)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    k[i] = fmaxf(v[h][i], -INFINITY); // a NaN is none
-            } else {
+                    for (int i = 0; i < 8; ++i)
+                        sum += ex2((v[h][i] - top) * 1.44269504f); // a NaN, and infinity minus itself, end here
+                sum = sum_over(sum, WIDTH);
+                bad |= !(sum == sum);
+                inv = 1.f / sum;
+                if (at == 0)
+                    row_max[r] = top, row_inv[r] = inv;
+            } else if (softmax) {
+                bool wrong = false;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float l = v[h][i];
-                    float s = softmax ? ex2((l - top) * 1.44269504f) * inv : rcp(1.f + ex2(l * -1.44269504f));
-                    if (c.bias)
-                        s += piece * 8 + i < E ? c.bias[piece * 8 + i] : 0.f;
-                    k[i] = l == -INFINITY ? -INFINITY : fmaxf(s, -INFINITY);
-                }
+                for (int h = 0; h < HELD; ++h)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        wrong |= !(v[h][i] < INFINITY);
+                const unsigned lanes = WIDTH == 32 ? FULL : ((1u << (WIDTH & 31)) - 1) << (sub * WIDTH);
+                bad |= (__ballot_sync(FULL, wrong) & lanes) != 0;
             }
-            if (bad)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    k[i] = -INFINITY;
-            float4 *to = (float4 *)(keys + r * pitch + piece * 8);
-            to[0] = make_float4(k[0], k[1], k[2], k[3]);
-            to[1] = make_float4(k[4], k[5], k[6], k[7]);
-            if (c.groups > 1 && c.group_top == 2) {
-                float best = k[0], next = -INFINITY;
+            for (int h = 0; h < HELD; ++h) {
+                const int piece = at + 32 * h;
+                float k[8];
+                if (by_logit) {
 #pragma unroll
-                for (int i = 1; i < 8; ++i) {
-                    next = fmaxf(next, fminf(best, k[i]));
-                    best = fmaxf(best, k[i]);
+                    for (int i = 0; i < 8; ++i)
+                        k[i] = fmaxf(v[h][i], -INFINITY); // a NaN is none
+                } else {
+                    if (softmax) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            k[i] = ex2((v[h][i] - top) * 1.44269504f) * inv;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            k[i] = rcp(1.f + ex2(v[h][i] * -1.44269504f));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        k[i] = fmaxf(k[i] + bias[h][i], -INFINITY);
+                    const float least = fminf(fminf(fminf(v[h][0], v[h][1]), fminf(v[h][2], v[h][3])), fminf(fminf(v[h][4], v[h][5]), fminf(v[h][6], v[h][7])));
+                    if (least == -INFINITY)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            k[i] = v[h][i] == -INFINITY ? -INFINITY : k[i];
                 }
-                first[r * piece_pitch + piece] = best, second[r * piece_pitch + piece] = next;
-            } else {
-                first[r * piece_pitch + piece] = max8(k);
+                if (bad)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        k[i] = -INFINITY;
+                float best, next = 0.f;
+                if (two)
+                    two_of(k, best, next);
+                else
+                    best = max8(k);
+                if (piece < pieces) {
+                    float4 *to = (float4 *)(keys + r * pitch + piece * 8);
+                    to[0] = make_float4(k[0], k[1], k[2], k[3]);
+                    to[1] = make_float4(k[4], k[5], k[6], k[7]);
+                }
+                if (piece < 4 * NB) { // -inf where there is none
+                    first[r * pp + place(piece)] = best;
+                    if (two)
+                        second[r * pp + place(piece)] = next;
+                }
             }
         }
     }
@@ -321,9 +390,8 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
     // four lanes a row from here on
     const int r = lane >> 2, l = lane & 3;
     const int64_t t = t0 + r;
-    float *my_keys = keys + r * pitch, *my_first = first + r * piece_pitch, *my_second = second + r * piece_pitch, *my_ranks = ranks + r * 33,
-          *my_chosen = chosen + r * SLOTS;
-    int *my_id = chosen_id + r * SLOTS;
+    float *my_keys = keys + r * pitch, *my_first = first + r * pp, *my_second = second + r * pp, *my_ranks = ranks + r * c.groups, *my_chosen = chosen + r * slots;
+    int *my_id = chosen_id + r * slots;
     const float unit = !by_logit && softmax ? row_inv[r] * 0x1p-18f : 0x1p-19f; // two scores are off by less together
     const auto near = [&](float a, float b, float times) { return !(a - b > times * (unit + 0x1p-22f * (fabsf(a) + fabsf(b)))); };
     bool unsure = false;
@@ -337,15 +405,15 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
             };
             if (aligned) {
                 for (int i = g * (per / 8); i < (g + 1) * (per / 8); ++i) {
-                    if (c.group_top == 2)
-                        next = fmaxf(next, my_second[i]);
-                    take(my_first[i]);
+                    if (two)
+                        next = fmaxf(next, my_second[place(i)]);
+                    take(my_first[place(i)]);
                 }
             } else {
                 for (int e = g * per; e < (g + 1) * per; ++e)
                     take(my_keys[e]);
             }
-            my_ranks[g] = c.group_top == 2 ? fmaxf(best + next, -INFINITY) : best;
+            my_ranks[g] = two ? fmaxf(best + next, -INFINITY) : best;
         }
         __syncwarp();
         float worst_kept = INFINITY, best_left = -INFINITY;
@@ -361,7 +429,7 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
             best_left = fmaxf(best_left, mine);
             if (aligned)
                 for (int i = g * (per / 8); i < (g + 1) * (per / 8); ++i)
-                    my_first[i] = -INFINITY;
+                    my_first[place(i)] = -INFINITY;
             else
                 for (int e = g * per; e < (g + 1) * per; ++e)
                     my_keys[e] = -INFINITY;
@@ -375,7 +443,7 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
                 float best = -INFINITY;
                 for (int e = i * 8; e < min(E, i * 8 + 8); ++e)
                     best = fmaxf(best, my_keys[e]);
-                my_first[i] = best;
+                my_first[place(i)] = best;
             }
             __syncwarp();
         }
@@ -383,7 +451,7 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
     float held[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-        held[i] = i * 4 + l < pieces ? my_first[i * 4 + l] : -INFINITY;
+        held[i] = my_first[l * NB + i];
     const int rounds = p.selected + (by_logit ? 0 : 1); // the first key that is not chosen, for its distance
 #pragma unroll 1
     for (int j = 0; j < rounds; ++j) {
@@ -425,42 +493,45 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
     // weights: a lane has every fourth choice
     const bool here = t < p.T;
     const T *row = logits + t * ld;
-    const auto logit = [&](int id) { return widen(row[id]); };
-    float top = -INFINITY, total = 0.f;
-    for (int j = l; j < p.selected && here; j += 4) {
-        const int id = my_id[j];
-        if (id < 0)
-            continue;
-        const float v = logit(id);
-        top = fmaxf(top, softmax ? v : fminf(v, 0.f));
-        if (!by_logit) {
+    constexpr int MINE = MOE_ROUTE_MAX_SELECTED / 4;
+    float v[MINE], top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int j = i * 4 + l, id = here && j < p.selected ? my_id[j] : -1;
+        v[i] = id >= 0 ? widen(row[id]) : -INFINITY;
+        top = fmaxf(top, softmax ? v[i] : fminf(v[i], 0.f));
+        if (!by_logit && id >= 0) {
             const int next = my_id[j + 1];
             if (next >= 0 && near(my_chosen[j], my_chosen[j + 1], 1.f)) // equal logits and biases are equal keys, whose order is known
-                unsure |= j == p.selected - 1 || v != logit(next) || (c.bias && c.bias[id] != c.bias[next]);
+                unsure |= j == p.selected - 1 || v[i] != widen(row[next]) || (c.bias && c.bias[id] != c.bias[next]);
         }
+        if (i * 4 + 4 >= p.selected)
+            break;
     }
     top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
     top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
-    __syncwarp(); // the keys have been compared
     const float ref = p.renormalize ? top : softmax ? row_max[r] : 0.f;
-    for (int j = l; j < p.selected && here; j += 4) {
-        const int id = my_id[j];
-        float w = 0.f;
-        if (id >= 0) {
-            const float v = logit(id);
-            // sigmoid(v) = exp(min(v, 0)) / (1 + exp(-|v|)): nothing underflows that matters to a quotient
-            w = softmax ? expf(v - ref) : expf(fminf(v, 0.f) - ref) / (1.f + expf(-fabsf(v)));
-        }
-        my_chosen[j] = w;
-        total += w;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        // sigmoid(v) = exp(min(v, 0)) / (1 + exp(-|v|)): nothing underflows that matters to a quotient
+        const float w = softmax ? ex2((v[i] - ref) * 1.44269504f) : ex2((fminf(v[i], 0.f) - ref) * 1.44269504f) * rcp(1.f + ex2(fabsf(v[i]) * -1.44269504f));
+        v[i] = v[i] > -INFINITY ? w : 0.f;
+        total += v[i];
+        if (i * 4 + 4 >= p.selected)
+            break;
     }
     total += __shfl_xor_sync(FULL, total, 1);
     total += __shfl_xor_sync(FULL, total, 2);
-    const float factor = p.renormalize ? (total > 0.f ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f;
-    for (int j = l; j < p.selected && here; j += 4) {
-        const int id = my_id[j];
-        ids[t * p.selected + j] = id;
-        weights[t * p.selected + j] = id < 0 ? 0.f : p.scale * (my_chosen[j] * factor);
+    const float factor = p.scale * (p.renormalize ? (total > 0.f ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int j = i * 4 + l;
+        if (here && j < p.selected) {
+            ids[t * p.selected + j] = my_id[j];
+            weights[t * p.selected + j] = v[i] > 0.f ? v[i] * factor : 0.f;
+        }
+        if (i * 4 + 4 >= p.selected)
+            break;
     }
     unsigned again = __ballot_sync(FULL, unsure && here);
     while (again) {
@@ -523,57 +594,56 @@ __global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__rest
         const int64_t t = t0 + r;
         const bool here = t < p.T && (!mask || mask[t]);
         const T *row = logits + t * ld;
-        const int *my_ids = ids + t * p.selected;
-        const float *my_d = dweights + t * p.selected;
-        const auto choice = [&](int j) {
-            const int id = here && j < p.selected ? my_ids[j] : -1;
-            return id < E ? id : -1;
-        };
-        float top = -INFINITY;
-        if (p.renormalize)
-            for (int j = l; j < p.selected; j += 4) {
-                const int id = choice(j);
-                if (id >= 0) {
-                    const float v = widen(row[id]);
-                    top = fmaxf(top, softmax ? v : fminf(v, 0.f));
-                }
-            }
-        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        constexpr int MINE = MOE_ROUTE_MAX_SELECTED / 4;
+        int id[MINE];
+        float v[MINE], d[MINE], top = -INFINITY, total = 0.f, dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int j = i * 4 + l;
+            id[i] = here && j < p.selected ? ids[t * p.selected + j] : -1;
+            if (id[i] >= E)
+                id[i] = -1;
+            v[i] = 0.f, d[i] = 0.f;
+            if (id[i] >= 0)
+                v[i] = widen(row[id[i]]), d[i] = dweights[t * p.selected + j], top = fmaxf(top, softmax ? v[i] : fminf(v[i], 0.f));
+            if (i * 4 + 4 >= p.selected)
+                break;
+        }
+        if (p.renormalize) {
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        }
         const float ref = p.renormalize ? top : softmax ? row_max[r] : 0.f;
-        const auto weight = [&](float v) { return softmax ? expf(v - ref) : expf(fminf(v, 0.f) - ref) / (1.f + expf(-fabsf(v))); };
-        float total = 0.f, dot = 0.f;
-        for (int j = l; j < p.selected; j += 4) {
-            const int id = choice(j);
-            if (id >= 0) {
-                const float w = weight(widen(row[id]));
-                total += w, dot += w * my_d[j];
-            }
+        float w[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            w[i] = softmax ? ex2((v[i] - ref) * 1.44269504f) : ex2((fminf(v[i], 0.f) - ref) * 1.44269504f) * rcp(1.f + ex2(fabsf(v[i]) * -1.44269504f));
+            w[i] = id[i] >= 0 ? w[i] : 0.f;
+            total += w[i], dot = fmaf(w[i], d[i], dot);
+            if (i * 4 + 4 >= p.selected)
+                break;
         }
         total += __shfl_xor_sync(FULL, total, 1), dot += __shfl_xor_sync(FULL, dot, 1);
         total += __shfl_xor_sync(FULL, total, 2), dot += __shfl_xor_sync(FULL, dot, 2);
-        const float factor = p.renormalize ? (total > 0.f ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f;
         const bool any = total > 0.f; // a choice was made (or weighs nothing)
-        dot *= any ? factor : 0.f;
+        const float factor = p.renormalize ? (any ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f;
+        dot = any ? dot * factor : 0.f;
         if (l == 0)
-            row_dot[r] = any ? dot : 0.f;
-#pragma unroll 1
-        for (int j0 = 0; j0 < p.selected; j0 += 4) {
-            const int id = choice(j0 + l);
-            float g = 0.f;
-            if (id >= 0) {
-                const float v = widen(row[id]), w = weight(v) * factor, d = my_d[j0 + l];
-                // 1 - sigmoid(v) = sigmoid(-v), without cancellation
-                const float rest = softmax ? 1.f : (v > 0.f ? expf(-v) : 1.f) / (1.f + expf(-fabsf(v)));
-                g = (p.renormalize ? w * (d - dot) : w * d) * rest;
-            }
+            row_dot[r] = dot;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            // 1 - sigmoid(v) = sigmoid(-v), without cancellation
+            const float rest = softmax ? 1.f : ex2(fmaxf(v[i], 0.f) * -1.44269504f) * rcp(1.f + ex2(fabsf(v[i]) * -1.44269504f));
+            const float g = w[i] * factor * (p.renormalize ? d[i] - dot : d[i]) * rest;
             // one of the four after the other: a caller's ids may name an expert twice
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (l == k && id >= 0)
-                    grads[r * pitch + id] += g;
+                if (l == k && id[i] >= 0)
+                    grads[r * pitch + id[i]] += g;
                 __syncwarp();
             }
+            if (i * 4 + 4 >= p.selected)
+                break;
         }
     }
     __syncwarp();
@@ -630,15 +700,18 @@ template <class T, int NB>
 static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const Choice &choice, const uint8_t *mask, int *ids, float *weights)
 {
     const int warps = THREADS / 32;
+    constexpr int most = warps * warp_words(4 * NB, NB, true, MOE_ROUTE_MAX_GROUPS, MOE_ROUTE_MAX_SELECTED) * 4;
+    static_assert(most <= 232448, "shared memory budget");
     static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
     const unsigned bit = 1u << (c.device & 15);
     if (!(ready.load() & bit)) {
-        TS2_CUDA(cudaFuncSetAttribute((const void *)route_forward_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, warps * warp_words(4 * NB) * 4));
+        TS2_CUDA(cudaFuncSetAttribute((const void *)route_forward_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         ready.fetch_or(bit);
     }
     const bool vec = (uintptr_t)logits % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    TS2_LAUNCH((route_forward_kernel<T, NB>), (unsigned)ceil_div(s.T, warps * ROWS), THREADS, (size_t)warps * warp_words((s.E + 7) / 8) * 4, c.stream,
-               (const T *)logits, ld, vec, s, choice, mask, ids, weights);
+    const size_t smem = (size_t)warps * warp_words((s.E + 7) / 8, NB, choice.groups > 1 && choice.group_top == 2, choice.groups, s.selected) * 4;
+    TS2_LAUNCH((route_forward_kernel<T, NB>), (unsigned)ceil_div(s.T, warps * ROWS), THREADS, smem, c.stream, (const T *)logits, ld, vec, s, choice, mask, ids,
+               weights);
     return TS2_OK;
 }
 template <class T>

@@ -7,9 +7,9 @@
 //     sigmoid              dl[e] = scale d[e] s[e] (1 - s[e])
 //     sigmoid, renormalised  dl[e] = scale w[e] (1 - s[e]) (d[e] - sum_j d[j] w[j])
 //
-// A warp takes 8 rows.  They come in a row at a time in pieces of 8 columns a lane, and their keys and every piece's largest key go to shared memory.  Then
-// four lanes have a row, each the largest keys of every fourth piece in registers: a choice is a maximum over those and over the four lanes, and only the piece
-// that it came from is looked at again.
+// A warp takes 4 rows (8 of up to 32 experts).  They come in a row at a time in pieces of 8 columns a lane, and their keys and every piece's largest key go to
+// shared memory.  Then 8 (4) lanes have a row, each the largest keys of every eighth piece in registers: a choice is a maximum over those and over the lanes, and
+// only the piece that it came from is looked at again.
 //
 // Keys are fp32 first.  They order as exact ones would where they differ by more than fp32 can be wrong, so a row in which two choices, the last choice and the
 // next key, or two groups at the border are nearer than that is done once more in fp64 by the whole warp.  Without a bias (and with groups ranked by one key)
@@ -172,12 +172,11 @@ __device__ __noinline__ void route_row_exactly(const T *__restrict__ row, const 
 
 // Shared memory of a warp, in 4-byte words: keys of ROWS rows (a pitch that keeps the rows' pieces in different banks), the largest and the second key of
 // their pieces, the groups' ranks, choices and what they weigh, and of the softmax the row's maximum and its sum's reciprocal.
-static constexpr int ROWS = 8, SLOTS = MOE_ROUTE_MAX_SELECTED + 1;
 __host__ __device__ constexpr int key_pitch(int pieces) { return (pieces + 3) / 4 * 32 + 4; }
-__host__ __device__ constexpr int piece_pitch(int held) { return held * 4 + 4; } // held: pieces of each of a row's four lanes
-__host__ __device__ constexpr int warp_words(int pieces, int held, bool second, int groups, int selected)
+__host__ __device__ constexpr int piece_pitch(int most) { return most + 4; } // most: pieces that a row may have
+__host__ __device__ constexpr int warp_words(int rows, int pieces, int most, bool second, int groups, int selected)
 {
-    return ROWS * (key_pitch(pieces) + piece_pitch(held) * (second ? 2 : 1) + (groups > 1 ? groups : 0) + 2 * (selected + 1) + 2) + 4;
+    return (rows * (key_pitch(pieces) + piece_pitch(most) * (second ? 2 : 1) + (groups > 1 ? groups : 0) + 2 * (selected + 1) + 2) + 3) / 4 * 4;
 }
 
 // eight neighbours from column e on as they lie in memory, -inf behind the last one and where there is nothing to read
@@ -223,12 +222,14 @@ __device__ __forceinline__ void load8(const T *row, int e, int E, bool vec, floa
 // over the `width` neighbouring lanes that share a row
 __device__ __forceinline__ float max_over(float v, int width)
 {
+#pragma unroll
     for (int o = width / 2; o > 0; o >>= 1)
         v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
     return v;
 }
 __device__ __forceinline__ float sum_over(float v, int width)
 {
+#pragma unroll
     for (int o = width / 2; o > 0; o >>= 1)
         v += __shfl_xor_sync(FULL, v, o);
     return v;
@@ -253,21 +254,22 @@ __device__ __forceinline__ void two_of(const float (&v)[8], float &best, float &
     best = fmaxf(a[0], a[2]), next = fmaxf(fminf(a[0], a[2]), fmaxf(b[0], b[2]));
 }
 
-// NB: pieces of 8 columns that each of the four lanes of a row has (E <= 32 NB)
-template <class T, int NB>
-__global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p, const Choice c,
+// L: lanes that share a row while choices are made; NB: pieces of 8 columns that each of them has (E <= 8 L NB)
+template <class T, int L, int NB>
+__global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) route_forward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p, const Choice c,
                                                                 const uint8_t *__restrict__ mask, int *ids, float *weights)
 {
     grid_dep_wait();
     // WIDTH: lanes that share a row while it comes in, HELD pieces each, STEP passes at a time
-    constexpr int WIDTH = NB >= 8 ? 32 : 4 * NB, HELD = NB > 8 ? NB / 8 : 1, PASSES = ROWS * WIDTH / 32, STEP = PASSES < 8 / HELD ? PASSES : 8 / HELD;
+    constexpr int ROWS = 32 / L, MOST = L * NB, WIDTH = MOST >= 32 ? 32 : MOST, HELD = MOST / WIDTH, PASSES = ROWS * WIDTH / 32, STEP = PASSES < 8 / HELD ? PASSES : 8 / HELD;
     extern __shared__ __align__(16) float route_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, pieces = (E + 7) / 8, per = E / c.groups;
-    const bool two = c.groups > 1 && c.group_top == 2;
-    constexpr int pp = piece_pitch(NB);
-    const int pitch = key_pitch(pieces), slots = p.selected + 1;
-    float *keys = route_smem + warp * warp_words(pieces, NB, two, c.groups, p.selected), *first = keys + ROWS * pitch, *second = first + ROWS * pp,
-          *ranks = second + (two ? ROWS * pp : 0), *chosen = ranks + (c.groups > 1 ? ROWS * c.groups : 0), *row_max = chosen + ROWS * slots,
+    // groups of 8, 16 .. 256 neighbours are ranked while they come in, others from what lies in shared memory
+    const bool two = c.groups > 1 && c.group_top == 2, coming = HELD == 1 && per >= 8 && (per & (per - 1)) == 0, kept_second = two && !coming;
+    constexpr int pp = piece_pitch(MOST);
+    const int pitch = key_pitch(pieces), slots = p.selected + 1, group_pieces = per >> 3, shift = coming ? 31 - __clz(group_pieces) : 0;
+    float *keys = route_smem + warp * warp_words(ROWS, pieces, MOST, kept_second, c.groups, p.selected), *first = keys + ROWS * pitch, *second = first + ROWS * pp,
+          *ranks = second + (kept_second ? ROWS * pp : 0), *chosen = ranks + (c.groups > 1 ? ROWS * c.groups : 0), *row_max = chosen + ROWS * slots,
           *row_inv = row_max + ROWS;
     int *chosen_id = (int *)(row_inv + ROWS);
     const int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * ROWS;
@@ -283,8 +285,8 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
             const int e = (at + 32 * h) * 8 + i;
             bias[h][i] = c.bias && e < E ? c.bias[e] : 0.f;
         }
-    // a piece's place among the largest keys: neighbours of a lane of the four side by side
-    const auto place = [&](int piece) { return (piece & 3) * NB + (piece >> 2); };
+    // a piece's place among the largest keys: those of a lane side by side
+    const auto place = [&](int piece) { return piece % L * NB + piece / L; };
 
     // rows come in
 #pragma unroll 1
@@ -377,81 +379,100 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
                     to[0] = make_float4(k[0], k[1], k[2], k[3]);
                     to[1] = make_float4(k[4], k[5], k[6], k[7]);
                 }
-                if (piece < 4 * NB) { // -inf where there is none
+                { // -inf where there is none
                     first[r * pp + place(piece)] = best;
-                    if (two)
+                    if (kept_second)
                         second[r * pp + place(piece)] = next;
+                }
+                if (c.groups > 1 && coming) { // over the lanes of a group
+                    for (int o = 1; o < group_pieces; o *= 2) {
+                        const float a = __shfl_xor_sync(FULL, best, o);
+                        if (two)
+                            next = fmaxf(fminf(best, a), fmaxf(next, __shfl_xor_sync(FULL, next, o)));
+                        best = fmaxf(best, a);
+                    }
+                    if (piece < pieces && (piece & (group_pieces - 1)) == 0)
+                        ranks[r * c.groups + (piece >> shift)] = two ? fmaxf(best + next, -INFINITY) : best;
                 }
             }
         }
     }
     __syncwarp();
 
-    // four lanes a row from here on
-    const int r = lane >> 2, l = lane & 3;
+    // L lanes a row from here on
+    const int r = lane / L, l = lane % L;
     const int64_t t = t0 + r;
     float *my_keys = keys + r * pitch, *my_first = first + r * pp, *my_second = second + r * pp, *my_ranks = ranks + r * c.groups, *my_chosen = chosen + r * slots;
     int *my_id = chosen_id + r * slots;
     const float unit = !by_logit && softmax ? row_inv[r] * 0x1p-18f : 0x1p-19f; // two scores are off by less together
     const auto near = [&](float a, float b, float times) { return !(a - b > times * (unit + 0x1p-22f * (fabsf(a) + fabsf(b)))); };
     bool unsure = false;
+    unsigned dropped = 0; // groups whose experts are not to be taken
     if (c.groups > 1) {
-        const bool aligned = per % 8 == 0; // a group is whole pieces
-        for (int g = l; g < c.groups; g += 4) {
-            float best = -INFINITY, next = -INFINITY;
-            const auto take = [&](float k) {
-                next = fmaxf(next, fminf(best, k));
-                best = fmaxf(best, k);
-            };
-            if (aligned) {
-                for (int i = g * (per / 8); i < (g + 1) * (per / 8); ++i) {
-                    if (two)
-                        next = fmaxf(next, my_second[place(i)]);
-                    take(my_first[place(i)]);
+        if (!coming) {
+            for (int g = l; g < c.groups; g += L) {
+                float best = -INFINITY, next = -INFINITY;
+                const auto take = [&](float k) {
+                    next = fmaxf(next, fminf(best, k));
+                    best = fmaxf(best, k);
+                };
+                if (per % 8 == 0) { // a group is whole pieces
+                    for (int i = g * group_pieces; i < (g + 1) * group_pieces; ++i) {
+                        if (two)
+                            next = fmaxf(next, my_second[place(i)]);
+                        take(my_first[place(i)]);
+                    }
+                } else {
+                    for (int e = g * per; e < (g + 1) * per; ++e)
+                        take(my_keys[e]);
                 }
-            } else {
-                for (int e = g * per; e < (g + 1) * per; ++e)
-                    take(my_keys[e]);
-            }
-            my_ranks[g] = two ? fmaxf(best + next, -INFINITY) : best;
-        }
-        __syncwarp();
-        float worst_kept = INFINITY, best_left = -INFINITY;
-        for (int g = l; g < c.groups; g += 4) {
-            const float mine = my_ranks[g];
-            int before = 0;
-            for (int h = 0; h < c.groups; ++h)
-                before += my_ranks[h] > mine || (my_ranks[h] == mine && h < g) ? 1 : 0;
-            if (before < c.kept && mine > -INFINITY) {
-                worst_kept = fminf(worst_kept, mine);
-                continue;
-            }
-            best_left = fmaxf(best_left, mine);
-            if (aligned)
-                for (int i = g * (per / 8); i < (g + 1) * (per / 8); ++i)
-                    my_first[place(i)] = -INFINITY;
-            else
-                for (int e = g * per; e < (g + 1) * per; ++e)
-                    my_keys[e] = -INFINITY;
-        }
-        worst_kept = fminf(worst_kept, __shfl_xor_sync(FULL, worst_kept, 1)), best_left = fmaxf(best_left, __shfl_xor_sync(FULL, best_left, 1));
-        worst_kept = fminf(worst_kept, __shfl_xor_sync(FULL, worst_kept, 2)), best_left = fmaxf(best_left, __shfl_xor_sync(FULL, best_left, 2));
-        unsure = !by_logit && best_left > -INFINITY && near(worst_kept, best_left, 2.f);
-        __syncwarp();
-        if (!aligned) { // what the pieces hold now
-            for (int i = l; i < pieces; i += 4) {
-                float best = -INFINITY;
-                for (int e = i * 8; e < min(E, i * 8 + 8); ++e)
-                    best = fmaxf(best, my_keys[e]);
-                my_first[place(i)] = best;
+                my_ranks[g] = two ? fmaxf(best + next, -INFINITY) : best;
             }
             __syncwarp();
         }
+        float worst_kept = INFINITY, best_left = -INFINITY;
+        for (int g = l; g < c.groups; g += L) {
+            const float mine = my_ranks[g];
+            int before = 0;
+            for (int h = 0; h < c.groups; ++h) {
+                const float other = my_ranks[h];
+                before += other > mine || (other == mine && h < g) ? 1 : 0;
+            }
+            if (before < c.kept && mine > -INFINITY) {
+                worst_kept = fminf(worst_kept, mine);
+            } else {
+                best_left = fmaxf(best_left, mine);
+                dropped |= 1u << g;
+            }
+        }
+        worst_kept = -max_over(-worst_kept, L), best_left = max_over(best_left, L);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1)
+            dropped |= __shfl_xor_sync(FULL, dropped, o);
+        unsure = !by_logit && best_left > -INFINITY && near(worst_kept, best_left, 2.f);
+        if (per % 8) { // pieces across groups: what is left of them
+            for (int i = l; i < pieces; i += L) {
+                float best = -INFINITY;
+                for (int e = i * 8; e < min(E, i * 8 + 8); ++e) {
+                    if (dropped >> (e / per) & 1)
+                        my_keys[e] = -INFINITY;
+                    best = fmaxf(best, my_keys[e]);
+                }
+                my_first[place(i)] = best;
+            }
+            dropped = 0;
+        }
+        __syncwarp();
     }
     float held[NB];
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < NB; ++i) {
         held[i] = my_first[l * NB + i];
+        if (dropped) {
+            const int piece = i * L + l, g = coming ? piece >> shift : piece / group_pieces;
+            held[i] = piece < pieces && (dropped >> g & 1) ? -INFINITY : held[i];
+        }
+    }
     const int rounds = p.selected + (by_logit ? 0 : 1); // the first key that is not chosen, for its distance
 #pragma unroll 1
     for (int j = 0; j < rounds; ++j) {
@@ -459,14 +480,15 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
 #pragma unroll
         for (int i = 1; i < NB; ++i)
             best = fmaxf(best, held[i]);
-        best = fmaxf(best, __shfl_xor_sync(FULL, best, 1));
-        best = fmaxf(best, __shfl_xor_sync(FULL, best, 2));
+        best = max_over(best, L);
         int piece = 1 << 20; // the first one with this key
 #pragma unroll
         for (int i = NB - 1; i >= 0; --i)
-            piece = held[i] == best ? i * 4 + l : piece;
-        int lowest = min(piece, __shfl_xor_sync(FULL, piece, 1));
-        lowest = min(lowest, __shfl_xor_sync(FULL, lowest, 2));
+            piece = held[i] == best ? i * L + l : piece;
+        int lowest = piece;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1)
+            lowest = min(lowest, __shfl_xor_sync(FULL, lowest, o));
         if (best == -INFINITY) {
             if (l == 0)
                 my_id[j] = -1, my_chosen[j] = -INFINITY;
@@ -484,20 +506,20 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
             my_keys[piece * 8 + i0] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
-                held[i] = i * 4 + l == piece ? rest : held[i];
+                held[i] = i * L + l == piece ? rest : held[i];
             my_id[j] = piece * 8 + i0, my_chosen[j] = best;
         }
     }
     __syncwarp();
 
-    // weights: a lane has every fourth choice
+    // weights: a lane has every L-th choice
     const bool here = t < p.T;
     const T *row = logits + t * ld;
-    constexpr int MINE = MOE_ROUTE_MAX_SELECTED / 4;
+    constexpr int MINE = MOE_ROUTE_MAX_SELECTED / L;
     float v[MINE], top = -INFINITY, total = 0.f;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-        const int j = i * 4 + l, id = here && j < p.selected ? my_id[j] : -1;
+        const int j = i * L + l, id = here && j < p.selected ? my_id[j] : -1;
         v[i] = id >= 0 ? widen(row[id]) : -INFINITY;
         top = fmaxf(top, softmax ? v[i] : fminf(v[i], 0.f));
         if (!by_logit && id >= 0) {
@@ -505,11 +527,10 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
             if (next >= 0 && near(my_chosen[j], my_chosen[j + 1], 1.f)) // equal logits and biases are equal keys, whose order is known
                 unsure |= j == p.selected - 1 || v[i] != widen(row[next]) || (c.bias && c.bias[id] != c.bias[next]);
         }
-        if (i * 4 + 4 >= p.selected)
+        if (i * L + L >= p.selected)
             break;
     }
-    top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+    top = max_over(top, L);
     const float ref = p.renormalize ? top : softmax ? row_max[r] : 0.f;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
@@ -517,102 +538,110 @@ __global__ void __launch_bounds__(THREADS) route_forward_kernel(const T *__restr
         const float w = softmax ? ex2((v[i] - ref) * 1.44269504f) : ex2((fminf(v[i], 0.f) - ref) * 1.44269504f) * rcp(1.f + ex2(fabsf(v[i]) * -1.44269504f));
         v[i] = v[i] > -INFINITY ? w : 0.f;
         total += v[i];
-        if (i * 4 + 4 >= p.selected)
+        if (i * L + L >= p.selected)
             break;
     }
-    total += __shfl_xor_sync(FULL, total, 1);
-    total += __shfl_xor_sync(FULL, total, 2);
+    total = sum_over(total, L);
     const float factor = p.scale * (p.renormalize ? (total > 0.f ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f);
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-        const int j = i * 4 + l;
+        const int j = i * L + l;
         if (here && j < p.selected) {
             ids[t * p.selected + j] = my_id[j];
             weights[t * p.selected + j] = v[i] > 0.f ? v[i] * factor : 0.f;
         }
-        if (i * 4 + 4 >= p.selected)
+        if (i * L + L >= p.selected)
             break;
     }
     unsigned again = __ballot_sync(FULL, unsure && here);
     while (again) {
-        const int i = (__ffs(again) - 1) >> 2;
-        again &= ~(15u << (4 * i));
+        const int i = (__ffs(again) - 1) / L;
+        again &= ~(((1u << L) - 1) << (L * i));
         __syncwarp();
         route_row_exactly(logits + (t0 + i) * ld, p, c, (double *)keys, ids + (t0 + i) * p.selected, weights + (t0 + i) * p.selected);
     }
 }
 
-// Gradients of a warp's 8 rows are put together in shared memory, zeros but for the choices, and leave a row at a time in pieces of 8 columns a lane; with a softmax
-// over all experts every column has its share.
-__host__ __device__ constexpr int backward_words(int pieces) { return ROWS * (key_pitch(pieces) + 3); }
-template <class T>
+// Gradients of a warp's rows are put together in shared memory, zeros but for the choices, and leave a row at a time in pieces of 8 columns a lane; with a softmax
+// over all experts (DENSE) every column has its share, of logits that stay in registers from the softmax to there.  L, NB: as above.
+__host__ __device__ constexpr int backward_words(int rows, int pieces) { return rows * (key_pitch(pieces) + 3) / 4 * 4 + 4; }
+template <class T, int L, int NB, bool DENSE>
 __global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p,
-                                                                      const uint8_t *__restrict__ mask, const int *__restrict__ ids,
-                                                                      const float *__restrict__ dweights, T *dlogits, int64_t ld_d, bool vec_d, bool add)
+                                                                 const uint8_t *__restrict__ mask, const int *__restrict__ ids,
+                                                                 const float *__restrict__ dweights, T *dlogits, int64_t ld_d, bool vec_d, bool add)
 {
     grid_dep_wait();
+    constexpr int ROWS = 32 / L, MOST = L * NB, WIDTH = MOST >= 32 ? 32 : MOST, HELD = MOST / WIDTH, PASSES = ROWS * WIDTH / 32;
     extern __shared__ __align__(16) float route_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, pieces = (E + 7) / 8, pitch = key_pitch(pieces);
-    float *grads = route_smem + warp * backward_words(pieces), *row_max = grads + ROWS * pitch, *row_inv = row_max + ROWS, *row_dot = row_inv + ROWS;
+    float *grads = route_smem + warp * backward_words(ROWS, pieces), *row_max = grads + ROWS * pitch, *row_inv = row_max + ROWS, *row_dot = row_inv + ROWS;
     const int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * ROWS;
     if (t0 >= p.T)
         return;
-    const bool softmax = p.score == TS2_SCORE_SOFTMAX, dense = softmax && !p.renormalize;
-    int width = 1; // lanes that share a row
-    while (width < pieces && width < 32)
-        width *= 2;
-    const int passes = max(1, ROWS * width / 32), at = lane & (width - 1), sub = lane / width;
+    const bool softmax = p.score == TS2_SCORE_SOFTMAX;
+    const int at = lane & (WIDTH - 1), sub = lane / WIDTH;
 
-    if (dense)
-#pragma unroll 1
-        for (int pass = 0; pass < passes; ++pass) {
-            const int r = pass * (32 / width) + sub;
-            const bool on = r < ROWS && t0 + r < p.T && (!mask || mask[t0 + r]);
-            float top = -INFINITY, sum = 0.f;
-            for (int i = at; i < pieces && on; i += width) {
-                float v[8];
-                load8(logits + (t0 + r) * ld, i * 8, E, vec, v);
-                // of what has come so far
-                const float now = fmaxf(top, max8(v)), ref = now == -INFINITY ? 0.f : now;
-                sum *= ex2((top - ref) * 1.44269504f);
+    Eight<T> raw[DENSE ? PASSES : 1][DENSE ? HELD : 1];
+    if constexpr (DENSE) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    sum += ex2((v[k] - ref) * 1.44269504f);
-                top = now;
-            }
-            const float all = max_over(top, width), ref = all == -INFINITY ? 0.f : all;
-            sum = sum_over(sum * ex2((top - ref) * 1.44269504f), width);
-            if (r < ROWS && at == 0)
-                row_max[r] = ref, row_inv[r] = 1.f / sum;
+        for (int s = 0; s < PASSES; ++s) {
+            const int64_t t = t0 + s * (32 / WIDTH) + sub;
+            const bool on = t < p.T && (!mask || mask[t]);
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+                raw[s][h].load(logits + t * ld, (at + 32 * h) * 8, E, vec, on && at + 32 * h < pieces);
         }
+    }
     for (int i = lane; i < ROWS * pitch / 4; i += 32)
         ((float4 *)grads)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (DENSE) {
+#pragma unroll
+        for (int s = 0; s < PASSES; ++s) {
+            float v[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                raw[s][h].widen_to(v);
+                top = fmaxf(top, max8(v));
+            }
+            top = max_over(top, WIDTH);
+            top = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                raw[s][h].widen_to(v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sum += ex2((v[i] - top) * 1.44269504f);
+            }
+            sum = sum_over(sum, WIDTH);
+            const int r = s * (32 / WIDTH) + sub;
+            if (at == 0)
+                row_max[r] = top, row_inv[r] = 1.f / sum;
+        }
+    }
     __syncwarp();
 
-    { // the gradients of the choices' logits over scale; four lanes a row, every fourth choice each
-        const int r = lane >> 2, l = lane & 3;
+    { // the gradients of the choices' logits over scale; L lanes a row, every L-th choice each
+        const int r = lane / L, l = lane % L;
         const int64_t t = t0 + r;
         const bool here = t < p.T && (!mask || mask[t]);
         const T *row = logits + t * ld;
-        constexpr int MINE = MOE_ROUTE_MAX_SELECTED / 4;
+        constexpr int MINE = MOE_ROUTE_MAX_SELECTED / L;
         int id[MINE];
         float v[MINE], d[MINE], top = -INFINITY, total = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-            const int j = i * 4 + l;
+            const int j = i * L + l;
             id[i] = here && j < p.selected ? ids[t * p.selected + j] : -1;
             if (id[i] >= E)
                 id[i] = -1;
             v[i] = 0.f, d[i] = 0.f;
             if (id[i] >= 0)
                 v[i] = widen(row[id[i]]), d[i] = dweights[t * p.selected + j], top = fmaxf(top, softmax ? v[i] : fminf(v[i], 0.f));
-            if (i * 4 + 4 >= p.selected)
+            if (i * L + L >= p.selected)
                 break;
         }
-        if (p.renormalize) {
-            top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
-        }
+        if (p.renormalize)
+            top = max_over(top, L);
         const float ref = p.renormalize ? top : softmax ? row_max[r] : 0.f;
         float w[MINE];
 #pragma unroll
@@ -620,11 +649,10 @@ __global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__rest
             w[i] = softmax ? ex2((v[i] - ref) * 1.44269504f) : ex2((fminf(v[i], 0.f) - ref) * 1.44269504f) * rcp(1.f + ex2(fabsf(v[i]) * -1.44269504f));
             w[i] = id[i] >= 0 ? w[i] : 0.f;
             total += w[i], dot = fmaf(w[i], d[i], dot);
-            if (i * 4 + 4 >= p.selected)
+            if (i * L + L >= p.selected)
                 break;
         }
-        total += __shfl_xor_sync(FULL, total, 1), dot += __shfl_xor_sync(FULL, dot, 1);
-        total += __shfl_xor_sync(FULL, total, 2), dot += __shfl_xor_sync(FULL, dot, 2);
+        total = sum_over(total, L), dot = sum_over(dot, L);
         const bool any = total > 0.f; // a choice was made (or weighs nothing)
         const float factor = p.renormalize ? (any ? 1.f / total : 0.f) : softmax ? row_inv[r] : 1.f;
         dot = any ? dot * factor : 0.f;
@@ -635,32 +663,36 @@ __global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__rest
             // 1 - sigmoid(v) = sigmoid(-v), without cancellation
             const float rest = softmax ? 1.f : ex2(fmaxf(v[i], 0.f) * -1.44269504f) * rcp(1.f + ex2(fabsf(v[i]) * -1.44269504f));
             const float g = w[i] * factor * (p.renormalize ? d[i] - dot : d[i]) * rest;
-            // one of the four after the other: a caller's ids may name an expert twice
+            // one lane after the other: a caller's ids may name an expert twice
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < L; ++k) {
                 if (l == k && id[i] >= 0)
                     grads[r * pitch + id[i]] += g;
                 __syncwarp();
             }
-            if (i * 4 + 4 >= p.selected)
+            if (i * L + L >= p.selected)
                 break;
         }
     }
     __syncwarp();
 
-#pragma unroll 1
-    for (int pass = 0; pass < passes; ++pass) {
-        const int r = pass * (32 / width) + sub;
+#pragma unroll
+    for (int s = 0; s < PASSES; ++s) {
+        const int r = s * (32 / WIDTH) + sub;
         const int64_t t = t0 + r;
-        if (r >= ROWS || t >= p.T)
+        if (t >= p.T)
             continue;
-        const float dot = dense ? row_dot[r] : 0.f, ref = dense ? row_max[r] : 0.f, share = dense && dot != 0.f ? dot * row_inv[r] : 0.f;
-        for (int i = at; i < pieces; i += width) {
+        const float ref = DENSE ? row_max[r] : 0.f, share = DENSE && row_dot[r] != 0.f ? row_dot[r] * row_inv[r] : 0.f;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const int i = at + 32 * h;
+            if (i >= pieces)
+                continue;
             const float4 a = *(const float4 *)(grads + r * pitch + i * 8), b = *(const float4 *)(grads + r * pitch + i * 8 + 4);
             float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (share != 0.f) {
+            if (DENSE && share != 0.f) {
                 float x[8];
-                load8(logits + t * ld, i * 8, E, vec, x);
+                raw[DENSE ? s : 0][DENSE ? h : 0].widen_to(x);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     v[k] = fmaf(-share, ex2((x[k] - ref) * 1.44269504f), v[k]);
@@ -669,59 +701,68 @@ __global__ void __launch_bounds__(THREADS) route_backward_kernel(const T *__rest
             const bool whole = vec_d && i * 8 + 8 <= E;
             constexpr int PER = 16 / sizeof(T);
 #pragma unroll
-            for (int h = 0; h < 8 / PER; ++h) {
+            for (int j = 0; j < 8 / PER; ++j) {
                 Piece<T, PER> q;
                 if (add) {
                     if (whole)
-                        q = *(const Piece<T, PER> *)(to + h * PER);
+                        q = *(const Piece<T, PER> *)(to + j * PER);
                     else
 #pragma unroll
                         for (int k = 0; k < PER; ++k)
-                            if (i * 8 + h * PER + k < E)
-                                q.v[k] = to[h * PER + k];
+                            if (i * 8 + j * PER + k < E)
+                                q.v[k] = to[j * PER + k];
                 }
 #pragma unroll
                 for (int k = 0; k < PER; ++k)
-                    q.v[k] = narrow<T>(add ? fmaf(p.scale, v[h * PER + k], widen(q.v[k])) : p.scale * v[h * PER + k]);
+                    q.v[k] = narrow<T>(add ? fmaf(p.scale, v[j * PER + k], widen(q.v[k])) : p.scale * v[j * PER + k]);
                 if (whole)
-                    *(Piece<T, PER> *)(to + h * PER) = q;
+                    *(Piece<T, PER> *)(to + j * PER) = q;
                 else
 #pragma unroll
                     for (int k = 0; k < PER; ++k)
-                        if (i * 8 + h * PER + k < E)
-                            to[h * PER + k] = q.v[k];
+                        if (i * 8 + j * PER + k < E)
+                            to[j * PER + k] = q.v[k];
             }
         }
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-template <class T, int NB>
+template <class T, int L, int NB>
 static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const Choice &choice, const uint8_t *mask, int *ids, float *weights)
 {
     const int warps = THREADS / 32;
-    constexpr int most = warps * warp_words(4 * NB, NB, true, MOE_ROUTE_MAX_GROUPS, MOE_ROUTE_MAX_SELECTED) * 4;
+    constexpr int most = warps * warp_words(32 / L, L * NB, L * NB, true, MOE_ROUTE_MAX_GROUPS, MOE_ROUTE_MAX_SELECTED) * 4;
     static_assert(most <= 232448, "shared memory budget");
     static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
     const unsigned bit = 1u << (c.device & 15);
     if (!(ready.load() & bit)) {
-        TS2_CUDA(cudaFuncSetAttribute((const void *)route_forward_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        TS2_CUDA(cudaFuncSetAttribute((const void *)route_forward_kernel<T, L, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         ready.fetch_or(bit);
     }
     const bool vec = (uintptr_t)logits % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    const size_t smem = (size_t)warps * warp_words((s.E + 7) / 8, NB, choice.groups > 1 && choice.group_top == 2, choice.groups, s.selected) * 4;
-    TS2_LAUNCH((route_forward_kernel<T, NB>), (unsigned)ceil_div(s.T, warps * ROWS), THREADS, smem, c.stream, (const T *)logits, ld, vec, s, choice, mask, ids,
+    const int per = s.E / choice.groups;
+    const bool coming = L * NB <= 32 && per >= 8 && (per & (per - 1)) == 0; // as in the kernel
+    const size_t smem = (size_t)warps * warp_words(32 / L, (s.E + 7) / 8, L * NB, choice.groups > 1 && choice.group_top == 2 && !coming, choice.groups, s.selected) * 4;
+    TS2_LAUNCH((route_forward_kernel<T, L, NB>), (unsigned)ceil_div(s.T, warps * (32 / L)), THREADS, smem, c.stream, (const T *)logits, ld, vec, s, choice, mask, ids,
                weights);
     return TS2_OK;
 }
 template <class T>
 static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const Choice &choice, const uint8_t *mask, int *ids, float *weights)
 {
-    const auto f = s.E <= 32 ? forward<T, 1> : s.E <= 64 ? forward<T, 2> : s.E <= 128 ? forward<T, 4> : s.E <= 256 ? forward<T, 8> : s.E <= 512 ? forward<T, 16>
-                                                                                                                                     : forward<T, 32>;
+    // 4 lanes a row take fewer instructions, 8 two times the warps.  Up to 128 experts 4 are faster (65537 x 128 19.2 against 24.1 us), beyond 8 (32768 x 256
+    // in groups 38.1 against 39.9); for the gradient, whose row has little to do, 8 are from 33 experts on (65537 x 128 22.8 against 27.4, 32768 x 256 8.9
+    // against 10.4).
+    const auto f = s.E <= 32    ? forward<T, 4, 1>
+                   : s.E <= 64  ? forward<T, 4, 2>
+                   : s.E <= 128 ? forward<T, 4, 4>
+                   : s.E <= 256 ? forward<T, 8, 4>
+                   : s.E <= 512 ? forward<T, 8, 8>
+                                : forward<T, 8, 16>;
     return f(c, s, logits, ld, choice, mask, ids, weights);
 }
-template <class T>
+template <class T, int L, int NB, bool DENSE>
 static int backward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const uint8_t *mask, const int *ids, const float *dweights,
                     void *dlogits, int64_t ld_d, bool add)
 {
@@ -729,14 +770,33 @@ static int backward(const Ctx &c, const RouteShape &s, const void *logits, int64
     static std::atomic<unsigned> ready{0}; // as above
     const unsigned bit = 1u << (c.device & 15);
     if (!(ready.load() & bit)) {
-        TS2_CUDA(cudaFuncSetAttribute((const void *)route_backward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      warps * backward_words(MOE_ROUTE_MAX_EXPERTS / 8) * 4));
+        TS2_CUDA(cudaFuncSetAttribute((const void *)route_backward_kernel<T, L, NB, DENSE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      warps * backward_words(32 / L, L * NB) * 4));
         ready.fetch_or(bit);
     }
     const auto aligned = [](const void *p, int64_t pitch) { return (uintptr_t)p % 16 == 0 && pitch * sizeof(T) % 16 == 0; };
-    TS2_LAUNCH((route_backward_kernel<T>), (unsigned)ceil_div(s.T, warps * ROWS), THREADS, (size_t)warps * backward_words((s.E + 7) / 8) * 4, c.stream,
+    TS2_LAUNCH((route_backward_kernel<T, L, NB, DENSE>), (unsigned)ceil_div(s.T, warps * (32 / L)), THREADS, (size_t)warps * backward_words(32 / L, (s.E + 7) / 8) * 4, c.stream,
                (const T *)logits, ld, aligned(logits, ld), s, mask, ids, dweights, (T *)dlogits, ld_d, aligned(dlogits, ld_d), add);
     return TS2_OK;
+}
+template <class T, bool DENSE>
+static int backward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const uint8_t *mask, const int *ids, const float *dweights,
+                    void *dlogits, int64_t ld_d, bool add)
+{
+    const auto f = s.E <= 32    ? backward<T, 4, 1, DENSE>
+                   : s.E <= 64  ? backward<T, 8, 1, DENSE>
+                   : s.E <= 128 ? backward<T, 8, 2, DENSE>
+                   : s.E <= 256 ? backward<T, 8, 4, DENSE>
+                   : s.E <= 512 ? backward<T, 8, 8, DENSE>
+                                : backward<T, 8, 16, DENSE>;
+    return f(c, s, logits, ld, mask, ids, dweights, dlogits, ld_d, add);
+}
+template <class T>
+static int backward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const uint8_t *mask, const int *ids, const float *dweights,
+                    void *dlogits, int64_t ld_d, bool add)
+{
+    return s.score == TS2_SCORE_SOFTMAX && !s.renormalize ? backward<T, true>(c, s, logits, ld, mask, ids, dweights, dlogits, ld_d, add)
+                                                          : backward<T, false>(c, s, logits, ld, mask, ids, dweights, dlogits, ld_d, add);
 }
 
 int moe_route_forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const float *bias, int groups, int groups_kept, int group_top,

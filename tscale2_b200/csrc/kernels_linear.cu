@@ -5,7 +5,8 @@
 // dw).  fp16 or bf16 operands, fp32 sums in tensor memory, two accumulators so that a tile's epilogue runs beside the next tile's products.  The
 // epilogue adds the bias, takes the activation and adds the residual in fp32, rounds once, and sends blocks of 32 rows x 128 bytes by TMA.
 // Large products are bound by the tensor pipe (under the part's power limit), small ones by the latency of a launch and the first loads.  Outputs of few tiles are
-// divided along K: partial tiles in fp32, added in their order by a second launch that runs the epilogue.
+// divided along K: partial tiles in fp32, added in their order by a second launch that runs the epilogue.  dw and dx are one launch: the units that take longer are
+// dealt out first, and the others even out what those leave.
 // Rows that TMA cannot address (a base or a pitch that is no multiple of 16 bytes) are copied to a pitch that it can.
 #include "elem_types.cuh"
 #include "kernels.cuh"
@@ -28,6 +29,7 @@ struct LinearArgs {
     int m, n; // rows and columns of the output
     int m_tiles, n_tiles, units, k_blocks, splits, kb_per_split;
     int kind, act;
+    bool a_mn; // the first operand is contiguous along the output's rows
     const float *bias;
     const void *res;
     int64_t res_ld;
@@ -36,8 +38,34 @@ struct LinearArgs {
     bool y_tma, z_tma, res_vec, bias_vec; // what 16-byte accesses can reach
     bool ends_whole;                      // a row of y and z is a multiple of 16 bytes
     float *part;
+};
+// The units of up to two products dealt out to pairs: those of the first one after the other to all pairs in turn.  Where they do not come out even, pairs that got
+// one less take `extra` units of the second each, about as long as one of the first; the rest goes to all pairs in turn.
+struct Deal {
+    int units[2], uneven, extra, early; // uneven: pairs with one more of the first; early: units of the second for those with one less
+    // sums of columns that the epilogue's warps add up before their first tile is there: [blocks][n] -> out
+    const float *sums;
+    float *sums_out;
+    int sums_n, sums_blocks;
     int32_t *status;
 };
+// the i-th unit of a pair: false behind the last one
+__device__ __forceinline__ bool unit_at(const Deal &d, int pair, int pairs, int i, int &which, int &unit)
+{
+    which = 0, unit = pair + i * pairs;
+    if (unit < d.units[0])
+        return true;
+    which = 1;
+    int j = i - (d.units[0] - pair + pairs - 1) / pairs;
+    if (pair >= d.uneven && d.extra) {
+        unit = pair - d.uneven + j * (pairs - d.uneven);
+        if (j < d.extra)
+            return unit < d.early;
+        j -= d.extra;
+    }
+    unit = d.early + pair + j * pairs;
+    return unit < d.units[1];
+}
 struct Unit {
     int row, col, kb0, kb1;
 };
@@ -156,13 +184,18 @@ __device__ __forceinline__ void tma_add_2d(const void *tmap, uint32_t src, int c
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------
-// A_MN, B_MN: that operand is contiguous along the output's rows (columns) instead of along K.  tmA, tmB: boxes of 64 along K x 128 (B of PN = 128: 64)
-// rows, or of 64 rows or columns x 64 along K; tmY, tmZ: blocks of 32 rows x 128 bytes; all 128-byte swizzle
-template <bool A_MN, bool B_MN, int PN, bool BF16>
+// BACK: up to two products, the second operand contiguous along the output's columns instead of along K, the first along its rows where its a_mn says so; else
+// one, both operands contiguous along K.  A, B: boxes of 64 along K x 128 (B of PN = 128: 64) rows, or of 64 rows or columns x 64 along K; Y, Z: blocks of 32
+// rows x 128 bytes; all 128-byte swizzle
+struct LinearMaps {
+    CUtensorMap A[2], B[2], Y[2], Z;
+};
+template <bool BACK, int PN, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    linear_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
-                          const __grid_constant__ CUtensorMap tmZ, const LinearArgs p)
+    linear_product_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearArgs arg0, const __grid_constant__ LinearArgs arg1,
+                          const __grid_constant__ Deal deal)
 {
+    constexpr bool B_MN = BACK;
     constexpr int PART = PN / 2, STAGE = HALF + PART * BK * 2;
     extern __shared__ uint8_t linear_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)linear_smem + 1023) & ~(uintptr_t)1023); // the same offset in both CTAs
@@ -185,8 +218,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
-        prefetch_tmap(&tmA);
-        prefetch_tmap(&tmB);
+        prefetch_tmap(&maps.A[0]);
+        prefetch_tmap(&maps.B[0]);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
@@ -198,7 +231,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_fence_after();
     grid_dep_wait();
     const uint32_t tmem_base = *tmem_slot;
-    const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+    const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+    int which = 0, u = 0; // the unit at work
+    const auto args = [&]() -> const LinearArgs & { return BACK && which ? arg1 : arg0; };
 
     if (warp == 0) {
         // TMA producer of the CTA's halves; all copies of a stage complete on the leader's barrier
@@ -206,8 +241,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             int stage = 0, issued = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int u = first; u < p.units && ok; u += step) {
-                const Unit un = unit_of<PN>(p, u);
+            for (int i = 0; ok && unit_at(deal, pair, pairs, i, which, u); ++i) {
+                const Unit un = unit_of<PN>(args(), u);
+                const bool a_mn = BACK && args().a_mn;
+                const CUtensorMap *tmA = &maps.A[BACK ? which : 0], *tmB = &maps.B[BACK ? which : 0];
                 const int am = un.row + (int)rank * 128, bn = un.col + (int)rank * PART;
                 for (int kb = un.kb0; kb < un.kb1; ++kb) {
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
@@ -218,18 +255,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (rank == 0)
                         mbar_arrive_expect_tx(full0 + 8 * stage, 2 * STAGE);
                     const uint32_t sa = smem_u32(smem + stage * STAGE), sb = sa + HALF;
-                    if constexpr (A_MN) {
-                        tma_load_2d_pair(sa, &tmA, fb, am, kb * BK);
-                        tma_load_2d_pair(sa + BK * 128, &tmA, fb, am + 64, kb * BK);
+                    if (a_mn) {
+                        tma_load_2d_pair(sa, tmA, fb, am, kb * BK);
+                        tma_load_2d_pair(sa + BK * 128, tmA, fb, am + 64, kb * BK);
                     } else {
-                        tma_load_2d_pair(sa, &tmA, fb, kb * BK, am);
+                        tma_load_2d_pair(sa, tmA, fb, kb * BK, am);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
                         for (int j = 0; j < PART / 64; ++j)
-                            tma_load_2d_pair(sb + j * BK * 128, &tmB, fb, bn + 64 * j, kb * BK);
+                            tma_load_2d_pair(sb + j * BK * 128, tmB, fb, bn + 64 * j, kb * BK);
                     } else {
-                        tma_load_2d_pair(sb, &tmB, fb, kb * BK, bn);
+                        tma_load_2d_pair(sb, tmB, fb, kb * BK, bn);
                     }
                     ++issued;
                     if (++stage == STAGES) {
@@ -255,13 +292,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     } else if (warp == 1) {
         // MMA issuer (leader)
         if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                                       ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
+            constexpr uint32_t idesc0 = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(PN >> 3) << 17) |
+                                        ((uint32_t)(PM >> 4) << 24);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
-            for (int u = first; u < p.units && ok; u += step) {
-                const Unit un = unit_of<PN>(p, u);
+            for (int i = 0; ok && unit_at(deal, pair, pairs, i, which, u); ++i) {
+                const Unit un = unit_of<PN>(args(), u);
+                const bool a_mn = BACK && args().a_mn;
+                const uint32_t idesc = idesc0 | (a_mn ? 1u << 15 : 0u), a_step = a_mn ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
                 if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag))
                     break;
                 tc_fence_after();
@@ -273,11 +312,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     }
                     tc_fence_after();
                     const uint32_t a = smem_u32(smem + stage * STAGE), b = a + HALF;
-                    const uint64_t adesc = umma_smem_desc(a, A_MN ? BK * 128 : 16, 1024), bdesc = umma_smem_desc(b, B_MN ? BK * 128 : 16, 1024);
-                    constexpr uint64_t a_step = A_MN ? (16 * 128) >> 4 : 2, b_step = B_MN ? (16 * 128) >> 4 : 2; // 16 of K, in 16-byte units
+                    const uint64_t adesc = umma_smem_desc(a, a_mn ? BK * 128 : 16, 1024), bdesc = umma_smem_desc(b, B_MN ? BK * 128 : 16, 1024);
+                    constexpr uint32_t b_step = B_MN ? (16 * 128) >> 4 : 2;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        umma_pair<1>(tmem_d, adesc + k * a_step, bdesc + k * b_step, idesc, kb > un.kb0 || k > 0 ? 1u : 0u);
+                        umma_pair<1>(tmem_d, adesc + (uint64_t)(k * a_step), bdesc + (uint64_t)(k * b_step), idesc, kb > un.kb0 || k > 0 ? 1u : 0u);
                     commit_both(empty0 + 8 * stage);
                     if (++stage == STAGES) {
                         stage = 0;
@@ -315,8 +354,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             return b;
         };
         const auto piece = [&](uint8_t *block, int row, int q) { return (uint4 *)(block + row * 128 + ((q ^ (row & 7)) << 4)); };
-        const bool halves = p.kind == TS2_OUT_F16 || p.kind == TS2_OUT_BF16;
-        for (int u = first; u < p.units; u += step) {
+        if (BACK && deal.sums_out) // no tile is there for a while
+            for (int at = ((int)blockIdx.x * EPI_WARPS + ew) * 32 + lane; at < deal.sums_n; at += (int)gridDim.x * EPI_WARPS * 32) {
+                float sum = 0.f;
+#pragma unroll 4
+                for (int i = 0; i < deal.sums_blocks; ++i)
+                    sum += deal.sums[(int64_t)i * deal.sums_n + at];
+                deal.sums_out[at] = sum;
+            }
+        for (int i = 0; unit_at(deal, pair, pairs, i, which, u); ++i) {
+            const LinearArgs &p = args();
+            const CUtensorMap *tmY = &maps.Y[BACK ? which : 0];
+            const bool halves = p.kind == TS2_OUT_F16 || p.kind == TS2_OUT_BF16;
             const Unit un = unit_of<PN>(p, u);
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PN + part * PART;
             const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
@@ -431,17 +480,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (y_tma && lane == 0 && left < p.n) {
                     if (p.kind == KIND_PARTIAL)
-                        tma_store_2d(&tmY, smem_u32(yb), left - un.col, u * PM + row0 - un.row);
+                        tma_store_2d(tmY, smem_u32(yb), left - un.col, u * PM + row0 - un.row);
                     else if (p.kind == TS2_OUT_F32_ADD)
-                        tma_add_2d(&tmY, smem_u32(yb), left, row0);
+                        tma_add_2d(tmY, smem_u32(yb), left, row0);
                     else
-                        tma_store_2d(&tmY, smem_u32(yb), left, row0);
+                        tma_store_2d(tmY, smem_u32(yb), left, row0);
                 }
                 if (lane == 0)
                     bulk_commit(); // a group for every block taken, with or without a store
                 if (halves && p.z) {
                     if (z_tma && lane == 0 && left < p.n)
-                        tma_store_2d(&tmZ, smem_u32(zb), left, row0);
+                        tma_store_2d(&maps.Z, smem_u32(zb), left, row0);
                     if (lane == 0)
                         bulk_commit();
                 }
@@ -484,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     if (threadIdx.x == 0 && *abort_flag)
-        atomicOr(p.status, TS2_STATUS_WAIT_TIMEOUT);
+        atomicOr(deal.status, TS2_STATUS_WAIT_TIMEOUT);
 }
 
 // The K ranges of a product added in their order, and its epilogue: 4 columns a thread
@@ -657,60 +706,92 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 4 : 1) linear_few_ke
         cluster_sync(); // nobody reads this CTA's sums any more
 }
 
-// ---- dz and its column sums ------------------------------------------------------------------------------------------------
-// A block takes 128 columns and rows b, b + blocks, ... of 16: dz = dy act'(z) rounded to 16 bits (dz null: not wanted), and the sums of the unrounded
-// dz over its rows (sums null: not wanted).  Bound by reading dy and z.
-template <int ACT, bool BF16>
+// ---- dz and its column sums; rows at another pitch --------------------------------------------------------------------------
+// rows of 16-bit elements to a pitch that TMA can address
+struct PitchJob {
+    const uint16_t *from;
+    uint16_t *to;
+    int64_t from_ld, to_ld, rows;
+    int cols;
+};
+struct PitchJobs {
+    PitchJob job[2];
+    int n;
+};
+// A block of the first `layers` takes 128 columns and rows b, b + layers, ... of 16: dz = dy act'(z) rounded to 16 bits (dz null: not wanted), and the sums of
+// the unrounded dz over its rows (sums null: not wanted).  Bound by reading dy and z.  Where 16-byte accesses are not possible (VEC false) a lane has columns
+// that are 16 apart, so that neighbouring lanes read neighbours.  The layers behind copy rows.
+template <int ACT, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restrict__ dy, int64_t dy_ld, const uint16_t *__restrict__ z, int64_t z_ld,
-                                                        int64_t T, int n, bool vec, uint16_t *dz, int64_t dz_ld, float *sums)
+                                                        int64_t T, int n, int layers, uint16_t *dz, int64_t dz_ld, float *sums, const PitchJobs jobs)
 {
     grid_dep_wait();
+    if ((int)blockIdx.y >= layers) {
+        const int64_t worker = ((int64_t)(blockIdx.y - layers) * gridDim.x + blockIdx.x) * 8 + (threadIdx.x >> 5), workers = (int64_t)(gridDim.y - layers) * gridDim.x * 8;
+        for (int i = 0; i < jobs.n; ++i) {
+            const PitchJob &j = jobs.job[i];
+            for (int64_t r = worker; r < j.rows; r += workers)
+#pragma unroll 8
+                for (int c = threadIdx.x & 31; c < j.cols; c += 32)
+                    j.to[r * j.to_ld + c] = j.from[r * j.from_ld + c];
+        }
+        return;
+    }
     __shared__ float part[16][132];
-    const int c8 = (threadIdx.x & 15) * 8, col = blockIdx.x * 128 + c8, line = threadIdx.x >> 4;
+    const int sub = threadIdx.x & 15, line = threadIdx.x >> 4, col0 = blockIdx.x * 128;
+    const auto column = [&](int k) { return col0 + (VEC ? sub * 8 + k : sub + 16 * k); };
     float acc[8] = {};
-    const auto read = [&](const uint16_t *row, uint4 &raw) {
-        if (vec && col + 8 <= n) {
-            raw = *(const uint4 *)(row + col);
-        } else {
-            uint32_t w[4] = {};
+    const auto read = [&](const uint16_t *row, uint16_t (&v)[8]) {
+        if (VEC && column(0) + 8 <= n) {
+            const Piece<uint16_t, 8> q = *(const Piece<uint16_t, 8> *)(row + column(0));
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                w[k >> 1] |= col + k < n ? (uint32_t)row[col + k] << (16 * (k & 1)) : 0u;
-            raw = make_uint4(w[0], w[1], w[2], w[3]);
+                v[k] = q.v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = column(k) < n ? row[column(k)] : (uint16_t)0;
         }
     };
 #pragma unroll 2
-    for (int64_t t = (int64_t)blockIdx.y * 16 + line; t < T; t += (int64_t)gridDim.y * 16) {
-        uint4 a, b = make_uint4(0, 0, 0, 0);
+    for (int64_t t = (int64_t)blockIdx.y * 16 + line; t < T; t += (int64_t)layers * 16) {
+        uint16_t a[8], b[8];
         read(dy + t * dy_ld, a);
         if (ACT != TS2_ACT_NONE)
             read(z + t * z_ld, b);
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-        uint32_t o[4];
+        float d[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float2 d = unpack2<BF16>(aw[k]);
-            const float2 s = unpack2<BF16>(bw[k]);
+        for (int k = 0; k < 8; ++k) {
+            d[k] = widen16<BF16>(a[k]);
             if (ACT != TS2_ACT_NONE)
-                d.x *= activation_slope<ACT>(s.x), d.y *= activation_slope<ACT>(s.y);
-            acc[2 * k] += d.x, acc[2 * k + 1] += d.y;
-            o[k] = pack2<BF16>(d.x, d.y);
+                d[k] *= activation_slope<ACT>(widen16<BF16>(b[k]));
+            acc[k] += d[k];
         }
-        if (dz && col < n)
-            *(uint4 *)(dz + t * dz_ld + col) = make_uint4(o[0], o[1], o[2], o[3]); // the pitch is a multiple of 8
+        if (!dz)
+            continue;
+        uint16_t *to = dz + t * dz_ld;
+        if (VEC) {
+            if (column(0) < n) // the pitch is a multiple of 8
+                *(uint4 *)(to + column(0)) = make_uint4(pack2<BF16>(d[0], d[1]), pack2<BF16>(d[2], d[3]), pack2<BF16>(d[4], d[5]), pack2<BF16>(d[6], d[7]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (column(k) < n)
+                    to[column(k)] = (uint16_t)pack2<BF16>(d[k], 0.f);
+        }
     }
     if (!sums)
         return;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-        part[line][c8 + k] = acc[k];
+        part[line][column(k) - col0] = acc[k];
     __syncthreads();
-    if (threadIdx.x < 128 && blockIdx.x * 128 + threadIdx.x < n) {
+    if (threadIdx.x < 128 && col0 + (int)threadIdx.x < n) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             s += part[i][threadIdx.x];
-        sums[(int64_t)blockIdx.y * n + blockIdx.x * 128 + threadIdx.x] = s;
+        sums[(int64_t)blockIdx.y * n + col0 + threadIdx.x] = s;
     }
 }
 __global__ void __launch_bounds__(128) linear_sum_kernel(const float *__restrict__ sums, int n, int blocks, float *out)
@@ -720,17 +801,10 @@ __global__ void __launch_bounds__(128) linear_sum_kernel(const float *__restrict
     if (col >= n)
         return;
     float s = 0.f;
+#pragma unroll 4
     for (int b = 0; b < blocks; ++b)
         s += sums[(int64_t)b * n + col];
     out[col] = s;
-}
-// rows of 16-bit elements to a pitch that TMA can address
-__global__ void __launch_bounds__(256) linear_pitch_kernel(const uint16_t *__restrict__ from, int64_t from_ld, uint16_t *to, int64_t to_ld, int64_t rows, int cols)
-{
-    grid_dep_wait();
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8)
-        for (int c = threadIdx.x & 31; c < cols; c += 32)
-            to[r * to_ld + c] = from[r * from_ld + c];
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -757,97 +831,137 @@ int linear_map(CUtensorMap *tm, const void *base, int size, int64_t cols, int64_
 }
 bool tma_ok(const void *base, int64_t ld, int size) { return (uintptr_t)base % 16 == 0 && ld * size % 16 == 0; }
 
-// an operand: rows of 16-bit elements, where they lie or copied to a pitch that TMA can address
+// an operand: rows of 16-bit elements, where they lie or as a job copies them to a pitch that TMA can address
 struct Operand {
-    const void *p;
-    int64_t rows, ld;
-    int cols;
+    const void *p = nullptr;
+    int64_t rows = 0, ld = 0;
+    int cols = 0;
     Scratch copy;
     int rc = TS2_OK;
-    Operand(const Ctx &c, const void *from, int64_t from_ld, int64_t rows_, int cols_)
-        : p(from), rows(rows_), ld(from_ld), cols(cols_), copy(c, tma_ok(from, from_ld, 2) ? 0 : (size_t)rows_ * ceil_div(cols_, 8) * 16)
+    Operand(const Ctx &c, const void *from, int64_t from_ld, int64_t rows_, int cols_, PitchJobs &jobs)
+        : p(from), rows(rows_), ld(from_ld), cols(cols_), copy(c, !from || tma_ok(from, from_ld, 2) ? 0 : (size_t)rows_ * ceil_div(cols_, 8) * 16), rc(copy.rc)
     {
-        if (tma_ok(from, from_ld, 2))
+        if (!copy.p)
             return;
-        rc = copy.rc;
-        if (rc == TS2_OK) {
-            p = copy.p, ld = ceil_div(cols, 8) * 8;
-            rc = [&] {
-                TS2_LAUNCH(linear_pitch_kernel, (int)std::min<int64_t>(ceil_div(rows, 8), 8 * sm_count(c.device)), 256, 0, c.stream,
-                           (const uint16_t *)from, from_ld, (uint16_t *)copy.p, ld, rows, cols);
-                return (int)TS2_OK;
-            }();
-        }
+        p = copy.p, ld = ceil_div(cols, 8) * 8;
+        jobs.job[jobs.n++] = {(const uint16_t *)from, (uint16_t *)copy.p, from_ld, ld, rows, cols};
     }
 };
-
-// K ranges of a product, see below
-int choose_splits(int pairs, int64_t tiles, int k_blocks)
+template <int ACT, bool BF16>
+int prepare(const Ctx &c, const void *dy, int64_t dy_ld, const void *z, int64_t z_ld, int64_t T, int n, int layers, void *dz, int64_t dz_ld, float *sums,
+            const PitchJobs &jobs)
 {
-    double best = (double)ceil_div(tiles, pairs) * (k_blocks + 4);
-    int splits = 1;
-    for (int s = 2; s <= 64 && s <= k_blocks; ++s) {
-        const int per = (int)ceil_div(k_blocks, s), used = (int)ceil_div(k_blocks, per);
-        const double cost = (double)ceil_div(tiles * s, pairs) * (per + 4) + 10 + 0.1 * tiles * s;
-        if (used == s && cost < best)
-            best = cost, splits = s;
-    }
-    return splits;
+    const bool vec = tma_ok(dy, dy_ld, 2) && (ACT == TS2_ACT_NONE || tma_ok(z, z_ld, 2));
+    const int strips = layers ? (int)ceil_div(n, 128) : 4 * sm_count(c.device);
+    const dim3 grid(strips, layers + (jobs.n ? (int)ceil_div(4 * sm_count(c.device), strips) : 0));
+    if (vec)
+        TS2_LAUNCH((linear_dz_kernel<ACT, BF16, true>), grid, 256, 0, c.stream, (const uint16_t *)dy, dy_ld, (const uint16_t *)z, z_ld, T, n, layers,
+                   (uint16_t *)dz, dz_ld, sums, jobs);
+    else
+        TS2_LAUNCH((linear_dz_kernel<ACT, BF16, false>), grid, 256, 0, c.stream, (const uint16_t *)dy, dy_ld, (const uint16_t *)z, z_ld, T, n, layers,
+                   (uint16_t *)dz, dz_ld, sums, jobs);
+    return TS2_OK;
 }
 
-template <bool A_MN, bool B_MN, int PN, bool BF16>
-int product(const Ctx &c, const Operand &a, const Operand &b, int64_t K, LinearArgs p)
+// a product: operands and what its epilogue does; m = 0: none
+struct Product {
+    const Operand *a = nullptr, *b = nullptr;
+    int64_t K = 0;
+    LinearArgs p = {};
+};
+// How products are divided: tiles of 256 x PN, and the first one's K into ranges.  Times in K blocks of a whole tile, 0.33 us with its copies: a unit takes its
+// blocks and 4 more for its start and its epilogue, tiles of half the width 0.55 of that; joining takes a launch, 10, and 0.1 for every range of a tile.
+struct Plan {
+    int pn, splits;
+};
+Plan plan_of(int pairs, const Product *products, int n)
+{
+    Plan plan = {256, 1};
+    double best = 1e30;
+    for (const int pn : {256, 128}) {
+        const double width = pn == 256 ? 1. : 0.55;
+        const auto tiles = [&](const Product &q) { return (double)(ceil_div(q.p.m, PM) * ceil_div(q.p.n, pn)); };
+        const auto blocks = [&](const Product &q) { return ceil_div(q.K, BK); };
+        const double rest = n > 1 ? tiles(products[1]) * (blocks(products[1]) + 4.) : 0.;
+        for (int s = 1; s <= 64 && s <= blocks(products[0]); ++s) {
+            const int64_t per = ceil_div(blocks(products[0]), s);
+            if (ceil_div(blocks(products[0]), per) != s)
+                continue;
+            const double units = tiles(products[0]) * s, unit = per + 4.;
+            // alone in whole rounds; with a second product that evens them out, by the sum
+            double cost = n > 1 && rest > 0. ? std::max((units * unit + rest) / pairs, unit) + 0.5 * (blocks(products[1]) + 4.)
+                                             : (double)ceil_div((int64_t)units, pairs) * unit;
+            cost = width * cost + (s > 1 ? 10. + 0.1 * width * units : 0.);
+            if (cost < best)
+                best = cost, plan = {pn, s};
+        }
+    }
+    return plan;
+}
+
+template <bool BACK, int PN, bool BF16>
+int run_products(const Ctx &c, const Product *products, int n, int splits, Deal deal)
 {
     static std::atomic<unsigned> ready{0}; // a bit a device: it has been told how much shared memory the kernel takes
     const unsigned bit = 1u << (c.device & 15);
     if (!(ready.load() & bit)) {
-        TS2_CUDA(cudaFuncSetAttribute((const void *)linear_product_kernel<A_MN, B_MN, PN, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        TS2_CUDA(cudaFuncSetAttribute((const void *)linear_product_kernel<BACK, PN, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         ready.fetch_or(bit);
     }
-    const int pairs = sm_count(c.device) / 2, kind = p.kind;
-    p.m_tiles = (int)ceil_div(p.m, PM), p.n_tiles = (int)ceil_div(p.n, PN), p.k_blocks = (int)ceil_div(K, BK);
-    p.splits = choose_splits(pairs, (int64_t)p.m_tiles * p.n_tiles, p.k_blocks);
-    p.kb_per_split = (int)ceil_div(p.k_blocks, p.splits), p.units = p.m_tiles * p.n_tiles * p.splits;
-    p.status = device_status_word(c.device);
-    if (!p.status)
+    const int pairs = sm_count(c.device) / 2;
+    deal.status = device_status_word(c.device);
+    if (!deal.status)
         return fail(TS2_ERR_CUDA, "no device status word");
-    const int size = kind == TS2_OUT_F32 || kind == TS2_OUT_F32_ADD ? 4 : 2;
-    p.y_tma = tma_ok(p.y, p.y_ld, size), p.z_tma = tma_ok(p.z, p.z_ld, 2), p.res_vec = tma_ok(p.res, p.res_ld, 2), p.bias_vec = (uintptr_t)p.bias % 16 == 0;
-    p.ends_whole = p.n * size % 16 == 0;
-    Scratch part(c, p.splits > 1 ? (size_t)p.units * PM * PN * 4 : 0);
-    if (part.rc != TS2_OK)
-        return part.rc;
-    CUtensorMap ta, tb, ty = {}, tz = {};
-    int rc = linear_map(&ta, a.p, 2, a.cols, a.rows, a.ld, A_MN ? BK : 128);
-    if (rc == TS2_OK)
-        rc = linear_map(&tb, b.p, 2, b.cols, b.rows, b.ld, B_MN ? BK : PN / 2);
-    LinearArgs q = p; // of the product
-    if (p.splits > 1) {
-        q.kind = KIND_PARTIAL, q.y_tma = q.ends_whole = true, q.res = nullptr, q.z = nullptr, q.bias = nullptr, p.part = (float *)part.p;
+    LinearMaps maps = {};
+    LinearArgs args[2] = {}, join = {};
+    Scratch part(c, splits > 1 ? (size_t)ceil_div(products[0].p.m, PM) * ceil_div(products[0].p.n, PN) * splits * PM * PN * 4 : 0);
+    int rc = part.rc;
+    for (int i = 0; i < n && rc == TS2_OK; ++i) {
+        const Product &q = products[i];
+        LinearArgs &p = args[i];
+        p = q.p;
+        p.m_tiles = (int)ceil_div(p.m, PM), p.n_tiles = (int)ceil_div(p.n, PN), p.k_blocks = (int)ceil_div(q.K, BK);
+        p.splits = i == 0 ? splits : 1, p.kb_per_split = (int)ceil_div(p.k_blocks, p.splits), p.units = p.m_tiles * p.n_tiles * p.splits;
+        deal.units[i] = p.units;
+        const int size = p.kind == TS2_OUT_F32 || p.kind == TS2_OUT_F32_ADD ? 4 : 2;
+        p.y_tma = tma_ok(p.y, p.y_ld, size), p.z_tma = tma_ok(p.z, p.z_ld, 2), p.res_vec = tma_ok(p.res, p.res_ld, 2), p.bias_vec = (uintptr_t)p.bias % 16 == 0;
+        p.ends_whole = (int64_t)p.n * size % 16 == 0;
+        rc = linear_map(&maps.A[i], q.a->p, 2, q.a->cols, q.a->rows, q.a->ld, p.a_mn ? BK : 128);
         if (rc == TS2_OK)
-            rc = linear_map(&ty, part.p, 4, PN, (int64_t)p.units * PM, PN, 32);
-    } else {
-        if (rc == TS2_OK && p.y_tma)
-            rc = linear_map(&ty, p.y, size, p.n, p.m, p.y_ld, 32);
-        if (rc == TS2_OK && p.z && p.z_tma)
-            rc = linear_map(&tz, p.z, 2, p.n, p.m, p.z_ld, 32);
+            rc = linear_map(&maps.B[i], q.b->p, 2, q.b->cols, q.b->rows, q.b->ld, BACK ? BK : PN / 2);
+        if (p.splits > 1) {
+            p.part = (float *)part.p, join = p;
+            p.kind = KIND_PARTIAL, p.y_tma = p.ends_whole = true, p.res = nullptr, p.z = nullptr, p.bias = nullptr;
+            if (rc == TS2_OK)
+                rc = linear_map(&maps.Y[i], part.p, 4, PN, (int64_t)p.units * PM, PN, 32);
+        } else {
+            if (rc == TS2_OK && p.y_tma)
+                rc = linear_map(&maps.Y[i], p.y, size, p.n, p.m, p.y_ld, 32);
+            if (rc == TS2_OK && p.z && p.z_tma)
+                rc = linear_map(&maps.Z, p.z, 2, p.n, p.m, p.z_ld, 32);
+        }
     }
     if (rc != TS2_OK)
         return rc;
-    TS2_LAUNCH((linear_product_kernel<A_MN, B_MN, PN, BF16>), 2 * std::min(pairs, p.units), THREADS, SMEM, c.stream, ta, tb, ty, tz, q);
-    if (p.splits > 1)
-        TS2_LAUNCH((linear_join_kernel<PN, BF16>), (int)std::min<int64_t>(ceil_div((int64_t)p.m * ceil_div(p.n, 4), 256), 8 * sm_count(c.device)), 256, 0,
-                   c.stream, p, kind);
+    const int used = std::min(pairs, deal.units[0] + deal.units[1]);
+    deal.uneven = deal.units[0] % used;
+    if (deal.uneven && deal.units[1]) {
+        deal.extra = std::max(1, (int)((args[0].kb_per_split + 4. ) / (args[1].k_blocks + 4.) + 0.5));
+        deal.early = std::min(deal.units[1], deal.extra * (used - deal.uneven));
+    }
+    TS2_LAUNCH((linear_product_kernel<BACK, PN, BF16>), 2 * used, THREADS, SMEM, c.stream, maps, args[0], args[1], deal);
+    if (splits > 1)
+        TS2_LAUNCH((linear_join_kernel<PN, BF16>), (int)std::min<int64_t>(ceil_div((int64_t)join.m * ceil_div(join.n, 4), 256), 8 * sm_count(c.device)), 256, 0,
+                   c.stream, join, join.kind);
     return TS2_OK;
 }
-template <bool A_MN, bool B_MN>
-int product(const Ctx &c, bool bf16, const Operand &a, const Operand &b, int64_t K, const LinearArgs &p)
+template <bool BACK>
+int run_products(const Ctx &c, bool bf16, const Product *products, int n, const Deal &deal)
 {
-    // tiles of 256 x 128 where those of 256 x 256 would leave half of the device idle
-    const bool few = 2 * ceil_div(p.m, PM) * ceil_div(p.n, 256) <= sm_count(c.device) / 2;
-    if (few)
-        return bf16 ? product<A_MN, B_MN, 128, true>(c, a, b, K, p) : product<A_MN, B_MN, 128, false>(c, a, b, K, p);
-    return bf16 ? product<A_MN, B_MN, 256, true>(c, a, b, K, p) : product<A_MN, B_MN, 256, false>(c, a, b, K, p);
+    const Plan plan = plan_of(sm_count(c.device) / 2, products, n);
+    if (plan.pn == 128)
+        return bf16 ? run_products<BACK, 128, true>(c, products, n, plan.splits, deal) : run_products<BACK, 128, false>(c, products, n, plan.splits, deal);
+    return bf16 ? run_products<BACK, 256, true>(c, products, n, plan.splits, deal) : run_products<BACK, 256, false>(c, products, n, plan.splits, deal);
 }
 
 // tokens that take the form for a few
@@ -895,25 +1009,19 @@ int linear_forward(const Ctx &c, const LinearShape &s, const void *x, int64_t x_
         const bool vec = tma_ok(x, x_ld, 2) && tma_ok(w, w_ld, 2);
         return s.T <= 8 ? few<1>(c, s.type == TS2_OUT_BF16, vec, f) : few<2>(c, s.type == TS2_OUT_BF16, vec, f);
     }
-    const Operand a(c, x, x_ld, s.T, s.in), b(c, w, w_ld, s.out, s.in);
+    PitchJobs jobs = {};
+    const Operand a(c, x, x_ld, s.T, s.in, jobs), b(c, w, w_ld, s.out, s.in, jobs);
     if (a.rc != TS2_OK || b.rc != TS2_OK)
         return a.rc != TS2_OK ? a.rc : b.rc;
-    LinearArgs p = {};
+    if (jobs.n)
+        if (const int rc = prepare<TS2_ACT_NONE, false>(c, nullptr, 0, nullptr, 0, 0, 0, 0, nullptr, 0, nullptr, jobs))
+            return rc;
+    Product q;
+    q.a = &a, q.b = &b, q.K = s.in;
+    LinearArgs &p = q.p;
     p.m = (int)s.T, p.n = s.out, p.kind = s.type, p.act = s.act, p.bias = bias;
     p.res = residual, p.res_ld = residual_ld, p.y = y, p.y_ld = y_ld, p.z = z, p.z_ld = z_ld;
-    return product<false, false>(c, s.type == TS2_OUT_BF16, a, b, s.in, p);
-}
-
-template <int ACT, bool BF16>
-static int dz_of(const Ctx &c, const LinearShape &s, const void *dy, int64_t dy_ld, const void *z, int64_t z_ld, void *dz, int64_t dz_ld, float *sums,
-                 int blocks, float *dbias)
-{
-    const bool vec = tma_ok(dy, dy_ld, 2) && (ACT == TS2_ACT_NONE || tma_ok(z, z_ld, 2));
-    TS2_LAUNCH((linear_dz_kernel<ACT, BF16>), dim3((int)ceil_div(s.out, 128), blocks), 256, 0, c.stream, (const uint16_t *)dy, dy_ld, (const uint16_t *)z, z_ld,
-               s.T, s.out, vec, (uint16_t *)dz, dz_ld, sums);
-    if (dbias)
-        TS2_LAUNCH(linear_sum_kernel, (int)ceil_div(s.out, 128), 128, 0, c.stream, sums, s.out, blocks, dbias);
-    return TS2_OK;
+    return run_products<false>(c, s.type == TS2_OUT_BF16, &q, 1, {});
 }
 
 int linear_backward(const Ctx &c, const LinearShape &s, const void *dy, int64_t dy_ld, const void *z, int64_t z_ld, const void *x, int64_t x_ld,
@@ -929,46 +1037,47 @@ int linear_backward(const Ctx &c, const LinearShape &s, const void *dy, int64_t 
             TS2_CUDA(cudaMemsetAsync(dbias, 0, (size_t)s.out * 4, c.stream));
         return TS2_OK;
     }
-    // dz where it differs from dy, and the sums of its columns
+    // dz where it differs from dy, the sums of its columns, and operands at another pitch
     const bool own_dz = s.act != TS2_ACT_NONE && products;
-    const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.T, 64), 8 * sm_count(c.device) / ceil_div(s.out, 128)));
-    const int64_t dz_ld = ceil_div(s.out, 8) * 8;
-    const Scratch dz(c, own_dz ? (size_t)s.T * dz_ld * 2 : 0), sums(c, dbias ? (size_t)blocks * s.out * 4 : 0);
-    if (dz.rc != TS2_OK || sums.rc != TS2_OK)
-        return dz.rc != TS2_OK ? dz.rc : sums.rc;
-    if (own_dz || dbias) {
-        using F = int (*)(const Ctx &, const LinearShape &, const void *, int64_t, const void *, int64_t, void *, int64_t, float *, int, float *);
-        static const F forms[4][2] = {{dz_of<TS2_ACT_NONE, false>, dz_of<TS2_ACT_NONE, true>},
-                                      {dz_of<TS2_ACT_RELU, false>, dz_of<TS2_ACT_RELU, true>},
-                                      {dz_of<TS2_ACT_GELU, false>, dz_of<TS2_ACT_GELU, true>},
-                                      {dz_of<TS2_ACT_SILU, false>, dz_of<TS2_ACT_SILU, true>}};
-        if (const int rc = forms[s.act][bf16](c, s, dy, dy_ld, z, z_ld, dz.p, dz_ld, (float *)sums.p, blocks, dbias))
+    const int layers = own_dz || dbias ? (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.T, 64), 8 * sm_count(c.device) / ceil_div(s.out, 128))) : 0;
+    const int64_t own_ld = ceil_div(s.out, 8) * 8;
+    const Scratch dz(c, own_dz ? (size_t)s.T * own_ld * 2 : 0), sums(c, dbias ? (size_t)layers * s.out * 4 : 0);
+    PitchJobs jobs = {}, first = {};
+    const Operand b(c, dx ? w : nullptr, w_ld, s.out, s.in, jobs), a(c, dw ? x : nullptr, x_ld, s.T, s.in, jobs),
+        d(c, own_dz ? dz.p : products ? dy : nullptr, own_dz ? own_ld : dy_ld, s.T, s.out, first);
+    for (const int rc : {dz.rc, sums.rc, a.rc, b.rc, d.rc})
+        if (rc != TS2_OK)
+            return rc;
+    if (layers || jobs.n) {
+        using F = int (*)(const Ctx &, const void *, int64_t, const void *, int64_t, int64_t, int, int, void *, int64_t, float *, const PitchJobs &);
+        static const F forms[4][2] = {{prepare<TS2_ACT_NONE, false>, prepare<TS2_ACT_NONE, true>},
+                                      {prepare<TS2_ACT_RELU, false>, prepare<TS2_ACT_RELU, true>},
+                                      {prepare<TS2_ACT_GELU, false>, prepare<TS2_ACT_GELU, true>},
+                                      {prepare<TS2_ACT_SILU, false>, prepare<TS2_ACT_SILU, true>}};
+        if (const int rc = forms[s.act][bf16](c, dy, dy_ld, z, z_ld, s.T, s.out, layers, dz.p, own_ld, (float *)sums.p, jobs))
             return rc;
     }
-    if (!products)
+    if (first.n) // dy itself
+        if (const int rc = prepare<TS2_ACT_NONE, false>(c, nullptr, 0, nullptr, 0, 0, 0, 0, nullptr, 0, nullptr, first))
+            return rc;
+    if (!products) {
+        if (dbias)
+            TS2_LAUNCH(linear_sum_kernel, (int)ceil_div(s.out, 128), 128, 0, c.stream, (const float *)sums.p, s.out, layers, dbias);
         return TS2_OK;
-    const Operand d(c, own_dz ? dz.p : dy, own_dz ? dz_ld : dy_ld, s.T, s.out);
-    if (d.rc != TS2_OK)
-        return d.rc;
-    if (dx) {
-        const Operand b(c, w, w_ld, s.out, s.in);
-        if (b.rc != TS2_OK)
-            return b.rc;
-        LinearArgs p = {};
-        p.m = (int)s.T, p.n = s.in, p.kind = s.type, p.y = dx, p.y_ld = dx_ld;
-        if (const int rc = product<false, true>(c, bf16, d, b, s.out, p))
-            return rc;
     }
-    if (dw) {
-        const Operand b(c, x, x_ld, s.T, s.in);
-        if (b.rc != TS2_OK)
-            return b.rc;
-        LinearArgs p = {};
-        p.m = s.out, p.n = s.in, p.kind = dw_kind, p.y = dw, p.y_ld = dw_ld;
-        if (const int rc = product<true, true>(c, bf16, d, b, s.T, p))
-            return rc;
-    }
-    return TS2_OK;
+    // the product with the longer sums first: its units are the long ones, or are divided
+    Product of_w, of_x, q[2];
+    of_w.a = &d, of_w.b = &a, of_w.K = s.T;
+    of_w.p.m = s.out, of_w.p.n = s.in, of_w.p.a_mn = true, of_w.p.kind = dw_kind, of_w.p.y = dw, of_w.p.y_ld = dw_ld;
+    of_x.a = &d, of_x.b = &b, of_x.K = s.out;
+    of_x.p.m = (int)s.T, of_x.p.n = s.in, of_x.p.kind = s.type, of_x.p.y = dx, of_x.p.y_ld = dx_ld;
+    const int n = (dx ? 1 : 0) + (dw ? 1 : 0);
+    const bool w_first = dw && (!dx || s.T >= s.out);
+    q[0] = w_first ? of_w : of_x, q[1] = w_first ? of_x : of_w;
+    Deal deal = {};
+    if (dbias)
+        deal.sums = (const float *)sums.p, deal.sums_out = dbias, deal.sums_n = s.out, deal.sums_blocks = layers;
+    return run_products<true>(c, bf16, q, n, deal);
 }
 
 } // namespace ts2

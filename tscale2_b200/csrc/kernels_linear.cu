@@ -19,8 +19,8 @@ namespace ts2 {
 namespace {
 
 constexpr int PM = 256, BK = 64, HALF = 128 * BK * 2; // HALF: a CTA's 128 rows of an operand, one K block, bytes
-constexpr int STAGES = 4, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
-constexpr int BLOCK = 4096, SLOTS = 3; // an epilogue warp's blocks of 32 rows x 128 bytes on their way out
+constexpr int STAGES = 5, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int BLOCK = 4096, SLOTS = 2; // an epilogue warp's blocks of 32 rows x 128 bytes on their way out
 constexpr int STG_OFF = STAGES * 2 * HALF, BAR_OFF = STG_OFF + EPI_WARPS * SLOTS * BLOCK, SMEM = BAR_OFF + 256 + 1024;
 static_assert(SMEM <= 232448, "shared memory budget");
 enum { KIND_PARTIAL = 16 }; // beside TS2_OUT_*: fp32 partial tiles
@@ -97,62 +97,73 @@ __device__ __forceinline__ float rcp(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// 1 - Phi(|z|) and exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun for the error function (absolute error below 1.5e-7): a third of the instructions of
-// erff, and far below the rounding of a 16-bit result
-__device__ __forceinline__ float normal_tail(float z, float &e)
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+__device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
+__device__ __forceinline__ float2 minus_abs(float2 z) { return make_float2(-fabsf(z.x), -fabsf(z.y)); }
+__device__ __forceinline__ float2 sigmoid(float2 z) { return rcp(add2(ex2(mul2(z, both(-1.44269504f))), both(1.f))); }
+// 1 - Phi(|z|) and e = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun for the error function (absolute error below 1.5e-7): a third of the
+// instructions of erff, and far below the rounding of a 16-bit result
+__device__ __forceinline__ float2 normal_tail(float2 z, float2 minus_z, float2 &e)
 {
-    const float a = fabsf(z), t = rcp(fmaf(a, 0.3275911f * 0.70710678f, 1.f));
-    e = ex2(z * z * -0.72134752f);
-    return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f) * e;
+    const float2 t = rcp(fma2(minus_z, both(-0.3275911f * 0.70710678f), both(1.f)));
+    e = ex2(mul2(mul2(z, z), both(-0.72134752f)));
+    float2 q = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+    q = fma2(t, q, both(0.5f * 1.421413741f));
+    q = fma2(t, q, both(0.5f * -0.284496736f));
+    q = fma2(t, q, both(0.5f * 0.254829592f));
+    return mul2(q, mul2(t, e));
 }
 template <int ACT>
-__device__ __forceinline__ float activation(float z)
+__device__ __forceinline__ float2 activation(float2 z)
 {
     if (ACT == TS2_ACT_RELU)
-        return z < 0.f ? 0.f : z; // a NaN stays one
-    if (ACT == TS2_ACT_GELU) {
-        float e;
-        return fmaf(-fminf(fabsf(z), 64.f), normal_tail(z, e), z < 0.f ? 0.f : z); // z Phi(z) = max(z, 0) - |z| (1 - Phi(|z|))
+        return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y); // a NaN stays one
+    if (ACT == TS2_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| (1 - Phi(|z|)), the last term 0 far out
+        const float2 m = minus_abs(z);
+        float2 e;
+        const float2 tail = normal_tail(z, m, e);
+        return fma2(make_float2(fmaxf(m.x, -64.f), fmaxf(m.y, -64.f)), tail, make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f)));
     }
     if (ACT == TS2_ACT_SILU)
-        return z * rcp(1.f + ex2(z * -1.44269504f));
+        return mul2(z, sigmoid(z));
     return z;
 }
 template <int ACT>
-__device__ __forceinline__ float activation_slope(float z)
+__device__ __forceinline__ float2 activation_slope(float2 z)
 {
     if (ACT == TS2_ACT_RELU)
-        return z > 0.f ? 1.f : 0.f;
-    if (ACT == TS2_ACT_GELU) {
-        float e;
-        const float tail = normal_tail(z, e);
-        return fmaf(fminf(fmaxf(z, -64.f), 64.f) * 0.39894228f, e, z < 0.f ? tail : 1.f - tail);
+        return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+    if (ACT == TS2_ACT_GELU) { // Phi(z) + z phi(z), Phi(z) = 1/2 + sign(z) (1/2 - (1 - Phi(|z|)))
+        float2 e;
+        const float2 half = fma2(normal_tail(z, minus_abs(z), e), both(-1.f), both(0.5f));
+        const float2 phi = add2(make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y)), both(0.5f));
+        return fma2(mul2(z, both(0.39894228f)), e, phi);
     }
     if (ACT == TS2_ACT_SILU) {
-        const float s = rcp(1.f + ex2(z * -1.44269504f));
-        return s * fmaf(z, 1.f - s, 1.f);
+        const float2 s = sigmoid(z);
+        return mul2(s, fma2(z, fma2(s, both(-1.f), both(1.f)), both(1.f)));
     }
-    return 1.f;
+    return both(1.f);
+}
+template <int ACT, int N>
+__device__ __forceinline__ void activate_all(float (&v)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 y = activation<ACT>(make_float2(v[i], i + 1 < N ? v[i + 1 < N ? i + 1 : i] : 0.f));
+        v[i] = y.x;
+        if (i + 1 < N)
+            v[i + 1 < N ? i + 1 : i] = y.y;
+    }
 }
 template <int N>
 __device__ __forceinline__ void activate(int act, float (&v)[N])
 {
     switch (act) {
-    case TS2_ACT_RELU:
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            v[i] = activation<TS2_ACT_RELU>(v[i]);
-        break;
-    case TS2_ACT_GELU:
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            v[i] = activation<TS2_ACT_GELU>(v[i]);
-        break;
-    case TS2_ACT_SILU:
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            v[i] = activation<TS2_ACT_SILU>(v[i]);
-        break;
+    case TS2_ACT_RELU: activate_all<TS2_ACT_RELU>(v); break;
+    case TS2_ACT_GELU: activate_all<TS2_ACT_GELU>(v); break;
+    case TS2_ACT_SILU: activate_all<TS2_ACT_SILU>(v); break;
     default: break;
     }
 }
@@ -340,7 +351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         uint8_t *const slots = smem + STG_OFF + ew * SLOTS * BLOCK;
         int slot = 0, acc = 0;
         uint32_t acc_phase = 0;
-        // the next block; the store that last used it, three blocks before, has read it (a block for z is taken while y's has not left)
+        // the next block; the store that last used it, two blocks before, has read it (a block for z is taken while y's has not left)
         const auto take = [&](bool second) {
             uint8_t *b = slots + slot * BLOCK;
             slot = slot == SLOTS - 1 ? 0 : slot + 1;
@@ -740,51 +751,49 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restri
     __shared__ float part[16][132];
     const int sub = threadIdx.x & 15, line = threadIdx.x >> 4, col0 = blockIdx.x * 128;
     const auto column = [&](int k) { return col0 + (VEC ? sub * 8 + k : sub + 16 * k); };
-    float acc[8] = {};
-    const auto read = [&](const uint16_t *row, uint16_t (&v)[8]) {
+    float2 acc[4] = {};
+    const auto read = [&](const uint16_t *row, uint32_t (&v)[4]) {
         if (VEC && column(0) + 8 <= n) {
-            const Piece<uint16_t, 8> q = *(const Piece<uint16_t, 8> *)(row + column(0));
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                v[k] = q.v[k];
+            const uint4 q = *(const uint4 *)(row + column(0));
+            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                v[k] = column(k) < n ? row[column(k)] : (uint16_t)0;
+            for (int k = 0; k < 4; ++k)
+                v[k] = (column(2 * k) < n ? (uint32_t)row[column(2 * k)] : 0u) | (column(2 * k + 1) < n ? (uint32_t)row[column(2 * k + 1)] << 16 : 0u);
         }
     };
 #pragma unroll 2
     for (int64_t t = (int64_t)blockIdx.y * 16 + line; t < T; t += (int64_t)layers * 16) {
-        uint16_t a[8], b[8];
+        uint32_t a[4], b[4], o[4];
         read(dy + t * dy_ld, a);
         if (ACT != TS2_ACT_NONE)
             read(z + t * z_ld, b);
-        float d[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            d[k] = widen16<BF16>(a[k]);
+        for (int k = 0; k < 4; ++k) {
+            float2 d = unpack2<BF16>(a[k]);
             if (ACT != TS2_ACT_NONE)
-                d[k] *= activation_slope<ACT>(widen16<BF16>(b[k]));
-            acc[k] += d[k];
+                d = mul2(d, activation_slope<ACT>(unpack2<BF16>(b[k])));
+            acc[k] = add2(acc[k], d);
+            o[k] = pack2<BF16>(d.x, d.y);
         }
         if (!dz)
             continue;
         uint16_t *to = dz + t * dz_ld;
         if (VEC) {
             if (column(0) < n) // the pitch is a multiple of 8
-                *(uint4 *)(to + column(0)) = make_uint4(pack2<BF16>(d[0], d[1]), pack2<BF16>(d[2], d[3]), pack2<BF16>(d[4], d[5]), pack2<BF16>(d[6], d[7]));
+                *(uint4 *)(to + column(0)) = make_uint4(o[0], o[1], o[2], o[3]);
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (column(k) < n)
-                    to[column(k)] = (uint16_t)pack2<BF16>(d[k], 0.f);
+                    to[column(k)] = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
         }
     }
     if (!sums)
         return;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-        part[line][column(k) - col0] = acc[k];
+        part[line][column(k) - col0] = k & 1 ? acc[k >> 1].y : acc[k >> 1].x;
     __syncthreads();
     if (threadIdx.x < 128 && col0 + (int)threadIdx.x < n) {
         float s = 0.f;

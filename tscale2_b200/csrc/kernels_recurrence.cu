@@ -11,6 +11,7 @@
 // what each segment does to the state that enters it, from the last start of a sequence in it on.  The bound is memory
 // bandwidth (gate and x in, h out), for 16-bit arrays nearly the issue slots, too (23 instructions an element, two of them in
 // the unit of exponentials and reciprocals).  The order of every sum is fixed.
+#include "elem_types.cuh"
 #include "kernels.cuh"
 #include <algorithm>
 #include <climits>
@@ -80,32 +81,6 @@ __device__ __forceinline__ void store_state(float *p, int n, float2 v)
         p[1] = v.y;
 }
 
-// both channels in one instruction
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
-        "mov.b64 {%0, %1}, w;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
 // a = 1 / (1 + exp(-g)) and 1 - a, both with a small relative error (the product with log2 e is rounded: |g| 2^-24, and the three
 // instructions' own) however near to one the other is.  The exponent stops at 126, where a is 1e-38 and 1 - a is 1: beyond it exp(-g)
 // would be infinite and 1 - a = exp(-g) a not a number.  A NaN stays one.

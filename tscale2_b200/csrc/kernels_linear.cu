@@ -505,15 +505,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (lane == 0)
                         bulk_commit();
                 }
-                // rows that TMA cannot address: neighbours by neighbours
-                const auto by_rows = [&](const uint8_t *block, uint16_t *to, int64_t ld) {
-                    for (int i = 0; i < 32 && row0 + i < p.m; ++i)
+                // Rows that TMA cannot address: 8 lanes a row, each the 16 bytes behind the first 16-byte boundary that are its, put together from two
+                // neighbouring pieces; what lies before that boundary and behind the last one element by element.
+                const auto by_rows = [&](uint8_t *block, uint16_t *base, int64_t ld) {
+                    const int there = min(64, p.n - left), q = lane & 7; // there: elements of a row, not always above 0
+#pragma unroll 2
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + (lane >> 3);
+                        uint16_t *to = base + (row0 + r) * ld + left;
+                        const int head = -((int)(uintptr_t)to >> 1) & 7, whole = max(0, there - head) >> 3, behind = head + 8 * whole + q;
+                        if (row0 + r >= p.m)
+                            continue;
+                        const auto element = [&](int e) { return *((const uint16_t *)piece(block, r, e >> 3) + (e & 7)); };
+                        if (q < whole) {
+                            const uint4 x = *piece(block, r, q), y = head ? *piece(block, r, q + 1) : x;
+                            uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int k = h * 32 + lane;
-                            if (left + k < p.n)
-                                to[(row0 + i) * ld + left + k] = *(const uint16_t *)(block + i * 128 + (((k >> 3) ^ (i & 7)) << 4) + (k & 7) * 2);
+                            for (int k = 0; k < 6; ++k)
+                                w[k] = head & 4 ? w[k + 2] : w[k];
+#pragma unroll
+                            for (int k = 0; k < 5; ++k)
+                                w[k] = head & 2 ? w[k + 1] : w[k];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                w[k] = __funnelshift_r(w[k], w[k + 1], head & 1 ? 16 : 0);
+                            *(uint4 *)(to + head + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
+                        if (q < head && q < there)
+                            to[q] = element(q);
+                        if (behind < there)
+                            to[behind] = element(behind);
+                    }
                 };
                 if (!y_tma) {
                     if (halves) {
@@ -741,10 +763,19 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restri
         const int64_t worker = ((int64_t)(blockIdx.y - layers) * gridDim.x + blockIdx.x) * 8 + (threadIdx.x >> 5), workers = (int64_t)(gridDim.y - layers) * gridDim.x * 8;
         for (int i = 0; i < jobs.n; ++i) {
             const PitchJob &j = jobs.job[i];
-            for (int64_t r = worker; r < j.rows; r += workers)
-#pragma unroll 8
-                for (int c = threadIdx.x & 31; c < j.cols; c += 32)
-                    j.to[r * j.to_ld + c] = j.from[r * j.from_ld + c];
+            for (int64_t r = worker; r < j.rows; r += workers) {
+                // 4-byte words that hold an element of the row; where it begins with the upper half of one, halves of neighbours
+                const uint16_t *row = j.from + r * j.from_ld;
+                const bool odd = (uintptr_t)row & 2;
+                const uint32_t *from = (const uint32_t *)(row - odd);
+                uint32_t *to = (uint32_t *)(j.to + r * j.to_ld); // 16-byte aligned, with room for a multiple of 8
+                const int words = (j.cols + 1) / 2, last = (j.cols + odd - 1) / 2;
+#pragma unroll 4
+                for (int c = threadIdx.x & 31; c < words; c += 32) {
+                    const uint32_t a = from[c], b = odd && c < last ? from[c + 1] : 0u;
+                    to[c] = odd ? a >> 16 | b << 16 : a;
+                }
+            }
         }
         return;
     }

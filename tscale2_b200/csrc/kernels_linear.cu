@@ -18,7 +18,7 @@ namespace ts2 {
 
 namespace {
 
-constexpr int PM = 256, BK = 64, HALF = 128 * BK * 2; // HALF: a CTA's 128 rows of an operand, one K block, bytes
+constexpr int PM = 256, BK = 64, BAND = 8,  HALF = 128 * BK * 2; // HALF: a CTA's 128 rows of an operand, one K block, bytes
 constexpr int STAGES = 5, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
 constexpr int BLOCK = 4096, SLOTS = 2; // an epilogue warp's blocks of 32 rows x 128 bytes on their way out
 constexpr int STG_OFF = STAGES * 2 * HALF, BAR_OFF = STG_OFF + EPI_WARPS * SLOTS * BLOCK, SMEM = BAR_OFF + 256 + 1024;
@@ -69,15 +69,15 @@ __device__ __forceinline__ bool unit_at(const Deal &d, int pair, int pairs, int 
 struct Unit {
     int row, col, kb0, kb1;
 };
-// Units go through the output in bands of 8 rows of tiles, column by column, so that the tiles at work at a time share rows and columns of the operands in
+// Units go through the output in bands of BAND rows of tiles, column by column, so that the tiles at work at a time share rows and columns of the operands in
 // the L2; the K ranges of a tile are neighbours.
 template <int PN>
 __device__ __forceinline__ Unit unit_of(const LinearArgs &p, int u)
 {
-    const int tile = u / p.splits, split = u - tile * p.splits, band = tile / (8 * p.n_tiles), rest = tile - band * 8 * p.n_tiles;
-    const int high = min(8, p.m_tiles - band * 8), col = rest / high;
+    const int tile = u / p.splits, split = u - tile * p.splits, band = tile / (BAND * p.n_tiles), rest = tile - band * BAND * p.n_tiles;
+    const int high = min(BAND, p.m_tiles - band * BAND), col = rest / high;
     Unit t;
-    t.row = (band * 8 + rest - col * high) * PM;
+    t.row = (band * BAND + rest - col * high) * PM;
     t.col = col * PN;
     t.kb0 = split * p.kb_per_split;
     t.kb1 = min(p.k_blocks, t.kb0 + p.kb_per_split);
@@ -188,6 +188,28 @@ __device__ __forceinline__ float widen16(uint16_t v)
     return unpack2<BF16>(v).x;
 }
 
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 v)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t at)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint16_t ld_shared_u16(uint32_t at)
+{
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ void tma_add_2d(const void *tmap, uint32_t src, int c0, int c1)
 {
     asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src), "r"(c0), "r"(c1)
@@ -348,12 +370,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     } else {
         // epilogue: a warp takes 32 rows x PART columns, 32 columns at a time, thread = row
         const int quarter = warp & 3, ew = warp - 2, part = ew >> 2;
-        uint8_t *const slots = smem + STG_OFF + ew * SLOTS * BLOCK;
+        const uint32_t slots = smem_u32(smem) + STG_OFF + ew * SLOTS * BLOCK;
         int slot = 0, acc = 0;
         uint32_t acc_phase = 0;
         // the next block; the store that last used it, two blocks before, has read it (a block for z is taken while y's has not left)
         const auto take = [&](bool second) {
-            uint8_t *b = slots + slot * BLOCK;
+            const uint32_t b = slots + slot * BLOCK;
             slot = slot == SLOTS - 1 ? 0 : slot + 1;
             if (lane == 0) {
                 if (second)
@@ -364,7 +386,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             __syncwarp();
             return b;
         };
-        const auto piece = [&](uint8_t *block, int row, int q) { return (uint4 *)(block + row * 128 + ((q ^ (row & 7)) << 4)); };
+        const auto piece = [&](uint32_t block, int row, int q) { return block + row * 128 + ((q ^ (row & 7)) << 4); };
         if (BACK && deal.sums_out) // no tile is there for a while
             for (int at = ((int)blockIdx.x * EPI_WARPS + ew) * 32 + lane; at < deal.sums_n; at += (int)gridDim.x * EPI_WARPS * 32) {
                 float sum = 0.f;
@@ -380,8 +402,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const Unit un = unit_of<PN>(p, u);
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * PN + part * PART;
             const int row0 = un.row + (int)rank * 128 + quarter * 32, col0 = un.col + part * PART;
-            uint4 rows[4]; // of the next 32 columns of the residual: 4 lanes a row, 8 rows at a time
-            const auto fetch = [&](int col) {
+            if (p.res && row0 + lane < p.m) { // the residual into the L2 while the tile is multiplied
+                const uint16_t *from = (const uint16_t *)p.res + (row0 + lane) * p.res_ld;
+#pragma unroll
+                for (int k = 0; k < PART; k += 64)
+                    if (col0 + k < p.n)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(from + col0 + k));
+            }
+            uint4 ahead[2][4]; // of the next two times 32 columns of the residual: 4 lanes a row, 8 rows at a time
+            const auto fetch = [&](int col, uint4 (&rows)[4]) {
                 if (!p.res || col >= p.n)
                     return;
 #pragma unroll
@@ -402,14 +431,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     }
                 }
             };
-            fetch(col0);
+            fetch(col0, ahead[0]);
+            fetch(col0 + 32, ahead[1]);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag)))
                 break;
             tc_fence_after();
-            uint8_t *yb = nullptr, *zb = nullptr;
+            uint32_t yb = 0, zb = 0;
 #pragma unroll 1
-            for (int c = 0; c < PART / 32; ++c) {
-                const int col = col0 + c * 32, half = c & 1; // 16-bit results fill half of a block's rows
+            for (int c2 = 0; c2 < PART / 32; c2 += 2)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = c2 + half, col = col0 + c * 32; // 16-bit results fill half of a block's rows
                 uint32_t r[32];
                 __syncwarp(); // lane 0 comes from its stores
                 tmem_ld32(taddr + c * 32, r);
@@ -430,7 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     yb = take(false);
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        *piece(yb, lane, q) = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+                        st_shared(piece(yb, lane, q), make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]));
                 } else {
                     if (!half) {
                         yb = take(false);
@@ -440,10 +472,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (p.res) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            *piece(yb, 8 * i + (lane >> 2), 4 * half + (lane & 3)) = rows[i];
+                            st_shared(piece(yb, 8 * i + (lane >> 2), 4 * half + (lane & 3)), ahead[half][i]);
                         __syncwarp();
-                        if (c + 1 < PART / 32)
-                            fetch(col + 32);
+                        if (c + 2 < PART / 32)
+                            fetch(col + 64, ahead[half]);
                     }
                     if (p.bias) {
                         if (p.bias_vec && col + 32 <= p.n) {
@@ -462,15 +494,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (p.z) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            *piece(zb, lane, 4 * half + q) = make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
-                                                                        pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7]));
+                            st_shared(piece(zb, lane, 4 * half + q),
+                                      make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
+                                                 pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7])));
                     }
                     activate(p.act, v);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        uint4 *at = piece(yb, lane, 4 * half + q);
+                        const uint32_t at = piece(yb, lane, 4 * half + q);
                         if (p.res) {
-                            const uint4 raw = *at;
+                            const uint4 raw = ld_shared(at);
                             const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
@@ -478,8 +511,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                 v[8 * q + 2 * k] += f.x, v[8 * q + 2 * k + 1] += f.y;
                             }
                         }
-                        *at = make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
-                                         pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7]));
+                        st_shared(at, make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
+                                                 pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7])));
                     }
                     if (!half)
                         continue;
@@ -491,23 +524,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (y_tma && lane == 0 && left < p.n) {
                     if (p.kind == KIND_PARTIAL)
-                        tma_store_2d(tmY, smem_u32(yb), left - un.col, u * PM + row0 - un.row);
+                        tma_store_2d(tmY, yb, left - un.col, u * PM + row0 - un.row);
                     else if (p.kind == TS2_OUT_F32_ADD)
-                        tma_add_2d(tmY, smem_u32(yb), left, row0);
+                        tma_add_2d(tmY, yb, left, row0);
                     else
-                        tma_store_2d(tmY, smem_u32(yb), left, row0);
+                        tma_store_2d(tmY, yb, left, row0);
                 }
                 if (lane == 0)
                     bulk_commit(); // a group for every block taken, with or without a store
                 if (halves && p.z) {
                     if (z_tma && lane == 0 && left < p.n)
-                        tma_store_2d(&maps.Z, smem_u32(zb), left, row0);
+                        tma_store_2d(&maps.Z, zb, left, row0);
                     if (lane == 0)
                         bulk_commit();
                 }
                 // Rows that TMA cannot address: 8 lanes a row, each the 16 bytes behind the first 16-byte boundary that are its, put together from two
                 // neighbouring pieces; what lies before that boundary and behind the last one element by element.
-                const auto by_rows = [&](uint8_t *block, uint16_t *base, int64_t ld) {
+                const auto by_rows = [&](uint32_t block, uint16_t *base, int64_t ld) {
                     const int there = min(64, p.n - left), q = lane & 7; // there: elements of a row, not always above 0
 #pragma unroll 2
                     for (int i = 0; i < 8; ++i) {
@@ -516,9 +549,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         const int head = -((int)(uintptr_t)to >> 1) & 7, whole = max(0, there - head) >> 3, behind = head + 8 * whole + q;
                         if (row0 + r >= p.m)
                             continue;
-                        const auto element = [&](int e) { return *((const uint16_t *)piece(block, r, e >> 3) + (e & 7)); };
+                        const auto element = [&](int e) { return ld_shared_u16(piece(block, r, e >> 3) + (e & 7) * 2); };
                         if (q < whole) {
-                            const uint4 x = *piece(block, r, q), y = head ? *piece(block, r, q + 1) : x;
+                            const uint4 x = ld_shared(piece(block, r, q)), y = head ? ld_shared(piece(block, r, q + 1)) : x;
                             uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
                             for (int k = 0; k < 6; ++k)
@@ -544,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         for (int i = 0; i < 32 && row0 + i < p.m; ++i)
                             if (left + lane < p.n) {
                                 float *to = (float *)p.y + (row0 + i) * p.y_ld + left + lane;
-                                const float now = *(const float *)(yb + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4);
+                                const float now = ld_shared_f32(piece(yb, i, lane >> 2) + (lane & 3) * 4);
                                 *to = p.kind == TS2_OUT_F32_ADD ? *to + now : now;
                             }
                     }
@@ -578,8 +611,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const LinearArgs p, in
     const int64_t total = (int64_t)p.m * quads;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int row = (int)(i / quads), col = (int)(i - (int64_t)row * quads) * 4;
-        const int band = row / (8 * PM), high = min(8, p.m_tiles - band * 8);
-        const int tile = band * 8 * p.n_tiles + col / PN * high + row / PM - band * 8;
+        const int band = row / (BAND * PM), high = min(BAND, p.m_tiles - band * BAND);
+        const int tile = band * BAND * p.n_tiles + col / PN * high + row / PM - band * BAND;
         const float *from = p.part + ((int64_t)tile * p.splits * PM + row % PM) * PN + col % PN;
         float v[4] = {};
         for (int s = 0; s < p.splits; ++s) {

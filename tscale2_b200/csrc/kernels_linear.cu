@@ -409,6 +409,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (col0 + k < p.n)
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(from + col0 + k));
             }
+            if (p.bias && col0 + 4 * lane < p.n) { // and the bias into the L1
+                float ignored;
+                asm volatile("ld.global.ca.f32 %0, [%1];" : "=f"(ignored) : "l"(p.bias + col0 + 4 * lane));
+            }
             uint4 ahead[2][4]; // of the next two times 32 columns of the residual: 4 lanes a row, 8 rows at a time
             const auto fetch = [&](int col, uint4 (&rows)[4]) {
                 if (!p.res || col >= p.n)
@@ -796,17 +800,23 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restri
         const int64_t worker = ((int64_t)(blockIdx.y - layers) * gridDim.x + blockIdx.x) * 8 + (threadIdx.x >> 5), workers = (int64_t)(gridDim.y - layers) * gridDim.x * 8;
         for (int i = 0; i < jobs.n; ++i) {
             const PitchJob &j = jobs.job[i];
-            for (int64_t r = worker; r < j.rows; r += workers) {
+            const int words = (j.cols + 1) / 2, pieces = (words + 255) / 256; // 256 words of a row at a time
+            for (int64_t item = worker; item < j.rows * pieces; item += workers) {
+                const int64_t r = item / pieces;
+                const int begin = (int)(item - r * pieces) * 256;
                 // 4-byte words that hold an element of the row; where it begins with the upper half of one, halves of neighbours
                 const uint16_t *row = j.from + r * j.from_ld;
                 const bool odd = (uintptr_t)row & 2;
                 const uint32_t *from = (const uint32_t *)(row - odd);
                 uint32_t *to = (uint32_t *)(j.to + r * j.to_ld); // 16-byte aligned, with room for a multiple of 8
-                const int words = (j.cols + 1) / 2, last = (j.cols + odd - 1) / 2;
-#pragma unroll 4
-                for (int c = threadIdx.x & 31; c < words; c += 32) {
-                    const uint32_t a = from[c], b = odd && c < last ? from[c + 1] : 0u;
-                    to[c] = odd ? a >> 16 | b << 16 : a;
+                const int last = (j.cols + odd - 1) / 2;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int c = begin + k * 32 + (threadIdx.x & 31);
+                    if (c < words) {
+                        const uint32_t a = from[c], b = odd && c < last ? from[c + 1] : 0u;
+                        to[c] = odd ? a >> 16 | b << 16 : a;
+                    }
                 }
             }
         }
@@ -943,7 +953,7 @@ struct Product {
     LinearArgs p = {};
 };
 // How products are divided: tiles of 256 x PN, and the first one's K into ranges.  Times in K blocks of a whole tile, 0.33 us with its copies: a unit takes its
-// blocks and 4 more for its start and its epilogue, tiles of half the width 0.55 of that; joining takes a launch, 10, and 0.1 for every range of a tile.
+// blocks and 4 more for its start and its epilogue, tiles of half the width 0.75 of that (32768 x 2048 x 8192 742 us, with those 1100); joining takes a launch, 10, and 0.1 for every range of a tile.
 struct Plan {
     int pn, splits;
 };
@@ -952,7 +962,7 @@ Plan plan_of(int pairs, const Product *products, int n)
     Plan plan = {256, 1};
     double best = 1e30;
     for (const int pn : {256, 128}) {
-        const double width = pn == 256 ? 1. : 0.55;
+        const double width = pn == 256 ? 1. : 0.75;
         const auto tiles = [&](const Product &q) { return (double)(ceil_div(q.p.m, PM) * ceil_div(q.p.n, pn)); };
         const auto blocks = [&](const Product &q) { return ceil_div(q.K, BK); };
         const double rest = n > 1 ? tiles(products[1]) * (blocks(products[1]) + 4.) : 0.;

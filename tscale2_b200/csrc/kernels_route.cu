@@ -8,8 +8,10 @@
 //     sigmoid, renormalised  dl[e] = scale w[e] (1 - s[e]) (d[e] - sum_j d[j] w[j])
 //
 // A warp takes 4 rows (8 of up to 32 experts).  They come in a row at a time in pieces of 8 columns a lane, and their keys and every piece's largest key go to
-// shared memory.  Then 8 (4) lanes have a row, each the largest keys of every eighth piece in registers: a choice is a maximum over those and over the lanes, and
-// only the piece that it came from is looked at again.
+// shared memory.  Then 4 or 8 lanes have a row, each the largest keys of some neighbouring pieces in registers: a choice is a maximum over those and over the
+// lanes, and only the piece that it came from is looked at again, by all of them.  Bound by instructions, 540 a row of 256 sigmoid scores with a bias, in groups and
+// 8 choices (of 224 for the row itself, 72 for its keys, 105 for groups, 20 for a choice), at 2.1 a clock of an SM with 39 % of its warps: 35.6 us for 32768 rows,
+// whose bytes take 3; 18.3 us for 65537 rows of 128, 4 choices, whose bytes take 2.9.
 //
 // Keys are fp32 first.  They order as exact ones would where they differ by more than fp32 can be wrong, so a row in which two choices, the last choice and the
 // next key, or two groups at the border are nearer than that is done once more in fp64 by the whole warp.  Without a bias (and with groups ranked by one key)
@@ -285,9 +287,6 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
             const int e = (at + 32 * h) * 8 + i;
             bias[h][i] = c.bias && e < E ? c.bias[e] : 0.f;
         }
-    // a piece's place among the largest keys: those of a lane side by side
-    const auto place = [&](int piece) { return piece % L * NB + piece / L; };
-
     // rows come in
 #pragma unroll 1
     for (int pass0 = 0; pass0 < PASSES; pass0 += STEP) {
@@ -380,9 +379,9 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                     to[1] = make_float4(k[4], k[5], k[6], k[7]);
                 }
                 { // -inf where there is none
-                    first[r * pp + place(piece)] = best;
+                    first[r * pp + piece] = best;
                     if (kept_second)
-                        second[r * pp + place(piece)] = next;
+                        second[r * pp + piece] = next;
                 }
                 if (c.groups > 1 && coming) { // over the lanes of a group
                     for (int o = 1; o < group_pieces; o *= 2) {
@@ -419,8 +418,8 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                 if (per % 8 == 0) { // a group is whole pieces
                     for (int i = g * group_pieces; i < (g + 1) * group_pieces; ++i) {
                         if (two)
-                            next = fmaxf(next, my_second[place(i)]);
-                        take(my_first[place(i)]);
+                            next = fmaxf(next, my_second[i]);
+                        take(my_first[i]);
                     }
                 } else {
                     for (int e = g * per; e < (g + 1) * per; ++e)
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                         my_keys[e] = -INFINITY;
                     best = fmaxf(best, my_keys[e]);
                 }
-                my_first[place(i)] = best;
+                my_first[i] = best;
             }
             dropped = 0;
         }
@@ -467,48 +466,61 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
     float held[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-        held[i] = my_first[l * NB + i];
+        const int piece = l * NB + i; // neighbours
+        held[i] = my_first[piece];
         if (dropped) {
-            const int piece = i * L + l, g = coming ? piece >> shift : piece / group_pieces;
+            const int g = coming ? piece >> shift : piece / group_pieces;
             held[i] = piece < pieces && (dropped >> g & 1) ? -INFINITY : held[i];
         }
     }
     const int rounds = p.selected + (by_logit ? 0 : 1); // the first key that is not chosen, for its distance
 #pragma unroll 1
     for (int j = 0; j < rounds; ++j) {
-        float best = held[0];
+        float mine = held[0];
 #pragma unroll
         for (int i = 1; i < NB; ++i)
-            best = fmaxf(best, held[i]);
-        best = max_over(best, L);
-        int piece = 1 << 20; // the first one with this key
+            mine = fmaxf(mine, held[i]);
+        const float best = max_over(mine, L);
+        // the first lane with this key, and the first of its pieces
+        const int owner = __ffs(__ballot_sync(FULL, mine == best) >> (lane & ~(L - 1)) & ((1u << L) - 1)) - 1;
+        int at_i = 0;
 #pragma unroll
         for (int i = NB - 1; i >= 0; --i)
-            piece = held[i] == best ? i * L + l : piece;
-        int lowest = piece;
+            at_i = held[i] == best ? i : at_i;
+        at_i = __shfl_sync(FULL, at_i, owner, L);
+        const int piece = owner * NB + at_i;
+        const bool found = best > -INFINITY;
+        // the lanes look at the piece together: its first element with this key, and the largest of the others
+        constexpr int EACH = 8 / L;
+        float k[EACH];
+        int i0 = 8;
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1)
-            lowest = min(lowest, __shfl_xor_sync(FULL, lowest, o));
-        if (best == -INFINITY) {
-            if (l == 0)
-                my_id[j] = -1, my_chosen[j] = -INFINITY;
-        } else if (piece == lowest) { // this lane's: nobody else looks at the piece
-            const float4 a = *(const float4 *)(my_keys + piece * 8), b = *(const float4 *)(my_keys + piece * 8 + 4);
-            const float k[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            int i0 = 0;
+        for (int i = 0; i < EACH; ++i)
+            k[i] = my_keys[piece * 8 + l * EACH + i];
+        if constexpr (EACH == 1) {
+            i0 = __ffs(__ballot_sync(FULL, k[0] == best) >> (lane & ~(L - 1)) & ((1u << L) - 1)) - 1;
+        } else {
 #pragma unroll
-            for (int i = 7; i >= 0; --i)
-                i0 = k[i] == best ? i : i0;
-            float rest = -INFINITY;
+            for (int i = EACH - 1; i >= 0; --i)
+                i0 = k[i] == best ? l * EACH + i : i0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                rest = fmaxf(rest, i == i0 ? -INFINITY : k[i]);
-            my_keys[piece * 8 + i0] = -INFINITY;
+            for (int o = L / 2; o > 0; o >>= 1)
+                i0 = min(i0, __shfl_xor_sync(FULL, i0, o));
+        }
+        float rest = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            rest = l * EACH + i == i0 ? rest : fmaxf(rest, k[i]);
+        rest = max_over(rest, L);
+        if (found && l == owner) {
 #pragma unroll
             for (int i = 0; i < NB; ++i)
-                held[i] = i * L + l == piece ? rest : held[i];
-            my_id[j] = piece * 8 + i0, my_chosen[j] = best;
+                held[i] = i == at_i ? rest : held[i];
+            my_keys[piece * 8 + i0] = -INFINITY;
         }
+        if (l == 0)
+            my_id[j] = found ? piece * 8 + i0 : -1, my_chosen[j] = best;
+        __syncwarp(); // the key is gone for all lanes
     }
     __syncwarp();
 
@@ -751,8 +763,8 @@ static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_
 template <class T>
 static int forward(const Ctx &c, const RouteShape &s, const void *logits, int64_t ld, const Choice &choice, const uint8_t *mask, int *ids, float *weights)
 {
-    // 4 lanes a row take fewer instructions, 8 two times the warps.  Up to 128 experts 4 are faster (65537 x 128 19.2 against 24.1 us), beyond 8 (32768 x 256
-    // in groups 38.1 against 39.9); for the gradient, whose row has little to do, 8 are from 33 experts on (65537 x 128 22.8 against 27.4, 32768 x 256 8.9
+    // 4 lanes a row take fewer instructions, 8 two times the warps.  Up to 128 experts 4 are faster (65537 x 128 18.3 against 20.9 us), beyond 8 (32768 x 256
+    // in groups 35.6 against 39.2); for the gradient, whose row has little to do, 8 are from 33 experts on (65537 x 128 22.8 against 27.4, 32768 x 256 8.9
     // against 10.4).
     const auto f = s.E <= 32    ? forward<T, 4, 1>
                    : s.E <= 64  ? forward<T, 4, 2>

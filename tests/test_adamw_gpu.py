@@ -270,3 +270,36 @@ def test_same_bits_on_another_stream_and_replayed():
         for s in sets[1:]:
             for a, b in zip(sets[0], s):
                 assert all(torch.equal(a.view[k], b.view[k]) for k in a.view)
+
+
+def test_elements_beyond_32_bits():
+    """a tensor of 2^31 elements and some: its last ones, and the ones on both sides of 2^31"""
+    n, seed, step = (1 << 31) + 1000, 5, 3
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    m, v = (torch.zeros(n, device="cuda", dtype=torch.uint8) for _ in range(2))
+    ms, vs = (torch.zeros(-(-n // 32), device="cuda", dtype=torch.uint8) for _ in range(2))
+    at = [(1 << 31) - 64, n - 40]
+    parts = [slice(a, min(n, a + 128)) for a in at]
+    for s in parts:
+        g[s] = torch.randn(s.stop - s.start, device="cuda", generator=gen)
+    table = (capi.AdamwTensor * 1)()
+    t = table[0]
+    t.param, t.grad, t.m, t.v, t.m_scale, t.v_scale, t.copy, t.n, t.rate, t.decay = *(x.data_ptr() for x in (p, g, m, v, ms, vs)), None, n, 1.0, 0.0
+    check(capi.load_library().ts2_op_adamw(0, stream(), KIND["bf16"], 8, KIND["none"], C.cast(table, C.c_void_p), 1, RATE, B1, B2, EPS, step, 1.0, None, seed))
+    key = mix64(mix64((seed + step) & M64) ^ 0) & 0xFFFFFFFF
+    for s in parts:
+        first = s.start // 32 * 32
+        w = slice(first, s.stop)
+        grad = g[w].double().cpu().numpy()
+        x = ((np.arange(w.start, w.stop, dtype=np.uint64) * 0x9E3779B1 + key) & 0xFFFFFFFF).astype(np.uint32)
+        x = (x ^ (x >> np.uint32(16))) * np.uint32(0x85EBCA6B)
+        x = (x ^ (x >> np.uint32(13))) * np.uint32(0xC2B2AE35)
+        x = x ^ (x >> np.uint32(16))
+        for state, scale, now, u, second in ((m, ms, (1 - B1) * grad, x >> np.uint32(16), False), (v, vs, (1 - B2) * grad * grad, x & np.uint32(0xFFFF), True)):
+            code, sc = encode(now, u / 65536.0, second)
+            assert np.array_equal(state[w].cpu().numpy(), code)
+            assert np.array_equal(scale[first // 32:-(-w.stop // 32)].cpu().numpy(), sc)
+        want = -RATE * (1 - B1) * grad / (1 - B1 ** step) / (np.sqrt((1 - B2) * grad * grad / (1 - B2 ** step)) + EPS)
+        assert (np.abs(p[w].double().cpu().numpy() - want) <= 2.0 ** -20 * np.abs(want)).all()
+    assert (p[: 1 << 20] == 0).all() and (p[1 << 30: (1 << 30) + (1 << 20)] == 0).all()

@@ -298,3 +298,25 @@ def test_beyond_32_bit_offsets():
     near(dx, dz @ w.double(), half_step("f16", dz @ w.double()) + 2.0 ** -19 * (dz.abs() @ w.double().abs()))
     want = dz.T @ x.double()
     near(dw, want, half_step("f16", want) + (T / 8 + 8) * 2.0 ** -23 * (dz.abs().T @ x.double().abs()))
+
+
+def test_more_than_32_bits_of_outputs():
+    """2.3e9 results, kept ones and gradients: the last rows, and dw over all of them"""
+    T, n, m = 290_001, 64, 8000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, w = torch.randn((T, n), device="cuda", generator=gen).bfloat16(), (torch.randn((m, n), device="cuda", generator=gen) / 8).bfloat16()
+    y, z = (torch.zeros((T, m), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    lib = capi.load_library()
+    check(lib.ts2_op_linear_forward(0, stream(), KIND["bf16"], ACT["relu"], T, n, m, ptr(x), n, ptr(w), n, None, None, m, ptr(y), m, ptr(z), m))
+    tail = slice(T - 300, T)
+    z64 = x[tail].double() @ w.double().T
+    off = 20 * 2.0 ** -23 * (x[tail].double().abs() @ w.double().abs().T)
+    near(z[tail], z64, half_step("bf16", z64) + off)
+    near(y[tail], z64.clamp(min=0), half_step("bf16", z64) + off)
+    dx, dw = torch.zeros_like(x), torch.zeros((m, n), device="cuda")
+    check(lib.ts2_op_linear_backward(0, stream(), KIND["bf16"], ACT["relu"], T, n, m, ptr(y), m, ptr(z), m, ptr(x), n, ptr(w), n, ptr(dx), n, KIND["f32"], ptr(dw), n, None))
+    want = y[tail].double() @ w.double()  # dz = y where z > 0, and y is zero elsewhere
+    near(dx[tail], want, half_step("bf16", want) + (m / 8 + 8) * 2.0 ** -23 * (y[tail].double().abs() @ w.double().abs()))
+    cols = slice(m - 40, m)
+    want = y[:, cols].double().T @ x.double()
+    near(dw[cols], want, half_step("f32", want) + (T / 8 + 8) * 2.0 ** -23 * (y[:, cols].double().abs().T @ x.double().abs()))

@@ -7,7 +7,7 @@
 //     sigmoid              dl[e] = scale d[e] s[e] (1 - s[e])
 //     sigmoid, renormalised  dl[e] = scale w[e] (1 - s[e]) (d[e] - sum_j d[j] w[j])
 //
-// A warp takes 4 rows (8 of up to 32 experts).  They come in a row at a time in pieces of 8 columns a lane, and their keys and every piece's largest key go to
+// A warp takes 4 rows (8 of up to 128 experts).  They come in a row at a time in pieces of 8 columns a lane, and their keys and every piece's largest key go to
 // shared memory.  Then 4 or 8 lanes have a row, each the largest keys of some neighbouring pieces in registers: a choice is a maximum over those and over the
 // lanes, and only the piece that it came from is looked at again, by all of them.  Bound by instructions, 540 a row of 256 sigmoid scores with a bias, in groups and
 // 8 choices (of 224 for the row itself, 72 for its keys, 105 for groups, 20 for a choice), at 2.1 a clock of an SM with 39 % of its warps: 35.6 us for 32768 rows,

@@ -320,3 +320,12 @@ def test_more_than_32_bits_of_outputs():
     cols = slice(m - 40, m)
     want = y[:, cols].double().T @ x.double()
     near(dw[cols], want, half_step("f32", want) + (T / 8 + 8) * 2.0 ** -23 * (y[:, cols].double().abs().T @ x.double().abs()))
+
+
+@pytest.mark.parametrize("layout", ["tight", "odd pitch", "odd base"])
+@pytest.mark.parametrize("n", [1, 2, 3, 31, 63, 64, 65, 510, 511, 512, 513, 1022, 1023, 1024, 1025, 2048])
+def test_rows_that_are_copied_end_anywhere(n, layout):
+    """rows at an odd pitch or base come in as words, 512 elements at a time"""
+    forward("f16", "none", 40, n, 24, layout=layout, seed=n, bias=False, residual=False, kept=False)
+    backward("f16", "none", 70, n, 40, layout=layout, seed=n)
+    backward("bf16", "silu", 40, 30, n, layout=layout, seed=n)

@@ -786,11 +786,12 @@ struct PitchJob {
 };
 struct PitchJobs {
     PitchJob job[2];
+    int64_t items[2]; // pieces of rows
     int n;
 };
 // A block of the first `layers` takes 128 columns and rows b, b + layers, ... of 16: dz = dy act'(z) rounded to 16 bits (dz null: not wanted), and the sums of
-// the unrounded dz over its rows (sums null: not wanted).  Bound by reading dy and z.  Where 16-byte accesses are not possible (VEC false) a lane has columns
-// that are 16 apart, so that neighbouring lanes read neighbours.  The layers behind copy rows.
+// the unrounded dz over its rows (sums null: not wanted).  Bound by reading dy and z.  Where 16-byte accesses are not possible (VEC false) a lane has pairs of
+// columns that are 16 pairs apart, so that neighbouring lanes read neighbouring 4-byte words.  The layers behind copy rows.
 template <int ACT, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restrict__ dy, int64_t dy_ld, const uint16_t *__restrict__ z, int64_t z_ld,
                                                         int64_t T, int n, int layers, uint16_t *dz, int64_t dz_ld, float *sums, const PitchJobs jobs)
@@ -798,38 +799,61 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restri
     grid_dep_wait();
     if ((int)blockIdx.y >= layers) {
         const int64_t worker = ((int64_t)(blockIdx.y - layers) * gridDim.x + blockIdx.x) * 8 + (threadIdx.x >> 5), workers = (int64_t)(gridDim.y - layers) * gridDim.x * 8;
-        for (int i = 0; i < jobs.n; ++i) {
-            const PitchJob &j = jobs.job[i];
+        for (int64_t all = worker; all < jobs.items[0] + jobs.items[1]; all += workers) {
+            const bool second = all >= jobs.items[0];
+            const PitchJob &j = second ? jobs.job[1] : jobs.job[0];
+            const int64_t item = all - (second ? jobs.items[0] : 0);
             const int words = (j.cols + 1) / 2, pieces = (words + 255) / 256; // 256 words of a row at a time
-            for (int64_t item = worker; item < j.rows * pieces; item += workers) {
-                const int64_t r = item / pieces;
-                const int begin = (int)(item - r * pieces) * 256;
-                // 4-byte words that hold an element of the row; where it begins with the upper half of one, halves of neighbours
-                const uint16_t *row = j.from + r * j.from_ld;
-                const bool odd = (uintptr_t)row & 2;
-                const uint32_t *from = (const uint32_t *)(row - odd);
-                uint32_t *to = (uint32_t *)(j.to + r * j.to_ld); // 16-byte aligned, with room for a multiple of 8
-                const int last = (j.cols + odd - 1) / 2;
+            const int64_t r = pieces == 1 ? item : item / pieces;
+            const int begin = (int)(item - r * pieces) * 256 + (threadIdx.x & 31);
+            // 4-byte words that hold an element of the row; where it begins with the upper half of one, halves of neighbours
+            const uint16_t *row = j.from + r * j.from_ld;
+            const bool odd = (uintptr_t)row & 2;
+            const uint32_t *from = (const uint32_t *)(row - odd);
+            uint32_t *to = (uint32_t *)(j.to + r * j.to_ld); // 16-byte aligned, with room for a multiple of 8
+            const int last = (j.cols + odd - 1) / 2;
+            uint32_t w[9]; // all loads before the first store; w[8]: the word behind the piece, in lane 0
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                w[k] = begin + k * 32 < words ? from[begin + k * 32] : 0u;
+            if (odd) { // the word behind the row's last one may be needed, and no other
+                const int lane = threadIdx.x & 31;
+                w[8] = lane == 0 && begin + 256 <= last ? from[begin + 256] : 0u;
+                const uint32_t end = words <= last && words > begin - lane && words <= begin - lane + 256 ? from[words] : 0u;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int c = begin + k * 32 + (threadIdx.x & 31);
-                    if (c < words) {
-                        const uint32_t a = from[c], b = odd && c < last ? from[c + 1] : 0u;
-                        to[c] = odd ? a >> 16 | b << 16 : a;
-                    }
+                    const uint32_t beside = __shfl_down_sync(0xffffffffu, w[k], 1), first = __shfl_sync(0xffffffffu, w[k + 1], 0);
+                    uint32_t next = lane == 31 ? first : beside;
+                    if (begin + k * 32 + 1 == words)
+                        next = end;
+                    w[k] = w[k] >> 16 | next << 16;
                 }
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (begin + k * 32 < words)
+                    to[begin + k * 32] = w[k];
         }
         return;
     }
     __shared__ float part[16][132];
     const int sub = threadIdx.x & 15, line = threadIdx.x >> 4, col0 = blockIdx.x * 128;
-    const auto column = [&](int k) { return col0 + (VEC ? sub * 8 + k : sub + 16 * k); };
+    const auto column = [&](int k) { return col0 + (VEC ? sub * 8 + k : 2 * (sub + 16 * (k >> 1)) + (k & 1)); };
+    const bool full = col0 + 128 <= n;
     float2 acc[4] = {};
     const auto read = [&](const uint16_t *row, uint32_t (&v)[4]) {
         if (VEC && column(0) + 8 <= n) {
             const uint4 q = *(const uint4 *)(row + column(0));
             v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+        } else if (!VEC && full) { // words that hold an element of the row; halves of neighbours where it begins with the upper half of one
+            const bool odd = (uintptr_t)row & 2;
+            const uint32_t *words = (const uint32_t *)(row - odd) + col0 / 2 + sub;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = words[16 * k];
+                if (odd)
+                    v[k] = v[k] >> 16 | words[16 * k + 1] << 16;
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -856,6 +880,10 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restri
         if (VEC) {
             if (column(0) < n) // the pitch is a multiple of 8
                 *(uint4 *)(to + column(0)) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else if (full) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *(uint32_t *)(to + column(2 * k)) = o[k];
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -927,6 +955,7 @@ struct Operand {
         if (!copy.p)
             return;
         p = copy.p, ld = ceil_div(cols, 8) * 8;
+        jobs.items[jobs.n] = rows * ceil_div((cols + 1) / 2, 256);
         jobs.job[jobs.n++] = {(const uint16_t *)from, (uint16_t *)copy.p, from_ld, ld, rows, cols};
     }
 };
@@ -936,7 +965,7 @@ int prepare(const Ctx &c, const void *dy, int64_t dy_ld, const void *z, int64_t 
 {
     const bool vec = tma_ok(dy, dy_ld, 2) && (ACT == TS2_ACT_NONE || tma_ok(z, z_ld, 2));
     const int strips = layers ? (int)ceil_div(n, 128) : 4 * sm_count(c.device);
-    const dim3 grid(strips, layers + (jobs.n ? (int)ceil_div(4 * sm_count(c.device), strips) : 0));
+    const dim3 grid(strips, layers + (int)ceil_div(std::min<int64_t>(ceil_div(jobs.items[0] + jobs.items[1], 8), 8 * sm_count(c.device)), strips));
     if (vec)
         TS2_LAUNCH((linear_dz_kernel<ACT, BF16, true>), grid, 256, 0, c.stream, (const uint16_t *)dy, dy_ld, (const uint16_t *)z, z_ld, T, n, layers,
                    (uint16_t *)dz, dz_ld, sums, jobs);

@@ -21,7 +21,7 @@ ACT = {"none": capi.ACT_NONE, "relu": capi.ACT_RELU, "gelu": capi.ACT_GELU, "sil
 F = torch.nn.functional
 ACT64 = {"none": lambda z: z, "relu": torch.relu, "gelu": F.gelu, "silu": F.silu}
 # one token, fewer than a tile, tiles and one more, sizes that no 16-byte access divides; few and many tiles, short and long sums
-SIZES = [(1, 1, 1), (1, 256, 512), (2, 333, 7), (7, 64, 130), (16, 2048, 264), (17, 1000, 24), (33, 100, 1001), (129, 1024, 64), (300, 2048, 768), (513, 72, 520),
+SIZES = [(1, 1, 1), (1, 256, 512), (2, 333, 7), (7, 64, 130), (16, 2048, 264), (17, 1000, 24), (32, 4096, 40), (33, 100, 1001), (129, 1024, 64), (300, 2048, 768), (513, 72, 520),
          (1030, 4104, 256), (2049, 520, 2056)]
 
 

@@ -667,7 +667,10 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const LinearArgs p, in
 // Bound by reading W once.  A CTA takes 16 rows of W; its 8 warps, and those of the up to 8 CTAs of a cluster where W has few rows, divide K.  A lane reads 8
 // neighbours of two rows of W and of the tokens' x; four lanes' pieces are 32 of K, and as both operands come in the same order they are the fragments of two
 // m16n8k16 products as they lie in the registers.  Sums are added in the order of the warps and CTAs.
-constexpr int FEW_WARPS = 8, FEW_BATCH = 4; // FEW_BATCH: blocks of 32 of K on their way at a time
+constexpr int FEW_WARPS = 8;
+// Blocks of 32 of K on their way at a time: more of them, or more warps an SM with fewer registers.  us for 2048 x 8192 with 2 and 4: 1 token 8.5, 9.4; 16 tokens
+// 12.9, 12.0; 32 tokens 16.3, 21.2.
+constexpr int few_batch(int nt) { return nt == 2 ? 4 : 2; }
 struct FewArgs {
     int T, n, m; // tokens, columns of x and W, rows of W
     const uint16_t *x, *w, *res;
@@ -705,6 +708,7 @@ __device__ __forceinline__ uint4 eight_of(const uint16_t *row, int k, int n, boo
 template <int NT, bool BF16, bool VEC>
 __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 4 : 1) linear_few_kernel(const FewArgs p)
 {
+    constexpr int BATCH = few_batch(NT);
     __shared__ float part[FEW_WARPS][8 * NT][17], sums[8 * NT][17];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t rank = p.ranks > 1 ? cluster_rank() : 0;
@@ -715,10 +719,10 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 4 : 1) linear_few_ke
     const bool a_there = row0 + g < p.m, b_there = row0 + g + 8 < p.m;
     float c[NT][4] = {};
 #pragma unroll 1
-    for (int kb = kb0; kb < kb1; kb += FEW_BATCH) {
-        uint4 a[FEW_BATCH], b[FEW_BATCH], x[FEW_BATCH][NT];
+    for (int kb = kb0; kb < kb1; kb += BATCH) {
+        uint4 a[BATCH], b[BATCH], x[BATCH][NT];
 #pragma unroll
-        for (int i = 0; i < FEW_BATCH; ++i) {
+        for (int i = 0; i < BATCH; ++i) {
             const int k = (kb + i) * 32 + q * 8;
             const bool in = kb + i < kb1;
             a[i] = eight_of<VEC>(wa, k, p.n, in && a_there);
@@ -728,7 +732,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 4 : 1) linear_few_ke
                 x[i][t] = eight_of<VEC>(p.x + (int64_t)(8 * t + g) * p.x_ld, k, p.n, in && 8 * t + g < p.T);
         }
 #pragma unroll
-        for (int i = 0; i < FEW_BATCH; ++i)
+        for (int i = 0; i < BATCH; ++i)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 mma16<BF16>(c[t], a[i].x, b[i].x, a[i].y, b[i].y, x[i][t].x, x[i][t].y);
@@ -1076,8 +1080,9 @@ int run_products(const Ctx &c, bool bf16, const Product *products, int n, const 
     return bf16 ? run_products<BACK, 256, true>(c, products, n, plan.splits, deal) : run_products<BACK, 256, false>(c, products, n, plan.splits, deal);
 }
 
-// tokens that take the form for a few
-constexpr int FEW_TOKENS = 16;
+// Tokens that take the form for a few.  us by it and by tiles: 32 x 2048 x 8192 16.3, 19.2; 32 x 768 x 768 3.7, 10.1; 32 x 8192 x 2048 20.3, 19.5; beyond, what
+// the tokens' own reads cost grows with them.
+constexpr int FEW_TOKENS = 32;
 template <int NT, bool BF16, bool VEC>
 int few(const Ctx &c, const FewArgs &p)
 {
@@ -1115,11 +1120,12 @@ int linear_forward(const Ctx &c, const LinearShape &s, const void *x, int64_t x_
     if (s.T <= FEW_TOKENS) {
         FewArgs f = {(int)s.T, s.in, s.out, (const uint16_t *)x, (const uint16_t *)w, (const uint16_t *)residual, x_ld, w_ld, residual_ld, y_ld, z_ld, bias,
                      (uint16_t *)y, (uint16_t *)z, s.act, 1};
-        // CTAs for two an SM, each warp with a batch of K at least
-        while (f.ranks < 8 && ceil_div(s.out, 16) * f.ranks < 2 * sm_count(c.device) && s.in >= 2 * f.ranks * FEW_WARPS * FEW_BATCH * 32)
+        // CTAs for two an SM, each warp with 128 of K at least
+        while (f.ranks < 8 && ceil_div(s.out, 16) * f.ranks < 2 * sm_count(c.device) && s.in >= 2 * f.ranks * FEW_WARPS * 4 * 32)
             f.ranks *= 2;
         const bool vec = tma_ok(x, x_ld, 2) && tma_ok(w, w_ld, 2);
-        return s.T <= 8 ? few<1>(c, s.type == TS2_OUT_BF16, vec, f) : few<2>(c, s.type == TS2_OUT_BF16, vec, f);
+        const auto form = s.T <= 8 ? few<1> : s.T <= 16 ? few<2> : few<4>;
+        return form(c, s.type == TS2_OUT_BF16, vec, f);
     }
     PitchJobs jobs = {};
     const Operand a(c, x, x_ld, s.T, s.in, jobs), b(c, w, w_ld, s.out, s.in, jobs);

@@ -629,7 +629,7 @@ int ts2_op_moe_route_backward(int device, void *stream, int type, int score, con
  * step * floor(|value| / step + u); a v that is not zero stays at or above the smallest step.  u of element j of tensor i: the upper (m) or lower (v)
  * 16 bits of h / 2^16, h = mix32(j * 0x9E3779B1 + key), key = the lower 32 bits of mix64(mix64(seed + step) ^ i); mix32: the finaliser of
  * MurmurHash3, mix64: SplitMix64's next output for that state.  Moments are summed in fp64 there, so that nothing but u decides.  A NaN or
- * an infinity in a gradient makes the moments of its 32 neighbours NaN from the next step on.
+ * an infinity in a gradient, or a moment of 2^128 or more, makes the moments of its 32 neighbours NaN from the next step on.
  * n up to 2^40 elements and 2^40 in all, beta1 and beta2 in [0, 1), eps at least 2^-126 (a v below that counts as zero beside it), up to 2^20 tensors; tensors may not overlap. */
 typedef struct ts2_adamw_tensor {
     float *param;

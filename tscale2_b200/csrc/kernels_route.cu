@@ -14,8 +14,9 @@
 // whose bytes take 3; 18.3 us for 65537 rows of 128, 4 choices, whose bytes take 2.9.
 //
 // Keys are fp32 first.  They order as exact ones would where they differ by more than fp32 can be wrong, so a row in which two choices, the last choice and the
-// next key, or two groups at the border are nearer than that is done once more in fp64 by the whole warp.  Without a bias (and with groups ranked by one key)
-// the logits themselves are the keys, and exact.
+// next key, or two groups at the border are nearer than that is done once more in fp64 by the whole warp.  A group's rank of two keys is off by what those are
+// rounded by, which is not small where a large bias and one of the other sign cancel, so a rank carries the size of its keys.  Without a bias (and with groups
+// ranked by one key) the logits themselves are the keys, and exact.
 #include "elem_types.cuh"
 #include "kernels.cuh"
 #include <algorithm>
@@ -173,12 +174,12 @@ __device__ __noinline__ void route_row_exactly(const T *__restrict__ row, const 
 }
 
 // Shared memory of a warp, in 4-byte words: keys of ROWS rows (a pitch that keeps the rows' pieces in different banks), the largest and the second key of
-// their pieces, the groups' ranks, choices and what they weigh, and of the softmax the row's maximum and its sum's reciprocal.
+// their pieces, the groups' ranks and the sizes of the keys in them, choices and what they weigh, and of the softmax the row's maximum and its sum's reciprocal.
 __host__ __device__ constexpr int key_pitch(int pieces) { return (pieces + 3) / 4 * 32 + 4; }
 __host__ __device__ constexpr int piece_pitch(int most) { return most + 4; } // most: pieces that a row may have
 __host__ __device__ constexpr int warp_words(int rows, int pieces, int most, bool second, int groups, int selected)
 {
-    return (rows * (key_pitch(pieces) + piece_pitch(most) * (second ? 2 : 1) + (groups > 1 ? groups : 0) + 2 * (selected + 1) + 2) + 3) / 4 * 4;
+    return (rows * (key_pitch(pieces) + piece_pitch(most) * (second ? 2 : 1) + (groups > 1 ? 2 * groups : 0) + 2 * (selected + 1) + 2) + 3) / 4 * 4;
 }
 
 // eight neighbours from column e on as they lie in memory, -inf behind the last one and where there is nothing to read
@@ -271,7 +272,8 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
     constexpr int pp = piece_pitch(MOST);
     const int pitch = key_pitch(pieces), slots = p.selected + 1, group_pieces = per >> 3, shift = coming ? 31 - __clz(group_pieces) : 0;
     float *keys = route_smem + warp * warp_words(ROWS, pieces, MOST, kept_second, c.groups, p.selected), *first = keys + ROWS * pitch, *second = first + ROWS * pp,
-          *ranks = second + (kept_second ? ROWS * pp : 0), *chosen = ranks + (c.groups > 1 ? ROWS * c.groups : 0), *row_max = chosen + ROWS * slots,
+          *ranks = second + (kept_second ? ROWS * pp : 0), *sizes = ranks + (c.groups > 1 ? ROWS * c.groups : 0), *chosen = sizes + (c.groups > 1 ? ROWS * c.groups : 0),
+          *row_max = chosen + ROWS * slots,
           *row_inv = row_max + ROWS;
     int *chosen_id = (int *)(row_inv + ROWS);
     const int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * ROWS;
@@ -390,8 +392,10 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                             next = fmaxf(fminf(best, a), fmaxf(next, __shfl_xor_sync(FULL, next, o)));
                         best = fmaxf(best, a);
                     }
-                    if (piece < pieces && (piece & (group_pieces - 1)) == 0)
+                    if (piece < pieces && (piece & (group_pieces - 1)) == 0) {
                         ranks[r * c.groups + (piece >> shift)] = two ? fmaxf(best + next, -INFINITY) : best;
+                        sizes[r * c.groups + (piece >> shift)] = two ? fabsf(best) + fabsf(next) : fabsf(best);
+                    }
                 }
             }
         }
@@ -401,10 +405,10 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
     // L lanes a row from here on
     const int r = lane / L, l = lane % L;
     const int64_t t = t0 + r;
-    float *my_keys = keys + r * pitch, *my_first = first + r * pp, *my_second = second + r * pp, *my_ranks = ranks + r * c.groups, *my_chosen = chosen + r * slots;
+    float *my_keys = keys + r * pitch, *my_first = first + r * pp, *my_second = second + r * pp, *my_ranks = ranks + r * c.groups, *my_sizes = sizes + r * c.groups, *my_chosen = chosen + r * slots;
     int *my_id = chosen_id + r * slots;
     const float unit = !by_logit && softmax ? row_inv[r] * 0x1p-18f : 0x1p-19f; // two scores are off by less together
-    const auto near = [&](float a, float b, float times) { return !(a - b > times * (unit + 0x1p-22f * (fabsf(a) + fabsf(b)))); };
+    const auto near = [&](float a, float b) { return !(a - b > unit + 0x1p-22f * (fabsf(a) + fabsf(b))); };
     bool unsure = false;
     unsigned dropped = 0; // groups whose experts are not to be taken
     if (c.groups > 1) {
@@ -426,10 +430,11 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                         take(my_keys[e]);
                 }
                 my_ranks[g] = two ? fmaxf(best + next, -INFINITY) : best;
+                my_sizes[g] = two ? fabsf(best) + fabsf(next) : fabsf(best);
             }
             __syncwarp();
         }
-        float worst_kept = INFINITY, best_left = -INFINITY;
+        float worst_kept = INFINITY, best_left = -INFINITY; // as far down and up as they may be: two scores, two keys' roundings and the sum's
         for (int g = l; g < c.groups; g += L) {
             const float mine = my_ranks[g];
             int before = 0;
@@ -437,10 +442,11 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                 const float other = my_ranks[h];
                 before += other > mine || (other == mine && h < g) ? 1 : 0;
             }
+            const float off = mine < INFINITY ? unit + 0x1p-21f * my_sizes[g] : 0.f;
             if (before < c.kept && mine > -INFINITY) {
-                worst_kept = fminf(worst_kept, mine);
+                worst_kept = fminf(worst_kept, mine - off);
             } else {
-                best_left = fmaxf(best_left, mine);
+                best_left = mine > -INFINITY ? fmaxf(best_left, mine + off) : best_left;
                 dropped |= 1u << g;
             }
         }
@@ -448,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1)
             dropped |= __shfl_xor_sync(FULL, dropped, o);
-        unsure = !by_logit && best_left > -INFINITY && near(worst_kept, best_left, 2.f);
+        unsure = !by_logit && best_left > -INFINITY && !(worst_kept > best_left);
         if (per % 8) { // pieces across groups: what is left of them
             for (int i = l; i < pieces; i += L) {
                 float best = -INFINITY;
@@ -536,7 +542,7 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
         top = fmaxf(top, softmax ? v[i] : fminf(v[i], 0.f));
         if (!by_logit && id >= 0) {
             const int next = my_id[j + 1];
-            if (next >= 0 && near(my_chosen[j], my_chosen[j + 1], 1.f)) // equal logits and biases are equal keys, whose order is known
+            if (next >= 0 && near(my_chosen[j], my_chosen[j + 1])) // equal logits and biases are equal keys, whose order is known
                 unsure |= j == p.selected - 1 || v[i] != widen(row[next]) || (c.bias && c.bias[id] != c.bias[next]);
         }
         if (i * L + L >= p.selected)

@@ -601,7 +601,8 @@ int ts2_op_linear_backward(int device, void *stream, int type, int act, int64_t 
  * can be chosen; up to 32 groups.  ids [T][selected]: the largest keys, descending; the lower index first among equal ones, of groups too.  Keys that differ
  * are told apart as in fp64, without a bias by the logits themselves.  weights fp32 [T][selected]: scale * score, with
  * renormalize scale * score / sum of the token's chosen scores.
- * An expert whose logit is -inf or whose key is -inf or NaN is not chosen, and does not count in its group (a NaN or +inf logit takes out a whole softmax row);
+ * An expert whose logit is -inf or whose key is -inf or NaN is not chosen, and does not count in its group, which is not kept where fewer than group_top experts
+ * count in it (a NaN or +inf logit takes out a whole softmax row);
  * where too few are left, ids ends with -1, weights with 0.  Tokens with a zero byte in token_mask [T] (optional) have ids -1 and weights 0, whatever
  * their logits are.  expert_count up to 1024, selected up to 32 and to the experts of groups_kept groups, T up to 2^30. */
 #define TS2_SCORE_SOFTMAX 0

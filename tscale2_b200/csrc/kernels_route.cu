@@ -257,6 +257,9 @@ __device__ __forceinline__ void two_of(const float (&v)[8], float &best, float &
     best = fmaxf(a[0], a[2]), next = fmaxf(fminf(a[0], a[2]), fmaxf(b[0], b[2]));
 }
 
+// half the sum of two keys, which does not overflow where both are fp32's lowest or largest value; -inf where one of them is none
+__device__ __forceinline__ float half_sum(float best, float next) { return next > -INFINITY ? fmaf(0.5f, best, 0.5f * next) : -INFINITY; }
+
 // L: lanes that share a row while choices are made; NB: pieces of 8 columns that each of them has (E <= 8 L NB)
 template <class T, int L, int NB>
 __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) route_forward_kernel(const T *__restrict__ logits, int64_t ld, bool vec, const RouteShape p, const Choice c,
@@ -393,8 +396,8 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                         best = fmaxf(best, a);
                     }
                     if (piece < pieces && (piece & (group_pieces - 1)) == 0) {
-                        ranks[r * c.groups + (piece >> shift)] = two ? fmaxf(best + next, -INFINITY) : best;
-                        sizes[r * c.groups + (piece >> shift)] = two ? fabsf(best) + fabsf(next) : fabsf(best);
+                        ranks[r * c.groups + (piece >> shift)] = two ? half_sum(best, next) : best;
+                        sizes[r * c.groups + (piece >> shift)] = two ? half_sum(fabsf(best), fabsf(next)) : fabsf(best);
                     }
                 }
             }
@@ -429,12 +432,12 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                     for (int e = g * per; e < (g + 1) * per; ++e)
                         take(my_keys[e]);
                 }
-                my_ranks[g] = two ? fmaxf(best + next, -INFINITY) : best;
-                my_sizes[g] = two ? fabsf(best) + fabsf(next) : fabsf(best);
+                my_ranks[g] = two ? half_sum(best, next) : best;
+                my_sizes[g] = two ? half_sum(fabsf(best), fabsf(next)) : fabsf(best);
             }
             __syncwarp();
         }
-        float worst_kept = INFINITY, best_left = -INFINITY; // as far down and up as they may be: two scores, two keys' roundings and the sum's
+        float worst_kept = INFINITY, best_left = -INFINITY; // as far down and up as they may be: scores, and the roundings of keys and sum
         for (int g = l; g < c.groups; g += L) {
             const float mine = my_ranks[g];
             int before = 0;
@@ -442,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, NB <= 4 ? 8 : NB * L == 32 ? 5 : 4) r
                 const float other = my_ranks[h];
                 before += other > mine || (other == mine && h < g) ? 1 : 0;
             }
-            const float off = mine < INFINITY ? unit + 0x1p-21f * my_sizes[g] : 0.f;
+            const float off = mine < INFINITY ? 0.5f * unit + 0x1p-21f * my_sizes[g] : 0.f;
             if (before < c.kept && mine > -INFINITY) {
                 worst_kept = fminf(worst_kept, mine - off);
             } else {

@@ -107,16 +107,19 @@ __device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), e
 __device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
 __device__ __forceinline__ float2 minus_abs(float2 z) { return make_float2(-fabsf(z.x), -fabsf(z.y)); }
 __device__ __forceinline__ float2 sigmoid(float2 z) { return rcp(add2(ex2(mul2(z, both(-1.44269504f))), both(1.f))); }
-// 1 - Phi(|z|) and e = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun for the error function (absolute error below 1.5e-7): a third of the
-// instructions of erff, and far below the rounding of a 16-bit result
+// 1 - Phi(|z|) = e t P(t) with e = exp(-z^2 / 2), t = 1 / (1 + 0.2575 |z|).  P: a fit of degree 6 for |z| up to 14, by a linear program over 1500 Chebyshev nodes in t that
+// bounds the absolute error near zero and the relative one in the tail, whose values a 16-bit result keeps.  In fp32 it is off by 2.2e-7 at most, and of itself by
+// 2e-6 at 3, 3e-6 at 6, 1e-5 at 13 (what e's exponent is rounded by; half a step of fp16 is 4.9e-4): a third of the instructions of erff.  Beyond 13.2 e is 0.
 __device__ __forceinline__ float2 normal_tail(float2 z, float2 minus_z, float2 &e)
 {
-    const float2 t = rcp(fma2(minus_z, both(-0.3275911f * 0.70710678f), both(1.f)));
+    const float2 t = rcp(fma2(minus_z, both(-0.257499993f), both(1.f)));
     e = ex2(mul2(mul2(z, z), both(-0.72134752f)));
-    float2 q = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
-    q = fma2(t, q, both(0.5f * 1.421413741f));
-    q = fma2(t, q, both(0.5f * -0.284496736f));
-    q = fma2(t, q, both(0.5f * 0.254829592f));
+    float2 q = fma2(t, both(-0.0768212900f), both(0.251779079f));
+    q = fma2(t, q, both(-0.136068970f));
+    q = fma2(t, q, both(0.185658634f));
+    q = fma2(t, q, both(0.0655971989f));
+    q = fma2(t, q, both(0.107425064f));
+    q = fma2(t, q, both(0.102430306f));
     return mul2(q, mul2(t, e));
 }
 template <int ACT>

@@ -39,3 +39,22 @@ def test_gelu(kind, T, n, m):
         want = torch.where(z64 < 0, z64 * tail(-z64), z64 * (1 - tail(z64)))
         off = (y.double() - want).abs() - half_step(kind, want) - 1.01 * ((2.0 ** -17 + 2.0 ** -23 * z64 ** 2) * z64.abs() * tail(z64.abs()) + 2.0 ** -22 * want.abs()) - 2.0 ** -120
         assert off.max() <= 0, (low, z[off.argmax() % m].item(), off.max().item())
+
+
+# rows without 16-byte alignment take other loads
+@pytest.mark.parametrize("m", [4096, 4001])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_slope_of_gelu(kind, m):
+    """of one token dbias is the unrounded dz, and dw = dz x is dz rounded"""
+    for low, high in ((-14, -3), (-6, 0), (-1e-2, 1e-2), (0, 14)):
+        z = grid(kind, low, high, m).view(1, m)
+        dy, x = torch.ones((1, m), device="cuda", dtype=TYPE[kind]), torch.ones((1, 8), device="cuda", dtype=TYPE[kind])
+        dw, db = torch.zeros((m, 8), device="cuda"), torch.zeros(m, device="cuda")
+        check(capi.load_library().ts2_op_linear_backward(0, stream(), KIND[kind], ACT["gelu"], 1, 8, m, ptr(dy), m, ptr(z), m, ptr(x), 8, None, 8, None, 8, KIND["f32"], ptr(dw), 8,
+                                                         ptr(db)))
+        z64 = z[0].double()
+        part = tail(z64.abs()) - z64.abs() * density(z64)  # the slope at -|z|
+        want = torch.where(z64 < 0, part, 1 - part)
+        off = 1.01 * ((2.0 ** -17 + 2.0 ** -23 * z64 ** 2) * (tail(z64.abs()) + z64.abs() * density(z64)) + 2.0 ** -23 * want.abs()) + 2.0 ** -120
+        assert ((db - want).abs() <= off).all(), (low, z64[((db - want).abs() - off).argmax()].item())
+        assert ((dw.double() - want[:, None]).abs() <= (off + half_step(kind, want))[:, None]).all()

@@ -107,10 +107,10 @@ __device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), e
 __device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
 __device__ __forceinline__ float2 minus_abs(float2 z) { return make_float2(-fabsf(z.x), -fabsf(z.y)); }
 __device__ __forceinline__ float2 sigmoid(float2 z) { return rcp(add2(ex2(mul2(z, both(-1.44269504f))), both(1.f))); }
-// 1 - Phi(|z|) = e t P(t) with e = exp(-z^2 / 2), t = 1 / (1 + 0.2575 |z|).  P: a fit of degree 6 for |z| up to 14, by a linear program over 1500 Chebyshev nodes in t that
+// 1 - Phi(|z|) = e g with e = exp(-z^2 / 2) and g = t P(t), t = 1 / (1 + 0.2575 |z|).  P: a fit of degree 6 for |z| up to 14, by a linear program over 1500 Chebyshev nodes in t that
 // bounds the absolute error near zero and the relative one in the tail, whose values a 16-bit result keeps.  In fp32 it is off by 2.2e-7 at most, and of itself by
 // 2e-6 at 3, 3e-6 at 6, 1e-5 at 13 (what e's exponent is rounded by; half a step of fp16 is 4.9e-4): a third of the instructions of erff.  Beyond 13.2 e is 0.
-__device__ __forceinline__ float2 normal_tail(float2 z, float2 minus_z, float2 &e)
+__device__ __forceinline__ void normal_tail(float2 z, float2 minus_z, float2 &g, float2 &e)
 {
     const float2 t = rcp(fma2(minus_z, both(-0.257499993f), both(1.f)));
     e = ex2(mul2(mul2(z, z), both(-0.72134752f)));
@@ -120,7 +120,7 @@ __device__ __forceinline__ float2 normal_tail(float2 z, float2 minus_z, float2 &
     q = fma2(t, q, both(0.0655971989f));
     q = fma2(t, q, both(0.107425064f));
     q = fma2(t, q, both(0.102430306f));
-    return mul2(q, mul2(t, e));
+    g = mul2(t, q);
 }
 template <int ACT>
 __device__ __forceinline__ float2 activation(float2 z)
@@ -129,9 +129,9 @@ __device__ __forceinline__ float2 activation(float2 z)
         return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y); // a NaN stays one
     if (ACT == TS2_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| (1 - Phi(|z|)), the last term 0 far out
         const float2 m = minus_abs(z);
-        float2 e;
-        const float2 tail = normal_tail(z, m, e);
-        return fma2(make_float2(fmaxf(m.x, -64.f), fmaxf(m.y, -64.f)), tail, make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f)));
+        float2 g, e;
+        normal_tail(z, m, g, e);
+        return fma2(make_float2(fmaxf(m.x, -64.f), fmaxf(m.y, -64.f)), mul2(g, e), make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f)));
     }
     if (ACT == TS2_ACT_SILU)
         return mul2(z, sigmoid(z));
@@ -142,11 +142,12 @@ __device__ __forceinline__ float2 activation_slope(float2 z)
 {
     if (ACT == TS2_ACT_RELU)
         return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
-    if (ACT == TS2_ACT_GELU) { // Phi(z) + z phi(z), Phi(z) = 1/2 + sign(z) (1/2 - (1 - Phi(|z|)))
-        float2 e;
-        const float2 half = fma2(normal_tail(z, minus_abs(z), e), both(-1.f), both(0.5f));
-        const float2 phi = add2(make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y)), both(0.5f));
-        return fma2(mul2(z, both(0.39894228f)), e, phi);
+    if (ACT == TS2_ACT_GELU) { // Phi(z) + z phi(z): e (g - |z| / sqrt(2 pi)) at -|z|, where nothing cancels but at the zero itself, and one minus that at |z|
+        const float2 m = minus_abs(z);
+        float2 g, e;
+        normal_tail(z, m, g, e);
+        const float2 low = mul2(e, fma2(make_float2(fmaxf(m.x, -64.f), fmaxf(m.y, -64.f)), both(0.39894228f), g));
+        return make_float2(z.x < 0.f ? low.x : 1.f - low.x, z.y < 0.f ? low.y : 1.f - low.y);
     }
     if (ACT == TS2_ACT_SILU) {
         const float2 s = sigmoid(z);

@@ -27,7 +27,7 @@ struct AdamwRecord {
     int64_t n;
     uint32_t chunk0; // the tensor's first chunk in the launch
     uint32_t key;
-    float keep, rate; // 1 - r decay, r / (1 - beta1^k)
+    float decay, rate; // r decay, r / (1 - beta1^k)
 };
 struct AdamwArgs {
     double beta1, beta2;
@@ -166,13 +166,14 @@ __device__ __forceinline__ void encode8(const double (&x)[8], const uint32_t (&h
     }
 }
 
-// a v below 2^-126 counts as zero beside eps (its root is below 2^-63)
+// A v below 2^-126 counts as zero beside eps (its root is below 2^-63).  The decay is taken off with the update, since 1 - r decay would be rounded to steps of 2^-24: r decay
+// of 1e-7 would be 1.2e-7 for every element and step.
 __device__ __forceinline__ float step_of(const AdamwArgs &a, const AdamwRecord &r, float p, float m, float v)
 {
     float root, inverse;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root, a.inv_c2, a.eps)));
-    return fmaf(p, r.keep, -r.rate * m * inverse);
+    return p - fmaf(r.decay, p, r.rate * m * inverse);
 }
 
 // what a thread reads in a turn, as it lies in memory
@@ -342,7 +343,7 @@ int adamw(const Ctx &c, int grad_type, int state_bits, int copy_type, const ts2_
         r.param = t.param, r.grad = t.grad, r.m = t.m, r.v = t.v, r.m_scale = t.m_scale, r.v_scale = t.v_scale, r.copy = t.copy, r.n = t.n;
         r.chunk0 = (uint32_t)chunks;
         r.key = (uint32_t)mix64(mix64(seed + (uint64_t)step) ^ (uint64_t)i);
-        r.keep = (float)(1. - (double)rate * t.rate * t.decay);
+        r.decay = (float)((double)rate * t.rate * t.decay);
         r.rate = (float)((double)rate * t.rate / c1);
         chunks += mine;
     }

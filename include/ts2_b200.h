@@ -588,8 +588,9 @@ int ts2_op_linear_forward(int device, void *stream, int type, int act, int64_t T
                           int64_t z_ld);
 /* Its backward pass: dz = dy act'(z), dx = dz W, dw = dz^T x, dbias = sum_t dz; the gradient of the residual is dy.  Each of dx, dw and dbias
  * may be null.  z: what the forward call left; not read where act is TS2_ACT_NONE.  x is read for dw only, w for dx only.  dx [T][in_dim] of `type`; dw
- * [out_dim][in_dim] of dw_kind: `type`, TS2_OUT_F32 or TS2_OUT_F32_ADD (dw +=); dbias fp32 [out_dim].  With an activation dz is rounded to
- * `type` for the two products (not for dbias).  T = 0 gives zeros.  All are gradients of the same sign. */
+ * [out_dim][in_dim] of dw_kind: `type`, TS2_OUT_F32 or TS2_OUT_F32_ADD (dw +=); dbias fp32 [out_dim].  With an activation dz is rounded to `type` for the two
+ * products (not for dbias), to an infinity beyond fp16's range, so that an fp32 dw shows it; fp16 results saturate.  T = 0 gives zeros.  All are gradients of
+ * the same sign. */
 int ts2_op_linear_backward(int device, void *stream, int type, int act, int64_t T, int64_t in_dim, int64_t out_dim, const void *dy, int64_t dy_ld,
                            const void *z, int64_t z_ld, const void *x, int64_t x_ld, const void *w, int64_t w_ld, void *dx, int64_t dx_ld,
                            int dw_kind, void *dw, int64_t dw_ld, float *dbias);

@@ -186,6 +186,15 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     const __half2 r = sat_half2(lo, hi);
     return *(const uint32_t *)&r;
 }
+// without saturation: infinite beyond the type's range
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2_open(float lo, float hi)
+{
+    if (BF16)
+        return pack2<true>(lo, hi);
+    const __half2 r = __floats2half2_rn(lo, hi);
+    return *(const uint32_t *)&r;
+}
 template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t v)
 {
@@ -802,7 +811,7 @@ struct PitchJobs {
     int64_t items[2]; // pieces of rows
     int n;
 };
-// A block of the first `layers` takes 128 columns and rows b, b + layers, ... of 16: dz = dy act'(z) rounded to 16 bits (dz null: not wanted), and the sums of
+// A block of the first `layers` takes 128 columns and rows b, b + layers, ... of 16: dz = dy act'(z) rounded to 16 bits, without saturation (dz null: not wanted), and the sums of
 // the unrounded dz over its rows (sums null: not wanted).  Bound by reading dy and z and writing dz (32768 x 8192 with GELU 303 us, 5.3 TB/s).  Where 16-byte accesses are not possible (VEC false) a lane has pairs of
 // columns that are 16 pairs apart, so that neighbouring lanes read neighbouring 4-byte words.  The layers behind copy rows.
 template <int ACT, bool BF16, bool VEC>
@@ -885,7 +894,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restri
             if (ACT != TS2_ACT_NONE)
                 d = mul2(d, activation_slope<ACT>(unpack2<BF16>(b[k])));
             acc[k] = add2(acc[k], d);
-            o[k] = pack2<BF16>(d.x, d.y);
+            o[k] = pack2_open<BF16>(d.x, d.y); // dw shows a gradient that left the range
         }
         if (!dz)
             continue;

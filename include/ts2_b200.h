@@ -602,10 +602,9 @@ int ts2_op_linear_backward(int device, void *stream, int type, int act, int64_t 
  * can be chosen; up to 32 groups.  ids [T][selected]: the largest keys, descending; the lower index first among equal ones, of groups too.  Keys that differ
  * are told apart as in fp64, without a bias by the logits themselves.  weights fp32 [T][selected]: scale * score, with
  * renormalize scale * score / sum of the token's chosen scores.
- * An expert whose logit is -inf or whose key is -inf or NaN is not chosen, and does not count in its group, which is not kept where fewer than group_top experts
- * count in it (a NaN or +inf logit takes out a whole softmax row);
- * where too few are left, ids ends with -1, weights with 0.  Tokens with a zero byte in token_mask [T] (optional) have ids -1 and weights 0, whatever
- * their logits are.  expert_count up to 1024, selected up to 32 and to the experts of groups_kept groups, T up to 2^30. */
+ * An expert whose logit is -inf or whose key is -inf or NaN is not chosen (a NaN or +inf logit takes out a whole softmax row), and does not count in its group;
+ * a group of fewer than group_top that count is not kept.  Where too few are left, ids ends with -1, weights with 0.  Tokens with a zero byte in token_mask
+ * [T] (optional) have ids -1 and weights 0, whatever their logits are.  expert_count up to 1024, selected up to 32 and to the experts of groups_kept groups, T up to 2^30. */
 #define TS2_SCORE_SOFTMAX 0
 #define TS2_SCORE_SIGMOID 1
 int ts2_op_moe_route_forward(int device, void *stream, int type, int score, const void *logits, int64_t ld, int64_t T, int expert_count, int selected,
@@ -618,8 +617,8 @@ int ts2_op_moe_route_backward(int device, void *stream, int type, int score, con
                               int renormalize, float scale, const uint8_t *token_mask, const int32_t *ids, const float *dweights, void *dlogits,
                               int64_t dlogits_ld, int add);
 
-/* One AdamW step of many tensors: with g = fp32(grad * grad_scale) (times *grad_scale_dev, optional, fp32 on the device: unscaling or clipping
- * that the host does not know yet), r = rate * the tensor's rate and k = step >= 1
+/* One AdamW step of many tensors: with g = fp32(grad * f), f = grad_scale or, with grad_scale_dev (optional, an fp32 factor on the device: unscaling or
+ * clipping that the host does not know yet), f = fp32(grad_scale * *grad_scale_dev), r = rate * the tensor's rate and k = step >= 1
  *     m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
  *     param = param (1 - r decay) - r m / (1 - beta1^k) / (sqrt(v / (1 - beta2^k)) + eps)
  * tensors: a host array, read before the call returns.  param fp32; grad of grad_type (TS2_OUT_F32, _F16 or _BF16); copy: param rounded to copy_type
@@ -630,8 +629,9 @@ int ts2_op_moe_route_backward(int device, void *stream, int type, int score, con
  * magnitude M of the 32, 2^(floor(log2 M) - 7).  A value is rounded to one of its two neighbours so that its expectation is itself: to
  * step * floor(|value| / step + u); a v that is not zero stays at or above the smallest step.  u of element j of tensor i: the upper (m) or lower (v)
  * 16 bits of h / 2^16, h = mix32(j * 0x9E3779B1 + key), key = the lower 32 bits of mix64(mix64(seed + step) ^ i); mix32: the finaliser of
- * MurmurHash3, mix64: SplitMix64's next output for that state.  Moments are summed in fp64 there, so that nothing but u decides.  A NaN or
- * an infinity in a gradient, or a moment of 2^128 or more, makes the moments of its 32 neighbours NaN from the next step on.
+ * MurmurHash3, mix64: SplitMix64's next output for that state.  Moments are summed in fp64 there, from the fp32 beta1, beta2 and
+ * g, so that nothing but u decides.  A NaN or an infinity in a gradient, or a moment of 2^128 or more, makes the moments of its 32 neighbours NaN from the
+ * next step on.
  * n up to 2^40 elements and 2^40 in all, beta1 and beta2 in [0, 1), eps at least 2^-126 (a v below that counts as zero beside it), up to 2^20 tensors; tensors may not overlap. */
 typedef struct ts2_adamw_tensor {
     float *param;

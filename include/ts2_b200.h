@@ -580,7 +580,7 @@ int ts2_op_orthogonalize(int device, void *stream, int type, const void *g, int6
  * y and z are rounded once.  residual may be y itself (same pitch): y += act(z).  A few tokens, the step of a generation, take a form
  * that is bound by reading W.  T up to 2^30, in_dim and out_dim up to 2^20, and ceil(T / 128) * ceil(d / 64) below 2^30 for d the larger of the two (2^30
  * tokens of 8128 columns; TS2_ERR_INVALID_ARG beyond, of the backward call too).  Scratch: x and w where TMA cannot address their rows (a base or a pitch
- * that is no multiple of 16 bytes), 2 * T * in_dim and 2 * out_dim * in_dim bytes. */
+ * that is no multiple of 16 bytes), 2 * T * in_dim and 2 * out_dim * in_dim bytes, and partial sums, up to 1 GB; none for up to 32 tokens. */
 #define TS2_ACT_NONE 0
 #define TS2_ACT_RELU 1
 #define TS2_ACT_GELU 2 /* z Phi(z), Phi of the error function */
@@ -592,7 +592,7 @@ int ts2_op_linear_forward(int device, void *stream, int type, int act, int64_t T
  * may be null.  z: what the forward call left; not read where act is TS2_ACT_NONE.  x is read for dw only, w for dx only.  dx [T][in_dim] of `type`; dw
  * [out_dim][in_dim] of dw_kind: `type`, TS2_OUT_F32 or TS2_OUT_F32_ADD (dw +=); dbias fp32 [out_dim].  With an activation dz is rounded to `type` for the two
  * products (not for dbias), to an infinity beyond fp16's range, so that an fp32 dw shows it; fp16 results saturate.  T = 0 gives zeros.  All are gradients of
- * the same sign.  Scratch: dz, 2 * T * out_dim bytes, with an activation, and copies as in the forward call (dy's without one).
+ * the same sign.  Scratch: dz, 2 * T * out_dim bytes, with an activation, copies as in the forward call (dy's without one), and partial sums, up to 1 GB.
  * The library's pool keeps 2 GB between calls; a call that needs more maps it each time, tens of milliseconds: fewer tokens a call avoid it. */
 int ts2_op_linear_backward(int device, void *stream, int type, int act, int64_t T, int64_t in_dim, int64_t out_dim, const void *dy, int64_t dy_ld,
                            const void *z, int64_t z_ld, const void *x, int64_t x_ld, const void *w, int64_t w_ld, void *dx, int64_t dx_ld,

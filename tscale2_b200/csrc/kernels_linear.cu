@@ -1008,6 +1008,9 @@ struct Product {
 struct Plan {
     int pn, splits;
 };
+// Bytes of partial tiles.  Large outputs gain less from K ranges than one part in 40, and their partials would have to be mapped in each call: dw of 18048 x 24224 over
+// 222160 tokens 217 ms without ranges, 219 with two and 3.5 GB of partials.
+constexpr double MOST_PARTIALS = SCRATCH_KEEP_BYTES / 2;
 Plan plan_of(int pairs, const Product *products, int n)
 {
     Plan plan = {256, 1};
@@ -1022,6 +1025,8 @@ Plan plan_of(int pairs, const Product *products, int n)
             if (ceil_div(blocks(products[0]), per) != s)
                 continue;
             const double units = tiles(products[0]) * s, unit = per + 4.;
+            if (s > 1 && units * PM * pn * 4 > MOST_PARTIALS)
+                continue;
             // alone in whole rounds; with a second product that evens them out, by the sum
             double cost = n > 1 && rest > 0. ? std::max((units * unit + rest) / pairs, unit) + 0.5 * (blocks(products[1]) + 4.)
                                              : (double)ceil_div((int64_t)units, pairs) * unit;

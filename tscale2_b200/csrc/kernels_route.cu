@@ -27,13 +27,6 @@ namespace ts2 {
 static constexpr int THREADS = 128;
 static constexpr unsigned FULL = 0xffffffffu;
 
-__device__ __forceinline__ double warp_max(double v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        v = fmax(v, __shfl_xor_sync(FULL, v, o));
-    return v;
-}
 // over the warp: the largest key, the lowest index among equal ones; -1 where all are -inf
 __device__ __forceinline__ int warp_best(double key, int at)
 {
@@ -215,13 +208,6 @@ struct Eight {
             v[i] = widen(q[i / PER].v[i % PER]);
     }
 };
-template <class T>
-__device__ __forceinline__ void load8(const T *row, int e, int E, bool vec, float (&v)[8])
-{
-    Eight<T> q;
-    q.load(row, e, E, vec, true);
-    q.widen_to(v);
-}
 // over the `width` neighbouring lanes that share a row
 __device__ __forceinline__ float max_over(float v, int width)
 {

@@ -1,4 +1,5 @@
-// Element types of the operators beside the engine: fp32, fp16 (results saturate) and bf16 arrays, a 16-byte piece at a time; arithmetic on pairs of fp32.
+// Element types of the operators beside the engine: fp32, fp16 (results saturate) and bf16 arrays, a 16-byte piece at a time; arithmetic on pairs of fp32; the hardware's
+// exponential and reciprocal.
 #pragma once
 #include "common.cuh"
 
@@ -20,7 +21,23 @@ struct alignas(VEC * sizeof(T)) Piece {
     T v[VEC];
 };
 
-// both channels in one instruction
+// 2^x and 1 / x, to 2^-22 of themselves; numbers below 2^-126 are zero
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+__device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
+
+// both of a pair in one instruction
 __device__ __forceinline__ float2 mul2(float2 a, float2 b)
 {
     float2 r;

@@ -90,21 +90,7 @@ __device__ __forceinline__ Unit unit_of(const LinearArgs &p, int u)
 }
 
 // ---- activations ----------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float ex2(float x)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float rcp(float x)
-{
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
-__device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
 __device__ __forceinline__ float2 minus_abs(float2 z) { return make_float2(-fabsf(z.x), -fabsf(z.y)); }
 __device__ __forceinline__ float2 sigmoid(float2 z) { return rcp(add2(ex2(mul2(z, both(-1.44269504f))), both(1.f))); }
 // 1 - Phi(|z|) = e g with e = exp(-z^2 / 2) and g = t P(t), t = 1 / (1 + 0.2575 |z|).  P: a fit of degree 6 for |z| up to 14, by a linear program over 1500 Chebyshev nodes in t that

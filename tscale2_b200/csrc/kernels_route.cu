@@ -66,18 +66,6 @@ struct Choice { // what the forward pass needs beside a RouteShape
     const float *bias;
     int groups, kept, group_top;
 };
-__device__ __forceinline__ float ex2(float x)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float rcp(float x)
-{
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 
 // One row by the whole warp, its keys in fp64: any row, and slow
 template <class T>

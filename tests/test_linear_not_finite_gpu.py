@@ -60,3 +60,33 @@ def test_products_beyond_fp16_show(T, n, m, act, slope):
     assert torch.isinf(dw[at[1]]).all() and abs(db[at[1]] - db0[at[1]] - (65504 - 1) * slope).item() < 1e-3 * 65504
     others = torch.arange(m, device="cuda") != at[1]
     assert torch.equal(dw[others], dw0[others])
+
+
+# a few tokens in each of their forms, tiles, K ranges; rows without 16-byte alignment
+@pytest.mark.parametrize("T,n,m", [(4, 64, 96), (13, 64, 96), (31, 40, 33), (40, 64, 96), (300, 333, 335), (70, 8192, 136)])
+@pytest.mark.parametrize("layout", ["tight", "odd base"])
+@pytest.mark.parametrize("act", list(ACT))
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_inputs_that_are_not_finite(kind, act, T, n, m, layout):
+    """a token's x of inf, NaN and -inf: act of it, by the formula (-inf / inf of SiLU is none), and every other token as it was"""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    t = TYPE[kind]
+    xs = torch.randn((T, n), device="cuda", generator=gen)
+    w = rows((torch.randn((m, n), device="cuda", generator=gen).abs() + 0.5).to(t), layout)
+    out = []
+    for bad in (False, True):
+        if bad:
+            xs[0, n // 2], xs[1, 0], xs[2, n - 1] = INF, NAN, -INF
+        x, y, z = rows(xs.to(t), layout), rows(torch.zeros((T, m), device="cuda", dtype=t), layout), rows(torch.zeros((T, m), device="cuda", dtype=t), layout)
+        check(capi.load_library().ts2_op_linear_forward(0, stream(), KIND[kind], ACT[act], T, n, m, x.ptr, x.ld, w.ptr, w.ld, None, None, m, y.ptr, y.ld, z.ptr, z.ld))
+        assert y.around_is_kept() and z.around_is_kept()
+        out.append((y.t.clone(), z.t.clone()))
+    (y0, z0), (y, z) = out
+    assert torch.equal(y[3:], y0[3:]) and torch.equal(z[3:], z0[3:])
+    most = INF if kind == "bf16" else 65504.0  # fp16 results saturate
+    assert (z[0] == most).all() and torch.isnan(z[1]).all() and (z[2] == -most).all()
+    assert (y[0] == most).all() and torch.isnan(y[1]).all()
+    if act == "silu":
+        assert torch.isnan(y[2]).all()
+    else:
+        assert (y[2] == (-most if act == "none" else 0)).all()

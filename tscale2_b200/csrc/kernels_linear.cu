@@ -9,7 +9,7 @@
 // dealt out first, and the others even out what those leave.
 // Rows that TMA cannot address (a base or a pitch that is no multiple of 16 bytes) are copied to a pitch that it can.
 //
-// One by one, 32768 x 2048 x 8192: without activation 742 us (1.48 PFLOP/s), with GELU and z 807; both gradients 1480 (1.49 PFLOP/s).  In a row the part's power limit takes
+// One by one, 32768 x 2048 x 8192: without activation 742 us (1.48 PFLOP/s), with GELU and z 816; both gradients 1480 to 1515 (1.45 to 1.49 PFLOP/s).  In a row the part's power limit takes
 // the clock to 1.3 GHz: 853 to 881 us without activation where a library product of the same operands takes 834.  A tile takes 18.5 k clocks, of which 16.8 k are
 // products and the ring waits 2.6 k for copies; five stages are what fits beside two blocks of staging a warp (four stages and three blocks 2 % slower).  Sums over
 // a K of 256 or less are bound by the epilogue, 9 k clocks a tile.
@@ -92,10 +92,11 @@ __device__ __forceinline__ Unit unit_of(const LinearArgs &p, int u)
 // ---- activations ----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 minus_abs(float2 z) { return make_float2(-fabsf(z.x), -fabsf(z.y)); }
+// zero below -87.3, where z sigmoid(z) is below 2^-119
 __device__ __forceinline__ float2 sigmoid(float2 z) { return rcp(add2(ex2(mul2(z, both(-1.44269504f))), both(1.f))); }
 // 1 - Phi(|z|) = e g with e = exp(-z^2 / 2) and g = t P(t), t = 1 / (1 + 0.2575 |z|).  P: a fit of degree 6 for |z| up to 14, by a linear program over 1500 Chebyshev nodes in t that
 // bounds the absolute error near zero and the relative one in the tail, whose values a 16-bit result keeps.  In fp32 it is off by 2.2e-7 at most, and of itself by
-// 2e-6 at 3, 3e-6 at 6, 1e-5 at 13 (what e's exponent is rounded by; half a step of fp16 is 4.9e-4): a third of the instructions of erff.  Beyond 13.2 e is 0.
+// 2e-6 at 3, 3e-6 at 6, 1e-5 at 13 (what e's exponent is rounded by); half a step of fp16 is 4.9e-4.  Beyond 13.2 e is 0.
 __device__ __forceinline__ void normal_tail(float2 z, float2 minus_z, float2 &g, float2 &e)
 {
     const float2 t = rcp(fma2(minus_z, both(-0.257499993f), both(1.f)));
@@ -798,7 +799,7 @@ struct PitchJobs {
     int n;
 };
 // A block of the first `layers` takes 128 columns and rows b, b + layers, ... of 16: dz = dy act'(z) rounded to 16 bits, without saturation (dz null: not wanted), and the sums of
-// the unrounded dz over its rows (sums null: not wanted).  Bound by reading dy and z and writing dz (32768 x 8192 with GELU 303 us, 5.3 TB/s).  Where 16-byte accesses are not possible (VEC false) a lane has pairs of
+// the unrounded dz over its rows (sums null: not wanted).  Bound by reading dy and z and writing dz (32768 x 8192 with GELU 312 us, 5.2 TB/s).  Where 16-byte accesses are not possible (VEC false) a lane has pairs of
 // columns that are 16 pairs apart, so that neighbouring lanes read neighbouring 4-byte words.  The layers behind copy rows.
 template <int ACT, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const uint16_t *__restrict__ dy, int64_t dy_ld, const uint16_t *__restrict__ z, int64_t z_ld,

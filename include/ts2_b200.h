@@ -603,7 +603,7 @@ int ts2_op_linear_backward(int device, void *stream, int type, int act, int64_t 
  * bias fp32 [expert_count] (optional) moves the choice and not the weights.  With groups > 1 the experts are that many groups of neighbours
  * (groups divides expert_count); a group's rank is the sum of its group_top (1 or 2) largest keys, and only experts of the groups_kept first groups
  * can be chosen; up to 32 groups.  ids [T][selected]: the largest keys, descending; the lower index first among equal ones, of groups too.  Keys that differ
- * are told apart as in fp64, without a bias by the logits themselves.  weights fp32 [T][selected]: scale * score, with
+ * are told apart as in fp64; without a bias experts, and groups ranked by one key, go by the logits themselves.  weights fp32 [T][selected]: scale * score, with
  * renormalize scale * score / sum of the token's chosen scores.
  * An expert whose logit is -inf or whose key is -inf or NaN is not chosen (a NaN or +inf logit takes out a whole softmax row), and does not count in its group;
  * a group of fewer than group_top that count is not kept.  Where too few are left, ids ends with -1, weights with 0.  Tokens with a zero byte in token_mask

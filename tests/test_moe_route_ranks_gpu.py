@@ -4,7 +4,7 @@ ids are those of the definition in float64: ranks that differ by more than fp64 
 groups, whose scores differ at random, are told apart."""
 import pytest
 
-from test_moe_route_gpu import case
+from test_moe_route_gpu import KIND, SCORE, capi, case, check, ptr, stream
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -32,3 +32,17 @@ def test_the_smallest_such_row():
     logits = torch.tensor([[-0.35720438, 1.0258067, 2.0709758, -1.0468799]], device="cuda")
     b = torch.tensor([1e4, -1e4, 1e4, -1e4], device="cuda")
     case("f32", "sigmoid", 1, 4, 2, True, 2, 1, 2, logits=logits, b=b)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,kept", GROUPS)
+def test_groups_of_one_key_without_a_bias_go_by_logits(score, E, groups, kept):
+    """logits of some hundred, whose scores float64 takes for one, or for zero"""
+    T, per, k = 200, E // groups, min(4, kept * E // groups)
+    l = 300 * torch.randn((T, E), device="cuda", generator=torch.Generator(device="cuda").manual_seed(E))
+    ids, w = torch.zeros((T, k), device="cuda", dtype=torch.int32), torch.zeros((T, k), device="cuda")
+    check(capi.load_library().ts2_op_moe_route_forward(0, stream(), KIND["f32"], SCORE[score], ptr(l), E, T, E, k, None, groups, kept, 1, 1, 1.0, None, ptr(ids), ptr(w)))
+    order = torch.sort(l.view(T, groups, per).amax(2), dim=1, descending=True, stable=True).indices[:, :kept]
+    keep = torch.zeros((T, groups), device="cuda", dtype=torch.bool).scatter_(1, order, True)
+    want = torch.sort(torch.where(keep.repeat_interleave(per, 1), l, float("-inf")), dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(ids, want.int())
